@@ -335,6 +335,88 @@ CCE_API int cce_backward_peer(const void* e, const void* c, const void* bias, in
                               void* workspace, size_t workspace_bytes, const CcePeerGroup* group,
                               void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Losses on per-token log-probabilities.  No counterpart in the reference
+ * (whose library ends at the cross-entropy); the policy and the preference
+ * loss that a head's log-probabilities are trained with.
+ *
+ * N tokens in one array; sequence s of S holds the tokens
+ * [cu_seqlens[s], cu_seqlens[s + 1]) (int32 offsets, non-decreasing), or with
+ * cu_seqlens = NULL the tokens [s N / S, (s + 1) N / S) (padded rows; N is a
+ * multiple of S).  Tokens of no sequence, and those whose mask byte is 0, add
+ * nothing and get a zero gradient; what they hold is not looked at.
+ * --------------------------------------------------------------------------- */
+
+/* reductions */
+#define CCE_REDUCE_MEAN      0  /* mean over the tokens that count (pairs)          */
+#define CCE_REDUCE_SUM       1
+#define CCE_REDUCE_SEQUENCE  2  /* mean over the sequences of their tokens' means   */
+#define CCE_REDUCE_NONE      3  /* one value per token (pair)                       */
+
+typedef struct CcePolicyParams {
+  double clip_low, clip_high;  /* ratios are clipped to [1 - clip_low, 1 + clip_high] */
+  double dual_clip;            /* > 1: loss of a negative advantage bounded by -dual_clip A; 0: not */
+  double kl_coef;              /* weight of e^q - 1 - q, q = ref_logp - logp           */
+  int32_t reduction;           /* CCE_REDUCE_*                                         */
+  int32_t advantage_per_token; /* advantages [N], else [S]                             */
+} CcePolicyParams;
+
+/* Workspace of the two forward calls (S = 2 pairs for the preference loss). */
+CCE_API size_t cce_token_loss_workspace_bytes(int64_t N, int64_t S);
+
+/*
+ * cce_policy_loss_forward -- clipped policy loss with a KL term.
+ *
+ *   logp, old_logp, ref_logp [N] dtype; old_logp NULL: ratio 1 (the policy
+ *            itself); ref_logp NULL: no KL term
+ *   advantages fp32 [N] or [S];  mask uint8 [N] or NULL
+ *   loss     fp32 out: [1], [N] with CCE_REDUCE_NONE
+ *   stats    fp32 out [2]: mean KL term, share of clipped tokens
+ *   coef     fp32 out [N], weight fp32 out [1 + S]: what the backward call
+ *            reads (the gradient is upstream * weight * coef)
+ */
+CCE_API int cce_policy_loss_forward(const void* logp, const void* old_logp, const void* ref_logp, int dtype,
+                                    const float* advantages, const uint8_t* mask, const int32_t* cu_seqlens,
+                                    int64_t N, int64_t S, const CcePolicyParams* params, float* loss, float* stats,
+                                    float* coef, float* weight, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+/* grad [N] in dtype; grad_loss fp32 [1], or [N] with CCE_REDUCE_NONE. */
+CCE_API int cce_policy_loss_backward(const float* coef, const float* weight, const float* grad_loss, int reduction,
+                                     const int32_t* cu_seqlens, int64_t N, int64_t S, int dtype, void* grad,
+                                     void* stream);
+
+/* kinds of preference loss, of gap = D_chosen - D_rejected (see below) */
+#define CCE_PREF_SIGMOID 0  /* -(1-ls) log s(h) - ls log s(-h), h = beta gap - margin, ls = label_smoothing */
+#define CCE_PREF_HINGE   1  /* max(0, 1 - h)                  */
+#define CCE_PREF_IPO     2  /* (gap - 1 / (2 beta))^2         */
+
+typedef struct CcePreferenceParams {
+  double beta, margin, label_smoothing;
+  int32_t kind;              /* CCE_PREF_*                                           */
+  int32_t reduction;         /* CCE_REDUCE_MEAN, _SUM or _NONE (over the pairs)      */
+  int32_t length_normalize;  /* D of a sequence divided by its number of tokens      */
+} CcePreferenceParams;
+
+/*
+ * cce_preference_loss_forward -- loss of `pairs` pairs of sequences; of the
+ * 2 pairs sequences, p is chosen over pairs + p.
+ *
+ *   logp, ref_logp [N] dtype (ref_logp nullable);  ref_sums fp32 [2 pairs]
+ *            or NULL: per-sequence sums in place of ref_logp
+ *   D_s = sum over the tokens that count of (logp - ref_logp), or of logp, - ref_sums[s]
+ *   loss     fp32 out: [1], [pairs] with CCE_REDUCE_NONE
+ *   rewards  fp32 out [2 pairs]: beta D_s
+ *   coef     fp32 out [2 pairs]: what the backward call reads
+ */
+CCE_API int cce_preference_loss_forward(const void* logp, const void* ref_logp, int dtype, const float* ref_sums,
+                                        const uint8_t* mask, const int32_t* cu_seqlens, int64_t N, int64_t pairs,
+                                        const CcePreferenceParams* params, float* loss, float* rewards, float* coef,
+                                        void* workspace, size_t workspace_bytes, void* stream);
+/* grad [N] in dtype; grad_loss fp32 [1], or [pairs] with CCE_REDUCE_NONE. */
+CCE_API int cce_preference_loss_backward(const float* coef, const float* grad_loss, int reduction,
+                                         const uint8_t* mask, const int32_t* cu_seqlens, int64_t N, int64_t pairs,
+                                         int dtype, void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

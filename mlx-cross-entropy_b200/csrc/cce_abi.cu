@@ -975,4 +975,135 @@ int cce_dequantize(const uint32_t* wq, const void* scales, const void* biases, i
   return CCE_OK;
 }
 
+// Sizes of a batch of sequences; S may be 0 only where no call needs sequences.
+static int check_tokens(int64_t N, int64_t S, const void* cu, int dtype, const char* what) {
+  if (N < 0 || S < 0 || N > INT32_MAX || S > INT32_MAX / 2)
+    return fail(CCE_ERR_SHAPE, "%s: bad sizes N=%lld S=%lld", what, (long long)N, (long long)S);
+  if (!dtype_ok(dtype)) return fail(CCE_ERR_DTYPE, "%s: unsupported dtype code %d", what, dtype);
+  if (cu == nullptr && S > 0 && N % S != 0)
+    return fail(CCE_ERR_SHAPE, "%s: N=%lld is not a multiple of S=%lld padded rows", what, (long long)N, (long long)S);
+  return CCE_OK;
+}
+
+size_t cce_token_loss_workspace_bytes(int64_t N, int64_t S) {
+  return N < 0 || S < 0 ? 0 : cce::token_loss_workspace_bytes(N, S);
+}
+
+int cce_policy_loss_forward(const void* logp, const void* old_logp, const void* ref_logp, int dtype,
+                            const float* advantages, const uint8_t* mask, const int32_t* cu_seqlens, int64_t N,
+                            int64_t S, const CcePolicyParams* params, float* loss, float* stats, float* coef,
+                            float* weight, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cce_policy_loss_forward";
+  int rc = check_tokens(N, S, cu_seqlens, dtype, what);
+  if (rc) return rc;
+  if (!params) return fail(CCE_ERR_ARG, "%s: NULL params", what);
+  if (!(params->clip_low >= 0.0 && params->clip_low <= 1.0) || !(params->clip_high >= 0.0))
+    return fail(CCE_ERR_ARG, "%s: clip_low must be in [0, 1] and clip_high >= 0, got %g and %g", what,
+                params->clip_low, params->clip_high);
+  if (!(params->dual_clip == 0.0 || params->dual_clip > 1.0))
+    return fail(CCE_ERR_ARG, "%s: dual_clip must be 0 or above 1, got %g", what, params->dual_clip);
+  if (params->kl_coef != params->kl_coef) return fail(CCE_ERR_ARG, "%s: kl_coef is NaN", what);
+  const int red = params->reduction;
+  if (red < CCE_REDUCE_MEAN || red > CCE_REDUCE_NONE) return fail(CCE_ERR_ARG, "%s: reduction code %d", what, red);
+  if (!loss && !(red == CCE_REDUCE_NONE && N == 0)) return fail(CCE_ERR_ARG, "%s: NULL loss", what);
+  if (!stats || !weight || (N > 0 && (!logp || !coef || (!advantages && (params->advantage_per_token || S > 0)))))
+    return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  rc = check_arch();
+  if (rc) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (N == 0) {
+    if (red != CCE_REDUCE_NONE) CCE_CUDA_CHECK(cudaMemsetAsync(loss, 0, sizeof(float), s), what);
+    CCE_CUDA_CHECK(cudaMemsetAsync(stats, 0, 2 * sizeof(float), s), what);
+    CCE_CUDA_CHECK(cudaMemsetAsync(weight, 0, (size_t)(1 + S) * sizeof(float), s), what);
+    return CCE_OK;
+  }
+  const size_t need = cce::token_loss_workspace_bytes(N, S);
+  if (!workspace || workspace_bytes < need)
+    return fail(CCE_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu", what, workspace_bytes, need);
+  const cce::PolicyArgs a{logp, old_logp, ref_logp, dtype, advantages, params->advantage_per_token, mask, cu_seqlens,
+                          N, S, red, params->clip_low, params->clip_high, params->dual_clip,
+                          ref_logp ? params->kl_coef : 0.0, loss, stats, coef, weight};
+  CCE_CUDA_CHECK(cce::policy_forward(a, workspace, s), what);
+  return CCE_OK;
+}
+
+int cce_policy_loss_backward(const float* coef, const float* weight, const float* grad_loss, int reduction,
+                             const int32_t* cu_seqlens, int64_t N, int64_t S, int dtype, void* grad, void* stream) {
+  const char* what = "cce_policy_loss_backward";
+  int rc = check_tokens(N, S, cu_seqlens, dtype, what);
+  if (rc) return rc;
+  if (reduction < CCE_REDUCE_MEAN || reduction > CCE_REDUCE_NONE)
+    return fail(CCE_ERR_ARG, "%s: reduction code %d", what, reduction);
+  if (N == 0) return CCE_OK;
+  if (!coef || !weight || !grad_loss || !grad) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  rc = check_arch();
+  if (rc) return rc;
+  CCE_CUDA_CHECK(cce::policy_backward(coef, weight, grad_loss, reduction == CCE_REDUCE_NONE, reduction, cu_seqlens, N,
+                                      S, dtype, grad, (cudaStream_t)stream),
+                 what);
+  return CCE_OK;
+}
+
+int cce_preference_loss_forward(const void* logp, const void* ref_logp, int dtype, const float* ref_sums,
+                                const uint8_t* mask, const int32_t* cu_seqlens, int64_t N, int64_t pairs,
+                                const CcePreferenceParams* params, float* loss, float* rewards, float* coef,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cce_preference_loss_forward";
+  int rc = check_tokens(N, pairs < 0 ? -1 : 2 * pairs, cu_seqlens, dtype, what);
+  if (rc) return rc;
+  if (!params) return fail(CCE_ERR_ARG, "%s: NULL params", what);
+  if (params->kind < CCE_PREF_SIGMOID || params->kind > CCE_PREF_IPO)
+    return fail(CCE_ERR_ARG, "%s: kind code %d", what, params->kind);
+  const int red = params->reduction;
+  if (red != CCE_REDUCE_MEAN && red != CCE_REDUCE_SUM && red != CCE_REDUCE_NONE)
+    return fail(CCE_ERR_ARG, "%s: reduction code %d", what, red);
+  if (!(params->beta > 0.0) || params->margin != params->margin)
+    return fail(CCE_ERR_ARG, "%s: beta must be positive and margin a number, got %g and %g", what, params->beta,
+                params->margin);
+  if (!(params->label_smoothing >= 0.0 && params->label_smoothing <= 0.5))
+    return fail(CCE_ERR_ARG, "%s: label_smoothing must be in [0, 0.5], got %g", what, params->label_smoothing);
+  if (ref_logp && ref_sums) return fail(CCE_ERR_ARG, "%s: ref_logp and ref_sums exclude each other", what);
+  if (!loss && !(red == CCE_REDUCE_NONE && pairs == 0)) return fail(CCE_ERR_ARG, "%s: NULL loss", what);
+  if (pairs > 0 && (!rewards || !coef || (N > 0 && !logp)))
+    return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  rc = check_arch();
+  if (rc) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (pairs == 0) {
+    if (red != CCE_REDUCE_NONE) CCE_CUDA_CHECK(cudaMemsetAsync(loss, 0, sizeof(float), s), what);
+    return CCE_OK;
+  }
+  const size_t need = cce::token_loss_workspace_bytes(N, 2 * pairs);
+  if (!workspace || workspace_bytes < need)
+    return fail(CCE_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu", what, workspace_bytes, need);
+  const cce::PreferenceArgs a{logp, ref_logp, dtype, ref_sums, mask, cu_seqlens, N, pairs, params->kind, red,
+                              params->length_normalize, params->beta, params->margin, params->label_smoothing, loss,
+                              rewards, coef};
+  CCE_CUDA_CHECK(cce::preference_forward(a, workspace, s), what);
+  return CCE_OK;
+}
+
+int cce_preference_loss_backward(const float* coef, const float* grad_loss, int reduction, const uint8_t* mask,
+                                 const int32_t* cu_seqlens, int64_t N, int64_t pairs, int dtype, void* grad,
+                                 void* stream) {
+  const char* what = "cce_preference_loss_backward";
+  int rc = check_tokens(N, pairs < 0 ? -1 : 2 * pairs, cu_seqlens, dtype, what);
+  if (rc) return rc;
+  if (reduction != CCE_REDUCE_MEAN && reduction != CCE_REDUCE_SUM && reduction != CCE_REDUCE_NONE)
+    return fail(CCE_ERR_ARG, "%s: reduction code %d", what, reduction);
+  if (N == 0) return CCE_OK;
+  if (!grad || (pairs > 0 && (!coef || !grad_loss))) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  rc = check_arch();
+  if (rc) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (pairs == 0) {
+    CCE_CUDA_CHECK(cudaMemsetAsync(grad, 0, (size_t)N * dtype_size(dtype), s), what);
+    return CCE_OK;
+  }
+  CCE_CUDA_CHECK(cce::preference_backward(coef, grad_loss, reduction == CCE_REDUCE_NONE, mask, cu_seqlens, N, pairs,
+                                          dtype, grad, s),
+                 what);
+  return CCE_OK;
+}
+
 }  // extern "C"

@@ -131,6 +131,39 @@ cudaError_t tc_grad_c(const BwdChunkArgs& a, void* grad_c, cudaStream_t stream);
 // one bounded pipeline wait that nothing satisfies: records `code` after limit_ns
 cudaError_t tc_selftest_wait(uint64_t limit_ns, int code, cudaStream_t stream);
 
+// ---- losses on per-token log-probabilities (token_loss.cu) ----
+// Sequences: offsets cu[S + 1] into the N tokens, or (cu == nullptr) S rows of N / S tokens.
+struct PolicyArgs {
+  const void *logp, *old, *ref;  // [N] of dtype; old, ref nullable
+  int dtype;
+  const float* adv;              // [N] (adv_token) or [S]
+  int adv_token;
+  const uint8_t* mask;           // [N], nullable
+  const int32_t* cu;
+  int64_t N, S;
+  int reduction;                 // CCE_REDUCE_*
+  double clip_low, clip_high, dual_clip, kl_coef;
+  float *loss, *stats, *coef, *weight;  // [1] or [N], [2], [N], [1 + S]
+};
+struct PreferenceArgs {
+  const void *logp, *ref;        // [N] of dtype; ref nullable
+  int dtype;
+  const float* ref_seq;          // [2 pairs], nullable
+  const uint8_t* mask;           // [N], nullable
+  const int32_t* cu;             // S = 2 pairs
+  int64_t N, pairs;
+  int kind, reduction, by_length;  // CCE_PREF_*, CCE_REDUCE_*
+  double beta, margin, smoothing;
+  float *loss, *rewards, *coef;  // [1] or [pairs], [2 pairs], [2 pairs]
+};
+size_t token_loss_workspace_bytes(int64_t N, int64_t S);
+cudaError_t policy_forward(const PolicyArgs& a, void* ws, cudaStream_t stream);
+cudaError_t policy_backward(const float* coef, const float* weight, const float* up, int up_token, int reduction,
+                            const int32_t* cu, int64_t N, int64_t S, int dtype, void* grad, cudaStream_t stream);
+cudaError_t preference_forward(const PreferenceArgs& a, void* ws, cudaStream_t stream);
+cudaError_t preference_backward(const float* coef, const float* up, int up_pair, const uint8_t* mask, const int32_t* cu,
+                                int64_t N, int64_t pairs, int dtype, void* grad, cudaStream_t stream);
+
 // ---- cross-rank grad_e exchange (peer.cu) ----
 namespace peer {
 // partial rows src[nslab][N][D] fp32 -> their owners' receive slots; raises `pushed`

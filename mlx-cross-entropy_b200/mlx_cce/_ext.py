@@ -58,6 +58,8 @@ EXPORTED_SYMBOLS = (
     "cce_peer_buffer_bytes", "cce_peer_buffer_alloc", "cce_peer_buffer_open", "cce_peer_buffer_close",
     "cce_peer_buffer_free", "cce_backward_peer", "cce_mma_flops",
     "cce_forward_q_workspace_bytes", "cce_forward_q", "cce_backward_q_workspace_bytes", "cce_backward_q",
+    "cce_token_loss_workspace_bytes", "cce_policy_loss_forward", "cce_policy_loss_backward",
+    "cce_preference_loss_forward", "cce_preference_loss_backward",
 )
 
 
@@ -71,6 +73,22 @@ class CcePeerGroup(ctypes.Structure):
     """Mirror of ``CcePeerGroup`` (include/cce_b200.h)."""
     _fields_ = [("rank", ctypes.c_int32), ("world", ctypes.c_int32), ("wait_limit_ns", ctypes.c_int64),
                 ("bytes", ctypes.c_size_t), ("bases", ctypes.c_void_p * CCE_PEER_MAX_WORLD)]
+
+
+class CcePolicyParams(ctypes.Structure):
+    """Mirror of ``CcePolicyParams`` (include/cce_b200.h)."""
+    _fields_ = [("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double), ("dual_clip", ctypes.c_double),
+                ("kl_coef", ctypes.c_double), ("reduction", ctypes.c_int32), ("advantage_per_token", ctypes.c_int32)]
+
+
+class CcePreferenceParams(ctypes.Structure):
+    """Mirror of ``CcePreferenceParams`` (include/cce_b200.h)."""
+    _fields_ = [("beta", ctypes.c_double), ("margin", ctypes.c_double), ("label_smoothing", ctypes.c_double),
+                ("kind", ctypes.c_int32), ("reduction", ctypes.c_int32), ("length_normalize", ctypes.c_int32)]
+
+
+CCE_REDUCE_MEAN, CCE_REDUCE_SUM, CCE_REDUCE_SEQUENCE, CCE_REDUCE_NONE = 0, 1, 2, 3
+CCE_PREF_SIGMOID, CCE_PREF_HINGE, CCE_PREF_IPO = 0, 1, 2
 
 _DTYPE_CODE = {torch.float32: CCE_F32, torch.float16: CCE_F16, torch.bfloat16: CCE_BF16}
 
@@ -140,6 +158,19 @@ def _load():
     lib.cce_backward_peer.argtypes = [c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
                                       c_i64, c_i64, c_int, c_int, c_f, c_vp, c_vp, c_vp, c_vp, c_vp,
                                       c_sz, ctypes.POINTER(CcePeerGroup), c_vp]
+    lib.cce_token_loss_workspace_bytes.restype = c_sz
+    lib.cce_token_loss_workspace_bytes.argtypes = [c_i64, c_i64]
+    lib.cce_policy_loss_forward.restype = c_int
+    lib.cce_policy_loss_forward.argtypes = [c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_i64,
+                                            ctypes.POINTER(CcePolicyParams), c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]
+    lib.cce_policy_loss_backward.restype = c_int
+    lib.cce_policy_loss_backward.argtypes = [c_vp, c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]
+    lib.cce_preference_loss_forward.restype = c_int
+    lib.cce_preference_loss_forward.argtypes = [c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_i64,
+                                                ctypes.POINTER(CcePreferenceParams), c_vp, c_vp, c_vp, c_vp, c_sz,
+                                                c_vp]
+    lib.cce_preference_loss_backward.restype = c_int
+    lib.cce_preference_loss_backward.argtypes = [c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]
     return lib
 
 
@@ -498,6 +529,87 @@ def dequantize(wq, scales, biases, group_size: int, bits: int, dtype, out=None, 
                             int(group_size), int(bits), dtype_code(dtype, what), _ptr(out), _stream(stream))
     _check(rc, what)
     return out
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def on_device(dev):
+    """Context in which a library call for tensors on ``dev`` is made."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def policy_forward(logp, old, ref, adv, mask, cu, S, params):
+    """``cce_policy_loss_forward`` on checked contiguous tensors.
+
+    Returns (loss, stats [2], coef [N + 1 + S]: per-token coefficients, then weights).
+    """
+    dev, N = logp.device, logp.numel()
+    with on_device(dev):
+        f32 = dict(dtype=torch.float32, device=dev)
+        none = params.reduction == CCE_REDUCE_NONE
+        loss = torch.empty(logp.shape if none else (), **f32)
+        stats = torch.empty((2,), **f32)
+        off = (N + 3) // 4 * 4
+        coef = torch.empty((off + 1 + S,), **f32)
+        ws_bytes = lib.cce_token_loss_workspace_bytes(N, S)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+        c = coef.data_ptr()
+        rc = lib.cce_policy_loss_forward(_addr(logp), _addr(old), _addr(ref), _DTYPE_CODE[logp.dtype], _addr(adv),
+                                         _addr(mask), _addr(cu), N, S, params, loss.data_ptr(), stats.data_ptr(), c,
+                                         c + 4 * off, ws.data_ptr(), ws_bytes,
+                                         torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_policy_loss_forward")
+    return loss, stats, coef
+
+
+def policy_backward(coef, grad_loss, reduction, cu, N, S, shape, dtype):
+    """``cce_policy_loss_backward``: the gradient with respect to logp."""
+    dev = coef.device
+    with on_device(dev):
+        grad = torch.empty(shape, dtype=dtype, device=dev)
+        c = coef.data_ptr()
+        rc = lib.cce_policy_loss_backward(c, c + 4 * ((N + 3) // 4 * 4), grad_loss.data_ptr(), reduction, _addr(cu), N,
+                                          S, _DTYPE_CODE[dtype], grad.data_ptr(),
+                                          torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_policy_loss_backward")
+    return grad
+
+
+def preference_forward(logp, ref, ref_sums, mask, cu, pairs, params):
+    """``cce_preference_loss_forward`` on checked contiguous tensors.
+
+    Returns (loss, rewards [2 pairs], coef [2 pairs]).
+    """
+    dev, N = logp.device, logp.numel()
+    with on_device(dev):
+        f32 = dict(dtype=torch.float32, device=dev)
+        loss = torch.empty((pairs,) if params.reduction == CCE_REDUCE_NONE else (), **f32)
+        rewards = torch.empty((2 * pairs,), **f32)
+        coef = torch.empty((2 * pairs,), **f32)
+        ws_bytes = lib.cce_token_loss_workspace_bytes(N, 2 * pairs)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+        rc = lib.cce_preference_loss_forward(_addr(logp), _addr(ref), _DTYPE_CODE[logp.dtype], _addr(ref_sums),
+                                             _addr(mask), _addr(cu), N, pairs, params, loss.data_ptr(),
+                                             rewards.data_ptr(), coef.data_ptr(), ws.data_ptr(), ws_bytes,
+                                             torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_preference_loss_forward")
+    return loss, rewards, coef
+
+
+def preference_backward(coef, grad_loss, reduction, mask, cu, N, pairs, shape, dtype):
+    """``cce_preference_loss_backward``: the gradient with respect to logp."""
+    dev = coef.device
+    with on_device(dev):
+        grad = torch.empty(shape, dtype=dtype, device=dev)
+        rc = lib.cce_preference_loss_backward(coef.data_ptr(), grad_loss.data_ptr(), reduction, _addr(mask), _addr(cu),
+                                              N, pairs, _DTYPE_CODE[dtype], grad.data_ptr(),
+                                              torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_preference_loss_backward")
+    return grad
 
 
 # ---------------------------------------------------------------------------
