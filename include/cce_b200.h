@@ -417,6 +417,71 @@ CCE_API int cce_preference_loss_backward(const float* coef, const float* grad_lo
                                          const uint8_t* mask, const int32_t* cu_seqlens, int64_t N, int64_t pairs,
                                          int dtype, void* grad, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The head's log-probabilities and the distillation loss.  No counterpart in
+ * the reference.  Rows that do not count (targets equal to ignore_index, mask
+ * bytes of 0) are taken out before the GEMMs; the logits are accumulated in
+ * two levels to float32 accuracy, and the gradients are exact (no filter).
+ *
+ * A forward call fills `saved` (cce_*_saved_bytes), which the backward call of
+ * the same sizes reads; c and bias must not have changed in between.
+ * --------------------------------------------------------------------------- */
+
+CCE_API size_t cce_logp_saved_bytes(int64_t N, int64_t D, int64_t V, int dtype);
+CCE_API size_t cce_logp_forward_workspace_bytes(int64_t N, int64_t V);
+CCE_API size_t cce_logp_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags);
+
+/*
+ * cce_logp_forward -- log softmax(e c^T + bias) at the targets.
+ *
+ *   targets  [N] of target_bytes (4: int32, 8: int64), unsanitised ids in
+ *            [0, V); rows whose target is ignore_index (has_ignore != 0) are left out
+ *   logp     [N] fp32 out (0 for rows left out);  mask uint8 [N] out (1: counts)
+ */
+CCE_API int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dtype, const void* targets,
+                             int target_bytes, int64_t ignore_index, int has_ignore, int64_t N, int64_t D, int64_t V,
+                             int dtype, float* logp, uint8_t* mask, void* saved, size_t saved_bytes, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* Gradients for the cotangents grad_logp [N] fp32; flags CCE_NEED_DE / _DC / _DBIAS. */
+CCE_API int cce_logp_backward(const void* c, const void* bias, int bias_dtype, const float* grad_logp, int64_t N,
+                              int64_t D, int64_t V, int dtype, int flags, const void* saved, size_t saved_bytes,
+                              void* grad_e, void* grad_c, float* grad_bias, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+#define CCE_DISTILL_MAX_K 1024
+
+typedef struct CceDistillParams {
+  double temperature;  /* the student's logits are divided by it                        */
+  int32_t tail;        /* 0: teacher probabilities softmax(teacher_logp / temperature)
+                          over its K entries; else e^teacher_logp as given, and the
+                          mass they leave over against the student's outside of them   */
+  int32_t reduction;   /* CCE_REDUCE_MEAN (rows with an entry), _SUM or _NONE           */
+} CceDistillParams;
+
+CCE_API size_t cce_distill_saved_bytes(int64_t N, int64_t D, int64_t V, int64_t K, int dtype);
+CCE_API size_t cce_distill_forward_workspace_bytes(int64_t N, int64_t V, int64_t K);
+CCE_API size_t cce_distill_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags);
+
+/*
+ * cce_distill_forward -- KL divergence from a teacher's K entries per row to
+ * the student softmax((e c^T + bias) / temperature).
+ *
+ *   teacher_ids  [N][K] of id_bytes (4 or 8), any order; ids outside of [0, V)
+ *                are absent entries, entries of the same id add their mass
+ *   teacher_logp [N][K] fp32;  mask uint8 [N] or NULL
+ *   loss     fp32 out: [1], [N] with CCE_REDUCE_NONE
+ */
+CCE_API int cce_distill_forward(const void* e, const void* c, const void* bias, int bias_dtype,
+                                const void* teacher_ids, int id_bytes, const float* teacher_logp, const uint8_t* mask,
+                                int64_t N, int64_t D, int64_t V, int64_t K, int dtype, const CceDistillParams* params,
+                                float* loss, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* grad_loss fp32 [1], or [N] with CCE_REDUCE_NONE; flags as cce_logp_backward. */
+CCE_API int cce_distill_backward(const void* c, const void* bias, int bias_dtype, const float* grad_loss, int64_t N,
+                                 int64_t D, int64_t V, int64_t K, int dtype, const CceDistillParams* params, int flags,
+                                 const void* saved, size_t saved_bytes, void* grad_e, void* grad_c, float* grad_bias,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

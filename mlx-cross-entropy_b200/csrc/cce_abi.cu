@@ -645,16 +645,27 @@ size_t cce_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, 
   return backward_ws_bytes(N, D, V, dtype, flags, false);
 }
 
+// Packed rows of a loss on log-probabilities (`e`, d_nll, lse and targets are
+// those of the packed rows; grad_e goes back to the batch's rows).
+struct RowsBwd {
+  cce::RowsView R;
+  cce::TopkView topk;    // distillation: the listed columns, d_nll the others' coefficient
+  const float* d;        // cotangent of each packed row (0: not computed)
+  float logit_scale;
+  float* bias_part;      // [ceil(N / 32)][chunk rows] when grad_bias is requested (tensor-core path)
+};
+
 // cce_backward, cce_backward_peer when `pg` is given (grad_e summed over the
 // group through the exchange buffers), and cce_backward_q when `qh` is given
 // (c is a quantised head: every vocabulary chunk is expanded into one of two
 // workspace buffers on a side stream while the previous chunk's GEMMs run).
+// With `rb` the gradients of a loss on log-probabilities, exact (no filter).
 static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, const void* bias, int bias_dtype,
                          const int32_t* targets, const float* lse, const float* d_nll,
                          const float* tile_max, int64_t N, int64_t D, int64_t V, int64_t v_offset,
                          int dtype, int flags, float filter_log_eps, void* grad_e, void* grad_c,
                          float* grad_bias, int64_t* skip_stats, void* workspace, size_t workspace_bytes,
-                         const CcePeerGroup* pg, void* stream) {
+                         const CcePeerGroup* pg, const RowsBwd* rb, void* stream) {
   int rc = check_sizes(N, D, V, dtype);
   if (rc) return rc;
   if (bias && !dtype_ok(bias_dtype)) return fail(CCE_ERR_DTYPE, "unsupported bias dtype code %d", bias_dtype);
@@ -682,7 +693,7 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
     if (need_db) CCE_CUDA_CHECK(cudaMemsetAsync(grad_bias, 0, (size_t)V * sizeof(float), s), "memset grad_bias");
     return CCE_OK;
   }
-  if (!e || (!c && !qh) || !targets || !lse || !d_nll || !tile_max)
+  if (!e || (!c && !qh) || !lse || !d_nll || (!rb && (!targets || !tile_max)))
     return fail(CCE_ERR_ARG, "cce_backward: NULL required pointer");
   // (a quantised head's chunks live in the workspace: its alignment stands for c's)
   const bool tc = !force_simt() && cce::tc_backward_supported(e, qh ? workspace : c, D, dtype) &&
@@ -733,17 +744,28 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
   }
   if (p.tc) CCE_CUDA_CHECK(cudaMemsetAsync(counters, 0, p.counter_bytes, s), "cce_backward memset counters");
   if (keep_t) CCE_CUDA_CHECK(cudaMemsetAsync(keep_t, 0, p.keep_t_bytes, s), "cce_backward memset mask table");
-  if (scale) CCE_CUDA_CHECK(cce::launch_pow2_absmax(d_nll, N, scale, s), "cce_backward scale");
+  // (a distillation's dlogits are at most the cotangent in magnitude, so its power of two fits them)
+  if (scale) CCE_CUDA_CHECK(cce::launch_pow2_absmax(rb ? rb->d : d_nll, N, scale, s), "cce_backward scale");
 
-  CCE_CUDA_CHECK(cce::launch_block_mask(tile_max, lse, targets, d_nll, N, V, v_offset, filter_log_eps,
-                                        (flags & CCE_NO_FILTER) != 0, keep, keep_t, p.keep_t_ld, skip_stats, s),
-                 "cce_backward mask");
+  if (rb)
+    CCE_CUDA_CHECK(cce::launch_live_mask(rb->d, N, V, keep, keep_t, p.keep_t_ld, s), "cce_backward mask");
+  else
+    CCE_CUDA_CHECK(cce::launch_block_mask(tile_max, lse, targets, d_nll, N, V, v_offset, filter_log_eps,
+                                          (flags & CCE_NO_FILTER) != 0, keep, keep_t, p.keep_t_ld, skip_stats, s),
+                   "cce_backward mask");
   if (need_db) CCE_CUDA_CHECK(cudaMemsetAsync(grad_bias, 0, (size_t)V * sizeof(float), s), "memset grad_bias");
   if (dl_lists)
     CCE_CUDA_CHECK(cce::tc_dlogits_lists(keep, N, D, V, p.vc, dl_lists, counters, s), "cce_backward dlogits lists");
 
   cce::BwdChunkArgs a{e, c, nullptr, bias, bias_dtype, targets, lse, d_nll, keep, keep_t, p.keep_t_ld, N, D, V,
-                      v_offset, dtype, 0, 0, p.vc, dl, need_db ? grad_bias : nullptr, nullptr, scale};
+                      v_offset, dtype, 0, 0, p.vc, dl, need_db && !rb ? grad_bias : nullptr, nullptr, scale};
+  if (rb) {
+    a.topk = rb->topk;
+    a.d_row = rb->d;
+    a.logit_scale = rb->logit_scale;
+    if (need_db && p.tc) a.bias_part = rb->bias_part;
+  }
+  const int64_t bias_parts = p.tc ? cce::ceil_div(N, 32) : N;  // (CUDA cores: the fp32 dlogits themselves)
   const int64_t nchunks = cce::ceil_div(V, p.vc);
   const size_t esz = dtype_size(dtype);
   SideStreams* ss = nullptr;
@@ -791,7 +813,12 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
       a.c_chunk = static_cast<const char*>(c) + (size_t)a.vc0 * (size_t)D * esz;
     }
     if (p.tc) {
+      if (a.bias_part)
+        CCE_CUDA_CHECK(cudaMemsetAsync(a.bias_part, 0, (size_t)bias_parts * p.vc * sizeof(float), s), "cce_backward memset");
       CCE_CUDA_CHECK(cce::tc_dlogits(a, s), "cce_backward tc dlogits");
+      if (a.bias_part)
+        CCE_CUDA_CHECK(cce::launch_bias_sum(a.bias_part, bias_parts, p.vc, a.vc_len, scale, grad_bias + a.vc0, s),
+                       "cce_backward grad_bias");
       CCE_CUDA_CHECK(cudaEventRecord(ss->ev_l, s), "cce_backward record");
       CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->se, ss->ev_l, 0), "cce_backward wait");
       CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->sc, ss->ev_l, 0), "cce_backward wait");
@@ -802,6 +829,9 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
           CCE_CUDA_CHECK(cce::peer::launch_reduce_gather(push.peers, push.layout, cce::peer::kSlotsPerSrc, N, D,
                                                          out_dtype, grad_e, wait_ns, ss->se),
                          "cce_backward_peer exchange");
+        else if (last && rb)
+          CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, acc + N * D, rb->R.pos, N, D, out_dtype, grad_e, ss->se),
+                         "cce_backward scatter grad_e");
         else if (last)
           CCE_CUDA_CHECK(cce::launch_sum2_f32(acc, acc + N * D, grad_e, out_dtype, N * D, ss->se),
                          "cce_backward sum grad_e");
@@ -815,12 +845,18 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
       }
     } else {
       CCE_CUDA_CHECK(cce::simt_dlogits(a, s), "cce_backward simt dlogits");
+      if (rb && need_db)
+        CCE_CUDA_CHECK(cce::launch_bias_sum((const float*)dl, bias_parts, p.vc, a.vc_len, nullptr, grad_bias + a.vc0, s),
+                       "cce_backward grad_bias");
       if (need_de) CCE_CUDA_CHECK(cce::simt_grad_e(a, acc, ch > 0, part, p.splits, s), "cce_backward simt grad_e");
       if (need_dc) CCE_CUDA_CHECK(cce::simt_grad_c(a, grad_c, s), "cce_backward simt grad_c");
       if (need_de && last && exchange) {
         CCE_CUDA_CHECK(cce::peer::launch_push(push.peers, push.layout, acc, 1, N, D, s), "cce_backward_peer push");
         CCE_CUDA_CHECK(cce::peer::launch_reduce_gather(push.peers, push.layout, 1, N, D, out_dtype, grad_e, wait_ns, s),
                        "cce_backward_peer exchange");
+      } else if (need_de && last && rb) {
+        CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, nullptr, rb->R.pos, N, D, out_dtype, grad_e, s),
+                       "cce_backward scatter grad_e");
       } else if (need_de && last && !(flags & CCE_DE_F32)) {
         CCE_CUDA_CHECK(cce::launch_cast_f32(acc, grad_e, dtype, N * D, s), "cce_backward cast grad_e");
       }
@@ -837,7 +873,7 @@ int cce_backward(const void* e, const void* c, const void* bias, int bias_dtype,
                  void* stream) {
   return backward_impl(e, c, nullptr, bias, bias_dtype, targets, lse, d_nll, tile_max, N, D, V, v_offset, dtype,
                        flags, filter_log_eps, grad_e, grad_c, grad_bias, skip_stats, workspace, workspace_bytes,
-                       nullptr, stream);
+                       nullptr, nullptr, stream);
 }
 
 int cce_backward_peer(const void* e, const void* c, const void* bias, int bias_dtype,
@@ -855,7 +891,7 @@ int cce_backward_peer(const void* e, const void* c, const void* bias, int bias_d
       return fail(CCE_ERR_ARG, "cce_backward_peer: buffer of rank %d is NULL or not 16-byte aligned", r);
   return backward_impl(e, c, nullptr, bias, bias_dtype, targets, lse, d_nll, tile_max, N, D, V, v_offset, dtype,
                        flags, filter_log_eps, grad_e, grad_c, grad_bias, skip_stats, workspace, workspace_bytes, group,
-                       stream);
+                       nullptr, stream);
 }
 
 size_t cce_backward_q_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
@@ -869,7 +905,7 @@ int cce_backward_q(const void* e, const CceQuantHead* head, const void* bias, in
   if (!head) return fail(CCE_ERR_ARG, "cce_backward_q: NULL head");
   return backward_impl(e, nullptr, head, bias, bias_dtype, targets, lse, d_nll, tile_max, N, D, V, v_offset, dtype,
                        flags, filter_log_eps, grad_e, nullptr, grad_bias, skip_stats, workspace, workspace_bytes,
-                       nullptr, stream);
+                       nullptr, nullptr, stream);
 }
 
 size_t cce_peer_buffer_bytes(int64_t N, int64_t D, int world, int out_dtype) {
@@ -1104,6 +1140,296 @@ int cce_preference_loss_backward(const float* coef, const float* grad_loss, int 
                                           dtype, grad, s),
                  what);
   return CCE_OK;
+}
+
+}  // extern "C"
+
+// ---- the head's log-probabilities and the distillation loss ----
+
+namespace {
+
+// Consecutive 256-byte aligned parts of a buffer (base nullptr: sizes only).
+struct Parts {
+  char* base;
+  size_t used = 0;
+  template <typename X>
+  X* take(size_t n) {
+    X* p = base ? reinterpret_cast<X*>(base + used) : nullptr;
+    used += align_up(n * sizeof(X));
+    return p;
+  }
+};
+
+// What the forward calls leave for the backward calls.
+struct RowsSaved {
+  cce::RowsView R;
+  float* lse;       // distillation: over the columns outside of the list
+  float* A;         // distillation
+  float* weight;    // distillation [1]
+  cce::TopkView topk;
+  void* e;          // packed rows
+  size_t bytes;
+};
+
+RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
+  Parts p{static_cast<char*>(base)};
+  RowsSaved r{};
+  r.R.count = p.take<int32_t>(1);
+  r.R.row_of = p.take<int32_t>(N);
+  r.R.pos = p.take<int32_t>(N);
+  if (K == 0) r.R.targets = p.take<int32_t>(N);
+  r.lse = p.take<float>(N);
+  if (K > 0) {
+    r.A = p.take<float>(N);
+    r.weight = p.take<float>(1);
+    r.topk.K = (int)K;
+    r.topk.tiles1 = (int)cce::ceil_div(V, cce::kTopkTile) + 1;
+    r.topk.sid = p.take<int32_t>((size_t)N * K);
+    r.topk.start = p.take<uint16_t>((size_t)N * r.topk.tiles1);
+    r.topk.z = p.take<float>((size_t)N * K);
+  }
+  r.e = p.take<char>((size_t)N * D * dtype_size(dtype));
+  r.bytes = p.used;
+  return r;
+}
+
+struct RowsFwdWs {
+  float *part_m, *part_s, *tgt, *p, *rest;
+  cce::DistillSum* sums;
+  size_t bytes;
+};
+
+RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t V, int64_t K) {
+  Parts p{static_cast<char*>(base)};
+  RowsFwdWs w{};
+  const size_t parts = (size_t)cce::ceil_div(V, cce::kSimtLseTile) * N;
+  w.part_m = p.take<float>(parts);
+  w.part_s = p.take<float>(parts);
+  if (K == 0) {
+    w.tgt = p.take<float>(N);
+  } else {
+    w.p = p.take<float>((size_t)N * K);
+    w.rest = p.take<float>(N);
+    w.sums = p.take<cce::DistillSum>(cce::distill_blocks(N));
+  }
+  w.bytes = p.used;
+  return w;
+}
+
+struct RowsBwdWs {
+  void* base;  // backward_impl's own
+  size_t base_bytes;
+  float *d, *dA, *bias_part;
+  size_t bytes;
+};
+
+RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, int flags, bool topk) {
+  Parts p{static_cast<char*>(base)};
+  RowsBwdWs w{};
+  w.base_bytes = backward_ws_bytes(N, D, V, dtype, flags, false);
+  w.base = p.take<char>(w.base_bytes);
+  w.d = p.take<float>(N);
+  if (topk) w.dA = p.take<float>(N);
+  if ((flags & CCE_NEED_DBIAS) && tc_candidate(dtype, D))
+    w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * plan_backward(N, D, V, dtype, flags, true).vc);
+  w.bytes = p.used;
+  return w;
+}
+
+int check_rows(int64_t N, int64_t D, int64_t V, int64_t K, int dtype, const char* what) {
+  int rc = check_sizes(N, D, V, dtype);
+  if (rc) return rc;
+  if (N > INT32_MAX || V > (1ll << 30))
+    return fail(CCE_ERR_SHAPE, "%s: sizes out of supported range N=%lld V=%lld", what, (long long)N, (long long)V);
+  if (V == 0) return fail(CCE_ERR_SHAPE, "%s: V must be positive", what);
+  if (K < 0 || K > CCE_DISTILL_MAX_K)
+    return fail(CCE_ERR_SHAPE, "%s: K=%lld is outside of [1, %d]", what, (long long)K, CCE_DISTILL_MAX_K);
+  return CCE_OK;
+}
+
+int check_distill(const CceDistillParams* p, const char* what) {
+  if (!p) return fail(CCE_ERR_ARG, "%s: NULL params", what);
+  if (!(p->temperature > 0.0) || p->temperature > 1e30)
+    return fail(CCE_ERR_ARG, "%s: temperature must be positive, got %g", what, p->temperature);
+  if (p->reduction != CCE_REDUCE_MEAN && p->reduction != CCE_REDUCE_SUM && p->reduction != CCE_REDUCE_NONE)
+    return fail(CCE_ERR_ARG, "%s: reduction code %d", what, p->reduction);
+  return CCE_OK;
+}
+
+cudaError_t rows_logits(const cce::FwdArgs& f, cudaStream_t s) {
+  // (the packed copy of e is aligned whatever e was)
+  return !force_simt() && cce::tc_supported(f.e, f.c, f.D, f.dtype) ? cce::tc_logits(f, s) : cce::simt_logits(f, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t cce_logp_saved_bytes(int64_t N, int64_t D, int64_t V, int dtype) {
+  return N < 0 || D < 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_saved(nullptr, N, D, V, 0, dtype).bytes;
+}
+
+size_t cce_logp_forward_workspace_bytes(int64_t N, int64_t V) {
+  return N < 0 || V <= 0 ? 0 : rows_fwd_ws(nullptr, N, V, 0).bytes;
+}
+
+size_t cce_logp_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
+  return N < 0 || D <= 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_bwd_ws(nullptr, N, D, V, dtype, flags, false).bytes;
+}
+
+int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dtype, const void* targets,
+                     int target_bytes, int64_t ignore_index, int has_ignore, int64_t N, int64_t D, int64_t V, int dtype,
+                     float* logp, uint8_t* mask, void* saved, size_t saved_bytes, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  const char* what = "cce_logp_forward";
+  int rc = check_rows(N, D, V, 0, dtype, what);
+  if (rc) return rc;
+  if (bias && !dtype_ok(bias_dtype)) return fail(CCE_ERR_DTYPE, "%s: unsupported bias dtype code %d", what, bias_dtype);
+  if (target_bytes != 4 && target_bytes != 8)
+    return fail(CCE_ERR_ARG, "%s: targets of %d bytes (4 or 8 expected)", what, target_bytes);
+  if (N == 0) return CCE_OK;
+  if (!e || !c || !targets || !logp || !mask) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  const RowsSaved v = rows_saved(saved, N, D, V, 0, dtype);
+  const RowsFwdWs w = rows_fwd_ws(workspace, N, V, 0);
+  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
+    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
+                v.bytes, workspace_bytes, w.bytes);
+  rc = check_arch();
+  if (rc) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  CCE_CUDA_CHECK(cce::launch_rows_pack(e, dtype, N, D, targets, target_bytes, ignore_index, has_ignore, nullptr, v.R,
+                                       mask, logp, v.e, w.tgt, s),
+                 what);
+  cce::FwdArgs f{v.e, c, bias, bias_dtype, v.R.targets, N, D, V, 0, dtype, nullptr, w.part_m, w.part_s, w.tgt};
+  f.rows = v.R.count;
+  CCE_CUDA_CHECK(rows_logits(f, s), what);
+  CCE_CUDA_CHECK(cce::launch_rows_logp(w.part_m, w.part_s, cce::ceil_div(V, cce::kSimtLseTile), N, v.R, w.tgt, v.lse,
+                                       logp, s),
+                 what);
+  return CCE_OK;
+}
+
+int cce_logp_backward(const void* c, const void* bias, int bias_dtype, const float* grad_logp, int64_t N, int64_t D,
+                      int64_t V, int dtype, int flags, const void* saved, size_t saved_bytes, void* grad_e,
+                      void* grad_c, float* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cce_logp_backward";
+  int rc = check_rows(N, D, V, 0, dtype, what);
+  if (rc) return rc;
+  if (flags & ~(CCE_NEED_DE | CCE_NEED_DC | CCE_NEED_DBIAS))
+    return fail(CCE_ERR_ARG, "%s: unknown flag bits 0x%x", what, flags);
+  if (N == 0)
+    return backward_impl(nullptr, c, nullptr, bias, bias_dtype, nullptr, nullptr, nullptr, nullptr, N, D, V, 0, dtype,
+                         flags, 0.f, grad_e, grad_c, grad_bias, nullptr, workspace, workspace_bytes, nullptr, nullptr,
+                         stream);
+  if (!grad_logp || !c) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  const RowsSaved v = rows_saved(const_cast<void*>(saved), N, D, V, 0, dtype);
+  const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags, false);
+  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
+    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
+                v.bytes, workspace_bytes, w.bytes);
+  rc = check_arch();
+  if (rc) return rc;
+  // d logp / dz = onehot - softmax: the negative of the cross-entropy's
+  CCE_CUDA_CHECK(cce::launch_rows_cotangent(grad_logp, 1, nullptr, -1.f, v.R, N, nullptr, w.d, nullptr,
+                                            (cudaStream_t)stream),
+                 what);
+  const RowsBwd rb{v.R, cce::TopkView{}, w.d, 1.f, w.bias_part};
+  return backward_impl(v.e, c, nullptr, bias, bias_dtype, v.R.targets, v.lse, w.d, nullptr, N, D, V, 0, dtype, flags,
+                       0.f, grad_e, grad_c, grad_bias, nullptr, w.base, w.base_bytes, nullptr, &rb, stream);
+}
+
+size_t cce_distill_saved_bytes(int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
+  if (N < 0 || D < 0 || V <= 0 || K < 1 || K > CCE_DISTILL_MAX_K || !dtype_ok(dtype)) return 0;
+  return rows_saved(nullptr, N, D, V, K, dtype).bytes;
+}
+
+size_t cce_distill_forward_workspace_bytes(int64_t N, int64_t V, int64_t K) {
+  return N < 0 || V <= 0 || K < 1 || K > CCE_DISTILL_MAX_K ? 0 : rows_fwd_ws(nullptr, N, V, K).bytes;
+}
+
+size_t cce_distill_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
+  return N < 0 || D <= 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_bwd_ws(nullptr, N, D, V, dtype, flags, true).bytes;
+}
+
+int cce_distill_forward(const void* e, const void* c, const void* bias, int bias_dtype, const void* teacher_ids,
+                        int id_bytes, const float* teacher_logp, const uint8_t* mask, int64_t N, int64_t D, int64_t V,
+                        int64_t K, int dtype, const CceDistillParams* params, float* loss, void* saved,
+                        size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cce_distill_forward";
+  int rc = check_rows(N, D, V, K, dtype, what);
+  if (rc) return rc;
+  if (K < 1) return fail(CCE_ERR_SHAPE, "%s: K=%lld is outside of [1, %d]", what, (long long)K, CCE_DISTILL_MAX_K);
+  if (bias && !dtype_ok(bias_dtype)) return fail(CCE_ERR_DTYPE, "%s: unsupported bias dtype code %d", what, bias_dtype);
+  rc = check_distill(params, what);
+  if (rc) return rc;
+  if (id_bytes != 4 && id_bytes != 8)
+    return fail(CCE_ERR_ARG, "%s: teacher ids of %d bytes (4 or 8 expected)", what, id_bytes);
+  const int red = params->reduction;
+  if (!loss && !(red == CCE_REDUCE_NONE && N == 0)) return fail(CCE_ERR_ARG, "%s: NULL loss", what);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (N == 0) {
+    rc = check_arch();
+    if (rc) return rc;
+    if (red != CCE_REDUCE_NONE) CCE_CUDA_CHECK(cudaMemsetAsync(loss, 0, sizeof(float), s), what);
+    return CCE_OK;
+  }
+  if (!e || !c || !teacher_ids || !teacher_logp) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  const RowsSaved v = rows_saved(saved, N, D, V, K, dtype);
+  const RowsFwdWs w = rows_fwd_ws(workspace, N, V, K);
+  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
+    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
+                v.bytes, workspace_bytes, w.bytes);
+  rc = check_arch();
+  if (rc) return rc;
+  CCE_CUDA_CHECK(cce::launch_rows_pack(e, dtype, N, D, nullptr, 0, 0, 0, mask, v.R, nullptr,
+                                       red == CCE_REDUCE_NONE ? loss : nullptr, v.e, nullptr, s),
+                 what);
+  CCE_CUDA_CHECK(cce::launch_topk_prep(teacher_ids, id_bytes, teacher_logp, N, V, (int)K, params->temperature,
+                                       params->tail, v.R, v.topk, w.p, w.rest, s),
+                 what);
+  cce::FwdArgs f{v.e, c, bias, bias_dtype, nullptr, N, D, V, 0, dtype, nullptr, w.part_m, w.part_s, nullptr};
+  f.rows = v.R.count;
+  f.scale = (float)(1.0 / params->temperature);
+  f.topk = v.topk;
+  CCE_CUDA_CHECK(rows_logits(f, s), what);
+  CCE_CUDA_CHECK(cce::launch_distill_rows(w.part_m, w.part_s, cce::ceil_div(V, cce::kSimtLseTile), N, V, v.R, v.topk,
+                                          w.p, w.rest, red, v.lse, v.A, w.sums, loss, v.weight, s),
+                 what);
+  return CCE_OK;
+}
+
+int cce_distill_backward(const void* c, const void* bias, int bias_dtype, const float* grad_loss, int64_t N, int64_t D,
+                         int64_t V, int64_t K, int dtype, const CceDistillParams* params, int flags, const void* saved,
+                         size_t saved_bytes, void* grad_e, void* grad_c, float* grad_bias, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  const char* what = "cce_distill_backward";
+  int rc = check_rows(N, D, V, K, dtype, what);
+  if (rc) return rc;
+  if (K < 1) return fail(CCE_ERR_SHAPE, "%s: K=%lld is outside of [1, %d]", what, (long long)K, CCE_DISTILL_MAX_K);
+  rc = check_distill(params, what);
+  if (rc) return rc;
+  if (flags & ~(CCE_NEED_DE | CCE_NEED_DC | CCE_NEED_DBIAS))
+    return fail(CCE_ERR_ARG, "%s: unknown flag bits 0x%x", what, flags);
+  if (N == 0)
+    return backward_impl(nullptr, c, nullptr, bias, bias_dtype, nullptr, nullptr, nullptr, nullptr, N, D, V, 0, dtype,
+                         flags, 0.f, grad_e, grad_c, grad_bias, nullptr, workspace, workspace_bytes, nullptr, nullptr,
+                         stream);
+  if (!grad_loss || !c) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
+  const RowsSaved v = rows_saved(const_cast<void*>(saved), N, D, V, K, dtype);
+  const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags, true);
+  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
+    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
+                v.bytes, workspace_bytes, w.bytes);
+  rc = check_arch();
+  if (rc) return rc;
+  // dlogits are by the logits before the temperature: one factor 1 / T in the cotangent
+  CCE_CUDA_CHECK(cce::launch_rows_cotangent(grad_loss, params->reduction == CCE_REDUCE_NONE, v.weight,
+                                            (float)(1.0 / params->temperature), v.R, N, v.A, w.d, w.dA,
+                                            (cudaStream_t)stream),
+                 what);
+  const RowsBwd rb{v.R, v.topk, w.d, (float)(1.0 / params->temperature), w.bias_part};
+  return backward_impl(v.e, c, nullptr, bias, bias_dtype, nullptr, v.lse, w.dA, nullptr, N, D, V, 0, dtype, flags, 0.f,
+                       grad_e, grad_c, grad_bias, nullptr, w.base, w.base_bytes, nullptr, &rb, stream);
 }
 
 }  // extern "C"

@@ -21,6 +21,27 @@ int report_error(int code, const char* msg);
 // context or resets a device.
 bool current_context_id(unsigned long long* id);
 
+// Rows that count, moved to the front in order (rows_kernels.cu): their number,
+// the batch row of each packed row, the packed row of each batch row (-1: left
+// out), the packed rows' targets (nullptr: none).
+struct RowsView {
+  int32_t* count;
+  int32_t* row_of;
+  int32_t* pos;
+  int32_t* targets;
+};
+
+// Per packed row up to K listed columns: sid[row][K] sorted and distinct,
+// start[row][tiles1] the first entry of every kTopkTile-column tile (the last:
+// the number of entries), z[row][K] a value per entry.
+constexpr int kTopkTile = 256;
+struct TopkView {
+  const int32_t* sid = nullptr;
+  const uint16_t* start = nullptr;
+  float* z = nullptr;
+  int K = 0, tiles1 = 0;
+};
+
 struct FwdArgs {
   const void* e;
   const void* c;
@@ -33,6 +54,10 @@ struct FwdArgs {
   float* part_m;    // [P][N] (workspace): row max over each kernel tile, P = ceil(V / lse_tile)
   float* part_s;    // [P][N] (workspace): row sum of exp(logit - part_m) over the same columns
   float* tgt;       // [N]
+  // row statistics for losses on log-probabilities (tc_logits, simt_logits): tile_max unused
+  const int32_t* rows = nullptr;  // rows that count (device)
+  float scale = 1.f;              // logits = scale (e c^T + bias)
+  TopkView topk{};                // columns left out of the sum, whose logits go to topk.z
 };
 
 struct BwdChunkArgs {
@@ -59,6 +84,12 @@ struct BwdChunkArgs {
   int* counters;         // 4 zeroed counters of this chunk (dlogits, grad_e, grad_c tile claims; the
                          // dlogits live-tile count) or nullptr
   const float* scale;    // fp16 tensor-core path: {s, 1/s} with s = 2^ceil(log2 max|d_nll|); else nullptr
+  // distillation: d_nll is the coefficient of the columns outside of the row's
+  // list (lse over those), a listed column's dlogit is topk.z * d_row
+  TopkView topk{};
+  const float* d_row = nullptr;
+  float logit_scale = 1.f;
+  float* bias_part = nullptr;    // [ceil(N / 32)][vc_ld] column sums of dlogits (zeroed); instead of grad_bias
   const int* dl_list = nullptr;  // the chunk's live dlogits tiles (tc_dlogits_lists), count in counters[3]
 };
 
@@ -83,7 +114,38 @@ cudaError_t launch_sum2_f32(const float* a, const float* b, void* dst, int dtype
 cudaError_t launch_pow2_absmax(const float* x, int64_t n, float* out, cudaStream_t stream);
 cudaError_t launch_fill_f32(float* dst, float v, int64_t n, cudaStream_t stream);
 
+// ---- rows of a batch, distillation (rows_kernels.cu) ----
+struct DistillSum {
+  double loss;
+  int32_t n;
+};
+cudaError_t launch_rows_pack(const void* e, int dtype, int64_t N, int64_t D, const void* targets, int target_bytes,
+                             int64_t ignore_index, int has_ignore, const uint8_t* mask, const RowsView& R,
+                             uint8_t* mask_out, float* per_row_out, void* e_packed, float* tgt, cudaStream_t stream);
+// lse (packed rows) and logp (batch rows) from P partials
+cudaError_t launch_rows_logp(const float* part_m, const float* part_s, int64_t P, int64_t N, const RowsView& R,
+                             const float* tgt, float* lse, float* logp, cudaStream_t stream);
+cudaError_t launch_topk_prep(const void* ids, int id_bytes, const float* logp, int64_t N, int64_t V, int K, double T,
+                             int tail, const RowsView& R, const TopkView& topk, float* p, float* rest,
+                             cudaStream_t stream);
+int64_t distill_blocks(int64_t N);  // entries of `sums`
+cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_t P, int64_t N, int64_t V,
+                                const RowsView& R, const TopkView& topk, const float* p, const float* rest,
+                                int reduction, float* lse_rest, float* A, DistillSum* sums, float* loss, float* weight,
+                                cudaStream_t stream);
+cudaError_t launch_rows_cotangent(const float* up, int up_row, const float* weight, float factor, const RowsView& R,
+                                  int64_t N, const float* A, float* d, float* dA, cudaStream_t stream);
+cudaError_t launch_live_mask(const float* d, int64_t N, int64_t V, uint8_t* keep, uint32_t* keep_t, int64_t keep_t_ld,
+                             cudaStream_t stream);
+// out[n] = a[pos[n]] (+ b[pos[n]] unless nullptr), 0 where pos[n] < 0
+cudaError_t launch_rows_scatter(const float* a, const float* b, const int32_t* pos, int64_t N, int64_t D, int dtype,
+                                void* out, cudaStream_t stream);
+cudaError_t launch_bias_sum(const float* part, int64_t parts, int64_t ld, int64_t cols, const float* scale, float* out,
+                            cudaStream_t stream);
+
 // ---- SIMT kernels (simt_kernels.cu): any dtype, any shape ----
+// row statistics of the rows that count (see FwdArgs)
+cudaError_t simt_logits(const FwdArgs& a, cudaStream_t stream);
 cudaError_t simt_forward(const FwdArgs& a, cudaStream_t stream);
 // vocabulary columns per LSE partial of simt_forward / tc_forward
 constexpr int64_t kSimtLseTile = 128;
@@ -109,6 +171,8 @@ int tc_read_status(bool reset);
 // the last reset; 0 = ok, -1 = read failed.
 int tc_read_mma_flops(uint64_t* out4, bool reset);
 cudaError_t tc_forward(const FwdArgs& a, cudaStream_t stream);
+// row statistics of the rows that count, two-level accumulation (see FwdArgs)
+cudaError_t tc_logits(const FwdArgs& a, cudaStream_t stream);
 cudaError_t tc_dlogits(const BwdChunkArgs& a, cudaStream_t stream);
 // Lists, per vocabulary chunk of vc rows, the dlogits work units with a kept
 // block in schedule order: chunk ch's ids at lists + ch * tc_dlogits_list_len(N, vc),

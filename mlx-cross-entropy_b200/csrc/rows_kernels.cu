@@ -1,0 +1,625 @@
+// Kernels around the head's GEMMs for losses on log-probabilities: packing the
+// rows that count, joining the row statistics, the teacher's entries and the
+// per-row part of the distillation loss, and bringing gradients back to the
+// batch's order.
+//
+// Rows that a mask or ignore_index leaves out (prompts, padding: a third of the
+// rows of a preference batch) are taken out before the GEMMs: the rows that
+// count move to the front of a copy of e, in order, and every GEMM runs on
+// those alone.  The copy moves 4 N D bytes (10 us at N = D = 4096) where the
+// GEMMs cost 3 us per row saved there.
+//
+// Distillation of a row with logits z (already divided by the temperature) and
+// teacher entries S with probabilities p_v (P their sum, r what they leave over):
+//     L = sum_S p_v (log p_v - log q_v) + r (log r - log q_r),  q_r = 1 - sum_S q_v
+//     dL/dz_v = (P + r) q_v - p_v                  for v in S
+//             = e^(z_v - lse_r) ((P + r) q_r - r)  for the others
+// lse_r, the log-sum-exp over the columns outside of S, is summed directly
+// (never as 1 - sum), so a tail of 1e-6 keeps its digits; the others'
+// gradient has one coefficient per row, and S is a list of K values per row.
+#include <type_traits>
+
+#include "kernels.cuh"
+
+namespace cce {
+namespace {
+
+// ---------------------------------------------------------------------------
+// packing
+// ---------------------------------------------------------------------------
+
+constexpr int kPackThreads = 1024;
+constexpr int kPackPer = 8;
+
+// One block walks the rows in order: a scan of the counting rows gives each its
+// place, so the packed order is the batch's and does not depend on scheduling.
+template <typename TT>  // target type; void: rows count by `mask` alone
+__global__ void __launch_bounds__(kPackThreads)
+rows_pack_kernel(const TT* __restrict__ targets, int64_t ignore_index, int has_ignore,
+                 const uint8_t* __restrict__ mask, int64_t N, const RowsView R, uint8_t* __restrict__ mask_out,
+                 float* __restrict__ per_row_out) {
+  __shared__ int warp_tot[32];
+  __shared__ int base_sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) base_sh = 0;
+  __syncthreads();
+  for (int64_t r0 = 0; r0 < N; r0 += kPackThreads * kPackPer) {
+    const int64_t n0 = r0 + (int64_t)threadIdx.x * kPackPer;
+    int32_t t[kPackPer];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < kPackPer; ++j) {
+      t[j] = 0;
+      if (n0 + j < N) {
+        bool ok = mask == nullptr || mask[n0 + j] != 0;
+        if constexpr (!std::is_void<TT>::value) {
+          const int64_t x = (int64_t)targets[n0 + j];
+          ok = ok && !(has_ignore && x == ignore_index);
+          t[j] = (int32_t)(x < INT32_MIN ? INT32_MIN : x > INT32_MAX ? INT32_MAX : x);
+        }
+        if (ok) bits |= 1u << j;
+      }
+    }
+    const int cnt = __popc(bits);
+    int incl = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) warp_tot[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+      int w = warp_tot[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+      }
+      warp_tot[lane] = w;
+    }
+    __syncthreads();
+    int at = base_sh + incl - cnt + (warp > 0 ? warp_tot[warp - 1] : 0);
+#pragma unroll
+    for (int j = 0; j < kPackPer; ++j) {
+      if (n0 + j < N) {
+        const bool ok = (bits >> j) & 1u;
+        R.pos[n0 + j] = ok ? at : -1;
+        if (mask_out) mask_out[n0 + j] = ok ? 1 : 0;
+        if (ok) {
+          R.row_of[at] = (int32_t)(n0 + j);
+          if constexpr (!std::is_void<TT>::value) R.targets[at] = t[j];
+          ++at;
+        } else if (per_row_out) {
+          per_row_out[n0 + j] = 0.f;
+        }
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) base_sh += warp_tot[31];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *R.count = base_sh;
+}
+
+// A warp per packed row: row i of the copy is row row_of[i] of e, zeros behind
+// the count (the grad_c GEMM multiplies those rows by zeros, so they must be
+// numbers).
+template <bool kVec>
+__global__ void __launch_bounds__(256)
+rows_gather_kernel(const uint8_t* __restrict__ e, int64_t N, int64_t row_bytes, const RowsView R, int has_targets,
+                   uint8_t* __restrict__ out, float* __restrict__ tgt) {
+  const int lane = threadIdx.x & 31;
+  const int64_t count = *R.count;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < N; i += (int64_t)gridDim.x * 8) {
+    const bool live = i < count;
+    const uint8_t* src = live ? e + (int64_t)R.row_of[i] * row_bytes : nullptr;
+    uint8_t* dst = out + i * row_bytes;
+    if constexpr (kVec) {
+      for (int64_t k = lane * 16; k < row_bytes; k += 32 * 16)
+        *reinterpret_cast<uint4*>(dst + k) =
+            live ? __ldg(reinterpret_cast<const uint4*>(src + k)) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int64_t k = lane * 2; k < row_bytes; k += 32 * 2)
+        *reinterpret_cast<uint16_t*>(dst + k) = live ? *reinterpret_cast<const uint16_t*>(src + k) : (uint16_t)0;
+    }
+    if (lane == 0) {
+      if (tgt) tgt[i] = 0.f;
+      if (has_targets && !live) R.targets[i] = 0;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// row statistics
+// ---------------------------------------------------------------------------
+
+constexpr int kStRows = 32;    // rows per block (a warp reads 128 contiguous bytes of the partials)
+constexpr int kStSlices = 32;
+
+__device__ __forceinline__ void fold(float& m, float& s, float mp, float sp) {
+  const float M = fmaxf(m, mp);
+  if (M == -INFINITY) return;
+  s = s * exp2f((m - M) * kLog2e) + sp * exp2f((mp - M) * kLog2e);
+  m = M;
+}
+
+// (max, sum) of the block's 32 rows over P partials, into sm[0][..], ss[0][..].
+__device__ __forceinline__ void fold_rows(const float* __restrict__ part_m, const float* __restrict__ part_s, int64_t P,
+                                          int64_t N, int64_t row, bool live, float (*sm)[kStRows],
+                                          float (*ss)[kStRows]) {
+  float m = -INFINITY, s = 0.f;
+  if (live) {
+    int64_t p = threadIdx.y;
+    for (; p + 3 * kStSlices < P; p += 4 * kStSlices) {  // four loads in flight
+      float mp[4], sp[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        mp[u] = part_m[(p + u * kStSlices) * N + row];
+        sp[u] = part_s[(p + u * kStSlices) * N + row];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) fold(m, s, mp[u], sp[u]);
+    }
+    for (; p < P; p += kStSlices) fold(m, s, part_m[p * N + row], part_s[p * N + row]);
+  }
+  sm[threadIdx.y][threadIdx.x] = m;
+  ss[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  for (int h = kStSlices / 2; h >= 1; h >>= 1) {
+    if (threadIdx.y < h) {
+      float M = sm[threadIdx.y][threadIdx.x], S = ss[threadIdx.y][threadIdx.x];
+      fold(M, S, sm[threadIdx.y + h][threadIdx.x], ss[threadIdx.y + h][threadIdx.x]);
+      sm[threadIdx.y][threadIdx.x] = M;
+      ss[threadIdx.y][threadIdx.x] = S;
+    }
+    __syncthreads();
+  }
+}
+
+// logp = (z_t - M) - log S: the target's logit against the row's maximum first,
+// so a log-probability near 0 is not the difference of two rounded large numbers.
+__global__ void __launch_bounds__(kStRows * kStSlices)
+rows_logp_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s, int64_t P, int64_t N,
+                 const RowsView R, const float* __restrict__ tgt, float* __restrict__ lse, float* __restrict__ logp) {
+  __shared__ float sm[kStSlices][kStRows], ss[kStSlices][kStRows];
+  const int64_t row = (int64_t)blockIdx.x * kStRows + threadIdx.x;
+  const bool live = row < *R.count;
+  fold_rows(part_m, part_s, P, N, row, live, sm, ss);
+  if (threadIdx.y == 0 && row < N) {
+    const float M = sm[0][threadIdx.x], L = logf(ss[0][threadIdx.x]);
+    // (rows behind the count: their softmax is 0)
+    lse[row] = live ? M + L : INFINITY;
+    if (live) logp[R.row_of[row]] = (tgt[row] - M) - L;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// distillation
+// ---------------------------------------------------------------------------
+
+constexpr int kPrepWarps = 4;
+
+// A warp per packed row: the teacher's entries sorted by column, entries of the
+// same column joined, absent ones (a column outside of [0, V)) dropped; their
+// probabilities; and where each 256-column tile's entries begin.
+template <typename TI>
+__global__ void __launch_bounds__(kPrepWarps * 32)
+topk_prep_kernel(const TI* __restrict__ ids, const float* __restrict__ logp, int K, int K2, int64_t N, int64_t V,
+                 float inv_t, int tail, const RowsView R, const TopkView T, float* __restrict__ p_out,
+                 float* __restrict__ rest_out) {
+  extern __shared__ unsigned long long keys_sh[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long* key = keys_sh + (size_t)warp * K2;
+  const int64_t i = (int64_t)blockIdx.x * kPrepWarps + warp;
+  const int64_t count = *R.count;
+  uint16_t* st = const_cast<uint16_t*>(T.start) + i * T.tiles1;
+  if (i >= N) return;
+  if (i >= count) {  // no entries
+    for (int t = lane; t < T.tiles1; t += 32) st[t] = 0;
+    return;
+  }
+  const int64_t src = (int64_t)R.row_of[i] * K;
+  constexpr unsigned long long kNone = 0xffffffffffffffffull;
+  float mx = -INFINITY;
+  bool nan = false;
+  for (int k = lane; k < K2; k += 32) {
+    unsigned long long x = kNone;
+    if (k < K) {
+      const int64_t v = (int64_t)ids[src + k];
+      if (v >= 0 && v < V) {
+        x = ((unsigned long long)v << 32) | (unsigned)k;
+        const float t = logp[src + k];
+        mx = fmaxf(mx, t);
+        nan = nan || t != t;
+      }
+    }
+    key[k] = x;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  nan = __any_sync(0xffffffffu, nan);
+  __syncwarp();
+  // bitonic sort by (column, place)
+  for (int size = 2; size <= K2; size <<= 1) {
+    for (int j = size >> 1; j > 0; j >>= 1) {
+      for (int k = lane; k < K2 / 2; k += 32) {
+        const int lo = 2 * j * (k / j) + k % j, hi = lo + j;
+        const bool up = (lo & size) == 0;
+        const unsigned long long x = key[lo], y = key[hi];
+        if ((x > y) == up) {
+          key[lo] = y;
+          key[hi] = x;
+        }
+      }
+      __syncwarp();
+    }
+  }
+  // renormalised: p = e^((t - max) / T) / Z; with a tail: p = e^t
+  float z = 0.f;
+  if (!tail) {
+    for (int k = lane; k < K2; k += 32)
+      if (key[k] != kNone) {
+        const float t = logp[src + (unsigned)key[k]];
+        if (t != -INFINITY) z += expf((t - mx) * inv_t);
+      }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if (nan) z = NAN;
+  }
+  int32_t* sid = const_cast<int32_t*>(T.sid) + i * K;
+  float* pr = p_out + i * K;
+  int n = 0;          // entries of distinct columns so far
+  double mass = 0.0;  // this lane's share of the sum of p
+  for (int k0 = 0; k0 < K2; k0 += 32) {
+    const int k = k0 + lane;
+    const unsigned long long x = k < K2 ? key[k] : kNone;
+    const bool head = x != kNone && (k == 0 || (key[k - 1] >> 32) != (x >> 32));
+    const unsigned heads = __ballot_sync(0xffffffffu, head);
+    if (head) {
+      double p = 0.0;
+      for (int j = k; j < K2 && key[j] != kNone && (key[j] >> 32) == (x >> 32); ++j) {
+        const float t = logp[src + (unsigned)key[j]];
+        if (tail) p += exp((double)t);
+        else if (z != z) p = NAN;
+        else if (t != -INFINITY) p += (double)(expf((t - mx) * inv_t) / z);
+      }
+      const int at = n + __popc(heads & ((1u << lane) - 1u));
+      sid[at] = (int32_t)(x >> 32);
+      pr[at] = (float)p;
+      mass += p;
+    }
+    n += __popc(heads);
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+  // what the entries leave over; nothing when every column is listed
+  if (lane == 0) {
+    const double r = 1.0 - mass;
+    rest_out[i] = tail && n > 0 && n < V ? (float)(r > 0.0 ? r : (r == r ? 0.0 : r)) : 0.f;
+  }
+  __syncwarp();
+  for (int t = lane; t < T.tiles1; t += 32) {
+    const int64_t col = (int64_t)t * kTopkTile;
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sid[mid] < col) lo = mid + 1;
+      else hi = mid;
+    }
+    st[t] = (uint16_t)lo;
+  }
+}
+
+// 32 rows per block: the statistics of the columns outside of S are joined, then
+// a warp per row takes the K entries: loss, the others' coefficient A, the
+// entries' gradients x (in place of their z).
+__global__ void __launch_bounds__(kStRows * kStSlices)
+distill_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s, int64_t P, int64_t N, int64_t V,
+                    const RowsView R, const TopkView T, const float* __restrict__ p_in,
+                    const float* __restrict__ rest_in, float* __restrict__ lse_rest, float* __restrict__ A,
+                    float* __restrict__ loss_row, DistillSum* __restrict__ sums) {
+  __shared__ float sm[kStSlices][kStRows], ss[kStSlices][kStRows];
+  __shared__ double tot[kStRows];
+  __shared__ int has[kStRows];
+  const int64_t row0 = (int64_t)blockIdx.x * kStRows;
+  const int64_t count = *R.count;
+  fold_rows(part_m, part_s, P, N, row0 + threadIdx.x, row0 + threadIdx.x < count, sm, ss);
+  const int w = threadIdx.y, lane = threadIdx.x;  // blockDim (32, 32): a warp per row
+  const int64_t i = row0 + w;
+  double loss = 0.0;
+  int ok = 0;
+  if (i < count) {
+    const int n = T.start[i * T.tiles1 + T.tiles1 - 1];
+    float* zr = T.z + i * T.K;
+    const float* pr = p_in + i * T.K;
+    const float rest = rest_in[i];
+    const float mr = sm[0][w], sr = ss[0][w];
+    float mx = mr, mass = 0.f;
+    for (int k = lane; k < n; k += 32) {
+      mx = fmaxf(mx, zr[k]);
+      mass += pr[k];
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    }
+    float top = 0.f;
+    for (int k = lane; k < n; k += 32) top += exp2f((zr[k] - mx) * kLog2e);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top += __shfl_xor_sync(0xffffffffu, top, o);
+    const bool others = n < V && mr != -INFINITY;
+    const float sr_mx = others ? sr * exp2f((mr - mx) * kLog2e) : 0.f;
+    const float S = top + sr_mx, logS = logf(S);
+    // an entry with a column but no mass anywhere (all e^-inf) says nothing
+    ok = n > 0 && !(mass == 0.f && rest == 0.f);
+    const float whole = mass + rest;
+    for (int k = lane; k < n; k += 32) {
+      const float p = pr[k], lz = zr[k] - mx;
+      if (ok && p != 0.f) loss += (double)(p * (logf(p) - (lz - logS)));
+      zr[k] = ok ? whole * (exp2f(lz * kLog2e) / S) - p : 0.f;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    if (lane == 0) {
+      // log q_r from the parts: (mr - mx) + log sr - log S
+      if (ok && rest != 0.f)
+        loss += others ? (double)(rest * (logf(rest) - ((mr - mx) + logf(sr) - logS))) : (double)INFINITY;
+      A[i] = ok && others ? whole * (sr_mx / S) - rest : 0.f;
+      lse_rest[i] = others ? mr + logf(sr) : INFINITY;
+      if (loss_row) loss_row[R.row_of[i]] = (float)loss;
+    }
+  } else if (i < N && lane == 0) {
+    A[i] = 0.f;
+    lse_rest[i] = INFINITY;
+  }
+  if (lane == 0) {
+    tot[w] = loss;
+    has[w] = ok;
+  }
+  __syncthreads();
+  if (w == 0) {
+    double l = tot[lane];
+    int n = has[lane];
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    if (lane == 0) sums[blockIdx.x] = DistillSum{l, n};
+  }
+}
+
+__global__ void __launch_bounds__(256)
+distill_final_kernel(const DistillSum* __restrict__ sums, int blocks, int reduction, float* __restrict__ loss,
+                     float* __restrict__ weight) {
+  __shared__ double l_sh[8], n_sh[8];
+  double l = 0.0, n = 0.0;
+  for (int b = threadIdx.x; b < blocks; b += 256) {
+    l += sums[b].loss;
+    n += (double)sums[b].n;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    l += __shfl_xor_sync(0xffffffffu, l, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    l_sh[threadIdx.x >> 5] = l;
+    n_sh[threadIdx.x >> 5] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    l = n = 0.0;
+    for (int w = 0; w < 8; ++w) {
+      l += l_sh[w];
+      n += n_sh[w];
+    }
+    const double c = reduction == CCE_REDUCE_MEAN ? (n > 0.0 ? n : 1.0) : 1.0;
+    if (reduction != CCE_REDUCE_NONE) loss[0] = (float)(l / c);
+    weight[0] = (float)(1.0 / c);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+
+// Cotangents of the packed rows: d = sign * up * weight * scale (0 behind the count), dA = d A.
+__global__ void rows_cotangent_kernel(const float* __restrict__ up, int up_row, const float* __restrict__ weight,
+                                      float factor, const RowsView R, int64_t N, const float* __restrict__ A,
+                                      float* __restrict__ d, float* __restrict__ dA) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= N) return;
+  float x = 0.f;
+  if (i < *R.count) x = up[up_row ? R.row_of[i] : 0] * (weight ? weight[0] * factor : factor);
+  d[i] = x;
+  if (dA) dA[i] = x == 0.f ? 0.f : x * A[i];
+}
+
+// Block mask of exact gradients: a row block is kept whole unless every row of
+// it has a zero cotangent.  grid (tile groups, row blocks)
+__global__ void __launch_bounds__(256)
+live_mask_kernel(const float* __restrict__ d, int64_t N, int64_t V, uint8_t* __restrict__ keep,
+                 uint32_t* __restrict__ keep_t, int64_t keep_t_ld) {
+  const int64_t i = blockIdx.y;
+  const int64_t r = i * kRowBlock + (threadIdx.x & (kRowBlock - 1));
+  const int live = __syncthreads_or(r < N && d[r] != 0.f);
+  const int64_t nVt = ceil_div(V, kStatTile);
+  const int64_t t0 = (int64_t)blockIdx.x * 1024;
+  for (int64_t t = t0 + threadIdx.x; t < nVt && t < t0 + 1024; t += 256) {
+    keep[i * nVt + t] = live ? 1 : 0;
+    if (keep_t && live && t % (128 / kStatTile) == 0)
+      atomicOr(&keep_t[t / (128 / kStatTile) * keep_t_ld + (i >> 5)], 1u << (i & 31));
+  }
+}
+
+// grad_e row n = a[pos[n]] (+ b[pos[n]]), 0 for rows that do not count.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256)
+rows_scatter_kernel(const float* __restrict__ a, const float* __restrict__ b, const int32_t* __restrict__ pos, int64_t N,
+                    int64_t D, T* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < N; n += (int64_t)gridDim.x * 8) {
+    const int64_t p = pos[n];
+    if constexpr (kVec) {
+      for (int64_t k = 4 * lane; k < D; k += 128) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p >= 0) {
+          x = *reinterpret_cast<const float4*>(a + p * D + k);
+          if (b) {
+            const float4 y = *reinterpret_cast<const float4*>(b + p * D + k);
+            x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+          }
+        }
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<float4*>(out + n * D + k) = x;
+        } else {
+          T h[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
+          *reinterpret_cast<uint2*>(out + n * D + k) = *reinterpret_cast<uint2*>(h);
+        }
+      }
+    } else {
+      for (int64_t k = lane; k < D; k += 32) {
+        float x = 0.f;
+        if (p >= 0) x = a[p * D + k] + (b ? b[p * D + k] : 0.f);
+        out[n * D + k] = from_f32<T>(x);
+      }
+    }
+  }
+}
+
+// grad_bias of a vocabulary chunk from partial column sums part[parts][ld], in
+// order: the same result every time, where atomics would add in any order.
+template <typename TO>
+__global__ void __launch_bounds__(256)
+bias_sum_kernel(const float* __restrict__ part, int64_t parts, int64_t ld, int64_t cols, const float* __restrict__ scale,
+                TO* __restrict__ out) {
+  __shared__ float sh[8][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < cols)
+    for (int64_t p = w; p < parts; p += 8) s += part[p * ld + c];
+  sh[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && c < cols) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sh[k][lane];
+    out[c] = s * (scale ? scale[0] : 1.f);
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+unsigned warps_grid(int64_t N) {
+  const int64_t b = ceil_div(N, 8);
+  return (unsigned)(b < 148 * 8 ? b : 148 * 8);
+}
+
+}  // namespace
+
+cudaError_t launch_rows_pack(const void* e, int dtype, int64_t N, int64_t D, const void* targets, int target_bytes,
+                             int64_t ignore_index, int has_ignore, const uint8_t* mask, const RowsView& R,
+                             uint8_t* mask_out, float* per_row_out, void* e_packed, float* tgt, cudaStream_t s) {
+  if (targets == nullptr)
+    rows_pack_kernel<void><<<1, kPackThreads, 0, s>>>(nullptr, 0, 0, mask, N, R, mask_out, per_row_out);
+  else if (target_bytes == 8)
+    rows_pack_kernel<int64_t><<<1, kPackThreads, 0, s>>>((const int64_t*)targets, ignore_index, has_ignore, mask, N, R,
+                                                         mask_out, per_row_out);
+  else
+    rows_pack_kernel<int32_t><<<1, kPackThreads, 0, s>>>((const int32_t*)targets, ignore_index, has_ignore, mask, N, R,
+                                                         mask_out, per_row_out);
+  cudaError_t err = launched();
+  if (err != cudaSuccess) return err;
+  const int64_t row_bytes = D * (dtype == CCE_F32 ? 4 : 2);
+  const bool vec = row_bytes % 16 == 0 && aligned16(e) && aligned16(e_packed);
+  if (vec)
+    rows_gather_kernel<true><<<warps_grid(N), 256, 0, s>>>((const uint8_t*)e, N, row_bytes, R, targets != nullptr,
+                                                           (uint8_t*)e_packed, tgt);
+  else
+    rows_gather_kernel<false><<<warps_grid(N), 256, 0, s>>>((const uint8_t*)e, N, row_bytes, R, targets != nullptr,
+                                                            (uint8_t*)e_packed, tgt);
+  return launched();
+}
+
+cudaError_t launch_rows_logp(const float* part_m, const float* part_s, int64_t P, int64_t N, const RowsView& R,
+                             const float* tgt, float* lse, float* logp, cudaStream_t s) {
+  rows_logp_kernel<<<(unsigned)ceil_div(N, kStRows), dim3(kStRows, kStSlices), 0, s>>>(part_m, part_s, P, N, R, tgt, lse,
+                                                                                       logp);
+  return launched();
+}
+
+cudaError_t launch_topk_prep(const void* ids, int id_bytes, const float* logp, int64_t N, int64_t V, int K, double T,
+                             int tail, const RowsView& R, const TopkView& topk, float* p, float* rest, cudaStream_t s) {
+  int K2 = 2;
+  while (K2 < K) K2 *= 2;
+  const size_t smem = (size_t)kPrepWarps * K2 * 8;  // at most 32 KB (K <= 1024)
+  const unsigned grid = (unsigned)ceil_div(N, kPrepWarps);
+  const float inv_t = (float)(1.0 / T);
+  if (id_bytes == 8)
+    topk_prep_kernel<int64_t><<<grid, kPrepWarps * 32, smem, s>>>((const int64_t*)ids, logp, K, K2, N, V, inv_t, tail, R,
+                                                                  topk, p, rest);
+  else
+    topk_prep_kernel<int32_t><<<grid, kPrepWarps * 32, smem, s>>>((const int32_t*)ids, logp, K, K2, N, V, inv_t, tail, R,
+                                                                  topk, p, rest);
+  return launched();
+}
+
+int64_t distill_blocks(int64_t N) { return ceil_div(N, kStRows); }
+
+cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_t P, int64_t N, int64_t V,
+                                const RowsView& R, const TopkView& topk, const float* p, const float* rest,
+                                int reduction, float* lse_rest, float* A, DistillSum* sums, float* loss, float* weight,
+                                cudaStream_t s) {
+  const int blocks = (int)distill_blocks(N);
+  distill_rows_kernel<<<blocks, dim3(kStRows, kStSlices), 0, s>>>(
+      part_m, part_s, P, N, V, R, topk, p, rest, lse_rest, A, reduction == CCE_REDUCE_NONE ? loss : nullptr, sums);
+  cudaError_t err = launched();
+  if (err != cudaSuccess) return err;
+  distill_final_kernel<<<1, 256, 0, s>>>(sums, blocks, reduction, loss, weight);
+  return launched();
+}
+
+cudaError_t launch_rows_cotangent(const float* up, int up_row, const float* weight, float factor, const RowsView& R,
+                                  int64_t N, const float* A, float* d, float* dA, cudaStream_t s) {
+  rows_cotangent_kernel<<<(unsigned)ceil_div(N, 256), 256, 0, s>>>(up, up_row, weight, factor, R, N, A, d, dA);
+  return launched();
+}
+
+cudaError_t launch_live_mask(const float* d, int64_t N, int64_t V, uint8_t* keep, uint32_t* keep_t, int64_t keep_t_ld,
+                             cudaStream_t s) {
+  const dim3 grid((unsigned)ceil_div(ceil_div(V, kStatTile), (int64_t)1024), (unsigned)ceil_div(N, kRowBlock));
+  live_mask_kernel<<<grid, 256, 0, s>>>(d, N, V, keep, keep_t, keep_t_ld);
+  return launched();
+}
+
+template <typename T>
+static cudaError_t scatter(const float* a, const float* b, const int32_t* pos, int64_t N, int64_t D, void* out,
+                           cudaStream_t s) {
+  const bool vec = D % 4 == 0 && aligned16(a) && aligned16(b) && aligned16(out);
+  if (vec)
+    rows_scatter_kernel<T, true><<<warps_grid(N), 256, 0, s>>>(a, b, pos, N, D, static_cast<T*>(out));
+  else
+    rows_scatter_kernel<T, false><<<warps_grid(N), 256, 0, s>>>(a, b, pos, N, D, static_cast<T*>(out));
+  return launched();
+}
+
+cudaError_t launch_rows_scatter(const float* a, const float* b, const int32_t* pos, int64_t N, int64_t D, int dtype,
+                                void* out, cudaStream_t s) {
+  switch (dtype) {
+    case CCE_F32: return scatter<float>(a, b, pos, N, D, out, s);
+    case CCE_F16: return scatter<__half>(a, b, pos, N, D, out, s);
+    case CCE_BF16: return scatter<__nv_bfloat16>(a, b, pos, N, D, out, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_bias_sum(const float* part, int64_t parts, int64_t ld, int64_t cols, const float* scale, float* out,
+                            cudaStream_t s) {
+  bias_sum_kernel<float><<<(unsigned)ceil_div(cols, 32), 256, 0, s>>>(part, parts, ld, cols, scale, out);
+  return launched();
+}
+
+}  // namespace cce

@@ -43,6 +43,7 @@
 #include "kernels.cuh"
 #include "schedule.cuh"
 #include "tc_ptx.cuh"
+#include "topk.cuh"
 
 namespace cce {
 namespace tc {
@@ -303,7 +304,9 @@ struct FwdEpi {
 // K4: dlogits of one vocabulary chunk
 // ---------------------------------------------------------------------------
 
-template <typename T, typename TB>
+// kTopk (distillation): d_nll and lse are the coefficient and log-sum-exp of the
+// columns outside of the row's list; the listed ones' values are given.
+template <typename T, typename TB, bool kTopk = false>
 struct DlogitsEpi {
   static constexpr bool kNarrowB = true;  // B rows loaded for a tile's live column run only
   static constexpr bool kPairLd = false;  // the epilogue reads TMEM two 32-column chunks at a time
@@ -323,10 +326,17 @@ struct DlogitsEpi {
   int mask_rows, mask_cols; // nRb, statistics tiles in the chunk
   int64_t N, V, v_offset, vc0, vc_end, ld;
   int dbl = 0;     // narrow tiles load two K-blocks per stage (kDblB0)
+  float* bias_part = nullptr;    // [ceil(N / 32)][ld] column sums of w (instead of grad_bias)
+  TopkView topk{};               // kTopk
+  const float* d_row = nullptr;
+  float logit_scale = 1.f;
 
+  struct NoCursor {};
   struct State {
     int64_t row, tl, col0;
     float g, L, s;   // g = d_nll / s
+    float dr;        // kTopk: d_row / s
+    typename std::conditional<kTopk, TopkCursor, NoCursor>::type cur;
     uint32_t kmask;  // kept statistics-tile column groups of the tile
     int y0;          // first row of this warp's 32-row slab
   };
@@ -367,7 +377,13 @@ struct DlogitsEpi {
     st.s = scale ? scale[0] : 1.f;
     st.g = ok ? d_nll[st.row] * (scale ? scale[1] : 1.f) : 0.f;
     st.L = ok ? lse[st.row] : 0.f;
-    st.tl = ok ? (int64_t)targets[st.row] - v_offset : -1;
+    if constexpr (kTopk) {
+      st.tl = -1;
+      st.dr = ok ? d_row[st.row] * (scale ? scale[1] : 1.f) : 0.f;
+      st.cur.open(topk, st.row, ok, st.col0 / kTopkTile);
+    } else {
+      st.tl = ok ? (int64_t)targets[st.row] - v_offset : -1;
+    }
     st.kmask = group_mask(mk, mb, nb);
     st.y0 = (int)(st.row - (threadIdx.x & 31));
   }
@@ -387,10 +403,24 @@ struct DlogitsEpi {
     for (int j = 0; j < 32; ++j) {
       float w = 0.f;
       if (kept && cb + j < vc_end) {
-        w = st.g * exp2f(fmaf(v[j] + b[j], kLog2e, -Ll));
-        if (cb + j == st.tl) w -= st.g;
+        if constexpr (kTopk) {
+          w = st.g * exp2f(((v[j] + b[j]) * logit_scale - st.L) * kLog2e);
+        } else {
+          w = st.g * exp2f(fmaf(v[j] + b[j], kLog2e, -Ll));
+          if (cb + j == st.tl) w -= st.g;
+        }
       }
       v[j] = w;
+    }
+    if constexpr (kTopk) {
+      int p;
+      const uint32_t bits = st.cur.take(cb, p);
+      if (__any_sync(0xffffffffu, bits != 0u)) {
+        const float* x = topk.z + st.row * topk.K + p;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if ((bits >> j) & 1u) v[j] = st.dr * __ldg(x + __popc(bits & ((1u << j) - 1u)));
+      }
     }
     // grad_c multiplies whole 128-column quarters (its M tiles): a quarter
     // with a kept group is stored whole (zeros in the others), the rest never
@@ -402,6 +432,10 @@ struct DlogitsEpi {
       const int lane = threadIdx.x & 31;
       const float colsum = warp_transpose_sum32(v);
       if (cb + lane < vc_end && colsum != 0.f) atomicAdd(grad_bias + cb + lane, colsum * st.s);
+    } else if (bias_part != nullptr && kept) {
+      const int lane = threadIdx.x & 31;
+      const float colsum = warp_transpose_sum32(v);
+      if (cb + lane < vc_end && st.y0 < N) bias_part[(int64_t)(st.y0 / 32) * ld + (cb - vc0) + lane] = colsum;
     }
   }
 
@@ -1495,7 +1529,7 @@ __global__ void __launch_bounds__(1024) dl_list_kernel(const uint8_t* keep, int6
     if (i < 32 ? ((bits >> i) & 1u) != 0 : live(u0 + i)) list[pos++] = u0 + i;
 }
 
-template <typename T, typename TB>
+template <typename T, typename TB, bool kTopk>
 cudaError_t dl_launch(const BwdChunkArgs& a, cudaStream_t s) {
   const bool bf16 = a.dtype == CCE_BF16;
   CUtensorMap tmA, tmB;
@@ -1509,11 +1543,15 @@ cudaError_t dl_launch(const BwdChunkArgs& a, cudaStream_t s) {
   }
   const int64_t vc_end = (a.vc0 + a.vc_len) < a.V ? (a.vc0 + a.vc_len) : a.V;
   sc.span = dlogits_span() ? 1 : 0;
-  DlogitsEpi<T, TB> epi{a.targets, a.lse, a.d_nll, a.bias, static_cast<T*>(a.dlogits), a.grad_bias,
+  DlogitsEpi<T, TB, kTopk> epi{a.targets, a.lse, a.d_nll, a.bias, static_cast<T*>(a.dlogits), a.grad_bias,
                         a.scale, a.keep + a.vc0 / kStatTile, ceil_div(a.V, kStatTile),
                         (int)ceil_div(a.N, kRowBlock), (int)ceil_div(a.vc_len, kStatTile),
                         a.N, a.V, a.v_offset, a.vc0, vc_end, a.vc_ld};
   epi.dbl = dlogits_double_k() ? 1 : 0;
+  epi.bias_part = a.bias_part;
+  epi.topk = a.topk;
+  epi.d_row = a.d_row;
+  epi.logit_scale = a.logit_scale;
   CUtensorMap tmC, tmB32;
   if (!make_tmap_out(&tmC, a.dlogits, a.dtype, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
   if (!make_tmap(&tmB32, cchunk, bf16, a.D, a.vc_len, a.D, BK, kStatTile)) return cudaErrorInvalidValue;
@@ -1543,22 +1581,44 @@ cudaError_t tc_forward(const FwdArgs& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-template <typename T>
+template <typename T, bool kTopk>
 cudaError_t dl_dispatch(const BwdChunkArgs& a, cudaStream_t s) {
   switch (a.bias == nullptr ? -1 : a.bias_dtype) {
-    case -1: return dl_launch<T, void>(a, s);
-    case CCE_F32: return dl_launch<T, float>(a, s);
-    case CCE_F16: return dl_launch<T, __half>(a, s);
-    case CCE_BF16: return dl_launch<T, __nv_bfloat16>(a, s);
+    case -1: return dl_launch<T, void, kTopk>(a, s);
+    case CCE_F32: return dl_launch<T, float, kTopk>(a, s);
+    case CCE_F16: return dl_launch<T, __half, kTopk>(a, s);
+    case CCE_BF16: return dl_launch<T, __nv_bfloat16, kTopk>(a, s);
   }
   return cudaErrorInvalidValue;
 }
 
+template <bool kTopk>
+cudaError_t dl_types(const BwdChunkArgs& a, cudaStream_t s) {
+  if (a.dtype == CCE_BF16) return dl_dispatch<__nv_bfloat16, kTopk>(a, s);
+  if (a.dtype == CCE_F16) return dl_dispatch<__half, kTopk>(a, s);
+  return cudaErrorNotSupported;
+}
+
 cudaError_t tc_dlogits(const BwdChunkArgs& a, cudaStream_t s) {
   if (a.N == 0 || a.vc_len == 0) return cudaSuccess;
-  if (a.dtype == CCE_BF16) return dl_dispatch<__nv_bfloat16>(a, s);
-  if (a.dtype == CCE_F16) return dl_dispatch<__half>(a, s);
-  return cudaErrorNotSupported;
+  return a.topk.sid ? dl_types<true>(a, s) : dl_types<false>(a, s);
+}
+
+namespace tc {
+namespace {
+#include "tc_logits.cuh"
+}  // namespace
+}  // namespace tc
+
+cudaError_t tc_logits(const FwdArgs& a, cudaStream_t s) {
+  if (a.N == 0 || a.V == 0) return cudaSuccess;
+  switch (a.bias == nullptr ? -1 : a.bias_dtype) {
+    case -1: return logits_dispatch<void>(a, s);
+    case CCE_F32: return logits_dispatch<float>(a, s);
+    case CCE_F16: return logits_dispatch<__half>(a, s);
+    case CCE_BF16: return logits_dispatch<__nv_bfloat16>(a, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 namespace {

@@ -32,7 +32,8 @@ from ._ext import FILTER_LOG_EPS, cce_backward_raw, cce_forward_raw, cut_cross_e
 __all__ = ["linear_cross_entropy", "cce_loss", "cut_cross_entropy", "LinearCrossEntropy",
            "cce_forward_raw", "cce_backward_raw", "FILTER_LOG_EPS", "QuantizedClassifier",
            "linear_cross_entropy_quantized", "policy_loss", "PolicyStats", "preference_loss",
-           "PreferenceRewards"]
+           "PreferenceRewards", "linear_log_probs", "linear_policy_loss", "linear_preference_loss",
+           "linear_distillation_loss"]
 
 
 def _cce(e, c, targets, bias, reduction, ignore_index, filter_log_eps, group, v_offset,
@@ -132,4 +133,5 @@ class LinearCrossEntropy(torch.nn.Module):
 
 
 from .quantized import QuantizedClassifier, linear_cross_entropy_quantized  # noqa: E402
-from .losses import PolicyStats, PreferenceRewards, policy_loss, preference_loss  # noqa: E402
+from .losses import (PolicyStats, PreferenceRewards, linear_distillation_loss,  # noqa: E402
+                     linear_log_probs, linear_policy_loss, linear_preference_loss, policy_loss, preference_loss)

@@ -60,6 +60,9 @@ EXPORTED_SYMBOLS = (
     "cce_forward_q_workspace_bytes", "cce_forward_q", "cce_backward_q_workspace_bytes", "cce_backward_q",
     "cce_token_loss_workspace_bytes", "cce_policy_loss_forward", "cce_policy_loss_backward",
     "cce_preference_loss_forward", "cce_preference_loss_backward",
+    "cce_logp_saved_bytes", "cce_logp_forward_workspace_bytes", "cce_logp_backward_workspace_bytes",
+    "cce_logp_forward", "cce_logp_backward", "cce_distill_saved_bytes", "cce_distill_forward_workspace_bytes",
+    "cce_distill_backward_workspace_bytes", "cce_distill_forward", "cce_distill_backward",
 )
 
 
@@ -87,6 +90,12 @@ class CcePreferenceParams(ctypes.Structure):
                 ("kind", ctypes.c_int32), ("reduction", ctypes.c_int32), ("length_normalize", ctypes.c_int32)]
 
 
+class CceDistillParams(ctypes.Structure):
+    """Mirror of ``CceDistillParams`` (include/cce_b200.h)."""
+    _fields_ = [("temperature", ctypes.c_double), ("tail", ctypes.c_int32), ("reduction", ctypes.c_int32)]
+
+
+CCE_DISTILL_MAX_K = 1024
 CCE_REDUCE_MEAN, CCE_REDUCE_SUM, CCE_REDUCE_SEQUENCE, CCE_REDUCE_NONE = 0, 1, 2, 3
 CCE_PREF_SIGMOID, CCE_PREF_HINGE, CCE_PREF_IPO = 0, 1, 2
 
@@ -171,6 +180,27 @@ def _load():
                                                 c_vp]
     lib.cce_preference_loss_backward.restype = c_int
     lib.cce_preference_loss_backward.argtypes = [c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]
+    for name, args in (("cce_logp_saved_bytes", [c_i64, c_i64, c_i64, c_int]),
+                       ("cce_logp_forward_workspace_bytes", [c_i64, c_i64]),
+                       ("cce_logp_backward_workspace_bytes", [c_i64, c_i64, c_i64, c_int, c_int]),
+                       ("cce_distill_saved_bytes", [c_i64, c_i64, c_i64, c_i64, c_int]),
+                       ("cce_distill_forward_workspace_bytes", [c_i64, c_i64, c_i64]),
+                       ("cce_distill_backward_workspace_bytes", [c_i64, c_i64, c_i64, c_int, c_int])):
+        getattr(lib, name).restype = c_sz
+        getattr(lib, name).argtypes = args
+    lib.cce_logp_forward.restype = c_int
+    lib.cce_logp_forward.argtypes = [c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_i64, c_int, c_i64, c_i64, c_i64, c_int,
+                                     c_vp, c_vp, c_vp, c_sz, c_vp, c_sz, c_vp]
+    lib.cce_logp_backward.restype = c_int
+    lib.cce_logp_backward.argtypes = [c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp, c_sz, c_vp,
+                                      c_vp, c_vp, c_vp, c_sz, c_vp]
+    lib.cce_distill_forward.restype = c_int
+    lib.cce_distill_forward.argtypes = [c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
+                                        c_int, ctypes.POINTER(CceDistillParams), c_vp, c_vp, c_sz, c_vp, c_sz, c_vp]
+    lib.cce_distill_backward.restype = c_int
+    lib.cce_distill_backward.argtypes = [c_vp, c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_int,
+                                         ctypes.POINTER(CceDistillParams), c_int, c_vp, c_sz, c_vp, c_vp, c_vp, c_vp,
+                                         c_sz, c_vp]
     return lib
 
 
@@ -610,6 +640,82 @@ def preference_backward(coef, grad_loss, reduction, mask, cu, N, pairs, shape, d
                                               torch.cuda.current_stream().cuda_stream)
     _check(rc, "cce_preference_loss_backward")
     return grad
+
+
+def _bias_code(bias):
+    return 0 if bias is None else _DTYPE_CODE[bias.dtype]
+
+
+def _bytes(n, dev):
+    return torch.empty((max(n, 1),), dtype=torch.uint8, device=dev)
+
+
+def logp_forward(e, c, bias, targets, ignore_index):
+    """``cce_logp_forward`` on checked contiguous tensors: (logp [N], mask [N], saved)."""
+    dev, (N, D), V, dt = e.device, e.shape, c.shape[0], _DTYPE_CODE[e.dtype]
+    with on_device(dev):
+        logp = torch.empty((N,), dtype=torch.float32, device=dev)
+        mask = torch.empty((N,), dtype=torch.bool, device=dev)
+        saved = _bytes(lib.cce_logp_saved_bytes(N, D, V, dt), dev)
+        ws = _bytes(lib.cce_logp_forward_workspace_bytes(N, V), dev)
+        rc = lib.cce_logp_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), targets.data_ptr(),
+                                  targets.element_size(), 0 if ignore_index is None else ignore_index,
+                                  ignore_index is not None, N, D, V, dt, logp.data_ptr(), mask.data_ptr(),
+                                  saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
+                                  torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_logp_forward")
+    return logp, mask, saved
+
+
+def _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias):
+    """Outputs and flags of the two backward calls on packed rows."""
+    dev, (V, D) = c.device, c.shape
+    ge = torch.empty((N, D), dtype=dtype, device=dev) if need_e else None
+    gc = torch.empty((V, D), dtype=c.dtype, device=dev) if need_c else None
+    gb = torch.empty((V,), dtype=torch.float32, device=dev) if need_bias else None
+    flags = (CCE_NEED_DE if need_e else 0) | (CCE_NEED_DC if need_c else 0) | (CCE_NEED_DBIAS if need_bias else 0)
+    return ge, gc, gb, flags
+
+
+def logp_backward(saved, c, bias, grad_logp, N, dtype, need_e, need_c, need_bias):
+    """``cce_logp_backward``: (grad_e, grad_c, grad_bias fp32); absent ones are None."""
+    dev, (V, D), dt = c.device, c.shape, _DTYPE_CODE[dtype]
+    with on_device(dev):
+        ge, gc, gb, flags = _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias)
+        ws = _bytes(lib.cce_logp_backward_workspace_bytes(N, D, V, dt, flags), dev)
+        rc = lib.cce_logp_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_logp.data_ptr(), N, D, V, dt,
+                                   flags, saved.data_ptr(), saved.numel(), _addr(ge), _addr(gc), _addr(gb),
+                                   ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_logp_backward")
+    return ge, gc, gb
+
+
+def distill_forward(e, c, bias, ids, teacher, mask, params):
+    """``cce_distill_forward`` on checked contiguous tensors: (loss, saved)."""
+    dev, (N, D), V, K, dt = e.device, e.shape, c.shape[0], ids.shape[1], _DTYPE_CODE[e.dtype]
+    with on_device(dev):
+        loss = torch.empty((N,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
+        saved = _bytes(lib.cce_distill_saved_bytes(N, D, V, K, dt), dev)
+        ws = _bytes(lib.cce_distill_forward_workspace_bytes(N, V, K), dev)
+        rc = lib.cce_distill_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), ids.data_ptr(),
+                                     ids.element_size(), teacher.data_ptr(), _addr(mask), N, D, V, K, dt, params,
+                                     loss.data_ptr(), saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
+                                     torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_distill_forward")
+    return loss, saved
+
+
+def distill_backward(saved, c, bias, grad_loss, N, K, dtype, params, need_e, need_c, need_bias):
+    """``cce_distill_backward``: (grad_e, grad_c, grad_bias fp32); absent ones are None."""
+    dev, (V, D), dt = c.device, c.shape, _DTYPE_CODE[dtype]
+    with on_device(dev):
+        ge, gc, gb, flags = _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias)
+        ws = _bytes(lib.cce_distill_backward_workspace_bytes(N, D, V, dt, flags), dev)
+        rc = lib.cce_distill_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_loss.data_ptr(), N, D, V, K,
+                                      dt, params, flags, saved.data_ptr(), saved.numel(), _addr(ge), _addr(gc),
+                                      _addr(gb), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    _check(rc, "cce_distill_backward")
+    return ge, gc, gb
 
 
 # ---------------------------------------------------------------------------

@@ -1,12 +1,21 @@
-"""Losses on a head's per-token log-probabilities: policy and preference losses.
+"""Losses on a head's log-probabilities: policy, preference and distillation losses.
 
-    logp = -linear_cross_entropy(hidden, weight, tokens, reduction="none")
-    loss = policy_loss(logp, old_logp, advantages, ref_logp=ref_logp, kl_coef=0.04)
+    loss = linear_policy_loss(hidden, weight, tokens, old_logp, advantages, ref_logp=ref_logp, kl_coef=0.04)
+    loss = linear_preference_loss(hidden, weight, tokens, ref_logp, cu_seqlens=offsets)
+    loss = linear_distillation_loss(hidden, weight, teacher_ids, teacher_logprobs, temperature=2.0)
 
-The reference ends at the cross-entropy; these are what its log-probabilities
-are trained with after pre-training.  Both run on the CUDA kernels of
-``csrc/token_loss.cu`` and are differentiable with respect to ``logp``; the
-other tensors are constants.
+The reference ends at the cross-entropy; these are what a head is trained with
+after pre-training.  ``linear_log_probs`` is the head's part of the first two
+(log-probabilities of given tokens, the [N, V] logits never materialised);
+``policy_loss`` and ``preference_loss`` take log-probabilities.  Hidden states,
+classifier, bias and log-probabilities are differentiable, the other tensors
+are constants.  Kernels: ``csrc/token_loss.cu``, ``csrc/rows_kernels.cu`` and
+the GEMMs of ``csrc/tc_kernels.cu`` / ``csrc/simt_kernels.cu``.
+
+The linear forms differ from ``linear_cross_entropy`` in two ways: gradients
+are exact (the filter of small softmax values is not applied: a policy
+gradient pushes the unlikely tokens too), and rows that do not count are taken
+out before the GEMMs.
 
 Tokens come as padded rows ``[S, T]`` (a row is a sequence) or packed in one
 dimension with ``cu_seqlens`` (int32 offsets ``[S + 1]``).  Tokens that
@@ -158,6 +167,49 @@ def _pairs(what, shape, cu_seqlens, dev):
     return S // 2, cu
 
 
+def _head(what, e, c, bias, rows_shape):
+    """Checked (e [N, D], c, bias), contiguous."""
+    if e.dim() < 2 or c.dim() != 2:
+        raise ValueError(f"[{what}] e must be [..., D] and c [V, D], got {tuple(e.shape)} and {tuple(c.shape)}")
+    if e.shape[:-1] != rows_shape:
+        raise ValueError(f"[{what}] e holds rows {tuple(e.shape[:-1])}, expected {tuple(rows_shape)}")
+    if e.shape[-1] != c.shape[1]:
+        raise ValueError(f"[{what}] c.shape[1] ({c.shape[1]}) must equal e.shape[-1] ({e.shape[-1]})")
+    if e.dtype != c.dtype:
+        raise ValueError(f"[{what}] e and c must share a dtype, got {e.dtype} and {c.dtype}")
+    _ext.dtype_code(e.dtype, what)
+    if bias is not None:
+        if bias.shape != (c.shape[0],):
+            raise ValueError(f"[{what}] bias must be [V={c.shape[0]}], got {tuple(bias.shape)}")
+        _ext.dtype_code(bias.dtype, what)
+    if c.shape[0] == 0 or c.shape[1] == 0:
+        raise ValueError(f"[{what}] c must not be empty, got {tuple(c.shape)}")
+    for name, t in (("e", e), ("c", c), ("bias", bias)):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"[{what}] {name} must be a CUDA tensor (no CPU implementation exists)")
+        if t.device != e.device:
+            raise ValueError(f"[{what}] {name} is on {t.device}, expected {e.device}")
+    return (e.reshape(-1, e.shape[-1]).contiguous(), c.contiguous(), None if bias is None else bias.contiguous())
+
+
+def _ids(what, name, t, dev):
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"[{what}] {name} must be int32 or int64, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"[{what}] {name} is on {t.device}, expected {dev}")
+    return t.contiguous()
+
+
+def _distill_params(what, temperature, tail, reduction):
+    if reduction not in PREFERENCE_REDUCTIONS:
+        raise ValueError(f"[{what}] Unknown reduction: {reduction}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"[{what}] temperature must be positive, got {temperature}")
+    return _ext.CceDistillParams(temperature, int(bool(tail)), PREFERENCE_REDUCTIONS[reduction])
+
+
 def _reference(what, ref_logp, logp, S):
     """(per-token reference or None, per-sequence sums or None)"""
     if ref_logp is None:
@@ -216,6 +268,47 @@ class PreferenceLossFunction(torch.autograd.Function):
         reduction, N, pairs, shape, dtype = ctx.meta
         g = grad_loss.to(torch.float32).contiguous()
         return (_ext.preference_backward(coef, g, reduction, mask, cu, N, pairs, shape, dtype),) + (None,) * 6
+
+
+class LogProbsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, e, c, bias, targets, ignore_index):
+        logp, mask, saved = _ext.logp_forward(e, c, bias, targets, ignore_index)
+        ctx.save_for_backward(c, bias, saved)
+        ctx.meta = (e.shape[0], e.dtype)
+        ctx.mark_non_differentiable(mask)
+        ctx.set_materialize_grads(False)
+        return logp, mask
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_logp, _grad_mask):
+        need = ctx.needs_input_grad
+        if grad_logp is None or not any(need[:3]):
+            return (None,) * 5
+        c, bias, saved = ctx.saved_tensors
+        ge, gc, gb = _ext.logp_backward(saved, c, bias, grad_logp.to(torch.float32).contiguous(), *ctx.meta, *need[:3])
+        return ge, gc, None if gb is None else gb.to(bias.dtype), None, None
+
+
+class DistillationFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, e, c, bias, ids, teacher, mask, params):
+        loss, saved = _ext.distill_forward(e, c, bias, ids, teacher, mask, params)
+        ctx.save_for_backward(c, bias, saved)
+        ctx.meta = (e.shape[0], ids.shape[1], e.dtype, params)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        need = ctx.needs_input_grad
+        if not any(need[:3]):
+            return (None,) * 7
+        c, bias, saved = ctx.saved_tensors
+        g = grad_loss.to(torch.float32).contiguous()
+        ge, gc, gb = _ext.distill_backward(saved, c, bias, g, *ctx.meta, *need[:3])
+        return (ge, gc, None if gb is None else gb.to(bias.dtype)) + (None,) * 4
 
 
 # ---------------------------------------------------------------------------
@@ -294,3 +387,111 @@ def preference_loss(logp, ref_logp=None, *, mask=None, cu_seqlens=None, beta=0.1
     loss, rewards = PreferenceLossFunction.apply(logp, ref, sums, _mask(what, mask, logp.shape, logp.device), cu,
                                                  pairs, params)
     return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
+
+
+def _log_probs(what, e, c, targets, bias, ignore_index):
+    """(logp, mask) in the targets' shape."""
+    e2, c, bias = _head(what, e, c, bias, targets.shape)
+    targets = _ids(what, "targets", targets, e.device)
+    logp, mask = LogProbsFunction.apply(e2, c, bias, targets.reshape(-1), ignore_index)
+    return logp.view(targets.shape), mask.view(targets.shape)
+
+
+def linear_log_probs(e, c, targets, bias=None, *, ignore_index=-100):
+    """Log-probabilities ``log softmax(e c^T + bias)`` of the target tokens.
+
+    Args:
+        e: hidden states ``[..., D]`` (float32, float16 or bfloat16)
+        c: classifier weights ``[V, D]`` in e's dtype
+        targets: token ids ``[...]`` in ``[0, V)`` (int32 or int64)
+        bias: optional classifier bias ``[V]``
+        ignore_index: rows with this target are left out (None: none)
+    Returns:
+        float32, shaped like ``targets``; 0 for rows left out.  Accurate to
+        float32 also for 16-bit inputs (``linear_cross_entropy`` is to 1e-3),
+        differentiable with respect to e, c and bias.
+    """
+    return _log_probs("linear_log_probs", e, c, targets, bias, ignore_index)[0]
+
+
+def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_logp=None, cu_seqlens=None, clip=0.2,
+                       clip_high=None, dual_clip=None, kl_coef=0.0, reduction="mean", ignore_index=-100,
+                       return_stats=False):
+    """``policy_loss`` of the head's log-probabilities of ``targets``.
+
+    e ``[..., D]``, c ``[V, D]`` and bias as in ``linear_log_probs``; targets are the
+    sampled tokens, ``[S, T]`` or packed ``[N]`` with ``cu_seqlens``; those equal to
+    ignore_index do not count.  old_logp and ref_logp are float32, shaped like
+    targets.  The other arguments and the result are those of ``policy_loss``.
+    """
+    what = "linear_policy_loss"
+    S, cu = _sequences(what, targets.shape, cu_seqlens, targets.device)
+    adv, per_token = _advantages(what, advantages, targets.shape, S, targets.device)
+    params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
+    logp, mask = _log_probs(what, e, c, targets, bias, ignore_index)
+    loss, stats = PolicyLossFunction.apply(logp, _like(what, "old_logp", old_logp, logp),
+                                           _like(what, "ref_logp", ref_logp, logp), adv, mask, cu, S, params)
+    return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
+
+
+def linear_preference_loss(e, c, targets, ref_logp=None, bias=None, *, cu_seqlens=None, beta=0.1, margin=0.0,
+                           loss_type="sigmoid", label_smoothing=0.0, length_normalize=False, reduction="mean",
+                           ignore_index=-100, return_rewards=False):
+    """``preference_loss`` of the head's log-probabilities of ``targets``.
+
+    e ``[..., D]``, c ``[V, D]`` and bias as in ``linear_log_probs``; targets are the
+    tokens of the sequences, ``[2 pairs, T]`` or packed ``[N]`` with ``cu_seqlens``,
+    chosen before rejected; those equal to ignore_index do not count.  ref_logp is
+    float32 per token, or per sequence ``[2 pairs]``.  The other arguments and the
+    result are those of ``preference_loss``.
+    """
+    what = "linear_preference_loss"
+    pairs, cu = _pairs(what, targets.shape, cu_seqlens, targets.device)
+    params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
+    logp, mask = _log_probs(what, e, c, targets, bias, ignore_index)
+    ref, sums = _reference(what, ref_logp, logp, 2 * pairs)
+    loss, rewards = PreferenceLossFunction.apply(logp, ref, sums, mask, cu, pairs, params)
+    return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
+
+
+def linear_distillation_loss(e, c, teacher_ids, teacher_logprobs, bias=None, *, temperature=1.0, tail=False, mask=None,
+                             reduction="mean"):
+    """KL divergence from a teacher known by its top K tokens to the head's softmax.
+
+    With ``q = softmax((e c^T + bias) / temperature)`` over the whole vocabulary and
+    the teacher's probabilities ``p`` of its K entries a row's loss is
+    ``sum p (log p - log q)``; with ``tail`` also ``r (log r - log q_r)`` of the mass
+    ``r = 1 - sum p`` that the entries leave over and the student's mass ``q_r``
+    outside of them.  (No factor ``temperature**2``.)
+
+    Args:
+        e: hidden states ``[..., D]`` (float32, float16 or bfloat16)
+        c: classifier weights ``[V, D]`` in e's dtype
+        teacher_ids: token ids ``[..., K]`` (int32 or int64, K <= 1024), in any order;
+            ids outside of ``[0, V)`` are absent entries (padding), entries of the
+            same id add their probabilities
+        teacher_logprobs: ``[..., K]`` log-probabilities or logits; p is their softmax
+            over the K entries at the temperature.  With ``tail``: log-probabilities
+            over the whole vocabulary at the temperature, used as they are
+        bias: optional classifier bias ``[V]``
+        mask: bool ``[...]``; False leaves a row out
+        reduction: "mean" over the rows that have an entry, "sum" or "none"
+    Returns:
+        float32 loss (scalar, or the rows' shape for reduction="none"), differentiable
+        with respect to e, c and bias.
+    """
+    what = "linear_distillation_loss"
+    params = _distill_params(what, temperature, tail, reduction)
+    if teacher_ids.dim() < 1 or teacher_ids.shape != teacher_logprobs.shape:
+        raise ValueError(f"[{what}] teacher_ids and teacher_logprobs must be [..., K] of one shape, got "
+                         f"{tuple(teacher_ids.shape)} and {tuple(teacher_logprobs.shape)}")
+    rows, K = teacher_ids.shape[:-1], teacher_ids.shape[-1]
+    if not 1 <= K <= _ext.CCE_DISTILL_MAX_K:
+        raise ValueError(f"[{what}] K must be in [1, {_ext.CCE_DISTILL_MAX_K}], got {K}")
+    e2, c, bias = _head(what, e, c, bias, rows)
+    ids = _ids(what, "teacher_ids", teacher_ids, e.device).view(-1, K)
+    if not teacher_logprobs.is_floating_point() or teacher_logprobs.device != e.device:
+        raise ValueError(f"[{what}] teacher_logprobs must be floating point on {e.device}")
+    teacher = teacher_logprobs.detach().to(torch.float32).contiguous()
+    loss = DistillationFunction.apply(e2, c, bias, ids, teacher, _mask(what, mask, rows, e.device), params)
+    return loss.view(rows) if reduction == "none" else loss
