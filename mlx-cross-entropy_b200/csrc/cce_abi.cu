@@ -744,8 +744,9 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
   }
   if (p.tc) CCE_CUDA_CHECK(cudaMemsetAsync(counters, 0, p.counter_bytes, s), "cce_backward memset counters");
   if (keep_t) CCE_CUDA_CHECK(cudaMemsetAsync(keep_t, 0, p.keep_t_bytes, s), "cce_backward memset mask table");
-  // (a distillation's dlogits are at most the cotangent in magnitude, so its power of two fits them)
-  if (scale) CCE_CUDA_CHECK(cce::launch_pow2_absmax(rb ? rb->d : d_nll, N, scale, s), "cce_backward scale");
+  // (dlogits are at most the cotangent in magnitude.  Exact gradients put the
+  // largest at 2^14 of fp16's 65504: a softmax value of 2^-28 is still a normal number)
+  if (scale) CCE_CUDA_CHECK(cce::launch_pow2_absmax(rb ? rb->d : d_nll, N, scale, rb ? 14 : 0, s), "cce_backward scale");
 
   if (rb)
     CCE_CUDA_CHECK(cce::launch_live_mask(rb->d, N, V, keep, keep_t, p.keep_t_ld, s), "cce_backward mask");

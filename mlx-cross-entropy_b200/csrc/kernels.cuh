@@ -110,8 +110,8 @@ cudaError_t launch_dequantize(const uint32_t* wq, const void* scales, const void
                               cudaStream_t stream);
 // dst[i] = a[i] + b[i], written in dtype (CCE_F32 / F16 / BF16)
 cudaError_t launch_sum2_f32(const float* a, const float* b, void* dst, int dtype, int64_t n, cudaStream_t stream);
-// out[0] = s = the power of two >= max |x| (1 if all zero), out[1] = 1 / s
-cudaError_t launch_pow2_absmax(const float* x, int64_t n, float* out, cudaStream_t stream);
+// out[0] = s = 2^-up times the power of two >= max |x| (1 if all zero), out[1] = 1 / s
+cudaError_t launch_pow2_absmax(const float* x, int64_t n, float* out, int up, cudaStream_t stream);
 cudaError_t launch_fill_f32(float* dst, float v, int64_t n, cudaStream_t stream);
 
 // ---- rows of a batch, distillation (rows_kernels.cu) ----

@@ -565,80 +565,94 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def on_device(dev):
-    """Context in which a library call for tensors on ``dev`` is made."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def _pad(n):
+    """Bytes up to the next multiple of 256."""
+    return (n + 255) & -256
 
 
+# The raw handle of a device's current stream, without a Stream object around it
+# (a few microseconds of a call whose kernels take less).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on_its_device(call):
+    """Runs a call of this module, whose first argument is a CUDA tensor, with that tensor's device current."""
+    def wrapped(t, *args):
+        if t.device.index == torch.cuda.current_device():
+            return call(t, *args)
+        with torch.cuda.device(t.device):
+            return call(t, *args)
+    return wrapped
+
+
+@_on_its_device
 def policy_forward(logp, old, ref, adv, mask, cu, S, params):
     """``cce_policy_loss_forward`` on checked contiguous tensors.
 
-    Returns (loss, stats [2], coef [N + 1 + S]: per-token coefficients, then weights).
+    Returns (loss, stats [2], state): state holds the per-token coefficients and
+    the weights for ``policy_backward``, and behind them the call's workspace.
     """
     dev, N = logp.device, logp.numel()
-    with on_device(dev):
-        f32 = dict(dtype=torch.float32, device=dev)
-        none = params.reduction == CCE_REDUCE_NONE
-        loss = torch.empty(logp.shape if none else (), **f32)
-        stats = torch.empty((2,), **f32)
-        off = (N + 3) // 4 * 4
-        coef = torch.empty((off + 1 + S,), **f32)
-        ws_bytes = lib.cce_token_loss_workspace_bytes(N, S)
-        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
-        c = coef.data_ptr()
-        rc = lib.cce_policy_loss_forward(_addr(logp), _addr(old), _addr(ref), _DTYPE_CODE[logp.dtype], _addr(adv),
-                                         _addr(mask), _addr(cu), N, S, params, loss.data_ptr(), stats.data_ptr(), c,
-                                         c + 4 * off, ws.data_ptr(), ws_bytes,
-                                         torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_policy_loss_forward")
-    return loss, stats, coef
+    loss = torch.empty(logp.shape if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
+    stats = torch.empty((2,), dtype=torch.float32, device=dev)
+    at_weight = _pad(4 * N)
+    at_ws = at_weight + _pad(4 * (1 + S))
+    ws_bytes = lib.cce_token_loss_workspace_bytes(N, S)
+    state = torch.empty((at_ws + ws_bytes,), dtype=torch.uint8, device=dev)
+    p = state.data_ptr()
+    rc = lib.cce_policy_loss_forward(logp.data_ptr(), _addr(old), _addr(ref), _DTYPE_CODE[logp.dtype], adv.data_ptr(),
+                                     _addr(mask), _addr(cu), N, S, params, loss.data_ptr(), stats.data_ptr(), p,
+                                     p + at_weight, p + at_ws, ws_bytes, _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_policy_loss_forward")
+    return loss, stats, state
 
 
-def policy_backward(coef, grad_loss, reduction, cu, N, S, shape, dtype):
+@_on_its_device
+def policy_backward(state, grad_loss, reduction, cu, N, S, shape, dtype):
     """``cce_policy_loss_backward``: the gradient with respect to logp."""
-    dev = coef.device
-    with on_device(dev):
-        grad = torch.empty(shape, dtype=dtype, device=dev)
-        c = coef.data_ptr()
-        rc = lib.cce_policy_loss_backward(c, c + 4 * ((N + 3) // 4 * 4), grad_loss.data_ptr(), reduction, _addr(cu), N,
-                                          S, _DTYPE_CODE[dtype], grad.data_ptr(),
-                                          torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_policy_loss_backward")
+    dev = state.device
+    grad = torch.empty(shape, dtype=dtype, device=dev)
+    p = state.data_ptr()
+    rc = lib.cce_policy_loss_backward(p, p + _pad(4 * N), grad_loss.data_ptr(), reduction, _addr(cu), N, S,
+                                      _DTYPE_CODE[dtype], grad.data_ptr(), _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_policy_loss_backward")
     return grad
 
 
+@_on_its_device
 def preference_forward(logp, ref, ref_sums, mask, cu, pairs, params):
     """``cce_preference_loss_forward`` on checked contiguous tensors.
 
-    Returns (loss, rewards [2 pairs], coef [2 pairs]).
+    Returns (loss, rewards [2 pairs], state): state holds the per-sequence
+    coefficients for ``preference_backward``, and behind them the call's workspace.
     """
     dev, N = logp.device, logp.numel()
-    with on_device(dev):
-        f32 = dict(dtype=torch.float32, device=dev)
-        loss = torch.empty((pairs,) if params.reduction == CCE_REDUCE_NONE else (), **f32)
-        rewards = torch.empty((2 * pairs,), **f32)
-        coef = torch.empty((2 * pairs,), **f32)
-        ws_bytes = lib.cce_token_loss_workspace_bytes(N, 2 * pairs)
-        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
-        rc = lib.cce_preference_loss_forward(_addr(logp), _addr(ref), _DTYPE_CODE[logp.dtype], _addr(ref_sums),
-                                             _addr(mask), _addr(cu), N, pairs, params, loss.data_ptr(),
-                                             rewards.data_ptr(), coef.data_ptr(), ws.data_ptr(), ws_bytes,
-                                             torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_preference_loss_forward")
-    return loss, rewards, coef
+    loss = torch.empty((pairs,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
+    rewards = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
+    at_ws = _pad(8 * pairs)
+    ws_bytes = lib.cce_token_loss_workspace_bytes(N, 2 * pairs)
+    state = torch.empty((at_ws + ws_bytes,), dtype=torch.uint8, device=dev)
+    p = state.data_ptr()
+    rc = lib.cce_preference_loss_forward(logp.data_ptr(), _addr(ref), _DTYPE_CODE[logp.dtype], _addr(ref_sums),
+                                         _addr(mask), _addr(cu), N, pairs, params, loss.data_ptr(),
+                                         rewards.data_ptr(), p, p + at_ws, ws_bytes, _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_preference_loss_forward")
+    return loss, rewards, state
 
 
-def preference_backward(coef, grad_loss, reduction, mask, cu, N, pairs, shape, dtype):
+@_on_its_device
+def preference_backward(state, grad_loss, reduction, mask, cu, N, pairs, shape, dtype):
     """``cce_preference_loss_backward``: the gradient with respect to logp."""
-    dev = coef.device
-    with on_device(dev):
-        grad = torch.empty(shape, dtype=dtype, device=dev)
-        rc = lib.cce_preference_loss_backward(coef.data_ptr(), grad_loss.data_ptr(), reduction, _addr(mask), _addr(cu),
-                                              N, pairs, _DTYPE_CODE[dtype], grad.data_ptr(),
-                                              torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_preference_loss_backward")
+    dev = state.device
+    grad = torch.empty(shape, dtype=dtype, device=dev)
+    rc = lib.cce_preference_loss_backward(state.data_ptr(), grad_loss.data_ptr(), reduction, _addr(mask), _addr(cu), N,
+                                          pairs, _DTYPE_CODE[dtype], grad.data_ptr(), _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_preference_loss_backward")
     return grad
 
 
@@ -650,20 +664,21 @@ def _bytes(n, dev):
     return torch.empty((max(n, 1),), dtype=torch.uint8, device=dev)
 
 
+@_on_its_device
 def logp_forward(e, c, bias, targets, ignore_index):
     """``cce_logp_forward`` on checked contiguous tensors: (logp [N], mask [N], saved)."""
     dev, (N, D), V, dt = e.device, e.shape, c.shape[0], _DTYPE_CODE[e.dtype]
-    with on_device(dev):
-        logp = torch.empty((N,), dtype=torch.float32, device=dev)
-        mask = torch.empty((N,), dtype=torch.bool, device=dev)
-        saved = _bytes(lib.cce_logp_saved_bytes(N, D, V, dt), dev)
-        ws = _bytes(lib.cce_logp_forward_workspace_bytes(N, V), dev)
-        rc = lib.cce_logp_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), targets.data_ptr(),
-                                  targets.element_size(), 0 if ignore_index is None else ignore_index,
-                                  ignore_index is not None, N, D, V, dt, logp.data_ptr(), mask.data_ptr(),
-                                  saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
-                                  torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_logp_forward")
+    logp = torch.empty((N,), dtype=torch.float32, device=dev)
+    mask = torch.empty((N,), dtype=torch.bool, device=dev)
+    saved = _bytes(lib.cce_logp_saved_bytes(N, D, V, dt), dev)
+    ws = _bytes(lib.cce_logp_forward_workspace_bytes(N, V), dev)
+    rc = lib.cce_logp_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), targets.data_ptr(),
+                              targets.element_size(), 0 if ignore_index is None else ignore_index,
+                              ignore_index is not None, N, D, V, dt, logp.data_ptr(), mask.data_ptr(),
+                              saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
+                              _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_logp_forward")
     return logp, mask, saved
 
 
@@ -677,44 +692,47 @@ def _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias):
     return ge, gc, gb, flags
 
 
+@_on_its_device
 def logp_backward(saved, c, bias, grad_logp, N, dtype, need_e, need_c, need_bias):
     """``cce_logp_backward``: (grad_e, grad_c, grad_bias fp32); absent ones are None."""
     dev, (V, D), dt = c.device, c.shape, _DTYPE_CODE[dtype]
-    with on_device(dev):
-        ge, gc, gb, flags = _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias)
-        ws = _bytes(lib.cce_logp_backward_workspace_bytes(N, D, V, dt, flags), dev)
-        rc = lib.cce_logp_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_logp.data_ptr(), N, D, V, dt,
-                                   flags, saved.data_ptr(), saved.numel(), _addr(ge), _addr(gc), _addr(gb),
-                                   ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_logp_backward")
+    ge, gc, gb, flags = _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias)
+    ws = _bytes(lib.cce_logp_backward_workspace_bytes(N, D, V, dt, flags), dev)
+    rc = lib.cce_logp_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_logp.data_ptr(), N, D, V, dt,
+                               flags, saved.data_ptr(), saved.numel(), _addr(ge), _addr(gc), _addr(gb),
+                               ws.data_ptr(), ws.numel(), _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_logp_backward")
     return ge, gc, gb
 
 
+@_on_its_device
 def distill_forward(e, c, bias, ids, teacher, mask, params):
     """``cce_distill_forward`` on checked contiguous tensors: (loss, saved)."""
     dev, (N, D), V, K, dt = e.device, e.shape, c.shape[0], ids.shape[1], _DTYPE_CODE[e.dtype]
-    with on_device(dev):
-        loss = torch.empty((N,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-        saved = _bytes(lib.cce_distill_saved_bytes(N, D, V, K, dt), dev)
-        ws = _bytes(lib.cce_distill_forward_workspace_bytes(N, V, K), dev)
-        rc = lib.cce_distill_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), ids.data_ptr(),
-                                     ids.element_size(), teacher.data_ptr(), _addr(mask), N, D, V, K, dt, params,
-                                     loss.data_ptr(), saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
-                                     torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_distill_forward")
+    loss = torch.empty((N,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
+    saved = _bytes(lib.cce_distill_saved_bytes(N, D, V, K, dt), dev)
+    ws = _bytes(lib.cce_distill_forward_workspace_bytes(N, V, K), dev)
+    rc = lib.cce_distill_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), ids.data_ptr(),
+                                 ids.element_size(), teacher.data_ptr(), _addr(mask), N, D, V, K, dt, params,
+                                 loss.data_ptr(), saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
+                                 _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_distill_forward")
     return loss, saved
 
 
+@_on_its_device
 def distill_backward(saved, c, bias, grad_loss, N, K, dtype, params, need_e, need_c, need_bias):
     """``cce_distill_backward``: (grad_e, grad_c, grad_bias fp32); absent ones are None."""
     dev, (V, D), dt = c.device, c.shape, _DTYPE_CODE[dtype]
-    with on_device(dev):
-        ge, gc, gb, flags = _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias)
-        ws = _bytes(lib.cce_distill_backward_workspace_bytes(N, D, V, dt, flags), dev)
-        rc = lib.cce_distill_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_loss.data_ptr(), N, D, V, K,
-                                      dt, params, flags, saved.data_ptr(), saved.numel(), _addr(ge), _addr(gc),
-                                      _addr(gb), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
-    _check(rc, "cce_distill_backward")
+    ge, gc, gb, flags = _rows_grads(c, bias, N, dtype, need_e, need_c, need_bias)
+    ws = _bytes(lib.cce_distill_backward_workspace_bytes(N, D, V, dt, flags), dev)
+    rc = lib.cce_distill_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_loss.data_ptr(), N, D, V, K,
+                                  dt, params, flags, saved.data_ptr(), saved.numel(), _addr(ge), _addr(gc),
+                                  _addr(gb), ws.data_ptr(), ws.numel(), _raw_stream(dev.index))
+    if rc:
+        _check(rc, "cce_distill_backward")
     return ge, gc, gb
 
 

@@ -55,6 +55,13 @@ class PreferenceRewards(NamedTuple):
 # argument checks
 # ---------------------------------------------------------------------------
 
+def _constant(t):
+    """t as a kernel input: contiguous, cut from the graph."""
+    if t.requires_grad:
+        t = t.detach()
+    return t.contiguous()
+
+
 def _offsets(what, cu_seqlens, dev):
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError(f"[{what}] cu_seqlens must be 1D with S + 1 offsets, got {tuple(cu_seqlens.shape)}")
@@ -89,7 +96,7 @@ def _like(what, name, t, logp):
         raise ValueError(f"[{what}] {name} must have logp's dtype {logp.dtype}, got {t.dtype}")
     if t.device != logp.device:
         raise ValueError(f"[{what}] {name} is on {t.device}, expected {logp.device}")
-    return t.detach().contiguous()
+    return _constant(t)
 
 
 def _mask(what, mask, shape, dev):
@@ -137,7 +144,7 @@ def _advantages(what, advantages, shape, S, dev):
         raise ValueError(f"[{what}] advantages must be floating point, got {advantages.dtype}")
     if advantages.device != dev:
         raise ValueError(f"[{what}] advantages are on {advantages.device}, expected {dev}")
-    return advantages.detach().to(torch.float32).contiguous(), per_token
+    return _constant(advantages.to(torch.float32)), per_token
 
 
 def _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction):
@@ -221,53 +228,64 @@ def _reference(what, ref_logp, logp, S):
                          f"got {tuple(ref_logp.shape)}")
     if not ref_logp.is_floating_point() or ref_logp.device != logp.device:
         raise ValueError(f"[{what}] ref_logp must be floating point on {logp.device}")
-    return None, ref_logp.detach().to(torch.float32).contiguous()
+    return None, _constant(ref_logp.to(torch.float32))
 
 
 # ---------------------------------------------------------------------------
 # autograd
 # ---------------------------------------------------------------------------
 
+def _first_order(backward):
+    """once_differentiable (a second derivative is an error, not a wrong zero), which
+    only costs its wrapping where a graph of the backward pass is recorded."""
+    recorded = once_differentiable(backward)
+
+    def wrapped(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return wrapped
+
+
 class PolicyLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, old, ref, adv, mask, cu, S, params):
-        loss, stats, coef = _ext.policy_forward(logp, old, ref, adv, mask, cu, S, params)
-        ctx.save_for_backward(coef, cu)
+        loss, stats, state = _ext.policy_forward(logp, old, ref, adv, mask, cu, S, params)
+        ctx.save_for_backward(state, cu)
         ctx.meta = (params.reduction, logp.numel(), S, logp.shape, logp.dtype)
         ctx.mark_non_differentiable(stats)
         ctx.set_materialize_grads(False)
         return loss, stats
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad_loss, _grad_stats):
         if grad_loss is None:
             return (None,) * 8
-        coef, cu = ctx.saved_tensors
+        state, cu = ctx.saved_tensors
         reduction, N, S, shape, dtype = ctx.meta
         g = grad_loss.to(torch.float32).contiguous()
-        return (_ext.policy_backward(coef, g, reduction, cu, N, S, shape, dtype),) + (None,) * 7
+        return (_ext.policy_backward(state, g, reduction, cu, N, S, shape, dtype),) + (None,) * 7
 
 
 class PreferenceLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logp, ref, ref_sums, mask, cu, pairs, params):
-        loss, rewards, coef = _ext.preference_forward(logp, ref, ref_sums, mask, cu, pairs, params)
-        ctx.save_for_backward(coef, mask, cu)
+        loss, rewards, state = _ext.preference_forward(logp, ref, ref_sums, mask, cu, pairs, params)
+        ctx.save_for_backward(state, mask, cu)
         ctx.meta = (params.reduction, logp.numel(), pairs, logp.shape, logp.dtype)
         ctx.mark_non_differentiable(rewards)
         ctx.set_materialize_grads(False)
         return loss, rewards
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad_loss, _grad_rewards):
         if grad_loss is None:
             return (None,) * 7
-        coef, mask, cu = ctx.saved_tensors
+        state, mask, cu = ctx.saved_tensors
         reduction, N, pairs, shape, dtype = ctx.meta
         g = grad_loss.to(torch.float32).contiguous()
-        return (_ext.preference_backward(coef, g, reduction, mask, cu, N, pairs, shape, dtype),) + (None,) * 6
+        return (_ext.preference_backward(state, g, reduction, mask, cu, N, pairs, shape, dtype),) + (None,) * 6
 
 
 class LogProbsFunction(torch.autograd.Function):
@@ -281,7 +299,7 @@ class LogProbsFunction(torch.autograd.Function):
         return logp, mask
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad_logp, _grad_mask):
         need = ctx.needs_input_grad
         if grad_logp is None or not any(need[:3]):
@@ -300,7 +318,7 @@ class DistillationFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad_loss):
         need = ctx.needs_input_grad
         if not any(need[:3]):
@@ -492,6 +510,6 @@ def linear_distillation_loss(e, c, teacher_ids, teacher_logprobs, bias=None, *, 
     ids = _ids(what, "teacher_ids", teacher_ids, e.device).view(-1, K)
     if not teacher_logprobs.is_floating_point() or teacher_logprobs.device != e.device:
         raise ValueError(f"[{what}] teacher_logprobs must be floating point on {e.device}")
-    teacher = teacher_logprobs.detach().to(torch.float32).contiguous()
+    teacher = _constant(teacher_logprobs.to(torch.float32))
     loss = DistillationFunction.apply(e2, c, bias, ids, teacher, _mask(what, mask, rows, e.device), params)
     return loss.view(rows) if reduction == "none" else loss
