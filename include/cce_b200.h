@@ -428,7 +428,7 @@ CCE_API int cce_preference_loss_backward(const float* coef, const float* grad_lo
  * --------------------------------------------------------------------------- */
 
 CCE_API size_t cce_logp_saved_bytes(int64_t N, int64_t D, int64_t V, int dtype);
-CCE_API size_t cce_logp_forward_workspace_bytes(int64_t N, int64_t V);
+CCE_API size_t cce_logp_forward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype);
 CCE_API size_t cce_logp_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags);
 
 /*
@@ -459,7 +459,7 @@ typedef struct CceDistillParams {
 } CceDistillParams;
 
 CCE_API size_t cce_distill_saved_bytes(int64_t N, int64_t D, int64_t V, int64_t K, int dtype);
-CCE_API size_t cce_distill_forward_workspace_bytes(int64_t N, int64_t V, int64_t K);
+CCE_API size_t cce_distill_forward_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t K, int dtype);
 CCE_API size_t cce_distill_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags);
 
 /*

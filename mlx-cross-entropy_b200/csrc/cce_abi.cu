@@ -135,6 +135,7 @@ struct BwdPlan {
   int splits;            // CUDA-core path: K splits of grad_e (partials part_bytes)
   size_t part_bytes;
   size_t list_bytes;     // tensor-core path: the dlogits live-tile lists of every chunk
+  int slabs;             // tensor-core path: K splits of grad_e
 };
 
 bool tc_candidate(int dtype, int64_t D) { return dtype != CCE_F32 && D % 8 == 0; }
@@ -160,7 +161,21 @@ bool dl_list_enabled() {
   return v;
 }
 
-BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool tc) {
+// K splits (fp32 slabs) of the tensor-core grad_e: two with the filter.  Exact
+// gradients of a few packed rows take as many as give every SM a work unit
+// (128 rows x 512 columns x a K range of at least 1024) within 64 MiB of slabs:
+// 331 x 1024 x 32000 has 6 such tiles, and its grad_e took 200 us in 12 units.
+int rows_slabs(int64_t N, int64_t D, int64_t vc) {
+  const int64_t tiles = cce::ceil_div(N > 0 ? N : 1, 128) * cce::ceil_div(D, 512);
+  int64_t s = cce::ceil_div(148, tiles);
+  const int64_t fit = (64ll << 20) / ((N > 0 ? N : 1) * D * 4);
+  if (s > fit) s = fit;
+  if (s > vc / 1024) s = vc / 1024;
+  if (s > 32) s = 32;
+  return s < 2 ? 2 : (int)s;
+}
+
+BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool tc, bool rows = false) {
   BwdPlan p{};
   p.tc = tc;
   const int64_t gran = tc ? 256 : 128;
@@ -184,6 +199,7 @@ BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, boo
   const int64_t vmax = cce::round_up(V > 0 ? V : 1, gran);
   if (vc > vmax) vc = vmax;
   p.vc = vc;
+  p.slabs = rows ? rows_slabs(N, D, vc) : 2;
   p.keep_bytes = align_up((size_t)cce::ceil_div(N, cce::kRowBlock) * (size_t)cce::ceil_div(V, cce::kStatTile));
   // grad_c's view of the mask: per 128-column tile a bit per row block
   p.keep_t_ld = tc ? cce::ceil_div(cce::ceil_div(N, cce::kRowBlock), 32) : 0;
@@ -193,13 +209,13 @@ BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, boo
   // (the two K halves of every chunk's grad_e GEMM), summed into grad_e at the
   // end; the SIMT path one [N][D] (none when grad_e itself is fp32).
   if (!(flags & CCE_NEED_DE)) p.acc_bytes = 0;
-  else if (tc) p.acc_bytes = align_up(2 * (size_t)N * (size_t)D * 4);
+  else if (tc) p.acc_bytes = align_up((size_t)p.slabs * (size_t)N * (size_t)D * 4);
   else p.acc_bytes = (flags & CCE_DE_F32) ? 0 : align_up((size_t)N * (size_t)D * 4);
   // four counters per vocabulary chunk: the tile claims of the three
   // dynamically scheduled kernels and the dlogits live-tile count
   const int64_t nch = cce::ceil_div(V > 0 ? V : 1, vc);
   p.counter_bytes = align_up((size_t)nch * 4 * sizeof(int));
-  p.list_bytes = (tc && dl_list_enabled()) ? align_up((size_t)nch * (size_t)cce::tc_dlogits_list_len(nrow, vc) * sizeof(int)) : 0;
+  p.list_bytes = (tc && !rows && dl_list_enabled()) ? align_up((size_t)nch * (size_t)cce::tc_dlogits_list_len(nrow, vc) * sizeof(int)) : 0;
   p.scale_bytes = (tc && dtype == CCE_F16) ? kAlign : 0;  // {s, 1/s} for fp16 dlogits
   p.splits = (!tc && (flags & CCE_NEED_DE)) ? cce::simt_grad_e_splits(N, D, vc) : 1;
   p.part_bytes = p.splits > 1 ? align_up((size_t)p.splits * (size_t)N * (size_t)D * 4) : 0;
@@ -489,11 +505,11 @@ static size_t chunk_buf_bytes(const BwdPlan& p, int64_t D, int dtype) {
   return align_up((size_t)p.vc * (size_t)D * dtype_size(dtype));
 }
 
-static size_t backward_ws_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool quant) {
+static size_t backward_ws_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool quant, bool rows = false) {
   const BwdPlan ps = plan_backward(N, D, V, dtype, flags, false);
   size_t b = plan_bytes(ps) + (quant ? 2 * chunk_buf_bytes(ps, D, dtype) : 0);
   if (tc_candidate(dtype, D)) {
-    const BwdPlan pt = plan_backward(N, D, V, dtype, flags, true);
+    const BwdPlan pt = plan_backward(N, D, V, dtype, flags, true, rows);
     const size_t t = plan_bytes(pt) + (quant ? 2 * chunk_buf_bytes(pt, D, dtype) : 0);
     if (t > b) b = t;
   }
@@ -698,8 +714,8 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
   // (a quantised head's chunks live in the workspace: its alignment stands for c's)
   const bool tc = !force_simt() && cce::tc_backward_supported(e, qh ? workspace : c, D, dtype) &&
                   aligned16(workspace) && (!need_de || aligned16(grad_e)) && (!need_dc || aligned16(grad_c));
-  const BwdPlan p = plan_backward(N, D, V, dtype, flags, tc);
-  const size_t need = backward_ws_bytes(N, D, V, dtype, flags, qh != nullptr);
+  const BwdPlan p = plan_backward(N, D, V, dtype, flags, tc, rb != nullptr);
+  const size_t need = backward_ws_bytes(N, D, V, dtype, flags, qh != nullptr, rb != nullptr);
   if (!workspace || workspace_bytes < need)
     return fail(CCE_ERR_WORKSPACE, "cce_backward: workspace %zu bytes < required %zu", workspace_bytes, need);
 
@@ -764,6 +780,8 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
     a.topk = rb->topk;
     a.d_row = rb->d;
     a.logit_scale = rb->logit_scale;
+    a.rows = rb->R.count;
+    a.slabs = p.slabs;
     if (need_db && p.tc) a.bias_part = rb->bias_part;
   }
   const int64_t bias_parts = p.tc ? cce::ceil_div(N, 32) : N;  // (CUDA cores: the fp32 dlogits themselves)
@@ -816,7 +834,7 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
     if (p.tc) {
       if (a.bias_part)
         CCE_CUDA_CHECK(cudaMemsetAsync(a.bias_part, 0, (size_t)bias_parts * p.vc * sizeof(float), s), "cce_backward memset");
-      CCE_CUDA_CHECK(cce::tc_dlogits(a, s), "cce_backward tc dlogits");
+      CCE_CUDA_CHECK(rb ? cce::tc_dlogits_rows(a, s) : cce::tc_dlogits(a, s), "cce_backward tc dlogits");
       if (a.bias_part)
         CCE_CUDA_CHECK(cce::launch_bias_sum(a.bias_part, bias_parts, p.vc, a.vc_len, scale, grad_bias + a.vc0, s),
                        "cce_backward grad_bias");
@@ -831,7 +849,7 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
                                                          out_dtype, grad_e, wait_ns, ss->se),
                          "cce_backward_peer exchange");
         else if (last && rb)
-          CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, acc + N * D, rb->R.pos, N, D, out_dtype, grad_e, ss->se),
+          CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, p.slabs, rb->R.pos, N, D, out_dtype, grad_e, ss->se),
                          "cce_backward scatter grad_e");
         else if (last)
           CCE_CUDA_CHECK(cce::launch_sum2_f32(acc, acc + N * D, grad_e, out_dtype, N * D, ss->se),
@@ -856,7 +874,7 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
         CCE_CUDA_CHECK(cce::peer::launch_reduce_gather(push.peers, push.layout, 1, N, D, out_dtype, grad_e, wait_ns, s),
                        "cce_backward_peer exchange");
       } else if (need_de && last && rb) {
-        CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, nullptr, rb->R.pos, N, D, out_dtype, grad_e, s),
+        CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, 1, rb->R.pos, N, D, out_dtype, grad_e, s),
                        "cce_backward scatter grad_e");
       } else if (need_de && last && !(flags & CCE_DE_F32)) {
         CCE_CUDA_CHECK(cce::launch_cast_f32(acc, grad_e, dtype, N * D, s), "cce_backward cast grad_e");
@@ -1169,8 +1187,13 @@ struct RowsSaved {
   float* weight;    // distillation [1]
   cce::TopkView topk;
   void* e;          // packed rows
+  cce::SplitView split;  // or their two parts (float32 on tensor cores)
   size_t bytes;
 };
+
+// float32 rows run on the tensor cores as two float16 parts (rows of the outputs
+// must start on 16-byte boundaries); others on the CUDA cores.
+bool split_path(int64_t D, int dtype) { return dtype == CCE_F32 && D % 4 == 0 && !force_simt() && cce::tc_available(); }
 
 RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
   Parts p{static_cast<char*>(base)};
@@ -1189,18 +1212,60 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
     r.topk.start = p.take<uint16_t>((size_t)N * r.topk.tiles1);
     r.topk.z = p.take<float>((size_t)N * K);
   }
-  r.e = p.take<char>((size_t)N * D * dtype_size(dtype));
+  if (split_path(D, dtype)) {
+    r.split.Dp = cce::round_up(D, 64);
+    float* se = p.take<float>(2);
+    r.split.se = se;
+    r.split.e_hi = p.take<uint16_t>((size_t)N * r.split.Dp);
+    r.split.e_lo = p.take<uint16_t>((size_t)N * r.split.Dp);
+  } else {
+    r.e = p.take<char>((size_t)N * D * dtype_size(dtype));
+  }
   r.bytes = p.used;
   return r;
+}
+
+// c's two parts, its scale, and the words the largest values go to.
+struct SplitWs {
+  void *c_hi, *c_lo;
+  float* sc;
+  uint32_t* words;
+};
+
+SplitWs split_ws(Parts& p, int64_t D, int64_t V, int dtype) {
+  SplitWs w{};
+  if (!split_path(D, dtype)) return w;
+  w.words = p.take<uint32_t>(2);
+  w.sc = p.take<float>(2);
+  w.c_hi = p.take<uint16_t>((size_t)V * cce::round_up(D, 64));
+  w.c_lo = p.take<uint16_t>((size_t)V * cce::round_up(D, 64));
+  return w;
+}
+
+// c into its parts (`v` gets them); with e != nullptr its packed rows into the saved ones too.
+cudaError_t split_operands(RowsSaved& v, const SplitWs& w, const void* e, const void* c, int64_t N, int64_t D,
+                           int64_t V, cudaStream_t s) {
+  v.split.c_hi = w.c_hi, v.split.c_lo = w.c_lo, v.split.sc = w.sc;
+  cudaError_t err = cudaMemsetAsync(w.words, 0, 2 * sizeof(uint32_t), s);
+  if (err != cudaSuccess) return err;
+  if (e) {
+    if ((err = cce::launch_absmax((const float*)e, N, D, &v.R, w.words + 1, s)) != cudaSuccess) return err;
+    if ((err = cce::launch_split((const float*)e, N, D, v.split.Dp, &v.R, w.words + 1, const_cast<float*>(v.split.se),
+                                 const_cast<void*>(v.split.e_hi), const_cast<void*>(v.split.e_lo), s)) != cudaSuccess)
+      return err;
+  }
+  if ((err = cce::launch_absmax((const float*)c, V, D, nullptr, w.words, s)) != cudaSuccess) return err;
+  return cce::launch_split((const float*)c, V, D, v.split.Dp, nullptr, w.words, w.sc, w.c_hi, w.c_lo, s);
 }
 
 struct RowsFwdWs {
   float *part_m, *part_s, *tgt, *p, *rest;
   cce::DistillSum* sums;
+  SplitWs split;
   size_t bytes;
 };
 
-RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t V, int64_t K) {
+RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
   Parts p{static_cast<char*>(base)};
   RowsFwdWs w{};
   const size_t parts = (size_t)cce::ceil_div(V, cce::kSimtLseTile) * N;
@@ -1213,28 +1278,119 @@ RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t V, int64_t K) {
     w.rest = p.take<float>(N);
     w.sums = p.take<cce::DistillSum>(cce::distill_blocks(N));
   }
+  w.split = split_ws(p, D, V, dtype);
   w.bytes = p.used;
   return w;
+}
+
+// Chunks and buffers of the float32 backward pass on tensor cores.
+struct SplitPlan {
+  int64_t vc;  // vocabulary rows of a chunk (both parts of its dlogits: 4 N vc bytes)
+  int slabs;   // K splits of grad_e
+};
+
+SplitPlan split_plan(int64_t N, int64_t D, int64_t V) {
+  const int64_t n = N > 0 ? N : 1;
+  const int64_t target = target_chunk_rows();
+  int64_t budget = n * 4 * target;
+  if (budget > kDlMaxBytes) budget = kDlMaxBytes;
+  if (budget < kDlMinBytes && target == kDlTargetRows) budget = kDlMinBytes;
+  SplitPlan p;
+  p.vc = budget / (n * 4) / 256 * 256;
+  if (p.vc < 256) p.vc = 256;
+  const int64_t vmax = cce::round_up(V, 256);
+  if (p.vc > vmax) p.vc = vmax;
+  // two units per SM of (128 rows, 256 columns, at least 512 of K), within 256 MiB of slabs
+  const int64_t tiles = cce::ceil_div(n, 128) * cce::ceil_div(D, 256);
+  int64_t sl = cce::ceil_div(2 * 148, tiles);
+  const int64_t fit = (256ll << 20) / (n * D * 4);
+  if (sl > fit) sl = fit;
+  if (sl > p.vc / 512) sl = p.vc / 512;
+  if (sl > 32) sl = 32;
+  p.slabs = sl < 1 ? 1 : (int)sl;
+  return p;
 }
 
 struct RowsBwdWs {
   void* base;  // backward_impl's own
   size_t base_bytes;
   float *d, *dA, *bias_part;
+  SplitWs split;
+  void *dl_hi, *dl_lo;
+  float *slabs, *scale;
   size_t bytes;
 };
 
 RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, int flags, bool topk) {
   Parts p{static_cast<char*>(base)};
   RowsBwdWs w{};
-  w.base_bytes = backward_ws_bytes(N, D, V, dtype, flags, false);
-  w.base = p.take<char>(w.base_bytes);
+  int64_t vc = 0;
+  if (split_path(D, dtype)) {
+    const SplitPlan sp = split_plan(N, D, V);
+    vc = sp.vc;
+    w.split = split_ws(p, D, V, dtype);
+    w.dl_hi = p.take<uint16_t>((size_t)N * vc);
+    w.dl_lo = p.take<uint16_t>((size_t)N * vc);
+    if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)sp.slabs * N * D);
+    w.scale = p.take<float>(2);
+  } else {
+    w.base_bytes = backward_ws_bytes(N, D, V, dtype, flags, false, true);
+    w.base = p.take<char>(w.base_bytes);
+    if (tc_candidate(dtype, D)) vc = plan_backward(N, D, V, dtype, flags, true, true).vc;
+  }
   w.d = p.take<float>(N);
   if (topk) w.dA = p.take<float>(N);
-  if ((flags & CCE_NEED_DBIAS) && tc_candidate(dtype, D))
-    w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * plan_backward(N, D, V, dtype, flags, true).vc);
+  if ((flags & CCE_NEED_DBIAS) && vc > 0) w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * vc);
   w.bytes = p.used;
   return w;
+}
+
+// Gradients of float32 rows from two-part operands: per vocabulary chunk the
+// dlogits' two parts, then grad_e's K splits into fp32 slabs and grad_c's rows.
+int split_backward(RowsSaved v, const RowsBwdWs& w, const RowsBwd& rb, const void* c, const void* bias, int bias_dtype,
+                   const float* g, int64_t N, int64_t D, int64_t V, int flags, void* grad_e, void* grad_c,
+                   float* grad_bias, cudaStream_t s) {
+  const char* what = "float32 backward";
+  const bool need_de = flags & CCE_NEED_DE, need_dc = flags & CCE_NEED_DC, need_db = flags & CCE_NEED_DBIAS;
+  if ((need_de && !aligned16(grad_e)) || (need_dc && !aligned16(grad_c)))
+    return fail(CCE_ERR_ALIGN, "%s: gradients must start on 16-byte boundaries", what);
+  const SplitPlan sp = split_plan(N, D, V);
+  CCE_CUDA_CHECK(split_operands(v, w.split, nullptr, c, N, D, V, s), what);
+  // the largest cotangent's dlogit at 2^13: hi and lo as in split_operands
+  CCE_CUDA_CHECK(cce::launch_pow2_absmax(rb.d, N, w.scale, 14, s), what);
+  cce::BwdChunkArgs a{};
+  a.bias = bias, a.bias_dtype = bias_dtype;
+  a.targets = v.R.targets, a.lse = v.lse, a.d_nll = g, a.d_row = rb.d;
+  a.N = N, a.D = D, a.V = V, a.dtype = CCE_F32;
+  a.vc_ld = sp.vc, a.dlogits = w.dl_hi, a.dlogits_lo = w.dl_lo, a.scale = w.scale;
+  a.topk = rb.topk, a.logit_scale = rb.logit_scale, a.rows = v.R.count, a.split = v.split;
+  a.bias_part = need_db ? w.bias_part : nullptr;
+  const int64_t parts = cce::ceil_div(N, 32);
+  for (a.vc0 = 0; a.vc0 < V; a.vc0 += sp.vc) {
+    a.vc_len = V - a.vc0 < sp.vc ? V - a.vc0 : sp.vc;
+    if (need_db) CCE_CUDA_CHECK(cudaMemsetAsync(w.bias_part, 0, (size_t)parts * sp.vc * sizeof(float), s), what);
+    CCE_CUDA_CHECK(cce::tc_dlogits_rows(a, s), what);
+    if (need_db)
+      CCE_CUDA_CHECK(cce::launch_bias_sum(w.bias_part, parts, sp.vc, a.vc_len, w.scale, grad_bias + a.vc0, s), what);
+    if (need_de) CCE_CUDA_CHECK(cce::tc_grad_e_split(a, w.slabs, sp.slabs, a.vc0 > 0, s), what);
+    if (need_dc) CCE_CUDA_CHECK(cce::tc_grad_c_split(a, (float*)grad_c, s), what);
+  }
+  if (need_de) CCE_CUDA_CHECK(cce::launch_rows_scatter(w.slabs, sp.slabs, v.R.pos, N, D, CCE_F32, grad_e, s), what);
+  return CCE_OK;
+}
+
+// Argument checks shared by the two backward calls; *done: nothing is left to do.
+int check_rows_backward(const void* bias, int bias_dtype, int64_t N, int64_t V, int64_t D, int dtype, int flags,
+                        const void* grad_e, const void* grad_c, const void* grad_bias, const char* what) {
+  if (flags & ~(CCE_NEED_DE | CCE_NEED_DC | CCE_NEED_DBIAS))
+    return fail(CCE_ERR_ARG, "%s: unknown flag bits 0x%x", what, flags);
+  if (bias && !dtype_ok(bias_dtype)) return fail(CCE_ERR_DTYPE, "%s: unsupported bias dtype code %d", what, bias_dtype);
+  if (((flags & CCE_NEED_DE) && N > 0 && !grad_e) || ((flags & CCE_NEED_DC) && !grad_c) ||
+      ((flags & CCE_NEED_DBIAS) && !grad_bias))
+    return fail(CCE_ERR_ARG, "%s: a requested gradient has a NULL output pointer", what);
+  if ((flags & CCE_NEED_DBIAS) && !bias) return fail(CCE_ERR_ARG, "%s: CCE_NEED_DBIAS without bias", what);
+  (void)V, (void)D, (void)dtype;
+  return CCE_OK;
 }
 
 int check_rows(int64_t N, int64_t D, int64_t V, int64_t K, int dtype, const char* what) {
@@ -1258,6 +1414,7 @@ int check_distill(const CceDistillParams* p, const char* what) {
 }
 
 cudaError_t rows_logits(const cce::FwdArgs& f, cudaStream_t s) {
+  if (f.split.e_hi) return cce::tc_logits(f, s);
   // (the packed copy of e is aligned whatever e was)
   return !force_simt() && cce::tc_supported(f.e, f.c, f.D, f.dtype) ? cce::tc_logits(f, s) : cce::simt_logits(f, s);
 }
@@ -1270,8 +1427,8 @@ size_t cce_logp_saved_bytes(int64_t N, int64_t D, int64_t V, int dtype) {
   return N < 0 || D < 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_saved(nullptr, N, D, V, 0, dtype).bytes;
 }
 
-size_t cce_logp_forward_workspace_bytes(int64_t N, int64_t V) {
-  return N < 0 || V <= 0 ? 0 : rows_fwd_ws(nullptr, N, V, 0).bytes;
+size_t cce_logp_forward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype) {
+  return N < 0 || D <= 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_fwd_ws(nullptr, N, D, V, 0, dtype).bytes;
 }
 
 size_t cce_logp_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
@@ -1290,8 +1447,8 @@ int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dt
     return fail(CCE_ERR_ARG, "%s: targets of %d bytes (4 or 8 expected)", what, target_bytes);
   if (N == 0) return CCE_OK;
   if (!e || !c || !targets || !logp || !mask) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
-  const RowsSaved v = rows_saved(saved, N, D, V, 0, dtype);
-  const RowsFwdWs w = rows_fwd_ws(workspace, N, V, 0);
+  RowsSaved v = rows_saved(saved, N, D, V, 0, dtype);
+  const RowsFwdWs w = rows_fwd_ws(workspace, N, D, V, 0, dtype);
   if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
     return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
                 v.bytes, workspace_bytes, w.bytes);
@@ -1303,6 +1460,10 @@ int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dt
                  what);
   cce::FwdArgs f{v.e, c, bias, bias_dtype, v.R.targets, N, D, V, 0, dtype, nullptr, w.part_m, w.part_s, w.tgt};
   f.rows = v.R.count;
+  if (v.split.Dp) {
+    CCE_CUDA_CHECK(split_operands(v, w.split, e, c, N, D, V, s), what);
+    f.split = v.split;
+  }
   CCE_CUDA_CHECK(rows_logits(f, s), what);
   CCE_CUDA_CHECK(cce::launch_rows_logp(w.part_m, w.part_s, cce::ceil_div(V, cce::kSimtLseTile), N, v.R, w.tgt, v.lse,
                                        logp, s),
@@ -1316,8 +1477,8 @@ int cce_logp_backward(const void* c, const void* bias, int bias_dtype, const flo
   const char* what = "cce_logp_backward";
   int rc = check_rows(N, D, V, 0, dtype, what);
   if (rc) return rc;
-  if (flags & ~(CCE_NEED_DE | CCE_NEED_DC | CCE_NEED_DBIAS))
-    return fail(CCE_ERR_ARG, "%s: unknown flag bits 0x%x", what, flags);
+  rc = check_rows_backward(bias, bias_dtype, N, V, D, dtype, flags, grad_e, grad_c, grad_bias, what);
+  if (rc) return rc;
   if (N == 0)
     return backward_impl(nullptr, c, nullptr, bias, bias_dtype, nullptr, nullptr, nullptr, nullptr, N, D, V, 0, dtype,
                          flags, 0.f, grad_e, grad_c, grad_bias, nullptr, workspace, workspace_bytes, nullptr, nullptr,
@@ -1335,6 +1496,9 @@ int cce_logp_backward(const void* c, const void* bias, int bias_dtype, const flo
                                             (cudaStream_t)stream),
                  what);
   const RowsBwd rb{v.R, cce::TopkView{}, w.d, 1.f, w.bias_part};
+  if (v.split.Dp)
+    return split_backward(v, w, rb, c, bias, bias_dtype, w.d, N, D, V, flags, grad_e, grad_c, grad_bias,
+                          (cudaStream_t)stream);
   return backward_impl(v.e, c, nullptr, bias, bias_dtype, v.R.targets, v.lse, w.d, nullptr, N, D, V, 0, dtype, flags,
                        0.f, grad_e, grad_c, grad_bias, nullptr, w.base, w.base_bytes, nullptr, &rb, stream);
 }
@@ -1344,8 +1508,9 @@ size_t cce_distill_saved_bytes(int64_t N, int64_t D, int64_t V, int64_t K, int d
   return rows_saved(nullptr, N, D, V, K, dtype).bytes;
 }
 
-size_t cce_distill_forward_workspace_bytes(int64_t N, int64_t V, int64_t K) {
-  return N < 0 || V <= 0 || K < 1 || K > CCE_DISTILL_MAX_K ? 0 : rows_fwd_ws(nullptr, N, V, K).bytes;
+size_t cce_distill_forward_workspace_bytes(int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
+  if (N < 0 || D <= 0 || V <= 0 || K < 1 || K > CCE_DISTILL_MAX_K || !dtype_ok(dtype)) return 0;
+  return rows_fwd_ws(nullptr, N, D, V, K, dtype).bytes;
 }
 
 size_t cce_distill_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
@@ -1375,8 +1540,8 @@ int cce_distill_forward(const void* e, const void* c, const void* bias, int bias
     return CCE_OK;
   }
   if (!e || !c || !teacher_ids || !teacher_logp) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
-  const RowsSaved v = rows_saved(saved, N, D, V, K, dtype);
-  const RowsFwdWs w = rows_fwd_ws(workspace, N, V, K);
+  RowsSaved v = rows_saved(saved, N, D, V, K, dtype);
+  const RowsFwdWs w = rows_fwd_ws(workspace, N, D, V, K, dtype);
   if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
     return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
                 v.bytes, workspace_bytes, w.bytes);
@@ -1390,6 +1555,10 @@ int cce_distill_forward(const void* e, const void* c, const void* bias, int bias
                  what);
   cce::FwdArgs f{v.e, c, bias, bias_dtype, nullptr, N, D, V, 0, dtype, nullptr, w.part_m, w.part_s, nullptr};
   f.rows = v.R.count;
+  if (v.split.Dp) {
+    CCE_CUDA_CHECK(split_operands(v, w.split, e, c, N, D, V, s), what);
+    f.split = v.split;
+  }
   f.scale = (float)(1.0 / params->temperature);
   f.topk = v.topk;
   CCE_CUDA_CHECK(rows_logits(f, s), what);
@@ -1409,8 +1578,8 @@ int cce_distill_backward(const void* c, const void* bias, int bias_dtype, const 
   if (K < 1) return fail(CCE_ERR_SHAPE, "%s: K=%lld is outside of [1, %d]", what, (long long)K, CCE_DISTILL_MAX_K);
   rc = check_distill(params, what);
   if (rc) return rc;
-  if (flags & ~(CCE_NEED_DE | CCE_NEED_DC | CCE_NEED_DBIAS))
-    return fail(CCE_ERR_ARG, "%s: unknown flag bits 0x%x", what, flags);
+  rc = check_rows_backward(bias, bias_dtype, N, V, D, dtype, flags, grad_e, grad_c, grad_bias, what);
+  if (rc) return rc;
   if (N == 0)
     return backward_impl(nullptr, c, nullptr, bias, bias_dtype, nullptr, nullptr, nullptr, nullptr, N, D, V, 0, dtype,
                          flags, 0.f, grad_e, grad_c, grad_bias, nullptr, workspace, workspace_bytes, nullptr, nullptr,
@@ -1429,6 +1598,9 @@ int cce_distill_backward(const void* c, const void* bias, int bias_dtype, const 
                                             (cudaStream_t)stream),
                  what);
   const RowsBwd rb{v.R, v.topk, w.d, (float)(1.0 / params->temperature), w.bias_part};
+  if (v.split.Dp)
+    return split_backward(v, w, rb, c, bias, bias_dtype, w.dA, N, D, V, flags, grad_e, grad_c, grad_bias,
+                          (cudaStream_t)stream);
   return backward_impl(v.e, c, nullptr, bias, bias_dtype, nullptr, v.lse, w.dA, nullptr, N, D, V, 0, dtype, flags, 0.f,
                        grad_e, grad_c, grad_bias, nullptr, w.base, w.base_bytes, nullptr, &rb, stream);
 }

@@ -42,6 +42,15 @@ struct TopkView {
   int K = 0, tiles1 = 0;
 };
 
+// Float32 operands as two float16 parts, x = (hi + lo) / s[0], rows padded with
+// zeros to Dp (a multiple of 64) columns; se, sc: {s, 1 / s} on the device.
+struct SplitView {
+  const void *e_hi = nullptr, *e_lo = nullptr;  // [N][Dp] packed rows
+  const void *c_hi = nullptr, *c_lo = nullptr;  // [V][Dp]
+  int64_t Dp = 0;
+  const float *se = nullptr, *sc = nullptr;
+};
+
 struct FwdArgs {
   const void* e;
   const void* c;
@@ -58,6 +67,7 @@ struct FwdArgs {
   const int32_t* rows = nullptr;  // rows that count (device)
   float scale = 1.f;              // logits = scale (e c^T + bias)
   TopkView topk{};                // columns left out of the sum, whose logits go to topk.z
+  SplitView split{};              // float32 inputs on tensor cores (e, c unused)
 };
 
 struct BwdChunkArgs {
@@ -89,6 +99,10 @@ struct BwdChunkArgs {
   TopkView topk{};
   const float* d_row = nullptr;
   float logit_scale = 1.f;
+  const int32_t* rows = nullptr; // packed rows that count (tc_dlogits_rows and the float32 gradients)
+  SplitView split{};             // float32 inputs on tensor cores (e, c_chunk unused)
+  void* dlogits_lo = nullptr;    // the dlogits' second part
+  int slabs = 2;                 // K splits of tc_grad_e
   float* bias_part = nullptr;    // [ceil(N / 32)][vc_ld] column sums of dlogits (zeroed); instead of grad_bias
   const int* dl_list = nullptr;  // the chunk's live dlogits tiles (tc_dlogits_lists), count in counters[3]
 };
@@ -137,9 +151,15 @@ cudaError_t launch_rows_cotangent(const float* up, int up_row, const float* weig
                                   int64_t N, const float* A, float* d, float* dA, cudaStream_t stream);
 cudaError_t launch_live_mask(const float* d, int64_t N, int64_t V, uint8_t* keep, uint32_t* keep_t, int64_t keep_t_ld,
                              cudaStream_t stream);
-// out[n] = a[pos[n]] (+ b[pos[n]] unless nullptr), 0 where pos[n] < 0
-cudaError_t launch_rows_scatter(const float* a, const float* b, const int32_t* pos, int64_t N, int64_t D, int dtype,
+// out[n] = sum over the slabs [N][D] of row pos[n], in order; 0 where pos[n] < 0
+cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, const int32_t* pos, int64_t N, int64_t D, int dtype,
                                 void* out, cudaStream_t stream);
+// largest |x| of the rows (those of R, if given) as the bits of a float, into *word (zeroed)
+cudaError_t launch_absmax(const float* x, int64_t rows, int64_t D, const RowsView* R, uint32_t* word,
+                          cudaStream_t stream);
+// x -> hi, lo [rows][Dp] and scale = {s, 1 / s}; R: the packed rows of x, zeros behind their count
+cudaError_t launch_split(const float* x, int64_t rows, int64_t D, int64_t Dp, const RowsView* R, const uint32_t* word,
+                         float* scale, void* hi, void* lo, cudaStream_t stream);
 cudaError_t launch_bias_sum(const float* part, int64_t parts, int64_t ld, int64_t cols, const float* scale, float* out,
                             cudaStream_t stream);
 
@@ -162,6 +182,7 @@ int simt_grad_e_splits(int64_t N, int64_t D, int64_t vc);
 cudaError_t simt_grad_c(const BwdChunkArgs& a, void* grad_c, cudaStream_t stream);
 
 // ---- tcgen05 kernels (tc_kernels.cu): 16-bit dtypes, D % 8 == 0 ----
+bool tc_available();  // the driver's tensor-map encoder was found
 bool tc_supported(const void* e, const void* c, int64_t D, int dtype);
 bool tc_backward_supported(const void* e, const void* c, int64_t D, int dtype);
 // Reads (and optionally clears) the tensor-core kernels' device status word:
@@ -173,6 +194,12 @@ int tc_read_mma_flops(uint64_t* out4, bool reset);
 cudaError_t tc_forward(const FwdArgs& a, cudaStream_t stream);
 // row statistics of the rows that count, two-level accumulation (see FwdArgs)
 cudaError_t tc_logits(const FwdArgs& a, cudaStream_t stream);
+// dlogits of a chunk's packed rows, no filter; float32 inputs (a.split): both parts
+cudaError_t tc_dlogits_rows(const BwdChunkArgs& a, cudaStream_t stream);
+// float32 gradients from split operands: slabs[num_slabs][N][D] (+)= the K splits
+// of dl c_chunk; grad_c rows of the chunk = dl^T e
+cudaError_t tc_grad_e_split(const BwdChunkArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t stream);
+cudaError_t tc_grad_c_split(const BwdChunkArgs& a, float* grad_c, cudaStream_t stream);
 cudaError_t tc_dlogits(const BwdChunkArgs& a, cudaStream_t stream);
 // Lists, per vocabulary chunk of vc rows, the dlogits work units with a kept
 // block in schedule order: chunk ch's ids at lists + ch * tc_dlogits_list_len(N, vc),

@@ -113,7 +113,7 @@ rows_gather_kernel(const uint8_t* __restrict__ e, int64_t N, int64_t row_bytes, 
   const int64_t count = *R.count;
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < N; i += (int64_t)gridDim.x * 8) {
     const bool live = i < count;
-    const uint8_t* src = live ? e + (int64_t)R.row_of[i] * row_bytes : nullptr;
+    const uint8_t* src = live ? e + (int64_t)R.row_of[i] * row_bytes : nullptr;  // (row_bytes 0: no copy)
     uint8_t* dst = out + i * row_bytes;
     if constexpr (kVec) {
       for (int64_t k = lane * 16; k < row_bytes; k += 32 * 16)
@@ -455,21 +455,24 @@ live_mask_kernel(const float* __restrict__ d, int64_t N, int64_t V, uint8_t* __r
   }
 }
 
-// grad_e row n = a[pos[n]] (+ b[pos[n]]), 0 for rows that do not count.
+// grad_e row n = the slabs' rows pos[n] added in order, 0 for rows that do not count.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256)
-rows_scatter_kernel(const float* __restrict__ a, const float* __restrict__ b, const int32_t* __restrict__ pos, int64_t N,
-                    int64_t D, T* __restrict__ out) {
+rows_scatter_kernel(const float* __restrict__ slabs, int num, const int32_t* __restrict__ pos, int64_t N, int64_t D,
+                    T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
+  const int64_t stride = N * D;
   for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < N; n += (int64_t)gridDim.x * 8) {
     const int64_t p = pos[n];
+    const float* row = slabs + p * D;
     if constexpr (kVec) {
       for (int64_t k = 4 * lane; k < D; k += 128) {
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         if (p >= 0) {
-          x = *reinterpret_cast<const float4*>(a + p * D + k);
-          if (b) {
-            const float4 y = *reinterpret_cast<const float4*>(b + p * D + k);
+          x = *reinterpret_cast<const float4*>(row + k);
+#pragma unroll 4
+          for (int z = 1; z < num; ++z) {
+            const float4 y = *reinterpret_cast<const float4*>(row + z * stride + k);
             x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
           }
         }
@@ -483,9 +486,85 @@ rows_scatter_kernel(const float* __restrict__ a, const float* __restrict__ b, co
     } else {
       for (int64_t k = lane; k < D; k += 32) {
         float x = 0.f;
-        if (p >= 0) x = a[p * D + k] + (b ? b[p * D + k] : 0.f);
+        if (p >= 0) {
+          x = row[k];
+          for (int z = 1; z < num; ++z) x += row[z * stride + k];
+        }
         out[n * D + k] = from_f32<T>(x);
       }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// float32 operands as two float16 parts
+// ---------------------------------------------------------------------------
+
+// The largest |x| as the bits of a float (their order is that of the values; NaN
+// and infinity come out on top), whatever order the blocks run in.
+__global__ void __launch_bounds__(256)
+absmax_kernel(const float* __restrict__ x, int64_t rows, int64_t D, const int32_t* __restrict__ row_of,
+              const int32_t* __restrict__ count, int vec, uint32_t* __restrict__ word) {
+  const int lane = threadIdx.x & 31;
+  if (count) rows = min(rows, (int64_t)*count);
+  uint32_t m = 0;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const float* p = x + (row_of ? row_of[r] : r) * D;
+    if (vec) {
+      for (int64_t k = 4 * lane; k < D; k += 128) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + k));
+        m = max(m, max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu)));
+      }
+    } else {
+      for (int64_t k = lane; k < D; k += 32) m = max(m, __float_as_uint(p[k]) & 0x7fffffffu);
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0 && m) atomicMax(word, m);
+}
+
+// s puts the largest value into [2^13, 2^14): hi = fp16(s x), lo = fp16(s x - hi)
+// together hold 22 bits of values down to 2^-14 of the largest, 2^-25 absolute
+// (in units of 1 / s) below.
+__global__ void __launch_bounds__(256)
+split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, const int32_t* __restrict__ row_of,
+             const int32_t* __restrict__ count, int vec, const uint32_t* __restrict__ word, float* __restrict__ scale,
+             __half* __restrict__ hi, __half* __restrict__ lo) {
+  const int lane = threadIdx.x & 31;
+  const float big = __uint_as_float(*word);
+  float s = 1.f;
+  if (big > 0.f && isfinite(big)) {
+    int ex;
+    frexpf(big, &ex);
+    s = ldexpf(1.f, min(110, max(-110, 14 - ex)));
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    scale[0] = s;
+    scale[1] = 1.f / s;
+  }
+  const int64_t live = count ? min(rows, (int64_t)*count) : rows;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const float* p = r < live ? x + (row_of ? row_of[r] : r) * D : nullptr;
+    for (int64_t k = 4 * lane; k < Dp; k += 128) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (p) {
+        if (vec && k + 4 <= D) {
+          const float4 y = __ldg(reinterpret_cast<const float4*>(p + k));
+          v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = k + j < D ? p[k + j] : 0.f;
+        }
+      }
+      __half h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float y = v[j] * s;
+        h[j] = __float2half_rn(y);
+        l[j] = __float2half_rn(y - __half2float(h[j]));
+      }
+      *reinterpret_cast<uint2*>(hi + r * Dp + k) = *reinterpret_cast<uint2*>(h);
+      *reinterpret_cast<uint2*>(lo + r * Dp + k) = *reinterpret_cast<uint2*>(l);
     }
   }
 }
@@ -535,7 +614,12 @@ cudaError_t launch_rows_pack(const void* e, int dtype, int64_t N, int64_t D, con
   if (err != cudaSuccess) return err;
   const int64_t row_bytes = D * (dtype == CCE_F32 ? 4 : 2);
   const bool vec = row_bytes % 16 == 0 && aligned16(e) && aligned16(e_packed);
-  if (vec)
+  if (e_packed == nullptr) {  // the rows themselves are copied elsewhere
+    if (tgt || targets)
+      rows_gather_kernel<true><<<warps_grid(N), 256, 0, s>>>(nullptr, N, 0, R, targets != nullptr, nullptr, tgt);
+    else
+      return cudaSuccess;
+  } else if (vec)
     rows_gather_kernel<true><<<warps_grid(N), 256, 0, s>>>((const uint8_t*)e, N, row_bytes, R, targets != nullptr,
                                                            (uint8_t*)e_packed, tgt);
   else
@@ -596,24 +680,38 @@ cudaError_t launch_live_mask(const float* d, int64_t N, int64_t V, uint8_t* keep
 }
 
 template <typename T>
-static cudaError_t scatter(const float* a, const float* b, const int32_t* pos, int64_t N, int64_t D, void* out,
+static cudaError_t scatter(const float* slabs, int num, const int32_t* pos, int64_t N, int64_t D, void* out,
                            cudaStream_t s) {
-  const bool vec = D % 4 == 0 && aligned16(a) && aligned16(b) && aligned16(out);
+  const bool vec = D % 4 == 0 && aligned16(slabs) && aligned16(out);
   if (vec)
-    rows_scatter_kernel<T, true><<<warps_grid(N), 256, 0, s>>>(a, b, pos, N, D, static_cast<T*>(out));
+    rows_scatter_kernel<T, true><<<warps_grid(N), 256, 0, s>>>(slabs, num, pos, N, D, static_cast<T*>(out));
   else
-    rows_scatter_kernel<T, false><<<warps_grid(N), 256, 0, s>>>(a, b, pos, N, D, static_cast<T*>(out));
+    rows_scatter_kernel<T, false><<<warps_grid(N), 256, 0, s>>>(slabs, num, pos, N, D, static_cast<T*>(out));
   return launched();
 }
 
-cudaError_t launch_rows_scatter(const float* a, const float* b, const int32_t* pos, int64_t N, int64_t D, int dtype,
+cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, const int32_t* pos, int64_t N, int64_t D, int dtype,
                                 void* out, cudaStream_t s) {
   switch (dtype) {
-    case CCE_F32: return scatter<float>(a, b, pos, N, D, out, s);
-    case CCE_F16: return scatter<__half>(a, b, pos, N, D, out, s);
-    case CCE_BF16: return scatter<__nv_bfloat16>(a, b, pos, N, D, out, s);
+    case CCE_F32: return scatter<float>(slabs, num_slabs, pos, N, D, out, s);
+    case CCE_F16: return scatter<__half>(slabs, num_slabs, pos, N, D, out, s);
+    case CCE_BF16: return scatter<__nv_bfloat16>(slabs, num_slabs, pos, N, D, out, s);
   }
   return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_absmax(const float* x, int64_t rows, int64_t D, const RowsView* R, uint32_t* word, cudaStream_t s) {
+  absmax_kernel<<<warps_grid(rows), 256, 0, s>>>(x, rows, D, R ? R->row_of : nullptr, R ? R->count : nullptr,
+                                                 D % 4 == 0 && aligned16(x), word);
+  return launched();
+}
+
+cudaError_t launch_split(const float* x, int64_t rows, int64_t D, int64_t Dp, const RowsView* R, const uint32_t* word,
+                         float* scale, void* hi, void* lo, cudaStream_t s) {
+  split_kernel<<<warps_grid(rows), 256, 0, s>>>(x, rows, D, Dp, R ? R->row_of : nullptr, R ? R->count : nullptr,
+                                                D % 4 == 0 && aligned16(x), word, scale, static_cast<__half*>(hi),
+                                                static_cast<__half*>(lo));
+  return launched();
 }
 
 cudaError_t launch_bias_sum(const float* part, int64_t parts, int64_t ld, int64_t cols, const float* scale, float* out,

@@ -304,9 +304,7 @@ struct FwdEpi {
 // K4: dlogits of one vocabulary chunk
 // ---------------------------------------------------------------------------
 
-// kTopk (distillation): d_nll and lse are the coefficient and log-sum-exp of the
-// columns outside of the row's list; the listed ones' values are given.
-template <typename T, typename TB, bool kTopk = false>
+template <typename T, typename TB>
 struct DlogitsEpi {
   static constexpr bool kNarrowB = true;  // B rows loaded for a tile's live column run only
   static constexpr bool kPairLd = false;  // the epilogue reads TMEM two 32-column chunks at a time
@@ -326,17 +324,10 @@ struct DlogitsEpi {
   int mask_rows, mask_cols; // nRb, statistics tiles in the chunk
   int64_t N, V, v_offset, vc0, vc_end, ld;
   int dbl = 0;     // narrow tiles load two K-blocks per stage (kDblB0)
-  float* bias_part = nullptr;    // [ceil(N / 32)][ld] column sums of w (instead of grad_bias)
-  TopkView topk{};               // kTopk
-  const float* d_row = nullptr;
-  float logit_scale = 1.f;
 
-  struct NoCursor {};
   struct State {
     int64_t row, tl, col0;
     float g, L, s;   // g = d_nll / s
-    float dr;        // kTopk: d_row / s
-    typename std::conditional<kTopk, TopkCursor, NoCursor>::type cur;
     uint32_t kmask;  // kept statistics-tile column groups of the tile
     int y0;          // first row of this warp's 32-row slab
   };
@@ -377,13 +368,7 @@ struct DlogitsEpi {
     st.s = scale ? scale[0] : 1.f;
     st.g = ok ? d_nll[st.row] * (scale ? scale[1] : 1.f) : 0.f;
     st.L = ok ? lse[st.row] : 0.f;
-    if constexpr (kTopk) {
-      st.tl = -1;
-      st.dr = ok ? d_row[st.row] * (scale ? scale[1] : 1.f) : 0.f;
-      st.cur.open(topk, st.row, ok, st.col0 / kTopkTile);
-    } else {
-      st.tl = ok ? (int64_t)targets[st.row] - v_offset : -1;
-    }
+    st.tl = ok ? (int64_t)targets[st.row] - v_offset : -1;
     st.kmask = group_mask(mk, mb, nb);
     st.y0 = (int)(st.row - (threadIdx.x & 31));
   }
@@ -403,24 +388,10 @@ struct DlogitsEpi {
     for (int j = 0; j < 32; ++j) {
       float w = 0.f;
       if (kept && cb + j < vc_end) {
-        if constexpr (kTopk) {
-          w = st.g * exp2f(((v[j] + b[j]) * logit_scale - st.L) * kLog2e);
-        } else {
-          w = st.g * exp2f(fmaf(v[j] + b[j], kLog2e, -Ll));
-          if (cb + j == st.tl) w -= st.g;
-        }
+        w = st.g * exp2f(fmaf(v[j] + b[j], kLog2e, -Ll));
+        if (cb + j == st.tl) w -= st.g;
       }
       v[j] = w;
-    }
-    if constexpr (kTopk) {
-      int p;
-      const uint32_t bits = st.cur.take(cb, p);
-      if (__any_sync(0xffffffffu, bits != 0u)) {
-        const float* x = topk.z + st.row * topk.K + p;
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if ((bits >> j) & 1u) v[j] = st.dr * __ldg(x + __popc(bits & ((1u << j) - 1u)));
-      }
     }
     // grad_c multiplies whole 128-column quarters (its M tiles): a quarter
     // with a kept group is stored whole (zeros in the others), the rest never
@@ -432,10 +403,6 @@ struct DlogitsEpi {
       const int lane = threadIdx.x & 31;
       const float colsum = warp_transpose_sum32(v);
       if (cb + lane < vc_end && colsum != 0.f) atomicAdd(grad_bias + cb + lane, colsum * st.s);
-    } else if (bias_part != nullptr && kept) {
-      const int lane = threadIdx.x & 31;
-      const float colsum = warp_transpose_sum32(v);
-      if (cb + lane < vc_end && st.y0 < N) bias_part[(int64_t)(st.y0 / 32) * ld + (cb - vc0) + lane] = colsum;
     }
   }
 
@@ -1372,14 +1339,14 @@ bool make_tmap_out(CUtensorMap* tm, const void* base, int dtype, int64_t inner, 
   return r == CUDA_SUCCESS;
 }
 
-// The two fp32 grad_e accumulator slabs acc2[2][N][D] as a 3-D map, written in
+// The fp32 grad_e accumulator slabs acc2[slabs][N][D] (two with the filter) as a 3-D map, written in
 // (16 x 32 x 1) boxes (64-byte rows, 64-byte swizzle); the slab index is the z
 // coordinate, so rows past N of one slab are clipped rather than spilling
 // into the other.
-bool make_tmap_acc2(CUtensorMap* tm, const float* acc2, int64_t D, int64_t N) {
+bool make_tmap_acc2(CUtensorMap* tm, const float* acc2, int64_t D, int64_t N, int slabs) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)N, 2};
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)N, (cuuint64_t)slabs};
   cuuint64_t strides[2] = {(cuuint64_t)(D * 4), (cuuint64_t)(N * D * 4)};
   cuuint32_t box[3] = {16, 32, 1};
   cuuint32_t estr[3] = {1, 1, 1};
@@ -1429,6 +1396,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 }  // namespace tc
 
 using namespace tc;
+
+bool tc_available() { return encode_fn() != nullptr; }
 
 bool tc_supported(const void* e, const void* c, int64_t D, int dtype) {
   return (dtype == CCE_BF16 || dtype == CCE_F16) && D % 8 == 0 && aligned16(e) && aligned16(c) &&
@@ -1529,7 +1498,7 @@ __global__ void __launch_bounds__(1024) dl_list_kernel(const uint8_t* keep, int6
     if (i < 32 ? ((bits >> i) & 1u) != 0 : live(u0 + i)) list[pos++] = u0 + i;
 }
 
-template <typename T, typename TB, bool kTopk>
+template <typename T, typename TB>
 cudaError_t dl_launch(const BwdChunkArgs& a, cudaStream_t s) {
   const bool bf16 = a.dtype == CCE_BF16;
   CUtensorMap tmA, tmB;
@@ -1543,15 +1512,11 @@ cudaError_t dl_launch(const BwdChunkArgs& a, cudaStream_t s) {
   }
   const int64_t vc_end = (a.vc0 + a.vc_len) < a.V ? (a.vc0 + a.vc_len) : a.V;
   sc.span = dlogits_span() ? 1 : 0;
-  DlogitsEpi<T, TB, kTopk> epi{a.targets, a.lse, a.d_nll, a.bias, static_cast<T*>(a.dlogits), a.grad_bias,
+  DlogitsEpi<T, TB> epi{a.targets, a.lse, a.d_nll, a.bias, static_cast<T*>(a.dlogits), a.grad_bias,
                         a.scale, a.keep + a.vc0 / kStatTile, ceil_div(a.V, kStatTile),
                         (int)ceil_div(a.N, kRowBlock), (int)ceil_div(a.vc_len, kStatTile),
                         a.N, a.V, a.v_offset, a.vc0, vc_end, a.vc_ld};
   epi.dbl = dlogits_double_k() ? 1 : 0;
-  epi.bias_part = a.bias_part;
-  epi.topk = a.topk;
-  epi.d_row = a.d_row;
-  epi.logit_scale = a.logit_scale;
   CUtensorMap tmC, tmB32;
   if (!make_tmap_out(&tmC, a.dlogits, a.dtype, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
   if (!make_tmap(&tmB32, cchunk, bf16, a.D, a.vc_len, a.D, BK, kStatTile)) return cudaErrorInvalidValue;
@@ -1581,32 +1546,27 @@ cudaError_t tc_forward(const FwdArgs& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-template <typename T, bool kTopk>
+template <typename T>
 cudaError_t dl_dispatch(const BwdChunkArgs& a, cudaStream_t s) {
   switch (a.bias == nullptr ? -1 : a.bias_dtype) {
-    case -1: return dl_launch<T, void, kTopk>(a, s);
-    case CCE_F32: return dl_launch<T, float, kTopk>(a, s);
-    case CCE_F16: return dl_launch<T, __half, kTopk>(a, s);
-    case CCE_BF16: return dl_launch<T, __nv_bfloat16, kTopk>(a, s);
+    case -1: return dl_launch<T, void>(a, s);
+    case CCE_F32: return dl_launch<T, float>(a, s);
+    case CCE_F16: return dl_launch<T, __half>(a, s);
+    case CCE_BF16: return dl_launch<T, __nv_bfloat16>(a, s);
   }
   return cudaErrorInvalidValue;
 }
 
-template <bool kTopk>
-cudaError_t dl_types(const BwdChunkArgs& a, cudaStream_t s) {
-  if (a.dtype == CCE_BF16) return dl_dispatch<__nv_bfloat16, kTopk>(a, s);
-  if (a.dtype == CCE_F16) return dl_dispatch<__half, kTopk>(a, s);
-  return cudaErrorNotSupported;
-}
-
 cudaError_t tc_dlogits(const BwdChunkArgs& a, cudaStream_t s) {
   if (a.N == 0 || a.vc_len == 0) return cudaSuccess;
-  return a.topk.sid ? dl_types<true>(a, s) : dl_types<false>(a, s);
+  if (a.dtype == CCE_BF16) return dl_dispatch<__nv_bfloat16>(a, s);
+  if (a.dtype == CCE_F16) return dl_dispatch<__half>(a, s);
+  return cudaErrorNotSupported;
 }
 
 namespace tc {
 namespace {
-#include "tc_logits.cuh"
+#include "tc_rows.cuh"
 }  // namespace
 }  // namespace tc
 
@@ -1621,6 +1581,23 @@ cudaError_t tc_logits(const FwdArgs& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
+cudaError_t tc_dlogits_rows(const BwdChunkArgs& a, cudaStream_t s) {
+  if (a.N == 0 || a.vc_len == 0) return cudaSuccess;
+  switch (a.bias == nullptr ? -1 : a.bias_dtype) {
+    case -1: return dlogits2_dispatch<void>(a, s);
+    case CCE_F32: return dlogits2_dispatch<float>(a, s);
+    case CCE_F16: return dlogits2_dispatch<__half>(a, s);
+    case CCE_BF16: return dlogits2_dispatch<__nv_bfloat16>(a, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t tc_grad_e_split(const BwdChunkArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
+  return grad_e_split(a, slabs, num_slabs, accumulate, s);
+}
+
+cudaError_t tc_grad_c_split(const BwdChunkArgs& a, float* grad_c, cudaStream_t s) { return grad_c_split(a, grad_c, s); }
+
 namespace {
 
 template <typename T>
@@ -1633,9 +1610,9 @@ cudaError_t grad_e_launch(const BwdChunkArgs& a, float* acc2, bool accumulate, c
   int b3d = 0;
   if (!make_tmap_mn(&tmB, cchunk, bf16, a.D, a.vc_len, a.D, (BN) / 64, &b3d))
     return cudaErrorInvalidValue;
-  if (!make_tmap_acc2(&tmC, acc2, a.D, a.N)) return cudaErrorInvalidValue;
+  if (!make_tmap_acc2(&tmC, acc2, a.D, a.N, a.slabs)) return cudaErrorInvalidValue;
   Sched sc{(int)ceil_div(a.N, BM), (int)ceil_div(a.D, BN), (int)ceil_div(a.vc_len, BK), 1, 0, b3d,
-           a.counters ? a.counters + 1 : nullptr, raster_group(a.N * a.vc_len * 2), 2};
+           a.counters ? a.counters + 1 : nullptr, raster_group(a.N * a.vc_len * 2), a.slabs};
   GradEEpi epi{a.scale, a.keep + a.vc0 / kStatTile, ceil_div(a.V, kStatTile), (int)ceil_div(a.N, kRowBlock),
                (int)ceil_div(a.vc_len, kStatTile), accumulate ? 1 : 0, acc2, a.N, a.D};
   if (push != nullptr) {

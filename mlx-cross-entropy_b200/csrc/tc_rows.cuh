@@ -1,0 +1,617 @@
+// The GEMMs of losses on log-probabilities over a batch's packed rows, with
+// two-level accumulation.  Part of tc_kernels.cu, after the engine whose
+// descriptors, tensor maps and output staging it uses.
+//
+//   LogitsEpi    z = scale (e c^T + bias): per row and 128-column half the online
+//                (max, sum of exp), the target's z, and for the distillation the z
+//                of the row's listed columns, which are left out of the sum
+//   DlogitsEpi2  the same z for one vocabulary chunk, then the dlogits
+//   OutEpi       float32 gradients (float32 inputs)
+//
+// 320 threads: a TMA warp, an MMA warp and 8 epilogue warps, one CTA per SM over
+// a static schedule of (128-row, 256-column) tiles.  There is no filter here: the
+// gradients are exact, and rows that do not count are not in the batch.
+//
+// Why a second level.  tcgen05.mma adds every K = 16 product into its fp32
+// accumulator rounding towards zero: a logit of 14 after 144 such steps is
+// about 1e-5 too small, always in the same direction, and sums of
+// log-probabilities over a sequence add that up.  Here an accumulator holds
+// only kSegKb K-blocks (256 products); the epilogue warps add each of those
+// partial logits to the total in their registers (128 per thread, round to
+// nearest).  The two TMEM accumulators take the segments in turn, so the MMAs
+// never wait for the adds: a segment's 16 MMAs take about 2000 cycles, its add
+// about 500 of the issue slots of the 8 epilogue warps.
+//
+// What is left of the drift is added back in expectation.  A step that rounds
+// an accumulator a towards zero loses on average half a unit in its last place,
+// 0.72 * 2^-24 |a| (mantissas spread evenly in their logarithm); over the 16
+// steps of a partial logit p that grows in a straight line 6 * 2^-24 |p|.  The
+// noise on the way makes it less, float16 products (22 bits, cut to the
+// accumulator's) make it more.  The partials are multiplied by 1 + k 2^-23 in the
+// same fused multiply-add, k (untruncate_of) from the root mean square error of
+// log-probabilities of 2048 peaked rows, V = 32000, in units of 1e-6 for
+// k = 0, 1, 2, 3, 4 (in brackets a library's float32 product):
+//   bfloat16, D = 2304     1.00 0.68 0.55 0.68 0.98   (5.1)
+//   bfloat16, D = 512      1.15 0.80 0.60 0.65 0.92   (2.2)
+//   float16, D = 2304      1.31 0.96 0.73 0.64 0.80   (6.5)
+//   float16, D = 512       2.30 1.94 1.63 1.37 1.20   (3.1)
+//   float32, D = 2304      1.69 1.60 1.63 1.73 1.92   (6.7)
+//   float32, D = 512       1.29 1.03 0.93 1.00 1.23   (3.0)
+// With one accumulator for all of K a bfloat16 D = 2304 head has 5.7.
+//
+// Float32 inputs.  x = (hi + lo) / s with hi, lo float16 and s a power of two that
+// puts the tensor's largest value below 2^14: hi holds 11 bits and lo the next 11.
+// A product runs as three passes over K, hi hi + hi lo + lo hi (lo lo is 2^-22 of
+// it), each on the tensor cores: 3 times the 16-bit work, where FFMA is 20 times
+// slower.  512 x 512 x 32000, loss and gradients: 2.75 ms on the CUDA cores.
+//
+// Rows are counted on the device (the batch without its masked rows), so row
+// tiles behind the count cost nothing.
+
+constexpr int kRgWarps = 8;                   // epilogue warps: two per TMEM lane quarter, a column half each
+constexpr int kRgThreads = 64 + 32 * kRgWarps;
+// K-blocks per accumulator segment: 4, 2 for split operands (accuracy is what they are for)
+__host__ __device__ constexpr int seg_kb(bool split) { return split ? 2 : 4; }
+constexpr size_t kRgSmem = 1024 + STAGES * (size_t)STAGE_BYTES + kRgWarps * 4096 + 256;
+
+struct RowsSched {
+  const int32_t* rows;   // rows that count, read at the kernel's start
+  int64_t N;             // their capacity
+  int m_rows, k_rows;    // M / K runs over the rows
+  int num_m, num_n, num_kb, ksplit, m_fast, group;
+  __device__ __forceinline__ Sched get(int64_t& count) const {
+    count = min((int64_t)__ldg(rows), N);
+    Sched s{};
+    s.num_m = m_rows ? (int)ceil_div(count, BM) : num_m;
+    s.num_n = num_n;
+    s.num_kb = k_rows ? (int)ceil_div(count, BK) : num_kb;
+    s.ksplit = ksplit;
+    s.m_fast = m_fast;
+    s.group = group;
+    return s;
+  }
+};
+
+// What an epilogue thread works on: its row of the tile, and the first of its
+// 128 columns.
+struct TileAt {
+  int64_t row, col0, rows;  // rows: those that count
+  int y0, ks, nb;           // first row of the warp's 32, K split, column tile
+};
+
+// 2^x, results below the normal range as 0 (they add nothing to a sum that holds a 1)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// z (accumulated in units of the split operands) += bias, -inf behind column V
+template <typename TB>
+__device__ __forceinline__ void add_bias(const void* bias, int64_t cb, int64_t V, float* v) {
+  if constexpr (!std::is_void<TB>::value) {
+    float b[32];
+    load_bias32<TB>(bias, cb, V, b);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += b[j];
+  }
+}
+
+// 1 / (s_a s_b) of split operands, 1 for whole ones: s[1] = 1 / s[0]
+__device__ __forceinline__ float unscale(const float* a, const float* b) { return a ? a[1] * b[1] : 1.f; }
+
+template <typename TB, bool kTopk>
+struct LogitsEpi {
+  static constexpr int kKind = 0;
+  static constexpr bool kStores = false;
+  const int32_t* targets;  // [N]
+  const void* bias;
+  float* part_m;           // [ceil(V / 128)][N]
+  float* part_s;
+  float* tgt;              // [N]
+  int64_t N, V;            // N: the arrays' stride
+  float scale;
+  const float *se, *sc;    // split operands' scales
+  TopkView topk;           // kTopk: the listed columns
+
+  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager&, const CUtensorMap*) const {
+    const bool live = t.row < t.rows;
+    const int64_t tl = (!kTopk && live) ? (int64_t)targets[t.row] - t.col0 : -1;  // the target's place in this half
+    TopkCursor cur;
+    if constexpr (kTopk) {
+      cur.open(topk, t.row, live, t.nb);
+      cur.skip_to(t.col0);
+    }
+    // The maximum is kept of the unscaled values; exponents are differences to
+    // it first, exact next to the maximum, then one product with scale log2 e.
+    float m = -INFINITY, sum = 0.f, tz = 0.f;
+    const float cexp = scale * kLog2e;
+    const float us = unscale(se, sc);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t cb = t.col0 + c * 32;
+      float* v = z + c * 32;
+      if (se) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= us;
+      }
+      add_bias<TB>(bias, cb, V, v);
+      if (cb + 32 > V) {
+        const int left = (int)(V - cb);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : -INFINITY;
+      }
+      if constexpr (kTopk) {
+        int p;
+        const uint32_t bits = cur.take(cb, p);
+        if (__any_sync(0xffffffffu, bits != 0u)) {
+          float* zo = topk.z + t.row * topk.K;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if ((bits >> j) & 1u) {
+              zo[p + __popc(bits & ((1u << j) - 1u))] = v[j] * scale;
+              v[j] = -INFINITY;
+            }
+          }
+        }
+      } else {
+        const int64_t at = tl - c * 32;
+        if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (at == j) tz = v[j];
+        }
+      }
+      float mc = v[0];
+#pragma unroll
+      for (int j = 1; j < 32; ++j) mc = fmaxf(mc, v[j]);
+      const float nm = fmaxf(m, mc);
+      if (nm != -INFINITY) {
+        float part = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) part += ex2((v[j] - nm) * cexp);
+        sum = sum * ex2((m - nm) * cexp) + part;
+        m = nm;
+      }
+    }
+    if (live) {
+      if (t.col0 < V) {
+        const int64_t idx = (t.col0 / 128) * N + t.row;
+        part_m[idx] = m * scale;
+        part_s[idx] = sum;
+      }
+      if constexpr (!kTopk)
+        if (tl >= 0 && tl < 128 && t.col0 + tl < V) tgt[t.row] = tz * scale;
+    }
+  }
+};
+
+// dlogits of one vocabulary chunk (columns relative to it).  Log-probabilities:
+// w = d (softmax - onehot).  Distillation: g e^(z - L) with the coefficient and
+// log-sum-exp of the columns outside of the row's list, d x for the listed ones.
+// float16 holds w / s (`scale` = {s, 1 / s}); split: hi + lo.
+template <typename T, typename TB, bool kTopk, bool kSplit>
+struct DlogitsEpi2 {
+  static constexpr int kKind = 1;
+  static constexpr bool kStores = true;
+  const int32_t* targets;
+  const float* lse;
+  const float* g;         // [N] d, or the coefficient
+  const float* d_row;     // [N] kTopk: d
+  const void* bias;       // of column 0 of the whole vocabulary
+  const float* scale;
+  float* bias_part;       // [ceil(N / 32)][ld] column sums of w, or nullptr
+  int64_t N, V, vc0, vc_end, ld;
+  float logit_scale;
+  const float *se, *sc;
+  TopkView topk;
+
+  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap* tm_lo) const {
+    const bool live = t.row < t.rows;
+    const float inv = scale ? scale[1] : 1.f;
+    const float G = live ? g[t.row] * inv : 0.f;
+    const float L = live ? lse[t.row] : INFINITY;
+    const float dr = kTopk && live ? d_row[t.row] * inv : 0.f;
+    const int64_t v0 = vc0 + t.col0;  // vocabulary id of column 0
+    const int64_t tl = (!kTopk && live) ? (int64_t)targets[t.row] - v0 : -1;
+    TopkCursor cur;
+    if constexpr (kTopk) {
+      cur.open(topk, t.row, live, (vc0 + (int64_t)t.nb * BN) / kTopkTile);
+      cur.skip_to(v0);
+    }
+    const float us = unscale(se, sc);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t cb = v0 + c * 32;
+      float(&v)[32] = *reinterpret_cast<float(*)[32]>(z + c * 32);
+      if constexpr (kSplit) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= us;
+      }
+      add_bias<TB>(bias, cb, vc_end, v);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = G * ex2((v[j] * logit_scale - L) * kLog2e);
+      if constexpr (kTopk) {
+        int p;
+        const uint32_t bits = cur.take(cb, p);
+        if (__any_sync(0xffffffffu, bits != 0u)) {
+          const float* x = topk.z + t.row * topk.K + p;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if ((bits >> j) & 1u) v[j] = dr * __ldg(x + __popc(bits & ((1u << j) - 1u)));
+        }
+      } else {
+        const int64_t at = tl - c * 32;
+        if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (at == j) v[j] -= G;
+        }
+      }
+      if (cb + 32 > vc_end) {  // (products of stored columns with rows of c behind the chunk)
+        const int left = (int)(vc_end - cb);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = j < left ? v[j] : 0.f;
+      }
+      if (t.y0 < N && cb < vc_end) {
+        if (bias_part != nullptr) {
+          float x[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = v[j];
+          const int lane = threadIdx.x & 31;
+          const float colsum = warp_transpose_sum32(x);
+          if (cb + lane < vc_end) bias_part[(int64_t)(t.y0 / 32) * ld + (cb - vc0) + lane] = colsum;
+        }
+        sg.template store16<T>(v, (int)(cb - vc0), t.y0);
+        if constexpr (kSplit) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] -= to_f32(from_f32<T>(v[j]));
+          const CUtensorMap* tm_hi = sg.tm;
+          sg.tm = tm_lo;
+          sg.template store16<T>(v, (int)(cb - vc0), t.y0);
+          sg.tm = tm_hi;
+        }
+      }
+    }
+  }
+};
+
+// out[ks][row][col] (+)= f1 f2 (A B), float32
+struct OutEpi {
+  static constexpr bool kStores = true;
+  const float *f1, *f2;
+  int add;
+  int64_t M, D;
+  int kind;  // slot in g_mma_cols
+  static constexpr int kKind = -1;  // (that of `kind`)
+
+  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
+    const float f = *f1 * *f2;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t col = t.col0 + c * 32;
+      if (col >= D || t.y0 >= M) continue;
+      float(&v)[32] = *reinterpret_cast<float(*)[32]>(z + c * 32);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= f;
+      sg.store_f32(v, (int)col, t.y0, t.ks, add != 0);
+    }
+  }
+};
+
+template <bool A_MN, bool B_MN, bool kSplit, class Epi>
+__global__ void __launch_bounds__(kRgThreads, 1)
+rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA2,
+                 const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmB2,
+                 const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmC2, const RowsSched rs,
+                 const Epi epi, const uint32_t idesc, const float untruncate) {
+  constexpr int kSegKb = seg_kb(kSplit);
+  constexpr int kPasses = kSplit ? 3 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  uint8_t* sA = smem_raw + pad;
+  uint8_t* sB = sA + STAGES * A_BYTES;
+  uint8_t* sOut = sB + STAGES * B_BYTES;  // 4 KB per epilogue warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + kRgWarps * 4096);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  int64_t rows;
+  const Sched sched = rs.get(rows);
+  const int units = sched.units();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(tfull + i, 1);
+      mbar_init(tempty + i, 32 * kRgWarps);
+    }
+    fence_barrier_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        int mb, nb, ks, kb0, kb1;
+        sched.coords(u, mb, nb, ks);
+        sched.krange(ks, kb0, kb1);
+        for (int p = 0; ok && p < kPasses; ++p) {  // hi hi, hi lo, lo hi
+          const CUtensorMap* ma = p == 2 ? &tmA2 : &tmA;
+          const CUtensorMap* mb_ = p == 1 ? &tmB2 : &tmB;
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait(empty + stage, phase ^ 1u, 11)) { ok = false; break; }
+            uint8_t* a = sA + stage * A_BYTES;
+            uint8_t* b = sB + stage * B_BYTES;
+            mbar_arrive_expect_tx(full + stage, STAGE_BYTES);
+            if constexpr (A_MN) tma_load_3d(a, ma, full + stage, 0, kb * BK, mb * (BM / 64));
+            else tma_load_2d(a, ma, full + stage, kb * BK, mb * BM);
+            if constexpr (B_MN) tma_load_3d(b, mb_, full + stage, 0, kb * BK, nb * (BN / 64));
+            else tma_load_2d(b, mb_, full + stage, kb * BK, nb * BN);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      unsigned long long mma_cols = 0;
+      const uint64_t adesc0 = A_MN ? smem_desc(smem_u32(sA), BOX_MN_BYTES, 1024) : smem_desc(smem_u32(sA), 16, 1024);
+      const uint64_t bdesc0 = B_MN ? smem_desc(smem_u32(sB), BOX_MN_BYTES, 1024) : smem_desc(smem_u32(sB), 16, 1024);
+      constexpr uint32_t a_kstep = (A_MN ? 2048u : 32u) >> 4;
+      constexpr uint32_t b_kstep = (B_MN ? 2048u : 32u) >> 4;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+        int mb, nb, ks, kb0, kb1;
+        sched.coords(u, mb, nb, ks);
+        sched.krange(ks, kb0, kb1);
+        const int n = (kb1 - kb0) * kPasses;
+        for (int k0 = 0; ok && k0 < n; k0 += kSegKb) {
+          if (!mbar_wait(tempty + acc, acc_phase ^ 1u, 12)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+          const int k1 = min(n, k0 + kSegKb);
+          uint32_t fresh = 1;
+          for (int k = k0; k < k1; ++k) {
+            if (!mbar_wait(full + stage, phase, 13)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t ad = adesc0 + (uint64_t)((stage * A_BYTES) >> 4);
+            const uint64_t bd = bdesc0 + (uint64_t)((stage * B_BYTES) >> 4);
+#pragma unroll
+            for (int i = 0; i < BK / 16; ++i) {
+              mma_f16(d, ad + i * a_kstep, bd + i * b_kstep, idesc, fresh ^ 1u);
+              fresh = 0;
+            }
+            mma_cols += (BK / 16) * BN;
+            mma_commit(empty + stage);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          if (!ok) break;
+          mma_commit(tfull + acc);
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1u;
+        }
+      }
+      if constexpr (Epi::kKind >= 0) atomicAdd(&g_mma_cols[Epi::kKind], mma_cols);
+      else atomicAdd(&g_mma_cols[epi.kind], mma_cols);
+    }
+    __syncwarp();
+  } else {
+    // ---------------- epilogue ----------------
+    const int q = warp & 3;           // TMEM lane quarter of this warp
+    const int h = (warp - 2) >> 2;    // column half
+    const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * 128);
+    Stager sg{&tmC, sOut + (warp - 2) * 4096, 0};
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      int mb, nb, ks, kb0, kb1;
+      sched.coords(u, mb, nb, ks);
+      sched.krange(ks, kb0, kb1);
+      const int n = (kb1 - kb0) * kPasses;
+      float z[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) z[j] = 0.f;
+#pragma unroll 1
+      for (int k0 = 0; k0 < n; k0 += kSegKb) {
+        // (one verdict for the warp: the TMEM reads below need all of its lanes)
+        ok = __all_sync(0xffffffffu, mbar_wait(tfull + acc, acc_phase, 14));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float v[32];
+          tmem_ld32(tbase + (uint32_t)(acc * BN + c * 32), v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[c * 32 + j] = fmaf(v[j], untruncate, z[c * 32 + j]);
+        }
+        tc_fence_before();
+        mbar_arrive(tempty + acc);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      if (!ok) break;
+      const int y0 = mb * BM + q * 32;
+      const TileAt t{(int64_t)y0 + lane, (int64_t)nb * BN + h * 128, rows, y0, ks, nb};
+      epi.finish(z, t, sg, &tmC2);
+    }
+    if constexpr (Epi::kStores) sg.drain();  // output boxes written before the kernel ends
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---- host side ----
+
+struct RowsMaps {
+  CUtensorMap A, A2, B, B2, C, C2;
+};
+
+// What a partial product is multiplied by (see the top of this file).
+float untruncate_of(bool split, bool bf16) { return 1.f + (split || bf16 ? 2.f : 3.f) * 1.1920929e-7f; }
+
+template <bool A_MN, bool B_MN, bool kSplit, class Epi>
+cudaError_t rows_gemm(const RowsMaps& m, const RowsSched& rs, const Epi& epi, bool bf16, int64_t max_units,
+                      cudaStream_t s) {
+  auto kern = rows_gemm_kernel<A_MN, B_MN, kSplit, Epi>;
+  static std::atomic<unsigned long long> attr_ctx[64];
+  cudaError_t err = ensure_smem_attr(kern, kRgSmem, attr_ctx);
+  if (err != cudaSuccess) return err;
+  if (max_units <= 0) return cudaSuccess;
+  const int grid = max_units < num_sms() ? (int)max_units : num_sms();
+  kern<<<grid, kRgThreads, kRgSmem, s>>>(m.A, m.A2, m.B, m.B2, m.C, m.C2, rs, epi, instr_desc(BM, BN, bf16, A_MN, B_MN),
+                                           untruncate_of(kSplit, bf16));
+  return launched();
+}
+
+// e (packed rows) and c, K-major: whole 16-bit operands or hi / lo.
+bool ec_maps(RowsMaps& m, const void* e, const void* c, const SplitView& sp, bool bf16, int64_t N, int64_t D, int64_t V,
+             int64_t v0) {
+  const bool split = sp.e_hi != nullptr;
+  const int64_t d = split ? sp.Dp : D;
+  const uint16_t* ch = static_cast<const uint16_t*>(split ? sp.c_hi : c);
+  const uint16_t* cl = static_cast<const uint16_t*>(sp.c_lo);
+  if (split) ch += v0 * d;  // (c is the chunk's first row already)
+  bool ok = make_tmap(&m.A, split ? sp.e_hi : e, bf16, d, N, d, BK, BM) && make_tmap(&m.B, ch, bf16, d, V, d, BK, BN);
+  m.A2 = m.A;
+  m.B2 = m.B;
+  if (split)
+    ok = ok && make_tmap(&m.A2, sp.e_lo, bf16, d, N, d, BK, BM) && make_tmap(&m.B2, cl + v0 * d, bf16, d, V, d, BK, BN);
+  m.C = m.C2 = m.A;  // (replaced where an epilogue stores)
+  return ok;
+}
+
+template <typename TB, bool kTopk>
+cudaError_t logits_launch(const FwdArgs& f, cudaStream_t s) {
+  const bool split = f.split.e_hi != nullptr, bf16 = !split && f.dtype == CCE_BF16;
+  RowsMaps m;
+  if (!ec_maps(m, f.e, f.c, f.split, bf16, f.N, f.D, f.V, 0)) return cudaErrorInvalidValue;
+  const int num_n = (int)ceil_div(f.V, BN);
+  const RowsSched rs{f.rows, f.N, 1, 0, 0, num_n, (int)ceil_div(split ? f.split.Dp : f.D, BK), 1, 1,
+                     raster_group(f.N * f.D * 2)};
+  const LogitsEpi<TB, kTopk> epi{f.targets, f.bias, f.part_m, f.part_s, f.tgt, f.N, f.V, f.scale,
+                                 f.split.se, f.split.sc, f.topk};
+  const int64_t units = ceil_div(f.N, BM) * num_n;
+  return split ? rows_gemm<false, false, true>(m, rs, epi, bf16, units, s)
+               : rows_gemm<false, false, false>(m, rs, epi, bf16, units, s);
+}
+
+template <typename TB>
+cudaError_t logits_dispatch(const FwdArgs& f, cudaStream_t s) {
+  return f.topk.sid ? logits_launch<TB, true>(f, s) : logits_launch<TB, false>(f, s);
+}
+
+template <typename T, typename TB, bool kTopk, bool kSplit>
+cudaError_t dlogits2_launch(const BwdChunkArgs& a, cudaStream_t s) {
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  RowsMaps m;
+  if (!ec_maps(m, a.e, a.c_chunk, a.split, bf16, a.N, a.D, a.vc_len, a.vc0)) return cudaErrorInvalidValue;
+  const int dt = bf16 ? CCE_BF16 : CCE_F16;
+  if (!make_tmap_out(&m.C, a.dlogits, dt, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
+  m.C2 = m.C;
+  if (kSplit && !make_tmap_out(&m.C2, a.dlogits_lo, dt, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
+  const int num_n = (int)ceil_div(a.vc_len, BN);
+  const RowsSched rs{a.rows, a.N, 1, 0, 0, num_n, (int)ceil_div(kSplit ? a.split.Dp : a.D, BK), 1, 1,
+                     raster_group(a.N * a.D * 2)};
+  const DlogitsEpi2<T, TB, kTopk, kSplit> epi{a.targets, a.lse, a.d_nll, a.d_row, a.bias, a.scale, a.bias_part, a.N, a.V,
+                                             a.vc0, a.vc0 + a.vc_len, a.vc_ld, a.logit_scale, a.split.se, a.split.sc,
+                                             a.topk};
+  return rows_gemm<false, false, kSplit>(m, rs, epi, bf16, ceil_div(a.N, BM) * num_n, s);
+}
+
+template <typename TB, bool kTopk>
+cudaError_t dlogits2_types(const BwdChunkArgs& a, cudaStream_t s) {
+  if (a.split.e_hi) return dlogits2_launch<__half, TB, kTopk, true>(a, s);
+  if (a.dtype == CCE_BF16) return dlogits2_launch<__nv_bfloat16, TB, kTopk, false>(a, s);
+  if (a.dtype == CCE_F16) return dlogits2_launch<__half, TB, kTopk, false>(a, s);
+  return cudaErrorNotSupported;
+}
+
+template <typename TB>
+cudaError_t dlogits2_dispatch(const BwdChunkArgs& a, cudaStream_t s) {
+  return a.topk.sid ? dlogits2_types<TB, true>(a, s) : dlogits2_types<TB, false>(a, s);
+}
+
+// float32 [z][rows][D] output, written in (16 x 32 x 1) boxes
+bool make_tmap_f32(CUtensorMap* tm, const float* out, int64_t D, int64_t rows, int64_t slabs) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)slabs};
+  cuuint64_t strides[2] = {(cuuint64_t)(D * 4), (cuuint64_t)(rows * D * 4)};
+  cuuint32_t box[3] = {16, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(out), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaError_t grad_e_split(const BwdChunkArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
+  const SplitView& sp = a.split;
+  RowsMaps m;
+  const uint16_t* ch = static_cast<const uint16_t*>(sp.c_hi) + a.vc0 * sp.Dp;
+  const uint16_t* cl = static_cast<const uint16_t*>(sp.c_lo) + a.vc0 * sp.Dp;
+  if (!make_tmap(&m.A, a.dlogits, false, a.vc_len, a.N, a.vc_ld, BK, BM) ||
+      !make_tmap(&m.A2, a.dlogits_lo, false, a.vc_len, a.N, a.vc_ld, BK, BM) ||
+      !make_tmap_mn3d(&m.B, ch, false, sp.Dp, a.vc_len, sp.Dp, BK, BN / 64) ||
+      !make_tmap_mn3d(&m.B2, cl, false, sp.Dp, a.vc_len, sp.Dp, BK, BN / 64) ||
+      !make_tmap_f32(&m.C, slabs, a.D, a.N, num_slabs))
+    return cudaErrorInvalidValue;
+  m.C2 = m.C;
+  const int num_n = (int)ceil_div(a.D, BN);
+  const RowsSched rs{a.rows, a.N, 1, 0, 0, num_n, (int)ceil_div(a.vc_len, BK), num_slabs, 1,
+                     raster_group(a.N * a.vc_len * 2)};
+  const OutEpi epi{a.scale, sp.sc + 1, accumulate ? 1 : 0, a.N, a.D, 2};
+  return rows_gemm<false, true, true>(m, rs, epi, false, ceil_div(a.N, BM) * num_n * num_slabs, s);
+}
+
+cudaError_t grad_c_split(const BwdChunkArgs& a, float* grad_c, cudaStream_t s) {
+  const SplitView& sp = a.split;
+  RowsMaps m;
+  const int64_t cols = round_up(a.vc_len, 64);  // (rows behind the chunk are clipped by the output's map)
+  if (!make_tmap_mn3d(&m.A, a.dlogits, false, cols, a.N, a.vc_ld, BK, BM / 64) ||
+      !make_tmap_mn3d(&m.A2, a.dlogits_lo, false, cols, a.N, a.vc_ld, BK, BM / 64) ||
+      !make_tmap_mn3d(&m.B, sp.e_hi, false, sp.Dp, a.N, sp.Dp, BK, BN / 64) ||
+      !make_tmap_mn3d(&m.B2, sp.e_lo, false, sp.Dp, a.N, sp.Dp, BK, BN / 64) ||
+      !make_tmap_f32(&m.C, grad_c + a.vc0 * a.D, a.D, a.vc_len, 1))
+    return cudaErrorInvalidValue;
+  m.C2 = m.C;
+  const int num_m = (int)ceil_div(a.vc_len, BM), num_n = (int)ceil_div(a.D, BN);
+  const RowsSched rs{a.rows, a.N, 0, 1, num_m, num_n, 0, 1, 0, raster_group(a.N * a.D * 2)};
+  const OutEpi epi{a.scale, sp.se + 1, 0, a.vc_len, a.D, 3};
+  return rows_gemm<true, true, true>(m, rs, epi, false, (int64_t)num_m * num_n, s);
+}

@@ -181,10 +181,10 @@ def _load():
     lib.cce_preference_loss_backward.restype = c_int
     lib.cce_preference_loss_backward.argtypes = [c_vp, c_vp, c_int, c_vp, c_vp, c_i64, c_i64, c_int, c_vp, c_vp]
     for name, args in (("cce_logp_saved_bytes", [c_i64, c_i64, c_i64, c_int]),
-                       ("cce_logp_forward_workspace_bytes", [c_i64, c_i64]),
+                       ("cce_logp_forward_workspace_bytes", [c_i64, c_i64, c_i64, c_int]),
                        ("cce_logp_backward_workspace_bytes", [c_i64, c_i64, c_i64, c_int, c_int]),
                        ("cce_distill_saved_bytes", [c_i64, c_i64, c_i64, c_i64, c_int]),
-                       ("cce_distill_forward_workspace_bytes", [c_i64, c_i64, c_i64]),
+                       ("cce_distill_forward_workspace_bytes", [c_i64, c_i64, c_i64, c_i64, c_int]),
                        ("cce_distill_backward_workspace_bytes", [c_i64, c_i64, c_i64, c_int, c_int])):
         getattr(lib, name).restype = c_sz
         getattr(lib, name).argtypes = args
@@ -671,7 +671,7 @@ def logp_forward(e, c, bias, targets, ignore_index):
     logp = torch.empty((N,), dtype=torch.float32, device=dev)
     mask = torch.empty((N,), dtype=torch.bool, device=dev)
     saved = _bytes(lib.cce_logp_saved_bytes(N, D, V, dt), dev)
-    ws = _bytes(lib.cce_logp_forward_workspace_bytes(N, V), dev)
+    ws = _bytes(lib.cce_logp_forward_workspace_bytes(N, D, V, dt), dev)
     rc = lib.cce_logp_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), targets.data_ptr(),
                               targets.element_size(), 0 if ignore_index is None else ignore_index,
                               ignore_index is not None, N, D, V, dt, logp.data_ptr(), mask.data_ptr(),
@@ -712,7 +712,7 @@ def distill_forward(e, c, bias, ids, teacher, mask, params):
     dev, (N, D), V, K, dt = e.device, e.shape, c.shape[0], ids.shape[1], _DTYPE_CODE[e.dtype]
     loss = torch.empty((N,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
     saved = _bytes(lib.cce_distill_saved_bytes(N, D, V, K, dt), dev)
-    ws = _bytes(lib.cce_distill_forward_workspace_bytes(N, V, K), dev)
+    ws = _bytes(lib.cce_distill_forward_workspace_bytes(N, D, V, K, dt), dev)
     rc = lib.cce_distill_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), ids.data_ptr(),
                                  ids.element_size(), teacher.data_ptr(), _addr(mask), N, D, V, K, dt, params,
                                  loss.data_ptr(), saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),

@@ -74,10 +74,14 @@ def test_abi_refusals():
     assert lib.cce_logp_backward(one, None, 0, one, 4, 8, 16, 2, 64, None, 0, None, None, None, None, 0,
                                  None) == _ext.CCE_ERR_ARG
     assert lib.cce_logp_backward(one, None, 0, one, 4, 8, 16, 2, 1, None, 0, None, None, None, None, 0,
+                                 None) == _ext.CCE_ERR_ARG  # grad_e is asked for and NULL
+    assert lib.cce_logp_backward(one, None, 0, one, 4, 8, 16, 2, 4, None, 0, None, None, one, None, 0,
+                                 None) == _ext.CCE_ERR_ARG  # grad_bias without a bias
+    assert lib.cce_logp_backward(one, None, 0, one, 4, 8, 16, 2, 1, None, 0, one, None, None, None, 0,
                                  None) == _ext.CCE_ERR_WORKSPACE
     assert lib.cce_distill_backward(one, None, 0, one, 4, 8, 16, 3, 2, ctypes.byref(p), 16, None, 0, None, None, None,
                                     None, 0, None) == _ext.CCE_ERR_ARG
-    assert lib.cce_distill_backward(one, None, 0, one, 4, 8, 16, 3, 2, ctypes.byref(p), 1, None, 0, None, None, None,
+    assert lib.cce_distill_backward(one, None, 0, one, 4, 8, 16, 3, 2, ctypes.byref(p), 1, None, 0, one, None, None,
                                     None, 0, None) == _ext.CCE_ERR_WORKSPACE
 
 
@@ -88,9 +92,14 @@ def test_saved_and_workspace_sizes():
     assert N * D * 2 < b < N * D * 2 + 64 * N + 4096     # the packed rows and a few values per row
     d = lib.cce_distill_saved_bytes(N, D, V, K, _ext.CCE_BF16)
     assert d >= N * D * 2 + N * K * 8 + N * (V // 256) * 2 and d < 2 * b
-    assert lib.cce_logp_forward_workspace_bytes(N, V) < N * V // 8   # never [N, V]
+    assert lib.cce_logp_forward_workspace_bytes(N, D, V, _ext.CCE_BF16) < N * V // 8   # never [N, V]
     flags = _ext.CCE_NEED_DE | _ext.CCE_NEED_DC
     plain = lib.cce_backward_workspace_bytes(N, D, V, _ext.CCE_BF16, flags)
-    assert plain < lib.cce_logp_backward_workspace_bytes(N, D, V, _ext.CCE_BF16, flags) < plain + 64 * N
+    # the same chunk buffers (without the filter's lists of live tiles) and a few values per row
+    rows = lib.cce_logp_backward_workspace_bytes(N, D, V, _ext.CCE_BF16, flags)
+    assert plain - (1 << 20) < rows < plain + 64 * N
+    # float32: both parts of c, and a bounded chunk of the dlogits' parts
+    f32 = lib.cce_logp_backward_workspace_bytes(N, D, V, _ext.CCE_F32, flags)
+    assert V * D * 4 < f32 < V * D * 4 + 3 * (1 << 29)
     assert lib.cce_distill_saved_bytes(N, D, V, 1025, _ext.CCE_BF16) == 0
     assert lib.cce_logp_saved_bytes(-1, D, V, _ext.CCE_BF16) == 0
