@@ -216,9 +216,9 @@ __global__ void fill_f32_kernel(float* __restrict__ dst, float v, int64_t n) {
 }
 
 // One block: s = smallest power of two >= max |x| (exact scaling for fp16
-// dlogits, which then lie in [-1, 1]), times 2^-up; s = 2^-up when every x is zero.
+// dlogits, which then lie in [-1, 1]); s = 1 when every x is zero.
 __global__ void __launch_bounds__(1024) pow2_absmax_kernel(const float* __restrict__ x, int64_t n,
-                                                           float* __restrict__ out, int up) {
+                                                           float* __restrict__ out) {
   __shared__ float red[32];
   float m = 0.f;
   for (int64_t i = threadIdx.x; i < n; i += blockDim.x) m = fmaxf(m, fabsf(x[i]));
@@ -237,7 +237,6 @@ __global__ void __launch_bounds__(1024) pow2_absmax_kernel(const float* __restri
         const float f = frexpf(m, &ex);  // m = f * 2^ex, f in [0.5, 1)
         s = ldexpf(1.f, f == 0.5f ? ex - 1 : ex);
       }
-      s = ldexpf(s, -up);
       out[0] = s;
       out[1] = 1.f / s;
     }
@@ -421,8 +420,8 @@ cudaError_t launch_dequantize(const uint32_t* wq, const void* scales, const void
   return cudaErrorInvalidValue;
 }
 
-cudaError_t launch_pow2_absmax(const float* x, int64_t n, float* out, int up, cudaStream_t stream) {
-  pow2_absmax_kernel<<<1, 1024, 0, stream>>>(x, n, out, up);
+cudaError_t launch_pow2_absmax(const float* x, int64_t n, float* out, cudaStream_t stream) {
+  pow2_absmax_kernel<<<1, 1024, 0, stream>>>(x, n, out);
   return launched();
 }
 

@@ -135,7 +135,6 @@ struct BwdPlan {
   int splits;            // CUDA-core path: K splits of grad_e (partials part_bytes)
   size_t part_bytes;
   size_t list_bytes;     // tensor-core path: the dlogits live-tile lists of every chunk
-  int slabs;             // tensor-core path: K splits of grad_e
 };
 
 bool tc_candidate(int dtype, int64_t D) { return dtype != CCE_F32 && D % 8 == 0; }
@@ -161,21 +160,7 @@ bool dl_list_enabled() {
   return v;
 }
 
-// K splits (fp32 slabs) of the tensor-core grad_e: two with the filter.  Exact
-// gradients of a few packed rows take as many as give every SM a work unit
-// (128 rows x 512 columns x a K range of at least 1024) within 64 MiB of slabs:
-// 331 x 1024 x 32000 has 6 such tiles, and its grad_e took 200 us in 12 units.
-int rows_slabs(int64_t N, int64_t D, int64_t vc) {
-  const int64_t tiles = cce::ceil_div(N > 0 ? N : 1, 128) * cce::ceil_div(D, 512);
-  int64_t s = cce::ceil_div(148, tiles);
-  const int64_t fit = (64ll << 20) / ((N > 0 ? N : 1) * D * 4);
-  if (s > fit) s = fit;
-  if (s > vc / 1024) s = vc / 1024;
-  if (s > 32) s = 32;
-  return s < 2 ? 2 : (int)s;
-}
-
-BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool tc, bool rows = false) {
+BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool tc) {
   BwdPlan p{};
   p.tc = tc;
   const int64_t gran = tc ? 256 : 128;
@@ -199,7 +184,6 @@ BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, boo
   const int64_t vmax = cce::round_up(V > 0 ? V : 1, gran);
   if (vc > vmax) vc = vmax;
   p.vc = vc;
-  p.slabs = rows ? rows_slabs(N, D, vc) : 2;
   p.keep_bytes = align_up((size_t)cce::ceil_div(N, cce::kRowBlock) * (size_t)cce::ceil_div(V, cce::kStatTile));
   // grad_c's view of the mask: per 128-column tile a bit per row block
   p.keep_t_ld = tc ? cce::ceil_div(cce::ceil_div(N, cce::kRowBlock), 32) : 0;
@@ -209,13 +193,13 @@ BwdPlan plan_backward(int64_t N, int64_t D, int64_t V, int dtype, int flags, boo
   // (the two K halves of every chunk's grad_e GEMM), summed into grad_e at the
   // end; the SIMT path one [N][D] (none when grad_e itself is fp32).
   if (!(flags & CCE_NEED_DE)) p.acc_bytes = 0;
-  else if (tc) p.acc_bytes = align_up((size_t)p.slabs * (size_t)N * (size_t)D * 4);
+  else if (tc) p.acc_bytes = align_up(2 * (size_t)N * (size_t)D * 4);
   else p.acc_bytes = (flags & CCE_DE_F32) ? 0 : align_up((size_t)N * (size_t)D * 4);
   // four counters per vocabulary chunk: the tile claims of the three
   // dynamically scheduled kernels and the dlogits live-tile count
   const int64_t nch = cce::ceil_div(V > 0 ? V : 1, vc);
   p.counter_bytes = align_up((size_t)nch * 4 * sizeof(int));
-  p.list_bytes = (tc && !rows && dl_list_enabled()) ? align_up((size_t)nch * (size_t)cce::tc_dlogits_list_len(nrow, vc) * sizeof(int)) : 0;
+  p.list_bytes = (tc && dl_list_enabled()) ? align_up((size_t)nch * (size_t)cce::tc_dlogits_list_len(nrow, vc) * sizeof(int)) : 0;
   p.scale_bytes = (tc && dtype == CCE_F16) ? kAlign : 0;  // {s, 1/s} for fp16 dlogits
   p.splits = (!tc && (flags & CCE_NEED_DE)) ? cce::simt_grad_e_splits(N, D, vc) : 1;
   p.part_bytes = p.splits > 1 ? align_up((size_t)p.splits * (size_t)N * (size_t)D * 4) : 0;
@@ -505,11 +489,11 @@ static size_t chunk_buf_bytes(const BwdPlan& p, int64_t D, int dtype) {
   return align_up((size_t)p.vc * (size_t)D * dtype_size(dtype));
 }
 
-static size_t backward_ws_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool quant, bool rows = false) {
+static size_t backward_ws_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags, bool quant) {
   const BwdPlan ps = plan_backward(N, D, V, dtype, flags, false);
   size_t b = plan_bytes(ps) + (quant ? 2 * chunk_buf_bytes(ps, D, dtype) : 0);
   if (tc_candidate(dtype, D)) {
-    const BwdPlan pt = plan_backward(N, D, V, dtype, flags, true, rows);
+    const BwdPlan pt = plan_backward(N, D, V, dtype, flags, true);
     const size_t t = plan_bytes(pt) + (quant ? 2 * chunk_buf_bytes(pt, D, dtype) : 0);
     if (t > b) b = t;
   }
@@ -661,27 +645,16 @@ size_t cce_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, 
   return backward_ws_bytes(N, D, V, dtype, flags, false);
 }
 
-// Packed rows of a loss on log-probabilities (`e`, d_nll, lse and targets are
-// those of the packed rows; grad_e goes back to the batch's rows).
-struct RowsBwd {
-  cce::RowsView R;
-  cce::TopkView topk;    // distillation: the listed columns, d_nll the others' coefficient
-  const float* d;        // cotangent of each packed row (0: not computed)
-  float logit_scale;
-  float* bias_part;      // [ceil(N / 32)][chunk rows] when grad_bias is requested (tensor-core path)
-};
-
 // cce_backward, cce_backward_peer when `pg` is given (grad_e summed over the
 // group through the exchange buffers), and cce_backward_q when `qh` is given
 // (c is a quantised head: every vocabulary chunk is expanded into one of two
 // workspace buffers on a side stream while the previous chunk's GEMMs run).
-// With `rb` the gradients of a loss on log-probabilities, exact (no filter).
 static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, const void* bias, int bias_dtype,
                          const int32_t* targets, const float* lse, const float* d_nll,
                          const float* tile_max, int64_t N, int64_t D, int64_t V, int64_t v_offset,
                          int dtype, int flags, float filter_log_eps, void* grad_e, void* grad_c,
                          float* grad_bias, int64_t* skip_stats, void* workspace, size_t workspace_bytes,
-                         const CcePeerGroup* pg, const RowsBwd* rb, void* stream) {
+                         const CcePeerGroup* pg, void* stream) {
   int rc = check_sizes(N, D, V, dtype);
   if (rc) return rc;
   if (bias && !dtype_ok(bias_dtype)) return fail(CCE_ERR_DTYPE, "unsupported bias dtype code %d", bias_dtype);
@@ -709,13 +682,13 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
     if (need_db) CCE_CUDA_CHECK(cudaMemsetAsync(grad_bias, 0, (size_t)V * sizeof(float), s), "memset grad_bias");
     return CCE_OK;
   }
-  if (!e || (!c && !qh) || !lse || !d_nll || (!rb && (!targets || !tile_max)))
+  if (!e || (!c && !qh) || !targets || !lse || !d_nll || !tile_max)
     return fail(CCE_ERR_ARG, "cce_backward: NULL required pointer");
   // (a quantised head's chunks live in the workspace: its alignment stands for c's)
   const bool tc = !force_simt() && cce::tc_backward_supported(e, qh ? workspace : c, D, dtype) &&
                   aligned16(workspace) && (!need_de || aligned16(grad_e)) && (!need_dc || aligned16(grad_c));
-  const BwdPlan p = plan_backward(N, D, V, dtype, flags, tc, rb != nullptr);
-  const size_t need = backward_ws_bytes(N, D, V, dtype, flags, qh != nullptr, rb != nullptr);
+  const BwdPlan p = plan_backward(N, D, V, dtype, flags, tc);
+  const size_t need = backward_ws_bytes(N, D, V, dtype, flags, qh != nullptr);
   if (!workspace || workspace_bytes < need)
     return fail(CCE_ERR_WORKSPACE, "cce_backward: workspace %zu bytes < required %zu", workspace_bytes, need);
 
@@ -760,31 +733,17 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
   }
   if (p.tc) CCE_CUDA_CHECK(cudaMemsetAsync(counters, 0, p.counter_bytes, s), "cce_backward memset counters");
   if (keep_t) CCE_CUDA_CHECK(cudaMemsetAsync(keep_t, 0, p.keep_t_bytes, s), "cce_backward memset mask table");
-  // (dlogits are at most the cotangent in magnitude.  Exact gradients put the
-  // largest at 2^14 of fp16's 65504: a softmax value of 2^-28 is still a normal number)
-  if (scale) CCE_CUDA_CHECK(cce::launch_pow2_absmax(rb ? rb->d : d_nll, N, scale, rb ? 14 : 0, s), "cce_backward scale");
+  if (scale) CCE_CUDA_CHECK(cce::launch_pow2_absmax(d_nll, N, scale, s), "cce_backward scale");
 
-  if (rb)
-    CCE_CUDA_CHECK(cce::launch_live_mask(rb->d, N, V, keep, keep_t, p.keep_t_ld, s), "cce_backward mask");
-  else
-    CCE_CUDA_CHECK(cce::launch_block_mask(tile_max, lse, targets, d_nll, N, V, v_offset, filter_log_eps,
-                                          (flags & CCE_NO_FILTER) != 0, keep, keep_t, p.keep_t_ld, skip_stats, s),
-                   "cce_backward mask");
+  CCE_CUDA_CHECK(cce::launch_block_mask(tile_max, lse, targets, d_nll, N, V, v_offset, filter_log_eps,
+                                        (flags & CCE_NO_FILTER) != 0, keep, keep_t, p.keep_t_ld, skip_stats, s),
+                 "cce_backward mask");
   if (need_db) CCE_CUDA_CHECK(cudaMemsetAsync(grad_bias, 0, (size_t)V * sizeof(float), s), "memset grad_bias");
   if (dl_lists)
     CCE_CUDA_CHECK(cce::tc_dlogits_lists(keep, N, D, V, p.vc, dl_lists, counters, s), "cce_backward dlogits lists");
 
   cce::BwdChunkArgs a{e, c, nullptr, bias, bias_dtype, targets, lse, d_nll, keep, keep_t, p.keep_t_ld, N, D, V,
-                      v_offset, dtype, 0, 0, p.vc, dl, need_db && !rb ? grad_bias : nullptr, nullptr, scale};
-  if (rb) {
-    a.topk = rb->topk;
-    a.d_row = rb->d;
-    a.logit_scale = rb->logit_scale;
-    a.rows = rb->R.count;
-    a.slabs = p.slabs;
-    if (need_db && p.tc) a.bias_part = rb->bias_part;
-  }
-  const int64_t bias_parts = p.tc ? cce::ceil_div(N, 32) : N;  // (CUDA cores: the fp32 dlogits themselves)
+                      v_offset, dtype, 0, 0, p.vc, dl, need_db ? grad_bias : nullptr, nullptr, scale};
   const int64_t nchunks = cce::ceil_div(V, p.vc);
   const size_t esz = dtype_size(dtype);
   SideStreams* ss = nullptr;
@@ -832,12 +791,7 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
       a.c_chunk = static_cast<const char*>(c) + (size_t)a.vc0 * (size_t)D * esz;
     }
     if (p.tc) {
-      if (a.bias_part)
-        CCE_CUDA_CHECK(cudaMemsetAsync(a.bias_part, 0, (size_t)bias_parts * p.vc * sizeof(float), s), "cce_backward memset");
-      CCE_CUDA_CHECK(rb ? cce::tc_dlogits_rows(a, s) : cce::tc_dlogits(a, s), "cce_backward tc dlogits");
-      if (a.bias_part)
-        CCE_CUDA_CHECK(cce::launch_bias_sum(a.bias_part, bias_parts, p.vc, a.vc_len, scale, grad_bias + a.vc0, s),
-                       "cce_backward grad_bias");
+      CCE_CUDA_CHECK(cce::tc_dlogits(a, s), "cce_backward tc dlogits");
       CCE_CUDA_CHECK(cudaEventRecord(ss->ev_l, s), "cce_backward record");
       CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->se, ss->ev_l, 0), "cce_backward wait");
       CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->sc, ss->ev_l, 0), "cce_backward wait");
@@ -848,9 +802,6 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
           CCE_CUDA_CHECK(cce::peer::launch_reduce_gather(push.peers, push.layout, cce::peer::kSlotsPerSrc, N, D,
                                                          out_dtype, grad_e, wait_ns, ss->se),
                          "cce_backward_peer exchange");
-        else if (last && rb)
-          CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, p.slabs, rb->R.pos, N, D, out_dtype, grad_e, ss->se),
-                         "cce_backward scatter grad_e");
         else if (last)
           CCE_CUDA_CHECK(cce::launch_sum2_f32(acc, acc + N * D, grad_e, out_dtype, N * D, ss->se),
                          "cce_backward sum grad_e");
@@ -864,18 +815,12 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
       }
     } else {
       CCE_CUDA_CHECK(cce::simt_dlogits(a, s), "cce_backward simt dlogits");
-      if (rb && need_db)
-        CCE_CUDA_CHECK(cce::launch_bias_sum((const float*)dl, bias_parts, p.vc, a.vc_len, nullptr, grad_bias + a.vc0, s),
-                       "cce_backward grad_bias");
       if (need_de) CCE_CUDA_CHECK(cce::simt_grad_e(a, acc, ch > 0, part, p.splits, s), "cce_backward simt grad_e");
       if (need_dc) CCE_CUDA_CHECK(cce::simt_grad_c(a, grad_c, s), "cce_backward simt grad_c");
       if (need_de && last && exchange) {
         CCE_CUDA_CHECK(cce::peer::launch_push(push.peers, push.layout, acc, 1, N, D, s), "cce_backward_peer push");
         CCE_CUDA_CHECK(cce::peer::launch_reduce_gather(push.peers, push.layout, 1, N, D, out_dtype, grad_e, wait_ns, s),
                        "cce_backward_peer exchange");
-      } else if (need_de && last && rb) {
-        CCE_CUDA_CHECK(cce::launch_rows_scatter(acc, 1, rb->R.pos, N, D, out_dtype, grad_e, s),
-                       "cce_backward scatter grad_e");
       } else if (need_de && last && !(flags & CCE_DE_F32)) {
         CCE_CUDA_CHECK(cce::launch_cast_f32(acc, grad_e, dtype, N * D, s), "cce_backward cast grad_e");
       }
@@ -892,7 +837,7 @@ int cce_backward(const void* e, const void* c, const void* bias, int bias_dtype,
                  void* stream) {
   return backward_impl(e, c, nullptr, bias, bias_dtype, targets, lse, d_nll, tile_max, N, D, V, v_offset, dtype,
                        flags, filter_log_eps, grad_e, grad_c, grad_bias, skip_stats, workspace, workspace_bytes,
-                       nullptr, nullptr, stream);
+                       nullptr, stream);
 }
 
 int cce_backward_peer(const void* e, const void* c, const void* bias, int bias_dtype,
@@ -910,7 +855,7 @@ int cce_backward_peer(const void* e, const void* c, const void* bias, int bias_d
       return fail(CCE_ERR_ARG, "cce_backward_peer: buffer of rank %d is NULL or not 16-byte aligned", r);
   return backward_impl(e, c, nullptr, bias, bias_dtype, targets, lse, d_nll, tile_max, N, D, V, v_offset, dtype,
                        flags, filter_log_eps, grad_e, grad_c, grad_bias, skip_stats, workspace, workspace_bytes, group,
-                       nullptr, stream);
+                       stream);
 }
 
 size_t cce_backward_q_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
@@ -924,7 +869,7 @@ int cce_backward_q(const void* e, const CceQuantHead* head, const void* bias, in
   if (!head) return fail(CCE_ERR_ARG, "cce_backward_q: NULL head");
   return backward_impl(e, nullptr, head, bias, bias_dtype, targets, lse, d_nll, tile_max, N, D, V, v_offset, dtype,
                        flags, filter_log_eps, grad_e, nullptr, grad_bias, skip_stats, workspace, workspace_bytes,
-                       nullptr, nullptr, stream);
+                       nullptr, stream);
 }
 
 size_t cce_peer_buffer_bytes(int64_t N, int64_t D, int world, int out_dtype) {
@@ -1179,6 +1124,12 @@ struct Parts {
   }
 };
 
+// Widths of the GEMMs' operands and outputs: rows start on 16-byte boundaries
+// (TMA), float16 parts of float32 fill whole 64-column blocks.  Other widths
+// run on padded copies.
+int64_t rows_dk(int64_t D, int dtype) { return cce::round_up(D, dtype == CCE_F32 ? 64 : 8); }
+int64_t rows_dout(int64_t D, int dtype) { return cce::round_up(D, dtype == CCE_F32 ? 4 : 8); }
+
 // What the forward calls leave for the backward calls.
 struct RowsSaved {
   cce::RowsView R;
@@ -1186,14 +1137,10 @@ struct RowsSaved {
   float* A;         // distillation
   float* weight;    // distillation [1]
   cce::TopkView topk;
-  void* e;          // packed rows
-  cce::SplitView split;  // or their two parts (float32 on tensor cores)
+  float* se;        // float32: scale of e's parts
+  void *e, *e_lo;   // packed rows [N][Dk]
   size_t bytes;
 };
-
-// float32 rows run on the tensor cores as two float16 parts (rows of the outputs
-// must start on 16-byte boundaries); others on the CUDA cores.
-bool split_path(int64_t D, int dtype) { return dtype == CCE_F32 && D % 4 == 0 && !force_simt() && cce::tc_available(); }
 
 RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
   Parts p{static_cast<char*>(base)};
@@ -1212,63 +1159,69 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
     r.topk.start = p.take<uint16_t>((size_t)N * r.topk.tiles1);
     r.topk.z = p.take<float>((size_t)N * K);
   }
-  if (split_path(D, dtype)) {
-    r.split.Dp = cce::round_up(D, 64);
-    float* se = p.take<float>(2);
-    r.split.se = se;
-    r.split.e_hi = p.take<uint16_t>((size_t)N * r.split.Dp);
-    r.split.e_lo = p.take<uint16_t>((size_t)N * r.split.Dp);
-  } else {
-    r.e = p.take<char>((size_t)N * D * dtype_size(dtype));
+  const size_t n = (size_t)N * rows_dk(D, dtype);
+  r.e = p.take<uint16_t>(n);
+  if (dtype == CCE_F32) {
+    r.e_lo = p.take<uint16_t>(n);
+    r.se = p.take<float>(2);
   }
   r.bytes = p.used;
   return r;
 }
 
-// c's two parts, its scale, and the words the largest values go to.
-struct SplitWs {
-  void *c_hi, *c_lo;
+// c as an operand: itself, a padded copy, or float16 parts with their scale.
+struct RowsC {
+  void *c, *c_lo;
   float* sc;
-  uint32_t* words;
+  uint32_t* words;  // largest values of c and e
 };
 
-SplitWs split_ws(Parts& p, int64_t D, int64_t V, int dtype) {
-  SplitWs w{};
-  if (!split_path(D, dtype)) return w;
-  w.words = p.take<uint32_t>(2);
-  w.sc = p.take<float>(2);
-  w.c_hi = p.take<uint16_t>((size_t)V * cce::round_up(D, 64));
-  w.c_lo = p.take<uint16_t>((size_t)V * cce::round_up(D, 64));
+RowsC rows_c(Parts& p, int64_t D, int64_t V, int dtype) {
+  RowsC w{};
+  const size_t n = (size_t)V * rows_dk(D, dtype);
+  if (dtype == CCE_F32) {
+    w.words = p.take<uint32_t>(2);
+    w.sc = p.take<float>(2);
+    w.c = p.take<uint16_t>(n);
+    w.c_lo = p.take<uint16_t>(n);
+  } else if (D % 8 != 0) {
+    w.c = p.take<uint16_t>(n);
+  }
   return w;
 }
 
-// c into its parts (`v` gets them); with e != nullptr its packed rows into the saved ones too.
-cudaError_t split_operands(RowsSaved& v, const SplitWs& w, const void* e, const void* c, int64_t N, int64_t D,
-                           int64_t V, cudaStream_t s) {
-  v.split.c_hi = w.c_hi, v.split.c_lo = w.c_lo, v.split.sc = w.sc;
-  cudaError_t err = cudaMemsetAsync(w.words, 0, 2 * sizeof(uint32_t), s);
-  if (err != cudaSuccess) return err;
-  if (e) {
-    if ((err = cce::launch_absmax((const float*)e, N, D, &v.R, w.words + 1, s)) != cudaSuccess) return err;
-    if ((err = cce::launch_split((const float*)e, N, D, v.split.Dp, &v.R, w.words + 1, const_cast<float*>(v.split.se),
-                                 const_cast<void*>(v.split.e_hi), const_cast<void*>(v.split.e_lo), s)) != cudaSuccess)
-      return err;
+// The operands' part of the GEMM arguments.  e != nullptr (the forward call):
+// its packed rows go to the saved copy first.
+cudaError_t rows_operands(cce::RowsGemmArgs& a, const RowsSaved& v, const RowsC& w, const void* e, const void* c,
+                          int64_t D, cudaStream_t s) {
+  a.e = v.e, a.e_lo = v.e_lo, a.se = v.se;
+  a.c = w.c ? w.c : c, a.c_lo = w.c_lo, a.sc = w.sc;
+  cudaError_t err = cudaSuccess;
+  if (a.dtype == CCE_F32) {
+    if ((err = cudaMemsetAsync(w.words, 0, 2 * sizeof(uint32_t), s)) != cudaSuccess) return err;
+    if (e) {
+      if ((err = cce::launch_absmax((const float*)e, a.N, D, &v.R, w.words + 1, s)) != cudaSuccess) return err;
+      if ((err = cce::launch_split((const float*)e, a.N, D, a.Dk, &v.R, w.words + 1, v.se, v.e, v.e_lo, s)) != cudaSuccess)
+        return err;
+    }
+    if ((err = cce::launch_absmax((const float*)c, a.V, D, nullptr, w.words, s)) != cudaSuccess) return err;
+    return cce::launch_split((const float*)c, a.V, D, a.Dk, nullptr, w.words, w.sc, w.c, w.c_lo, s);
   }
-  if ((err = cce::launch_absmax((const float*)c, V, D, nullptr, w.words, s)) != cudaSuccess) return err;
-  return cce::launch_split((const float*)c, V, D, v.split.Dp, nullptr, w.words, w.sc, w.c_hi, w.c_lo, s);
+  if (e && (err = cce::launch_rows_copy(e, a.N, D, D, &v.R, v.e, a.Dk, s)) != cudaSuccess) return err;
+  return w.c ? cce::launch_rows_copy(c, a.V, D, D, nullptr, w.c, a.Dk, s) : cudaSuccess;
 }
 
 struct RowsFwdWs {
   float *part_m, *part_s, *tgt, *p, *rest;
   cce::DistillSum* sums;
-  SplitWs split;
+  RowsC c;
   size_t bytes;
 };
 
 RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
   Parts p{static_cast<char*>(base)};
   RowsFwdWs w{};
-  const size_t parts = (size_t)cce::ceil_div(V, cce::kSimtLseTile) * N;
+  const size_t parts = (size_t)cce::ceil_div(V, 128) * N;
   w.part_m = p.take<float>(parts);
   w.part_s = p.take<float>(parts);
   if (K == 0) {
@@ -1278,119 +1231,71 @@ RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t D, int64_t V, int64_t K, in
     w.rest = p.take<float>(N);
     w.sums = p.take<cce::DistillSum>(cce::distill_blocks(N));
   }
-  w.split = split_ws(p, D, V, dtype);
+  w.c = rows_c(p, D, V, dtype);
   w.bytes = p.used;
   return w;
 }
 
-// Chunks and buffers of the float32 backward pass on tensor cores.
-struct SplitPlan {
-  int64_t vc;  // vocabulary rows of a chunk (both parts of its dlogits: 4 N vc bytes)
-  int slabs;   // K splits of grad_e
+// Vocabulary rows per backward chunk (its dlogits buffer: the filtered backward's
+// bounds) and K splits of grad_e.
+struct RowsPlan {
+  int64_t vc;
+  int slabs;
 };
 
-SplitPlan split_plan(int64_t N, int64_t D, int64_t V) {
-  const int64_t n = N > 0 ? N : 1;
+RowsPlan rows_plan(int64_t N, int64_t D, int64_t V, int dtype) {
+  const int64_t n = N > 0 ? N : 1, elt = dtype == CCE_F32 ? 4 : 2;
   const int64_t target = target_chunk_rows();
-  int64_t budget = n * 4 * target;
+  int64_t budget = n * elt * target;
   if (budget > kDlMaxBytes) budget = kDlMaxBytes;
   if (budget < kDlMinBytes && target == kDlTargetRows) budget = kDlMinBytes;
-  SplitPlan p;
-  p.vc = budget / (n * 4) / 256 * 256;
+  RowsPlan p;
+  p.vc = budget / (n * elt) / 256 * 256;
   if (p.vc < 256) p.vc = 256;
+  if (target == kDlTargetRows && n * 2 * target < kDlSmallNBytes) {
+    // few rows: longer chunks, up to 512 MiB and half of the vocabulary
+    const int64_t half = cce::round_up(cce::ceil_div(V, 2), 256);
+    int64_t grow = kDlSmallNGrowBytes / (n * elt) / 256 * 256;
+    if (grow > half) grow = half;
+    if (grow > p.vc) p.vc = grow;
+  }
   const int64_t vmax = cce::round_up(V, 256);
   if (p.vc > vmax) p.vc = vmax;
-  // two units per SM of (128 rows, 256 columns, at least 512 of K), within 256 MiB of slabs
+  // enough units of (128 rows, 256 columns, at least kMinK of K) for every SM to
+  // have two, within 256 MiB of fp32 slabs
+  constexpr int64_t kMinK = 512;
   const int64_t tiles = cce::ceil_div(n, 128) * cce::ceil_div(D, 256);
   int64_t sl = cce::ceil_div(2 * 148, tiles);
   const int64_t fit = (256ll << 20) / (n * D * 4);
   if (sl > fit) sl = fit;
-  if (sl > p.vc / 512) sl = p.vc / 512;
+  if (sl > p.vc / kMinK) sl = p.vc / kMinK;
   if (sl > 32) sl = 32;
   p.slabs = sl < 1 ? 1 : (int)sl;
   return p;
 }
 
 struct RowsBwdWs {
-  void* base;  // backward_impl's own
-  size_t base_bytes;
-  float *d, *dA, *bias_part;
-  SplitWs split;
-  void *dl_hi, *dl_lo;
-  float *slabs, *scale;
+  RowsC c;
+  void *dl, *dl_lo;
+  float *slabs, *scale, *bias_part;
+  void* grad_c;  // padded rows
   size_t bytes;
 };
 
-RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, int flags, bool topk) {
+RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, int flags) {
   Parts p{static_cast<char*>(base)};
   RowsBwdWs w{};
-  int64_t vc = 0;
-  if (split_path(D, dtype)) {
-    const SplitPlan sp = split_plan(N, D, V);
-    vc = sp.vc;
-    w.split = split_ws(p, D, V, dtype);
-    w.dl_hi = p.take<uint16_t>((size_t)N * vc);
-    w.dl_lo = p.take<uint16_t>((size_t)N * vc);
-    if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)sp.slabs * N * D);
-    w.scale = p.take<float>(2);
-  } else {
-    w.base_bytes = backward_ws_bytes(N, D, V, dtype, flags, false, true);
-    w.base = p.take<char>(w.base_bytes);
-    if (tc_candidate(dtype, D)) vc = plan_backward(N, D, V, dtype, flags, true, true).vc;
-  }
-  w.d = p.take<float>(N);
-  if (topk) w.dA = p.take<float>(N);
-  if ((flags & CCE_NEED_DBIAS) && vc > 0) w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * vc);
+  const RowsPlan pl = rows_plan(N, D, V, dtype);
+  const int64_t dout = rows_dout(D, dtype);
+  w.c = rows_c(p, D, V, dtype);
+  w.dl = p.take<uint16_t>((size_t)N * pl.vc);
+  if (dtype == CCE_F32) w.dl_lo = p.take<uint16_t>((size_t)N * pl.vc);
+  if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)pl.slabs * N * dout);
+  if (dtype != CCE_BF16) w.scale = p.take<float>(2);
+  if (flags & CCE_NEED_DBIAS) w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * pl.vc);
+  if ((flags & CCE_NEED_DC) && dout != D) w.grad_c = p.take<char>((size_t)V * dout * dtype_size(dtype));
   w.bytes = p.used;
   return w;
-}
-
-// Gradients of float32 rows from two-part operands: per vocabulary chunk the
-// dlogits' two parts, then grad_e's K splits into fp32 slabs and grad_c's rows.
-int split_backward(RowsSaved v, const RowsBwdWs& w, const RowsBwd& rb, const void* c, const void* bias, int bias_dtype,
-                   const float* g, int64_t N, int64_t D, int64_t V, int flags, void* grad_e, void* grad_c,
-                   float* grad_bias, cudaStream_t s) {
-  const char* what = "float32 backward";
-  const bool need_de = flags & CCE_NEED_DE, need_dc = flags & CCE_NEED_DC, need_db = flags & CCE_NEED_DBIAS;
-  if ((need_de && !aligned16(grad_e)) || (need_dc && !aligned16(grad_c)))
-    return fail(CCE_ERR_ALIGN, "%s: gradients must start on 16-byte boundaries", what);
-  const SplitPlan sp = split_plan(N, D, V);
-  CCE_CUDA_CHECK(split_operands(v, w.split, nullptr, c, N, D, V, s), what);
-  // the largest cotangent's dlogit at 2^13: hi and lo as in split_operands
-  CCE_CUDA_CHECK(cce::launch_pow2_absmax(rb.d, N, w.scale, 14, s), what);
-  cce::BwdChunkArgs a{};
-  a.bias = bias, a.bias_dtype = bias_dtype;
-  a.targets = v.R.targets, a.lse = v.lse, a.d_nll = g, a.d_row = rb.d;
-  a.N = N, a.D = D, a.V = V, a.dtype = CCE_F32;
-  a.vc_ld = sp.vc, a.dlogits = w.dl_hi, a.dlogits_lo = w.dl_lo, a.scale = w.scale;
-  a.topk = rb.topk, a.logit_scale = rb.logit_scale, a.rows = v.R.count, a.split = v.split;
-  a.bias_part = need_db ? w.bias_part : nullptr;
-  const int64_t parts = cce::ceil_div(N, 32);
-  for (a.vc0 = 0; a.vc0 < V; a.vc0 += sp.vc) {
-    a.vc_len = V - a.vc0 < sp.vc ? V - a.vc0 : sp.vc;
-    if (need_db) CCE_CUDA_CHECK(cudaMemsetAsync(w.bias_part, 0, (size_t)parts * sp.vc * sizeof(float), s), what);
-    CCE_CUDA_CHECK(cce::tc_dlogits_rows(a, s), what);
-    if (need_db)
-      CCE_CUDA_CHECK(cce::launch_bias_sum(w.bias_part, parts, sp.vc, a.vc_len, w.scale, grad_bias + a.vc0, s), what);
-    if (need_de) CCE_CUDA_CHECK(cce::tc_grad_e_split(a, w.slabs, sp.slabs, a.vc0 > 0, s), what);
-    if (need_dc) CCE_CUDA_CHECK(cce::tc_grad_c_split(a, (float*)grad_c, s), what);
-  }
-  if (need_de) CCE_CUDA_CHECK(cce::launch_rows_scatter(w.slabs, sp.slabs, v.R.pos, N, D, CCE_F32, grad_e, s), what);
-  return CCE_OK;
-}
-
-// Argument checks shared by the two backward calls; *done: nothing is left to do.
-int check_rows_backward(const void* bias, int bias_dtype, int64_t N, int64_t V, int64_t D, int dtype, int flags,
-                        const void* grad_e, const void* grad_c, const void* grad_bias, const char* what) {
-  if (flags & ~(CCE_NEED_DE | CCE_NEED_DC | CCE_NEED_DBIAS))
-    return fail(CCE_ERR_ARG, "%s: unknown flag bits 0x%x", what, flags);
-  if (bias && !dtype_ok(bias_dtype)) return fail(CCE_ERR_DTYPE, "%s: unsupported bias dtype code %d", what, bias_dtype);
-  if (((flags & CCE_NEED_DE) && N > 0 && !grad_e) || ((flags & CCE_NEED_DC) && !grad_c) ||
-      ((flags & CCE_NEED_DBIAS) && !grad_bias))
-    return fail(CCE_ERR_ARG, "%s: a requested gradient has a NULL output pointer", what);
-  if ((flags & CCE_NEED_DBIAS) && !bias) return fail(CCE_ERR_ARG, "%s: CCE_NEED_DBIAS without bias", what);
-  (void)V, (void)D, (void)dtype;
-  return CCE_OK;
 }
 
 int check_rows(int64_t N, int64_t D, int64_t V, int64_t K, int dtype, const char* what) {
@@ -1413,10 +1318,118 @@ int check_distill(const CceDistillParams* p, const char* what) {
   return CCE_OK;
 }
 
-cudaError_t rows_logits(const cce::FwdArgs& f, cudaStream_t s) {
-  if (f.split.e_hi) return cce::tc_logits(f, s);
-  // (the packed copy of e is aligned whatever e was)
-  return !force_simt() && cce::tc_supported(f.e, f.c, f.D, f.dtype) ? cce::tc_logits(f, s) : cce::simt_logits(f, s);
+// The device and what the operands' TMA loads ask of c.
+int check_rows_device(const void* c, int64_t D, int dtype, const char* what) {
+  int rc = check_arch();
+  if (rc) return rc;
+  if (!cce::tc_available()) return fail(CCE_ERR_CUDA, "%s: the driver's tensor-map encoder is unavailable", what);
+  if (dtype != CCE_F32 && D % 8 == 0 && !aligned16(c))
+    return fail(CCE_ERR_ALIGN, "%s: c must start on a 16-byte boundary", what);
+  return CCE_OK;
+}
+
+// Argument checks shared by the two backward calls.
+int check_rows_backward(const void* bias, int bias_dtype, int64_t N, int flags, const void* grad_e, const void* grad_c,
+                        const void* grad_bias, const char* what) {
+  if (flags & ~(CCE_NEED_DE | CCE_NEED_DC | CCE_NEED_DBIAS))
+    return fail(CCE_ERR_ARG, "%s: unknown flag bits 0x%x", what, flags);
+  if (bias && !dtype_ok(bias_dtype)) return fail(CCE_ERR_DTYPE, "%s: unsupported bias dtype code %d", what, bias_dtype);
+  if (((flags & CCE_NEED_DE) && N > 0 && !grad_e) || ((flags & CCE_NEED_DC) && !grad_c) ||
+      ((flags & CCE_NEED_DBIAS) && !grad_bias))
+    return fail(CCE_ERR_ARG, "%s: a requested gradient has a NULL output pointer", what);
+  if ((flags & CCE_NEED_DBIAS) && !bias) return fail(CCE_ERR_ARG, "%s: CCE_NEED_DBIAS without bias", what);
+  if ((flags & CCE_NEED_DC) && !aligned16(grad_c))
+    return fail(CCE_ERR_ALIGN, "%s: grad_c must start on a 16-byte boundary", what);
+  return CCE_OK;
+}
+
+// Gradients of the packed rows: per vocabulary chunk the dlogits, then grad_e's K
+// splits (added into fp32 slabs) beside grad_c's rows on two side streams.
+int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, const void* c, int64_t D, int flags,
+                  void* grad_e, void* grad_c, float* grad_bias, cudaStream_t s, const char* what) {
+  const bool need_de = flags & CCE_NEED_DE, need_dc = flags & CCE_NEED_DC, need_db = flags & CCE_NEED_DBIAS;
+  if (!need_de && !need_dc && !need_db) return CCE_OK;
+  const RowsPlan pl = rows_plan(a.N, D, a.V, a.dtype);
+  CCE_CUDA_CHECK(rows_operands(a, v, w.c, nullptr, c, D, s), what);
+  a.R = v.R, a.topk = v.topk, a.lse = v.lse, a.A = v.A;
+  a.dl = w.dl, a.dl_lo = w.dl_lo, a.vc_ld = pl.vc, a.scale = w.scale;
+  a.bias_part = need_db ? w.bias_part : nullptr;
+  if (w.scale) CCE_CUDA_CHECK(cce::launch_rows_scale(a.up, v.R, w.scale, s), what);
+  const bool fork = need_de && need_dc;
+  SideStreams* ss = nullptr;
+  cudaStream_t se = s, sc = s;
+  if (fork) {
+    int rc = side_streams(&ss);
+    if (rc) return rc;
+    se = ss->se, sc = ss->sc;
+  }
+  void* gc = w.grad_c ? w.grad_c : grad_c;
+  for (a.vc0 = 0; a.vc0 < a.V; a.vc0 += pl.vc) {
+    a.vc_len = a.V - a.vc0 < pl.vc ? a.V - a.vc0 : pl.vc;
+    if (fork && a.vc0 > 0) {  // the last chunk's dlogits have been read
+      CCE_CUDA_CHECK(cudaStreamWaitEvent(s, ss->ev_e, 0), what);
+      CCE_CUDA_CHECK(cudaStreamWaitEvent(s, ss->ev_c, 0), what);
+    }
+    CCE_CUDA_CHECK(cce::tc_dlogits_rows(a, s), what);
+    if (fork) {
+      CCE_CUDA_CHECK(cudaEventRecord(ss->ev_l, s), what);
+      CCE_CUDA_CHECK(cudaStreamWaitEvent(se, ss->ev_l, 0), what);
+      CCE_CUDA_CHECK(cudaStreamWaitEvent(sc, ss->ev_l, 0), what);
+    }
+    if (need_db)
+      CCE_CUDA_CHECK(cce::launch_bias_sum(w.bias_part, cce::ceil_div(a.N, 32), v.R, pl.vc, a.vc_len, w.scale,
+                                          grad_bias + a.vc0, s),
+                     what);
+    if (need_de) {
+      CCE_CUDA_CHECK(cce::tc_grad_e_rows(a, w.slabs, pl.slabs, a.vc0 > 0, se), what);
+      if (a.vc0 + pl.vc >= a.V)
+        CCE_CUDA_CHECK(cce::launch_rows_scatter(w.slabs, pl.slabs, a.Dout, v.R.pos, a.N, D, a.dtype, grad_e, se), what);
+    }
+    if (need_dc) {
+      CCE_CUDA_CHECK(cce::tc_grad_c_rows(a, gc, sc), what);
+      if (w.grad_c) {  // (16-bit units: two per float32)
+        const int64_t u = (int64_t)dtype_size(a.dtype) / 2;
+        const size_t row = dtype_size(a.dtype);
+        CCE_CUDA_CHECK(cce::launch_rows_copy((char*)gc + (size_t)a.vc0 * a.Dout * row, a.vc_len, D * u, a.Dout * u, nullptr,
+                                             (char*)grad_c + (size_t)a.vc0 * D * row, D * u, sc),
+                       what);
+      }
+    }
+    if (fork) {
+      CCE_CUDA_CHECK(cudaEventRecord(ss->ev_e, se), what);
+      CCE_CUDA_CHECK(cudaEventRecord(ss->ev_c, sc), what);
+    }
+  }
+  if (fork) {
+    CCE_CUDA_CHECK(cudaStreamWaitEvent(s, ss->ev_e, 0), what);
+    CCE_CUDA_CHECK(cudaStreamWaitEvent(s, ss->ev_c, 0), what);
+  }
+  return CCE_OK;
+}
+
+cce::RowsGemmArgs rows_args(const void* bias, int bias_dtype, int64_t N, int64_t D, int64_t V, int dtype) {
+  cce::RowsGemmArgs a{};
+  a.bias = bias, a.bias_dtype = bias_dtype, a.dtype = dtype;
+  a.N = N, a.V = V, a.Dk = rows_dk(D, dtype), a.Dout = rows_dout(D, dtype);
+  a.vc_len = V, a.scale_z = 1.f;
+  return a;
+}
+
+// No rows: every requested gradient is zero.
+int zero_grads(int64_t D, int64_t V, int dtype, int flags, void* grad_c, float* grad_bias, cudaStream_t s) {
+  if (flags & CCE_NEED_DC) CCE_CUDA_CHECK(cudaMemsetAsync(grad_c, 0, (size_t)V * D * dtype_size(dtype), s), "memset grad_c");
+  if (flags & CCE_NEED_DBIAS) CCE_CUDA_CHECK(cudaMemsetAsync(grad_bias, 0, (size_t)V * sizeof(float), s), "memset grad_bias");
+  return CCE_OK;
+}
+
+int check_space(const void* saved, size_t saved_bytes, size_t saved_need, const void* ws, size_t ws_bytes, size_t ws_need,
+                const char* what) {
+  if (!saved || saved_bytes < saved_need || !ws || ws_bytes < ws_need)
+    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
+                saved_need, ws_bytes, ws_need);
+  if (!aligned16(saved) || !aligned16(ws))
+    return fail(CCE_ERR_ALIGN, "%s: saved and workspace must start on 16-byte boundaries", what);
+  return CCE_OK;
 }
 
 }  // namespace
@@ -1432,7 +1445,7 @@ size_t cce_logp_forward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dty
 }
 
 size_t cce_logp_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
-  return N < 0 || D <= 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_bwd_ws(nullptr, N, D, V, dtype, flags, false).bytes;
+  return N < 0 || D <= 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_bwd_ws(nullptr, N, D, V, dtype, flags).bytes;
 }
 
 int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dtype, const void* targets,
@@ -1447,27 +1460,19 @@ int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dt
     return fail(CCE_ERR_ARG, "%s: targets of %d bytes (4 or 8 expected)", what, target_bytes);
   if (N == 0) return CCE_OK;
   if (!e || !c || !targets || !logp || !mask) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
-  RowsSaved v = rows_saved(saved, N, D, V, 0, dtype);
+  const RowsSaved v = rows_saved(saved, N, D, V, 0, dtype);
   const RowsFwdWs w = rows_fwd_ws(workspace, N, D, V, 0, dtype);
-  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
-    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
-                v.bytes, workspace_bytes, w.bytes);
-  rc = check_arch();
+  rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
+  if (!rc) rc = check_rows_device(c, D, dtype, what);
   if (rc) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  CCE_CUDA_CHECK(cce::launch_rows_pack(e, dtype, N, D, targets, target_bytes, ignore_index, has_ignore, nullptr, v.R,
-                                       mask, logp, v.e, w.tgt, s),
+  CCE_CUDA_CHECK(cce::launch_rows_pack(N, targets, target_bytes, ignore_index, has_ignore, nullptr, v.R, mask, logp, w.tgt, s),
                  what);
-  cce::FwdArgs f{v.e, c, bias, bias_dtype, v.R.targets, N, D, V, 0, dtype, nullptr, w.part_m, w.part_s, w.tgt};
-  f.rows = v.R.count;
-  if (v.split.Dp) {
-    CCE_CUDA_CHECK(split_operands(v, w.split, e, c, N, D, V, s), what);
-    f.split = v.split;
-  }
-  CCE_CUDA_CHECK(rows_logits(f, s), what);
-  CCE_CUDA_CHECK(cce::launch_rows_logp(w.part_m, w.part_s, cce::ceil_div(V, cce::kSimtLseTile), N, v.R, w.tgt, v.lse,
-                                       logp, s),
-                 what);
+  cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
+  a.R = v.R, a.part_m = w.part_m, a.part_s = w.part_s, a.tgt = w.tgt;
+  CCE_CUDA_CHECK(rows_operands(a, v, w.c, e, c, D, s), what);
+  CCE_CUDA_CHECK(cce::tc_logits(a, s), what);
+  CCE_CUDA_CHECK(cce::launch_rows_logp(w.part_m, w.part_s, cce::ceil_div(V, 128), N, v.R, w.tgt, v.lse, logp, s), what);
   return CCE_OK;
 }
 
@@ -1476,31 +1481,23 @@ int cce_logp_backward(const void* c, const void* bias, int bias_dtype, const flo
                       void* grad_c, float* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "cce_logp_backward";
   int rc = check_rows(N, D, V, 0, dtype, what);
+  if (!rc) rc = check_rows_backward(bias, bias_dtype, N, flags, grad_e, grad_c, grad_bias, what);
   if (rc) return rc;
-  rc = check_rows_backward(bias, bias_dtype, N, V, D, dtype, flags, grad_e, grad_c, grad_bias, what);
-  if (rc) return rc;
-  if (N == 0)
-    return backward_impl(nullptr, c, nullptr, bias, bias_dtype, nullptr, nullptr, nullptr, nullptr, N, D, V, 0, dtype,
-                         flags, 0.f, grad_e, grad_c, grad_bias, nullptr, workspace, workspace_bytes, nullptr, nullptr,
-                         stream);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (N == 0) {
+    rc = check_arch();
+    return rc ? rc : zero_grads(D, V, dtype, flags, grad_c, grad_bias, s);
+  }
   if (!grad_logp || !c) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
   const RowsSaved v = rows_saved(const_cast<void*>(saved), N, D, V, 0, dtype);
-  const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags, false);
-  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
-    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
-                v.bytes, workspace_bytes, w.bytes);
-  rc = check_arch();
+  const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags);
+  rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
+  if (!rc) rc = check_rows_device(c, D, dtype, what);
   if (rc) return rc;
-  // d logp / dz = onehot - softmax: the negative of the cross-entropy's
-  CCE_CUDA_CHECK(cce::launch_rows_cotangent(grad_logp, 1, nullptr, -1.f, v.R, N, nullptr, w.d, nullptr,
-                                            (cudaStream_t)stream),
-                 what);
-  const RowsBwd rb{v.R, cce::TopkView{}, w.d, 1.f, w.bias_part};
-  if (v.split.Dp)
-    return split_backward(v, w, rb, c, bias, bias_dtype, w.d, N, D, V, flags, grad_e, grad_c, grad_bias,
-                          (cudaStream_t)stream);
-  return backward_impl(v.e, c, nullptr, bias, bias_dtype, v.R.targets, v.lse, w.d, nullptr, N, D, V, 0, dtype, flags,
-                       0.f, grad_e, grad_c, grad_bias, nullptr, w.base, w.base_bytes, nullptr, &rb, stream);
+  cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
+  // d logp / dz = onehot - softmax: the negative of what the dlogits are
+  a.up = cce::Cotangent{grad_logp, nullptr, -1.f, 1};
+  return rows_backward(a, v, w, c, D, flags, grad_e, grad_c, grad_bias, s, what);
 }
 
 size_t cce_distill_saved_bytes(int64_t N, int64_t D, int64_t V, int64_t K, int dtype) {
@@ -1514,7 +1511,7 @@ size_t cce_distill_forward_workspace_bytes(int64_t N, int64_t D, int64_t V, int6
 }
 
 size_t cce_distill_backward_workspace_bytes(int64_t N, int64_t D, int64_t V, int dtype, int flags) {
-  return N < 0 || D <= 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_bwd_ws(nullptr, N, D, V, dtype, flags, true).bytes;
+  return N < 0 || D <= 0 || V <= 0 || !dtype_ok(dtype) ? 0 : rows_bwd_ws(nullptr, N, D, V, dtype, flags).bytes;
 }
 
 int cce_distill_forward(const void* e, const void* c, const void* bias, int bias_dtype, const void* teacher_ids,
@@ -1540,30 +1537,24 @@ int cce_distill_forward(const void* e, const void* c, const void* bias, int bias
     return CCE_OK;
   }
   if (!e || !c || !teacher_ids || !teacher_logp) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
-  RowsSaved v = rows_saved(saved, N, D, V, K, dtype);
+  const RowsSaved v = rows_saved(saved, N, D, V, K, dtype);
   const RowsFwdWs w = rows_fwd_ws(workspace, N, D, V, K, dtype);
-  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
-    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
-                v.bytes, workspace_bytes, w.bytes);
-  rc = check_arch();
+  rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
+  if (!rc) rc = check_rows_device(c, D, dtype, what);
   if (rc) return rc;
-  CCE_CUDA_CHECK(cce::launch_rows_pack(e, dtype, N, D, nullptr, 0, 0, 0, mask, v.R, nullptr,
-                                       red == CCE_REDUCE_NONE ? loss : nullptr, v.e, nullptr, s),
+  CCE_CUDA_CHECK(cce::launch_rows_pack(N, nullptr, 0, 0, 0, mask, v.R, nullptr, red == CCE_REDUCE_NONE ? loss : nullptr,
+                                       nullptr, s),
                  what);
   CCE_CUDA_CHECK(cce::launch_topk_prep(teacher_ids, id_bytes, teacher_logp, N, V, (int)K, params->temperature,
                                        params->tail, v.R, v.topk, w.p, w.rest, s),
                  what);
-  cce::FwdArgs f{v.e, c, bias, bias_dtype, nullptr, N, D, V, 0, dtype, nullptr, w.part_m, w.part_s, nullptr};
-  f.rows = v.R.count;
-  if (v.split.Dp) {
-    CCE_CUDA_CHECK(split_operands(v, w.split, e, c, N, D, V, s), what);
-    f.split = v.split;
-  }
-  f.scale = (float)(1.0 / params->temperature);
-  f.topk = v.topk;
-  CCE_CUDA_CHECK(rows_logits(f, s), what);
-  CCE_CUDA_CHECK(cce::launch_distill_rows(w.part_m, w.part_s, cce::ceil_div(V, cce::kSimtLseTile), N, V, v.R, v.topk,
-                                          w.p, w.rest, red, v.lse, v.A, w.sums, loss, v.weight, s),
+  cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
+  a.R = v.R, a.topk = v.topk, a.part_m = w.part_m, a.part_s = w.part_s;
+  a.scale_z = (float)(1.0 / params->temperature);
+  CCE_CUDA_CHECK(rows_operands(a, v, w.c, e, c, D, s), what);
+  CCE_CUDA_CHECK(cce::tc_logits(a, s), what);
+  CCE_CUDA_CHECK(cce::launch_distill_rows(w.part_m, w.part_s, cce::ceil_div(V, 128), N, V, v.R, v.topk, w.p, w.rest,
+                                          red, v.lse, v.A, w.sums, loss, v.weight, s),
                  what);
   return CCE_OK;
 }
@@ -1577,32 +1568,24 @@ int cce_distill_backward(const void* c, const void* bias, int bias_dtype, const 
   if (rc) return rc;
   if (K < 1) return fail(CCE_ERR_SHAPE, "%s: K=%lld is outside of [1, %d]", what, (long long)K, CCE_DISTILL_MAX_K);
   rc = check_distill(params, what);
+  if (!rc) rc = check_rows_backward(bias, bias_dtype, N, flags, grad_e, grad_c, grad_bias, what);
   if (rc) return rc;
-  rc = check_rows_backward(bias, bias_dtype, N, V, D, dtype, flags, grad_e, grad_c, grad_bias, what);
-  if (rc) return rc;
-  if (N == 0)
-    return backward_impl(nullptr, c, nullptr, bias, bias_dtype, nullptr, nullptr, nullptr, nullptr, N, D, V, 0, dtype,
-                         flags, 0.f, grad_e, grad_c, grad_bias, nullptr, workspace, workspace_bytes, nullptr, nullptr,
-                         stream);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (N == 0) {
+    rc = check_arch();
+    return rc ? rc : zero_grads(D, V, dtype, flags, grad_c, grad_bias, s);
+  }
   if (!grad_loss || !c) return fail(CCE_ERR_ARG, "%s: NULL required pointer", what);
   const RowsSaved v = rows_saved(const_cast<void*>(saved), N, D, V, K, dtype);
-  const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags, true);
-  if (!saved || saved_bytes < v.bytes || !workspace || workspace_bytes < w.bytes)
-    return fail(CCE_ERR_WORKSPACE, "%s: saved %zu bytes < required %zu or workspace %zu < %zu", what, saved_bytes,
-                v.bytes, workspace_bytes, w.bytes);
-  rc = check_arch();
+  const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags);
+  rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
+  if (!rc) rc = check_rows_device(c, D, dtype, what);
   if (rc) return rc;
+  cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
+  a.scale_z = (float)(1.0 / params->temperature);
   // dlogits are by the logits before the temperature: one factor 1 / T in the cotangent
-  CCE_CUDA_CHECK(cce::launch_rows_cotangent(grad_loss, params->reduction == CCE_REDUCE_NONE, v.weight,
-                                            (float)(1.0 / params->temperature), v.R, N, v.A, w.d, w.dA,
-                                            (cudaStream_t)stream),
-                 what);
-  const RowsBwd rb{v.R, v.topk, w.d, (float)(1.0 / params->temperature), w.bias_part};
-  if (v.split.Dp)
-    return split_backward(v, w, rb, c, bias, bias_dtype, w.dA, N, D, V, flags, grad_e, grad_c, grad_bias,
-                          (cudaStream_t)stream);
-  return backward_impl(v.e, c, nullptr, bias, bias_dtype, nullptr, v.lse, w.dA, nullptr, N, D, V, 0, dtype, flags, 0.f,
-                       grad_e, grad_c, grad_bias, nullptr, w.base, w.base_bytes, nullptr, &rb, stream);
+  a.up = cce::Cotangent{grad_loss, v.weight, a.scale_z, params->reduction == CCE_REDUCE_NONE};
+  return rows_backward(a, v, w, c, D, flags, grad_e, grad_c, grad_bias, s, what);
 }
 
 }  // extern "C"

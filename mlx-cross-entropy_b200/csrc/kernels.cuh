@@ -42,13 +42,44 @@ struct TopkView {
   int K = 0, tiles1 = 0;
 };
 
-// Float32 operands as two float16 parts, x = (hi + lo) / s[0], rows padded with
-// zeros to Dp (a multiple of 64) columns; se, sc: {s, 1 / s} on the device.
-struct SplitView {
-  const void *e_hi = nullptr, *e_lo = nullptr;  // [N][Dp] packed rows
-  const void *c_hi = nullptr, *c_lo = nullptr;  // [V][Dp]
-  int64_t Dp = 0;
-  const float *se = nullptr, *sc = nullptr;
+// The cotangent d of a batch row's log-probability or loss: factor * up (per row,
+// or one for all), times weight[0].
+struct Cotangent {
+  const float* up;
+  const float* weight;  // nullptr: 1
+  float factor;
+  int per_row;
+#ifdef __CUDACC__
+  __device__ __forceinline__ float of(int64_t packed, const int32_t* row_of) const {
+    return up[per_row ? row_of[packed] : 0] * (weight ? weight[0] * factor : factor);
+  }
+#endif
+};
+
+// GEMMs over a batch's packed rows (tc_rows.cuh), 16-bit operands; dtype CCE_F32:
+// float32 operands as two float16 parts, x = (hi + lo) / s[0] (e, c and e_lo,
+// c_lo; se, sc: {s, 1 / s} on the device).
+struct RowsGemmArgs {
+  const void *e, *e_lo;          // [N][Dk] packed rows, zeros behind the count
+  const void *c, *c_lo;          // [V][Dk]
+  const float *se, *sc;
+  const void* bias;              // [V] or nullptr
+  int bias_dtype, dtype;
+  RowsView R;
+  int64_t N, V, Dk, Dout;        // Dk: operands' width (a multiple of 8); Dout: the gradients'
+                                 // (of 8, float32 of 4); their columns behind D are zeros
+  int64_t vc0, vc_len;           // vocabulary rows of this call
+  float scale_z;                 // logits = scale_z (e c^T + bias)
+  TopkView topk;                 // the rows' listed columns (sid == nullptr: none)
+  // row statistics
+  float *part_m, *part_s, *tgt;  // [ceil(V / 128)][N] twice, [N]
+  // dlogits and gradients
+  const float *lse, *A;          // A: distillation
+  Cotangent up;
+  const float* scale;            // {s, 1 / s}: float16 dlogits hold w / s (nullptr: 1)
+  void *dl, *dl_lo;              // [N][vc_ld] 16-bit
+  int64_t vc_ld;
+  float* bias_part;              // [ceil(N / 32)][vc_ld] zeroed: column sums of dlogits, or nullptr
 };
 
 struct FwdArgs {
@@ -63,11 +94,6 @@ struct FwdArgs {
   float* part_m;    // [P][N] (workspace): row max over each kernel tile, P = ceil(V / lse_tile)
   float* part_s;    // [P][N] (workspace): row sum of exp(logit - part_m) over the same columns
   float* tgt;       // [N]
-  // row statistics for losses on log-probabilities (tc_logits, simt_logits): tile_max unused
-  const int32_t* rows = nullptr;  // rows that count (device)
-  float scale = 1.f;              // logits = scale (e c^T + bias)
-  TopkView topk{};                // columns left out of the sum, whose logits go to topk.z
-  SplitView split{};              // float32 inputs on tensor cores (e, c unused)
 };
 
 struct BwdChunkArgs {
@@ -94,16 +120,6 @@ struct BwdChunkArgs {
   int* counters;         // 4 zeroed counters of this chunk (dlogits, grad_e, grad_c tile claims; the
                          // dlogits live-tile count) or nullptr
   const float* scale;    // fp16 tensor-core path: {s, 1/s} with s = 2^ceil(log2 max|d_nll|); else nullptr
-  // distillation: d_nll is the coefficient of the columns outside of the row's
-  // list (lse over those), a listed column's dlogit is topk.z * d_row
-  TopkView topk{};
-  const float* d_row = nullptr;
-  float logit_scale = 1.f;
-  const int32_t* rows = nullptr; // packed rows that count (tc_dlogits_rows and the float32 gradients)
-  SplitView split{};             // float32 inputs on tensor cores (e, c_chunk unused)
-  void* dlogits_lo = nullptr;    // the dlogits' second part
-  int slabs = 2;                 // K splits of tc_grad_e
-  float* bias_part = nullptr;    // [ceil(N / 32)][vc_ld] column sums of dlogits (zeroed); instead of grad_bias
   const int* dl_list = nullptr;  // the chunk's live dlogits tiles (tc_dlogits_lists), count in counters[3]
 };
 
@@ -124,8 +140,8 @@ cudaError_t launch_dequantize(const uint32_t* wq, const void* scales, const void
                               cudaStream_t stream);
 // dst[i] = a[i] + b[i], written in dtype (CCE_F32 / F16 / BF16)
 cudaError_t launch_sum2_f32(const float* a, const float* b, void* dst, int dtype, int64_t n, cudaStream_t stream);
-// out[0] = s = 2^-up times the power of two >= max |x| (1 if all zero), out[1] = 1 / s
-cudaError_t launch_pow2_absmax(const float* x, int64_t n, float* out, int up, cudaStream_t stream);
+// out[0] = s = the power of two >= max |x| (1 if all zero), out[1] = 1 / s
+cudaError_t launch_pow2_absmax(const float* x, int64_t n, float* out, cudaStream_t stream);
 cudaError_t launch_fill_f32(float* dst, float v, int64_t n, cudaStream_t stream);
 
 // ---- rows of a batch, distillation (rows_kernels.cu) ----
@@ -133,9 +149,15 @@ struct DistillSum {
   double loss;
   int32_t n;
 };
-cudaError_t launch_rows_pack(const void* e, int dtype, int64_t N, int64_t D, const void* targets, int target_bytes,
-                             int64_t ignore_index, int has_ignore, const uint8_t* mask, const RowsView& R,
-                             uint8_t* mask_out, float* per_row_out, void* e_packed, float* tgt, cudaStream_t stream);
+// Row lists of the batch; mask_out and per_row_out (0 for rows left out) nullable;
+// tgt: a value per packed row, zeroed (with targets).
+cudaError_t launch_rows_pack(int64_t N, const void* targets, int target_bytes, int64_t ignore_index, int has_ignore,
+                             const uint8_t* mask, const RowsView& R, uint8_t* mask_out, float* per_row_out, float* tgt,
+                             cudaStream_t stream);
+// 16-bit rows: dst[i] = src[row_of[i]] (R; zeros behind the count), or src[i] (R == nullptr),
+// `cols` values each, zeros up to dst_ld
+cudaError_t launch_rows_copy(const void* src, int64_t rows, int64_t cols, int64_t src_ld, const RowsView* R, void* dst,
+                             int64_t dst_ld, cudaStream_t stream);
 // lse (packed rows) and logp (batch rows) from P partials
 cudaError_t launch_rows_logp(const float* part_m, const float* part_s, int64_t P, int64_t N, const RowsView& R,
                              const float* tgt, float* lse, float* logp, cudaStream_t stream);
@@ -147,25 +169,22 @@ cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_
                                 const RowsView& R, const TopkView& topk, const float* p, const float* rest,
                                 int reduction, float* lse_rest, float* A, DistillSum* sums, float* loss, float* weight,
                                 cudaStream_t stream);
-cudaError_t launch_rows_cotangent(const float* up, int up_row, const float* weight, float factor, const RowsView& R,
-                                  int64_t N, const float* A, float* d, float* dA, cudaStream_t stream);
-cudaError_t launch_live_mask(const float* d, int64_t N, int64_t V, uint8_t* keep, uint32_t* keep_t, int64_t keep_t_ld,
-                             cudaStream_t stream);
-// out[n] = sum over the slabs [N][D] of row pos[n], in order; 0 where pos[n] < 0
-cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, const int32_t* pos, int64_t N, int64_t D, int dtype,
-                                void* out, cudaStream_t stream);
+// out[n] = sum over the slabs [N][ld] of row pos[n], in order; 0 where pos[n] < 0
+cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, int64_t ld, const int32_t* pos, int64_t N, int64_t D,
+                                int dtype, void* out, cudaStream_t stream);
+// out = {s, 1 / s}, s the power of two >= the largest |d| of the rows, times 2^-14
+cudaError_t launch_rows_scale(const Cotangent& up, const RowsView& R, float* out, cudaStream_t stream);
 // largest |x| of the rows (those of R, if given) as the bits of a float, into *word (zeroed)
 cudaError_t launch_absmax(const float* x, int64_t rows, int64_t D, const RowsView* R, uint32_t* word,
                           cudaStream_t stream);
 // x -> hi, lo [rows][Dp] and scale = {s, 1 / s}; R: the packed rows of x, zeros behind their count
 cudaError_t launch_split(const float* x, int64_t rows, int64_t D, int64_t Dp, const RowsView* R, const uint32_t* word,
                          float* scale, void* hi, void* lo, cudaStream_t stream);
-cudaError_t launch_bias_sum(const float* part, int64_t parts, int64_t ld, int64_t cols, const float* scale, float* out,
-                            cudaStream_t stream);
+// column sums part[parts][ld] of 32 packed rows each -> out[cols], times scale[0]
+cudaError_t launch_bias_sum(const float* part, int64_t parts, const RowsView& R, int64_t ld, int64_t cols,
+                            const float* scale, float* out, cudaStream_t stream);
 
 // ---- SIMT kernels (simt_kernels.cu): any dtype, any shape ----
-// row statistics of the rows that count (see FwdArgs)
-cudaError_t simt_logits(const FwdArgs& a, cudaStream_t stream);
 cudaError_t simt_forward(const FwdArgs& a, cudaStream_t stream);
 // vocabulary columns per LSE partial of simt_forward / tc_forward
 constexpr int64_t kSimtLseTile = 128;
@@ -182,7 +201,6 @@ int simt_grad_e_splits(int64_t N, int64_t D, int64_t vc);
 cudaError_t simt_grad_c(const BwdChunkArgs& a, void* grad_c, cudaStream_t stream);
 
 // ---- tcgen05 kernels (tc_kernels.cu): 16-bit dtypes, D % 8 == 0 ----
-bool tc_available();  // the driver's tensor-map encoder was found
 bool tc_supported(const void* e, const void* c, int64_t D, int dtype);
 bool tc_backward_supported(const void* e, const void* c, int64_t D, int dtype);
 // Reads (and optionally clears) the tensor-core kernels' device status word:
@@ -192,14 +210,6 @@ int tc_read_status(bool reset);
 // the last reset; 0 = ok, -1 = read failed.
 int tc_read_mma_flops(uint64_t* out4, bool reset);
 cudaError_t tc_forward(const FwdArgs& a, cudaStream_t stream);
-// row statistics of the rows that count, two-level accumulation (see FwdArgs)
-cudaError_t tc_logits(const FwdArgs& a, cudaStream_t stream);
-// dlogits of a chunk's packed rows, no filter; float32 inputs (a.split): both parts
-cudaError_t tc_dlogits_rows(const BwdChunkArgs& a, cudaStream_t stream);
-// float32 gradients from split operands: slabs[num_slabs][N][D] (+)= the K splits
-// of dl c_chunk; grad_c rows of the chunk = dl^T e
-cudaError_t tc_grad_e_split(const BwdChunkArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t stream);
-cudaError_t tc_grad_c_split(const BwdChunkArgs& a, float* grad_c, cudaStream_t stream);
 cudaError_t tc_dlogits(const BwdChunkArgs& a, cudaStream_t stream);
 // Lists, per vocabulary chunk of vc rows, the dlogits work units with a kept
 // block in schedule order: chunk ch's ids at lists + ch * tc_dlogits_list_len(N, vc),
@@ -221,6 +231,15 @@ cudaError_t tc_grad_e(const BwdChunkArgs& a, float* acc2, bool accumulate, const
 cudaError_t tc_grad_c(const BwdChunkArgs& a, void* grad_c, cudaStream_t stream);
 // one bounded pipeline wait that nothing satisfies: records `code` after limit_ns
 cudaError_t tc_selftest_wait(uint64_t limit_ns, int code, cudaStream_t stream);
+
+// ---- GEMMs over packed rows (tc_rows.cuh) ----
+bool tc_available();  // the driver's tensor-map encoder was found
+cudaError_t tc_logits(const RowsGemmArgs& a, cudaStream_t stream);
+cudaError_t tc_dlogits_rows(const RowsGemmArgs& a, cudaStream_t stream);
+// slabs[num_slabs][N][Dout] (+)= the K splits of dl c (fp32)
+cudaError_t tc_grad_e_rows(const RowsGemmArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t stream);
+// grad_c rows [vc0, vc0 + vc_len) = dl^T e, row stride Dout
+cudaError_t tc_grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t stream);
 
 // ---- losses on per-token log-probabilities (token_loss.cu) ----
 // Sequences: offsets cu[S + 1] into the N tokens, or (cu == nullptr) S rows of N / S tokens.

@@ -37,7 +37,7 @@ template <typename TT>  // target type; void: rows count by `mask` alone
 __global__ void __launch_bounds__(kPackThreads)
 rows_pack_kernel(const TT* __restrict__ targets, int64_t ignore_index, int has_ignore,
                  const uint8_t* __restrict__ mask, int64_t N, const RowsView R, uint8_t* __restrict__ mask_out,
-                 float* __restrict__ per_row_out) {
+                 float* __restrict__ per_row_out, float* __restrict__ tgt) {
   __shared__ int warp_tot[32];
   __shared__ int base_sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -88,7 +88,10 @@ rows_pack_kernel(const TT* __restrict__ targets, int64_t ignore_index, int has_i
         if (mask_out) mask_out[n0 + j] = ok ? 1 : 0;
         if (ok) {
           R.row_of[at] = (int32_t)(n0 + j);
-          if constexpr (!std::is_void<TT>::value) R.targets[at] = t[j];
+          if constexpr (!std::is_void<TT>::value) {
+            R.targets[at] = t[j];
+            tgt[at] = 0.f;  // (stays for a target that is no column)
+          }
           ++at;
         } else if (per_row_out) {
           per_row_out[n0 + j] = 0.f;
@@ -102,30 +105,25 @@ rows_pack_kernel(const TT* __restrict__ targets, int64_t ignore_index, int has_i
   if (threadIdx.x == 0) *R.count = base_sh;
 }
 
-// A warp per packed row: row i of the copy is row row_of[i] of e, zeros behind
-// the count (the grad_c GEMM multiplies those rows by zeros, so they must be
-// numbers).
+// A warp per row of 16-bit values: dst[i] = src[row_of[i]], zeros behind the
+// count (the grad_c GEMM multiplies those rows by zeros, so they must be
+// numbers), or with no list dst[i] = src[i]; columns behind `cols` are zeros.
 template <bool kVec>
 __global__ void __launch_bounds__(256)
-rows_gather_kernel(const uint8_t* __restrict__ e, int64_t N, int64_t row_bytes, const RowsView R, int has_targets,
-                   uint8_t* __restrict__ out, float* __restrict__ tgt) {
+rows_copy_kernel(const uint16_t* __restrict__ src, int64_t rows, int64_t cols, int64_t src_ld,
+                 const int32_t* __restrict__ row_of, const int32_t* __restrict__ count, uint16_t* __restrict__ dst,
+                 int64_t dst_ld) {
   const int lane = threadIdx.x & 31;
-  const int64_t count = *R.count;
-  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < N; i += (int64_t)gridDim.x * 8) {
-    const bool live = i < count;
-    const uint8_t* src = live ? e + (int64_t)R.row_of[i] * row_bytes : nullptr;  // (row_bytes 0: no copy)
-    uint8_t* dst = out + i * row_bytes;
+  const int64_t live = count ? *count : rows;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows; i += (int64_t)gridDim.x * 8) {
+    const uint16_t* p = i < live ? src + (row_of ? row_of[i] : i) * src_ld : nullptr;
+    uint16_t* q = dst + i * dst_ld;
     if constexpr (kVec) {
-      for (int64_t k = lane * 16; k < row_bytes; k += 32 * 16)
-        *reinterpret_cast<uint4*>(dst + k) =
-            live ? __ldg(reinterpret_cast<const uint4*>(src + k)) : make_uint4(0u, 0u, 0u, 0u);
+      for (int64_t k = lane * 8; k < dst_ld; k += 256)
+        *reinterpret_cast<uint4*>(q + k) =
+            p && k < cols ? __ldg(reinterpret_cast<const uint4*>(p + k)) : make_uint4(0u, 0u, 0u, 0u);
     } else {
-      for (int64_t k = lane * 2; k < row_bytes; k += 32 * 2)
-        *reinterpret_cast<uint16_t*>(dst + k) = live ? *reinterpret_cast<const uint16_t*>(src + k) : (uint16_t)0;
-    }
-    if (lane == 0) {
-      if (tgt) tgt[i] = 0.f;
-      if (has_targets && !live) R.targets[i] = 0;
+      for (int64_t k = lane; k < dst_ld; k += 32) q[k] = p && k < cols ? p[k] : (uint16_t)0;
     }
   }
 }
@@ -426,65 +424,65 @@ distill_final_kernel(const DistillSum* __restrict__ sums, int blocks, int reduct
 // backward
 // ---------------------------------------------------------------------------
 
-// Cotangents of the packed rows: d = sign * up * weight * scale (0 behind the count), dA = d A.
-__global__ void rows_cotangent_kernel(const float* __restrict__ up, int up_row, const float* __restrict__ weight,
-                                      float factor, const RowsView R, int64_t N, const float* __restrict__ A,
-                                      float* __restrict__ d, float* __restrict__ dA) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= N) return;
-  float x = 0.f;
-  if (i < *R.count) x = up[up_row ? R.row_of[i] : 0] * (weight ? weight[0] * factor : factor);
-  d[i] = x;
-  if (dA) dA[i] = x == 0.f ? 0.f : x * A[i];
-}
-
-// Block mask of exact gradients: a row block is kept whole unless every row of
-// it has a zero cotangent.  grid (tile groups, row blocks)
-__global__ void __launch_bounds__(256)
-live_mask_kernel(const float* __restrict__ d, int64_t N, int64_t V, uint8_t* __restrict__ keep,
-                 uint32_t* __restrict__ keep_t, int64_t keep_t_ld) {
-  const int64_t i = blockIdx.y;
-  const int64_t r = i * kRowBlock + (threadIdx.x & (kRowBlock - 1));
-  const int live = __syncthreads_or(r < N && d[r] != 0.f);
-  const int64_t nVt = ceil_div(V, kStatTile);
-  const int64_t t0 = (int64_t)blockIdx.x * 1024;
-  for (int64_t t = t0 + threadIdx.x; t < nVt && t < t0 + 1024; t += 256) {
-    keep[i * nVt + t] = live ? 1 : 0;
-    if (keep_t && live && t % (128 / kStatTile) == 0)
-      atomicOr(&keep_t[t / (128 / kStatTile) * keep_t_ld + (i >> 5)], 1u << (i & 31));
+// One block: the largest |d| of the rows that count, as a power of two s (1 when
+// all are zero) times 2^-14: dlogits are at most d in magnitude, so w / s stays
+// below 2^14 in float16 and a softmax value of 2^-28 is still a normal number.
+__global__ void __launch_bounds__(1024) rows_scale_kernel(const Cotangent up, const RowsView R, float* __restrict__ out) {
+  __shared__ float red[32];
+  const int count = *R.count;
+  float m = 0.f;
+  for (int i = threadIdx.x; i < (up.per_row ? count : min(count, 1)); i += blockDim.x)
+    m = fmaxf(m, fabsf(up.of(i, R.row_of)));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) m = fmaxf(m, red[w]);
+    int ex = 0;
+    if (m > 0.f && isfinite(m)) {
+      const float f = frexpf(m, &ex);  // m = f * 2^ex, f in [0.5, 1)
+      if (f == 0.5f) --ex;
+    }
+    const float s = ldexpf(1.f, max(ex, -100) - 14);
+    out[0] = s;
+    out[1] = 1.f / s;
   }
 }
 
-// grad_e row n = the slabs' rows pos[n] added in order, 0 for rows that do not count.
+// grad_e row n = the slabs' rows pos[n] added in order, 0 for rows that do not
+// count; a warp per row and 128 columns (few rows with many slabs need the width).
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256)
-rows_scatter_kernel(const float* __restrict__ slabs, int num, const int32_t* __restrict__ pos, int64_t N, int64_t D,
-                    T* __restrict__ out) {
+rows_scatter_kernel(const float* __restrict__ slabs, int num, int64_t ld, const int32_t* __restrict__ pos, int64_t N,
+                    int64_t D, T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
-  const int64_t stride = N * D;
-  for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < N; n += (int64_t)gridDim.x * 8) {
+  const int64_t stride = N * ld;
+  const int64_t pieces = ceil_div(D, 128), items = N * pieces;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < items; i += (int64_t)gridDim.x * 8) {
+    const int64_t n = i / pieces, k0 = (i - n * pieces) * 128;
     const int64_t p = pos[n];
-    const float* row = slabs + p * D;
+    const float* row = slabs + p * ld;
     if constexpr (kVec) {
-      for (int64_t k = 4 * lane; k < D; k += 128) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p >= 0) {
-          x = *reinterpret_cast<const float4*>(row + k);
-#pragma unroll 4
-          for (int z = 1; z < num; ++z) {
-            const float4 y = *reinterpret_cast<const float4*>(row + z * stride + k);
-            x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-          }
-        }
-        if constexpr (sizeof(T) == 4) {
-          *reinterpret_cast<float4*>(out + n * D + k) = x;
-        } else {
-          T h[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
-          *reinterpret_cast<uint2*>(out + n * D + k) = *reinterpret_cast<uint2*>(h);
+      const int64_t k = k0 + 4 * lane;
+      if (k >= D) continue;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p >= 0) {
+        x = *reinterpret_cast<const float4*>(row + k);
+#pragma unroll 8
+        for (int z = 1; z < num; ++z) {
+          const float4 y = *reinterpret_cast<const float4*>(row + z * stride + k);
+          x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
       }
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(out + n * D + k) = x;
+      } else {
+        T h[4] = {from_f32<T>(x.x), from_f32<T>(x.y), from_f32<T>(x.z), from_f32<T>(x.w)};
+        *reinterpret_cast<uint2*>(out + n * D + k) = *reinterpret_cast<uint2*>(h);
+      }
     } else {
-      for (int64_t k = lane; k < D; k += 32) {
+      for (int64_t k = k0 + lane; k < D && k < k0 + 128; k += 32) {
         float x = 0.f;
         if (p >= 0) {
           x = row[k];
@@ -569,15 +567,15 @@ split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, c
   }
 }
 
-// grad_bias of a vocabulary chunk from partial column sums part[parts][ld], in
-// order: the same result every time, where atomics would add in any order.
-template <typename TO>
+// grad_bias of a vocabulary chunk from the column sums of 32 rows each, in order:
+// the same result every time, where atomics would add in any order.
 __global__ void __launch_bounds__(256)
-bias_sum_kernel(const float* __restrict__ part, int64_t parts, int64_t ld, int64_t cols, const float* __restrict__ scale,
-                TO* __restrict__ out) {
+bias_sum_kernel(const float* __restrict__ part, int64_t parts, const int32_t* __restrict__ count, int64_t ld,
+                int64_t cols, const float* __restrict__ scale, float* __restrict__ out) {
   __shared__ float sh[8][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  parts = min(parts, ceil_div(*count, 128) * 4);  // (those of the row tiles that were computed)
   float s = 0.f;
   if (c < cols)
     for (int64_t p = w; p < parts; p += 8) s += part[p * ld + c];
@@ -599,32 +597,36 @@ unsigned warps_grid(int64_t N) {
 
 }  // namespace
 
-cudaError_t launch_rows_pack(const void* e, int dtype, int64_t N, int64_t D, const void* targets, int target_bytes,
-                             int64_t ignore_index, int has_ignore, const uint8_t* mask, const RowsView& R,
-                             uint8_t* mask_out, float* per_row_out, void* e_packed, float* tgt, cudaStream_t s) {
+cudaError_t launch_rows_pack(int64_t N, const void* targets, int target_bytes, int64_t ignore_index, int has_ignore,
+                             const uint8_t* mask, const RowsView& R, uint8_t* mask_out, float* per_row_out, float* tgt,
+                             cudaStream_t s) {
   if (targets == nullptr)
-    rows_pack_kernel<void><<<1, kPackThreads, 0, s>>>(nullptr, 0, 0, mask, N, R, mask_out, per_row_out);
+    rows_pack_kernel<void><<<1, kPackThreads, 0, s>>>(nullptr, 0, 0, mask, N, R, mask_out, per_row_out, nullptr);
   else if (target_bytes == 8)
     rows_pack_kernel<int64_t><<<1, kPackThreads, 0, s>>>((const int64_t*)targets, ignore_index, has_ignore, mask, N, R,
-                                                         mask_out, per_row_out);
+                                                         mask_out, per_row_out, tgt);
   else
     rows_pack_kernel<int32_t><<<1, kPackThreads, 0, s>>>((const int32_t*)targets, ignore_index, has_ignore, mask, N, R,
-                                                         mask_out, per_row_out);
-  cudaError_t err = launched();
-  if (err != cudaSuccess) return err;
-  const int64_t row_bytes = D * (dtype == CCE_F32 ? 4 : 2);
-  const bool vec = row_bytes % 16 == 0 && aligned16(e) && aligned16(e_packed);
-  if (e_packed == nullptr) {  // the rows themselves are copied elsewhere
-    if (tgt || targets)
-      rows_gather_kernel<true><<<warps_grid(N), 256, 0, s>>>(nullptr, N, 0, R, targets != nullptr, nullptr, tgt);
-    else
-      return cudaSuccess;
-  } else if (vec)
-    rows_gather_kernel<true><<<warps_grid(N), 256, 0, s>>>((const uint8_t*)e, N, row_bytes, R, targets != nullptr,
-                                                           (uint8_t*)e_packed, tgt);
+                                                         mask_out, per_row_out, tgt);
+  return launched();
+}
+
+cudaError_t launch_rows_copy(const void* src, int64_t rows, int64_t cols, int64_t src_ld, const RowsView* R, void* dst,
+                             int64_t dst_ld, cudaStream_t s) {
+  const bool vec = ((cols | src_ld | dst_ld) & 7) == 0 && aligned16(src) && aligned16(dst);
+  const int32_t* row_of = R ? R->row_of : nullptr;
+  const int32_t* count = R ? R->count : nullptr;
+  if (vec)
+    rows_copy_kernel<true><<<warps_grid(rows), 256, 0, s>>>((const uint16_t*)src, rows, cols, src_ld, row_of, count,
+                                                            (uint16_t*)dst, dst_ld);
   else
-    rows_gather_kernel<false><<<warps_grid(N), 256, 0, s>>>((const uint8_t*)e, N, row_bytes, R, targets != nullptr,
-                                                            (uint8_t*)e_packed, tgt);
+    rows_copy_kernel<false><<<warps_grid(rows), 256, 0, s>>>((const uint16_t*)src, rows, cols, src_ld, row_of, count,
+                                                             (uint16_t*)dst, dst_ld);
+  return launched();
+}
+
+cudaError_t launch_rows_scale(const Cotangent& up, const RowsView& R, float* out, cudaStream_t s) {
+  rows_scale_kernel<<<1, 1024, 0, s>>>(up, R, out);
   return launched();
 }
 
@@ -666,36 +668,23 @@ cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_
   return launched();
 }
 
-cudaError_t launch_rows_cotangent(const float* up, int up_row, const float* weight, float factor, const RowsView& R,
-                                  int64_t N, const float* A, float* d, float* dA, cudaStream_t s) {
-  rows_cotangent_kernel<<<(unsigned)ceil_div(N, 256), 256, 0, s>>>(up, up_row, weight, factor, R, N, A, d, dA);
-  return launched();
-}
-
-cudaError_t launch_live_mask(const float* d, int64_t N, int64_t V, uint8_t* keep, uint32_t* keep_t, int64_t keep_t_ld,
-                             cudaStream_t s) {
-  const dim3 grid((unsigned)ceil_div(ceil_div(V, kStatTile), (int64_t)1024), (unsigned)ceil_div(N, kRowBlock));
-  live_mask_kernel<<<grid, 256, 0, s>>>(d, N, V, keep, keep_t, keep_t_ld);
-  return launched();
-}
-
 template <typename T>
-static cudaError_t scatter(const float* slabs, int num, const int32_t* pos, int64_t N, int64_t D, void* out,
+static cudaError_t scatter(const float* slabs, int num, int64_t ld, const int32_t* pos, int64_t N, int64_t D, void* out,
                            cudaStream_t s) {
-  const bool vec = D % 4 == 0 && aligned16(slabs) && aligned16(out);
-  if (vec)
-    rows_scatter_kernel<T, true><<<warps_grid(N), 256, 0, s>>>(slabs, num, pos, N, D, static_cast<T*>(out));
+  const unsigned grid = warps_grid(N * ceil_div(D, 128));
+  if (D % 4 == 0 && ld % 4 == 0 && aligned16(slabs) && aligned16(out))
+    rows_scatter_kernel<T, true><<<grid, 256, 0, s>>>(slabs, num, ld, pos, N, D, static_cast<T*>(out));
   else
-    rows_scatter_kernel<T, false><<<warps_grid(N), 256, 0, s>>>(slabs, num, pos, N, D, static_cast<T*>(out));
+    rows_scatter_kernel<T, false><<<grid, 256, 0, s>>>(slabs, num, ld, pos, N, D, static_cast<T*>(out));
   return launched();
 }
 
-cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, const int32_t* pos, int64_t N, int64_t D, int dtype,
-                                void* out, cudaStream_t s) {
+cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, int64_t ld, const int32_t* pos, int64_t N, int64_t D,
+                                int dtype, void* out, cudaStream_t s) {
   switch (dtype) {
-    case CCE_F32: return scatter<float>(slabs, num_slabs, pos, N, D, out, s);
-    case CCE_F16: return scatter<__half>(slabs, num_slabs, pos, N, D, out, s);
-    case CCE_BF16: return scatter<__nv_bfloat16>(slabs, num_slabs, pos, N, D, out, s);
+    case CCE_F32: return scatter<float>(slabs, num_slabs, ld, pos, N, D, out, s);
+    case CCE_F16: return scatter<__half>(slabs, num_slabs, ld, pos, N, D, out, s);
+    case CCE_BF16: return scatter<__nv_bfloat16>(slabs, num_slabs, ld, pos, N, D, out, s);
   }
   return cudaErrorInvalidValue;
 }
@@ -714,9 +703,9 @@ cudaError_t launch_split(const float* x, int64_t rows, int64_t D, int64_t Dp, co
   return launched();
 }
 
-cudaError_t launch_bias_sum(const float* part, int64_t parts, int64_t ld, int64_t cols, const float* scale, float* out,
-                            cudaStream_t s) {
-  bias_sum_kernel<float><<<(unsigned)ceil_div(cols, 32), 256, 0, s>>>(part, parts, ld, cols, scale, out);
+cudaError_t launch_bias_sum(const float* part, int64_t parts, const RowsView& R, int64_t ld, int64_t cols,
+                            const float* scale, float* out, cudaStream_t s) {
+  bias_sum_kernel<<<(unsigned)ceil_div(cols, 32), 256, 0, s>>>(part, parts, R.count, ld, cols, scale, out);
   return launched();
 }
 

@@ -8,10 +8,7 @@
 //    (w = d_nll * (exp(logit - lse) - [v == t]), cce.metal:276-281) and two
 //    plain GEMMs (dE += w @ c, dC = w^T @ e, cce.metal:284-304) instead of
 //    per-element atomics.
-#include <type_traits>
-
 #include "kernels.cuh"
-#include "topk.cuh"
 
 namespace cce {
 namespace {
@@ -85,100 +82,6 @@ __device__ __forceinline__ float bias_at(const void* bias, int64_t v) {
   return to_f32(reinterpret_cast<const TB*>(bias)[v]);
 }
 
-// Rows-and-list form of the two logits kernels (losses on log-probabilities).
-struct SimtRows {
-  const int32_t* rows;  // rows that count
-  float scale;          // logits = scale (e c^T + bias)
-  TopkView topk;        // listed columns (sid == nullptr: none)
-  const float* d_row;   // dlogits of a listed column = topk.z * d_row
-};
-
-// The tile's listed columns: row r's as bits of msk[r] (128 columns), its first
-// entry in base[r].  All threads take part; a barrier follows.
-struct ListedTile {
-  uint32_t msk[BM][BN / 32];
-  int base[BM];
-  __device__ __forceinline__ void load(const TopkView& t, int64_t r0, int64_t rows, int64_t v0) {
-    if (threadIdx.x < BM) {
-      const int r = threadIdx.x;
-      uint32_t m[BN / 32] = {0u, 0u, 0u, 0u};
-      TopkCursor cur;
-      cur.open(t, r0 + r, r0 + r < rows, v0 / kTopkTile);
-      cur.skip_to(v0);
-      int first;
-      base[r] = cur.p;
-#pragma unroll
-      for (int w = 0; w < BN / 32; ++w) m[w] = cur.take(v0 + 32 * w, first);
-#pragma unroll
-      for (int w = 0; w < BN / 32; ++w) msk[r][w] = m[w];
-    }
-    __syncthreads();
-  }
-  // Entry of column `col` of the tile in row r, -1 for none.
-  __device__ __forceinline__ int entry(int r, int col) const {
-    const int w = col >> 5;
-    const uint32_t bit = 1u << (col & 31);
-    if (!(msk[r][w] & bit)) return -1;
-    int p = base[r] + __popc(msk[r][w] & (bit - 1u));
-    for (int i = 0; i < w; ++i) p += __popc(msk[r][i]);
-    return p;
-  }
-};
-
-template <typename T, typename TB>
-__global__ void __launch_bounds__(THREADS)
-simt_logits_kernel(const T* __restrict__ e, const T* __restrict__ c, const void* __restrict__ bias,
-                   const int32_t* __restrict__ targets, int64_t N, int64_t D, int64_t V, const SimtRows X,
-                   float* __restrict__ part_m, float* __restrict__ part_s, float* __restrict__ tgt) {
-  const int64_t r0 = (int64_t)blockIdx.x * BM;
-  const int64_t rows = min((int64_t)__ldg(X.rows), N);
-  if (r0 >= rows) return;
-  const int64_t tile = blockIdx.y;
-  const int64_t v0 = tile * BN;
-  const bool listed = X.topk.sid != nullptr;
-  __shared__ ListedTile lt;
-  if (listed) lt.load(X.topk, r0, rows, v0);
-  float acc[4][8];
-  tile_logits<T>(e, c, rows, D, V, r0, v0, acc);
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = r0 + ty + 16 * i;
-    const int64_t tl = (!listed && row < rows) ? (int64_t)targets[row] - v0 : -1;
-    float x[8], m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t v = v0 + tx + 16 * j;
-      x[j] = -INFINITY;
-      if (v < V) {
-        x[j] = (acc[i][j] + (bias != nullptr ? bias_at<TB>(bias, v) : 0.f)) * X.scale;
-        if (tl == tx + 16 * j) tgt[row] = x[j];
-        if (listed && row < rows) {
-          const int p = lt.entry(ty + 16 * i, tx + 16 * j);
-          if (p >= 0) {
-            X.topk.z[row * X.topk.K + p] = x[j];
-            x[j] = -INFINITY;
-          }
-        }
-      }
-      m = fmaxf(m, x[j]);
-    }
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float s = 0.f;
-    if (m != -INFINITY) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s += exp2f((x[j] - m) * kLog2e);
-    }
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (tx == 0 && row < rows) {
-      part_m[tile * N + row] = m;
-      part_s[tile * N + row] = s;
-    }
-  }
-}
-
 template <typename T, typename TB>
 __global__ void __launch_bounds__(THREADS)
 simt_fwd_kernel(const T* __restrict__ e, const T* __restrict__ c, const void* __restrict__ bias,
@@ -249,13 +152,13 @@ simt_fwd_kernel(const T* __restrict__ e, const T* __restrict__ c, const void* __
   }
 }
 
-template <typename T, typename TB, bool kTopk>
+template <typename T, typename TB>
 __global__ void __launch_bounds__(THREADS)
 simt_dlogits_kernel(const T* __restrict__ e, const T* __restrict__ c, const void* __restrict__ bias,
                     const int32_t* __restrict__ targets, const float* __restrict__ lse,
                     const float* __restrict__ d_nll, const uint8_t* __restrict__ keep, int64_t N,
                     int64_t D, int64_t V, int64_t v_offset, int64_t vc0, int64_t vc_len, int64_t ld,
-                    float* __restrict__ dl, float* __restrict__ grad_bias, const SimtRows X) {
+                    float* __restrict__ dl, float* __restrict__ grad_bias) {
   const int64_t r0 = (int64_t)blockIdx.x * BM;
   const int64_t v0 = vc0 + (int64_t)blockIdx.y * BN;   // local vocab id of column 0
   const int64_t vend = min(vc0 + vc_len, V);
@@ -278,8 +181,6 @@ simt_dlogits_kernel(const T* __restrict__ e, const T* __restrict__ c, const void
   float acc[4][8];
   // c holds the chunk's rows: row 0 = local vocab id vc0
   tile_logits<T>(e, c, N, D, vend - vc0, r0, v0 - vc0, acc);
-  __shared__ typename std::conditional<kTopk, ListedTile, char>::type lt;
-  if constexpr (kTopk) lt.load(X.topk, r0, N, v0);
   __shared__ float colsum[BN];
   if (grad_bias) {
     for (int idx = threadIdx.x; idx < BN; idx += THREADS) colsum[idx] = 0.f;
@@ -300,22 +201,15 @@ simt_dlogits_kernel(const T* __restrict__ e, const T* __restrict__ c, const void
     if (row >= N) continue;
     const float g = d_nll[row];
     const float L = lse[row];
-    int64_t tl = -1;
-    if constexpr (!kTopk) tl = (int64_t)targets[row] - v_offset;
+    const int64_t tl = (int64_t)targets[row] - v_offset;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t v = v0 + tx + 16 * j;
       if (v < vend) {
         float w = 0.f;
         if ((kmask >> gof(j)) & 1u) {
-          if constexpr (kTopk) {
-            const int p = lt.entry(ty + 16 * i, tx + 16 * j);
-            w = p >= 0 ? X.d_row[row] * X.topk.z[row * X.topk.K + p]
-                       : g * exp2f(((acc[i][j] + bv[j]) * X.scale - L) * kLog2e);
-          } else {
-            w = g * exp2f((acc[i][j] + bv[j] - L) * kLog2e);
-            if (v == tl) w -= g;
-          }
+          w = g * exp2f((acc[i][j] + bv[j] - L) * kLog2e);
+          if (v == tl) w -= g;
         }
         dl[row * ld + (v - vc0)] = w;
         cs[j] += w;
@@ -437,17 +331,16 @@ cudaError_t fwd_dispatch_bias(const FwdArgs& a, cudaStream_t s) {
   return launched();
 }
 
-template <typename T, bool kTopk>
+template <typename T>
 cudaError_t dl_dispatch_bias(const BwdChunkArgs& a, cudaStream_t s) {
-  const SimtRows X{nullptr, a.logit_scale, a.topk, a.d_row};
   dim3 grid((unsigned)ceil_div(a.N, BM), (unsigned)ceil_div(a.vc_len, BN));
   const T* e = (const T*)a.e;
   const T* c = (const T*)a.c_chunk;
   float* dl = (float*)a.dlogits;
 #define CCE_DL_LAUNCH(TB)                                                                        \
-  simt_dlogits_kernel<T, TB, kTopk><<<grid, THREADS, 0, s>>>(e, c, a.bias, a.targets, a.lse, a.d_nll, a.keep, a.N,  \
-                                                             a.D, a.V, a.v_offset, a.vc0, a.vc_len, a.vc_ld, dl,   \
-                                                             a.grad_bias, X)
+  simt_dlogits_kernel<T, TB><<<grid, THREADS, 0, s>>>(e, c, a.bias, a.targets, a.lse, a.d_nll,    \
+                                                      a.keep, a.N, a.D, a.V, a.v_offset, a.vc0, \
+                                                      a.vc_len, a.vc_ld, dl, a.grad_bias)
   switch (a.bias == nullptr ? CCE_F32 : a.bias_dtype) {
     case CCE_F32: CCE_DL_LAUNCH(float); break;
     case CCE_F16: CCE_DL_LAUNCH(__half); break;
@@ -458,41 +351,7 @@ cudaError_t dl_dispatch_bias(const BwdChunkArgs& a, cudaStream_t s) {
   return launched();
 }
 
-template <typename T>
-cudaError_t logits_dispatch_bias(const FwdArgs& a, cudaStream_t s) {
-  const dim3 grid((unsigned)ceil_div(a.N, BM), (unsigned)ceil_div(a.V, BN));
-  const SimtRows X{a.rows, a.scale, a.topk, nullptr};
-  const T* e = (const T*)a.e;
-  const T* c = (const T*)a.c;
-  switch (a.bias == nullptr ? CCE_F32 : a.bias_dtype) {
-    case CCE_F32:
-      simt_logits_kernel<T, float><<<grid, THREADS, 0, s>>>(e, c, a.bias, a.targets, a.N, a.D, a.V, X, a.part_m,
-                                                            a.part_s, a.tgt);
-      break;
-    case CCE_F16:
-      simt_logits_kernel<T, __half><<<grid, THREADS, 0, s>>>(e, c, a.bias, a.targets, a.N, a.D, a.V, X, a.part_m,
-                                                             a.part_s, a.tgt);
-      break;
-    case CCE_BF16:
-      simt_logits_kernel<T, __nv_bfloat16><<<grid, THREADS, 0, s>>>(e, c, a.bias, a.targets, a.N, a.D, a.V, X,
-                                                                    a.part_m, a.part_s, a.tgt);
-      break;
-    default: return cudaErrorInvalidValue;
-  }
-  return launched();
-}
-
 }  // namespace
-
-cudaError_t simt_logits(const FwdArgs& a, cudaStream_t s) {
-  if (a.N == 0 || a.V == 0) return cudaSuccess;
-  switch (a.dtype) {
-    case CCE_F32: return logits_dispatch_bias<float>(a, s);
-    case CCE_F16: return logits_dispatch_bias<__half>(a, s);
-    case CCE_BF16: return logits_dispatch_bias<__nv_bfloat16>(a, s);
-  }
-  return cudaErrorInvalidValue;
-}
 
 cudaError_t simt_forward(const FwdArgs& a, cudaStream_t s) {
   if (a.N == 0 || a.V == 0) return cudaSuccess;
@@ -507,10 +366,9 @@ cudaError_t simt_forward(const FwdArgs& a, cudaStream_t s) {
 cudaError_t simt_dlogits(const BwdChunkArgs& a, cudaStream_t s) {
   if (a.N == 0 || a.vc_len == 0) return cudaSuccess;
   switch (a.dtype) {
-    case CCE_F32: return a.topk.sid ? dl_dispatch_bias<float, true>(a, s) : dl_dispatch_bias<float, false>(a, s);
-    case CCE_F16: return a.topk.sid ? dl_dispatch_bias<__half, true>(a, s) : dl_dispatch_bias<__half, false>(a, s);
-    case CCE_BF16:
-      return a.topk.sid ? dl_dispatch_bias<__nv_bfloat16, true>(a, s) : dl_dispatch_bias<__nv_bfloat16, false>(a, s);
+    case CCE_F32: return dl_dispatch_bias<float>(a, s);
+    case CCE_F16: return dl_dispatch_bias<__half>(a, s);
+    case CCE_BF16: return dl_dispatch_bias<__nv_bfloat16>(a, s);
   }
   return cudaErrorInvalidValue;
 }

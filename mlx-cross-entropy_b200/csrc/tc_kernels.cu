@@ -1339,14 +1339,14 @@ bool make_tmap_out(CUtensorMap* tm, const void* base, int dtype, int64_t inner, 
   return r == CUDA_SUCCESS;
 }
 
-// The fp32 grad_e accumulator slabs acc2[slabs][N][D] (two with the filter) as a 3-D map, written in
+// The two fp32 grad_e accumulator slabs acc2[2][N][D] as a 3-D map, written in
 // (16 x 32 x 1) boxes (64-byte rows, 64-byte swizzle); the slab index is the z
 // coordinate, so rows past N of one slab are clipped rather than spilling
 // into the other.
-bool make_tmap_acc2(CUtensorMap* tm, const float* acc2, int64_t D, int64_t N, int slabs) {
+bool make_tmap_acc2(CUtensorMap* tm, const float* acc2, int64_t D, int64_t N) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)N, (cuuint64_t)slabs};
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)N, 2};
   cuuint64_t strides[2] = {(cuuint64_t)(D * 4), (cuuint64_t)(N * D * 4)};
   cuuint32_t box[3] = {16, 32, 1};
   cuuint32_t estr[3] = {1, 1, 1};
@@ -1396,8 +1396,6 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 }  // namespace tc
 
 using namespace tc;
-
-bool tc_available() { return encode_fn() != nullptr; }
 
 bool tc_supported(const void* e, const void* c, int64_t D, int dtype) {
   return (dtype == CCE_BF16 || dtype == CCE_F16) && D % 8 == 0 && aligned16(e) && aligned16(c) &&
@@ -1570,8 +1568,9 @@ namespace {
 }  // namespace
 }  // namespace tc
 
-cudaError_t tc_logits(const FwdArgs& a, cudaStream_t s) {
-  if (a.N == 0 || a.V == 0) return cudaSuccess;
+bool tc_available() { return encode_fn() != nullptr; }
+
+cudaError_t tc_logits(const RowsGemmArgs& a, cudaStream_t s) {
   switch (a.bias == nullptr ? -1 : a.bias_dtype) {
     case -1: return logits_dispatch<void>(a, s);
     case CCE_F32: return logits_dispatch<float>(a, s);
@@ -1581,8 +1580,7 @@ cudaError_t tc_logits(const FwdArgs& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-cudaError_t tc_dlogits_rows(const BwdChunkArgs& a, cudaStream_t s) {
-  if (a.N == 0 || a.vc_len == 0) return cudaSuccess;
+cudaError_t tc_dlogits_rows(const RowsGemmArgs& a, cudaStream_t s) {
   switch (a.bias == nullptr ? -1 : a.bias_dtype) {
     case -1: return dlogits2_dispatch<void>(a, s);
     case CCE_F32: return dlogits2_dispatch<float>(a, s);
@@ -1592,11 +1590,19 @@ cudaError_t tc_dlogits_rows(const BwdChunkArgs& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-cudaError_t tc_grad_e_split(const BwdChunkArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
-  return grad_e_split(a, slabs, num_slabs, accumulate, s);
+cudaError_t tc_grad_e_rows(const RowsGemmArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
+  return a.dtype == CCE_F32 ? grad_e_rows<true>(a, slabs, num_slabs, accumulate, s)
+                            : grad_e_rows<false>(a, slabs, num_slabs, accumulate, s);
 }
 
-cudaError_t tc_grad_c_split(const BwdChunkArgs& a, float* grad_c, cudaStream_t s) { return grad_c_split(a, grad_c, s); }
+cudaError_t tc_grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t s) {
+  switch (a.dtype) {
+    case CCE_F32: return grad_c_rows<float, true>(a, grad_c, s);
+    case CCE_F16: return grad_c_rows<__half, false>(a, grad_c, s);
+    case CCE_BF16: return grad_c_rows<__nv_bfloat16, false>(a, grad_c, s);
+  }
+  return cudaErrorNotSupported;
+}
 
 namespace {
 
@@ -1610,9 +1616,9 @@ cudaError_t grad_e_launch(const BwdChunkArgs& a, float* acc2, bool accumulate, c
   int b3d = 0;
   if (!make_tmap_mn(&tmB, cchunk, bf16, a.D, a.vc_len, a.D, (BN) / 64, &b3d))
     return cudaErrorInvalidValue;
-  if (!make_tmap_acc2(&tmC, acc2, a.D, a.N, a.slabs)) return cudaErrorInvalidValue;
+  if (!make_tmap_acc2(&tmC, acc2, a.D, a.N)) return cudaErrorInvalidValue;
   Sched sc{(int)ceil_div(a.N, BM), (int)ceil_div(a.D, BN), (int)ceil_div(a.vc_len, BK), 1, 0, b3d,
-           a.counters ? a.counters + 1 : nullptr, raster_group(a.N * a.vc_len * 2), a.slabs};
+           a.counters ? a.counters + 1 : nullptr, raster_group(a.N * a.vc_len * 2), 2};
   GradEEpi epi{a.scale, a.keep + a.vc0 / kStatTile, ceil_div(a.V, kStatTile), (int)ceil_div(a.N, kRowBlock),
                (int)ceil_div(a.vc_len, kStatTile), accumulate ? 1 : 0, acc2, a.N, a.D};
   if (push != nullptr) {

@@ -50,8 +50,9 @@
 
 constexpr int kRgWarps = 8;                   // epilogue warps: two per TMEM lane quarter, a column half each
 constexpr int kRgThreads = 64 + 32 * kRgWarps;
-// K-blocks per accumulator segment: 4, 2 for split operands (accuracy is what they are for)
-__host__ __device__ constexpr int seg_kb(bool split) { return split ? 2 : 4; }
+// K-blocks per accumulator segment: 4 for logits, 2 for split operands (accuracy is
+// what they are for), 16 for gradients that are rounded to 16 bits.
+__host__ __device__ constexpr int seg_kb(bool split, bool grad) { return split ? 2 : grad ? 16 : 4; }
 constexpr size_t kRgSmem = 1024 + STAGES * (size_t)STAGE_BYTES + kRgWarps * 4096 + 256;
 
 struct RowsSched {
@@ -59,6 +60,7 @@ struct RowsSched {
   int64_t N;             // their capacity
   int m_rows, k_rows;    // M / K runs over the rows
   int num_m, num_n, num_kb, ksplit, m_fast, group;
+  int b3d = 1;           // MN-major B as one 3-D box (else one 2-D box per 64 columns)
   __device__ __forceinline__ Sched get(int64_t& count) const {
     count = min((int64_t)__ldg(rows), N);
     Sched s{};
@@ -187,7 +189,7 @@ struct LogitsEpi {
 };
 
 // dlogits of one vocabulary chunk (columns relative to it).  Log-probabilities:
-// w = d (softmax - onehot).  Distillation: g e^(z - L) with the coefficient and
+// w = d (softmax - onehot).  Distillation: A d e^(z - L) with the coefficient and
 // log-sum-exp of the columns outside of the row's list, d x for the listed ones.
 // float16 holds w / s (`scale` = {s, 1 / s}); split: hi + lo.
 template <typename T, typename TB, bool kTopk, bool kSplit>
@@ -196,22 +198,25 @@ struct DlogitsEpi2 {
   static constexpr bool kStores = true;
   const int32_t* targets;
   const float* lse;
-  const float* g;         // [N] d, or the coefficient
-  const float* d_row;     // [N] kTopk: d
+  Cotangent up;           // d of a row
+  const int32_t* row_of;
+  const float* A;         // [N] kTopk: coefficient over d
   const void* bias;       // of column 0 of the whole vocabulary
   const float* scale;
   float* bias_part;       // [ceil(N / 32)][ld] column sums of w, or nullptr
   int64_t N, V, vc0, vc_end, ld;
-  float logit_scale;
+  float scale_z;
   const float *se, *sc;
   TopkView topk;
 
   __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap* tm_lo) const {
     const bool live = t.row < t.rows;
     const float inv = scale ? scale[1] : 1.f;
-    const float G = live ? g[t.row] * inv : 0.f;
+    const float d = live ? up.of(t.row, row_of) : 0.f;
     const float L = live ? lse[t.row] : INFINITY;
-    const float dr = kTopk && live ? d_row[t.row] * inv : 0.f;
+    const float dr = d * inv;
+    // (a row that gets no gradient: 0 whatever its coefficient)
+    const float G = kTopk ? (live && d != 0.f ? A[t.row] * dr : 0.f) : dr;
     const int64_t v0 = vc0 + t.col0;  // vocabulary id of column 0
     const int64_t tl = (!kTopk && live) ? (int64_t)targets[t.row] - v0 : -1;
     TopkCursor cur;
@@ -230,7 +235,7 @@ struct DlogitsEpi2 {
       }
       add_bias<TB>(bias, cb, vc_end, v);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = G * ex2((v[j] * logit_scale - L) * kLog2e);
+      for (int j = 0; j < 32; ++j) v[j] = G * ex2((v[j] * scale_z - L) * kLog2e);
       if constexpr (kTopk) {
         int p;
         const uint32_t bits = cur.take(cb, p);
@@ -276,6 +281,28 @@ struct DlogitsEpi2 {
   }
 };
 
+// out[row][col] = f (A B) in T
+template <typename T>
+struct Out16Epi {
+  static constexpr int kKind = 3;
+  static constexpr bool kStores = true;
+  const float* f;  // {s, 1 / s} of float16 dlogits, or nullptr
+  int64_t M, D;
+
+  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
+    const float s = f ? *f : 1.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t col = t.col0 + c * 32;
+      if (col >= D || t.y0 >= M) continue;
+      float(&v)[32] = *reinterpret_cast<float(*)[32]>(z + c * 32);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= s;
+      sg.template store16<T>(v, (int)col, t.y0);
+    }
+  }
+};
+
 // out[ks][row][col] (+)= f1 f2 (A B), float32
 struct OutEpi {
   static constexpr bool kStores = true;
@@ -286,7 +313,7 @@ struct OutEpi {
   static constexpr int kKind = -1;  // (that of `kind`)
 
   __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
-    const float f = *f1 * *f2;
+    const float f = (f1 ? *f1 : 1.f) * (f2 ? *f2 : 1.f);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t col = t.col0 + c * 32;
@@ -305,7 +332,7 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                  const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmB2,
                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmC2, const RowsSched rs,
                  const Epi epi, const uint32_t idesc, const float untruncate) {
-  constexpr int kSegKb = seg_kb(kSplit);
+  constexpr int kSegKb = seg_kb(kSplit, B_MN);
   constexpr int kPasses = kSplit ? 3 : 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
@@ -365,8 +392,15 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             mbar_arrive_expect_tx(full + stage, STAGE_BYTES);
             if constexpr (A_MN) tma_load_3d(a, ma, full + stage, 0, kb * BK, mb * (BM / 64));
             else tma_load_2d(a, ma, full + stage, kb * BK, mb * BM);
-            if constexpr (B_MN) tma_load_3d(b, mb_, full + stage, 0, kb * BK, nb * (BN / 64));
-            else tma_load_2d(b, mb_, full + stage, kb * BK, nb * BN);
+            if constexpr (B_MN) {
+              if (rs.b3d) {
+                tma_load_3d(b, mb_, full + stage, 0, kb * BK, nb * (BN / 64));
+              } else {
+#pragma unroll
+                for (int j = 0; j < BN / 64; ++j)
+                  tma_load_2d(b + j * BOX_MN_BYTES, mb_, full + stage, nb * BN + j * 64, kb * BK);
+              }
+            } else tma_load_2d(b, mb_, full + stage, kb * BK, nb * BN);
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1u;
@@ -499,80 +533,78 @@ cudaError_t rows_gemm(const RowsMaps& m, const RowsSched& rs, const Epi& epi, bo
   return launched();
 }
 
-// e (packed rows) and c, K-major: whole 16-bit operands or hi / lo.
-bool ec_maps(RowsMaps& m, const void* e, const void* c, const SplitView& sp, bool bf16, int64_t N, int64_t D, int64_t V,
-             int64_t v0) {
-  const bool split = sp.e_hi != nullptr;
-  const int64_t d = split ? sp.Dp : D;
-  const uint16_t* ch = static_cast<const uint16_t*>(split ? sp.c_hi : c);
-  const uint16_t* cl = static_cast<const uint16_t*>(sp.c_lo);
-  if (split) ch += v0 * d;  // (c is the chunk's first row already)
-  bool ok = make_tmap(&m.A, split ? sp.e_hi : e, bf16, d, N, d, BK, BM) && make_tmap(&m.B, ch, bf16, d, V, d, BK, BN);
+// e (packed rows) and the chunk's rows of c, K-major: whole 16-bit operands or hi / lo.
+bool ec_maps(RowsMaps& m, const RowsGemmArgs& a) {
+  const bool bf16 = a.dtype == CCE_BF16, split = a.dtype == CCE_F32;
+  const int64_t off = a.vc0 * a.Dk;
+  bool ok = make_tmap(&m.A, a.e, bf16, a.Dk, a.N, a.Dk, BK, BM) &&
+            make_tmap(&m.B, static_cast<const uint16_t*>(a.c) + off, bf16, a.Dk, a.vc_len, a.Dk, BK, BN);
   m.A2 = m.A;
   m.B2 = m.B;
   if (split)
-    ok = ok && make_tmap(&m.A2, sp.e_lo, bf16, d, N, d, BK, BM) && make_tmap(&m.B2, cl + v0 * d, bf16, d, V, d, BK, BN);
+    ok = ok && make_tmap(&m.A2, a.e_lo, bf16, a.Dk, a.N, a.Dk, BK, BM) &&
+         make_tmap(&m.B2, static_cast<const uint16_t*>(a.c_lo) + off, bf16, a.Dk, a.vc_len, a.Dk, BK, BN);
   m.C = m.C2 = m.A;  // (replaced where an epilogue stores)
   return ok;
 }
 
+// Schedule of the two logits kernels: row tiles first, so that a column tile of c
+// is read once for all of them.
+RowsSched ec_sched(const RowsGemmArgs& a) {
+  return RowsSched{a.R.count, a.N, 1, 0, 0, (int)ceil_div(a.vc_len, BN), (int)ceil_div(a.Dk, BK), 1, 1,
+                   raster_group(a.N * a.Dk * 2)};
+}
+
 template <typename TB, bool kTopk>
-cudaError_t logits_launch(const FwdArgs& f, cudaStream_t s) {
-  const bool split = f.split.e_hi != nullptr, bf16 = !split && f.dtype == CCE_BF16;
+cudaError_t logits_launch(const RowsGemmArgs& a, cudaStream_t s) {
   RowsMaps m;
-  if (!ec_maps(m, f.e, f.c, f.split, bf16, f.N, f.D, f.V, 0)) return cudaErrorInvalidValue;
-  const int num_n = (int)ceil_div(f.V, BN);
-  const RowsSched rs{f.rows, f.N, 1, 0, 0, num_n, (int)ceil_div(split ? f.split.Dp : f.D, BK), 1, 1,
-                     raster_group(f.N * f.D * 2)};
-  const LogitsEpi<TB, kTopk> epi{f.targets, f.bias, f.part_m, f.part_s, f.tgt, f.N, f.V, f.scale,
-                                 f.split.se, f.split.sc, f.topk};
-  const int64_t units = ceil_div(f.N, BM) * num_n;
-  return split ? rows_gemm<false, false, true>(m, rs, epi, bf16, units, s)
-               : rows_gemm<false, false, false>(m, rs, epi, bf16, units, s);
+  if (!ec_maps(m, a)) return cudaErrorInvalidValue;
+  const RowsSched rs = ec_sched(a);
+  const LogitsEpi<TB, kTopk> epi{a.R.targets, a.bias, a.part_m, a.part_s, a.tgt, a.N, a.V, a.scale_z, a.se, a.sc, a.topk};
+  const int64_t units = ceil_div(a.N, BM) * rs.num_n;
+  return a.dtype == CCE_F32 ? rows_gemm<false, false, true>(m, rs, epi, false, units, s)
+                            : rows_gemm<false, false, false>(m, rs, epi, a.dtype == CCE_BF16, units, s);
 }
 
 template <typename TB>
-cudaError_t logits_dispatch(const FwdArgs& f, cudaStream_t s) {
-  return f.topk.sid ? logits_launch<TB, true>(f, s) : logits_launch<TB, false>(f, s);
+cudaError_t logits_dispatch(const RowsGemmArgs& a, cudaStream_t s) {
+  return a.topk.sid ? logits_launch<TB, true>(a, s) : logits_launch<TB, false>(a, s);
 }
 
 template <typename T, typename TB, bool kTopk, bool kSplit>
-cudaError_t dlogits2_launch(const BwdChunkArgs& a, cudaStream_t s) {
-  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+cudaError_t dlogits2_launch(const RowsGemmArgs& a, cudaStream_t s) {
   RowsMaps m;
-  if (!ec_maps(m, a.e, a.c_chunk, a.split, bf16, a.N, a.D, a.vc_len, a.vc0)) return cudaErrorInvalidValue;
-  const int dt = bf16 ? CCE_BF16 : CCE_F16;
-  if (!make_tmap_out(&m.C, a.dlogits, dt, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
+  const int dt = a.dtype == CCE_BF16 ? CCE_BF16 : CCE_F16;
+  if (!ec_maps(m, a) || !make_tmap_out(&m.C, a.dl, dt, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
   m.C2 = m.C;
-  if (kSplit && !make_tmap_out(&m.C2, a.dlogits_lo, dt, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
-  const int num_n = (int)ceil_div(a.vc_len, BN);
-  const RowsSched rs{a.rows, a.N, 1, 0, 0, num_n, (int)ceil_div(kSplit ? a.split.Dp : a.D, BK), 1, 1,
-                     raster_group(a.N * a.D * 2)};
-  const DlogitsEpi2<T, TB, kTopk, kSplit> epi{a.targets, a.lse, a.d_nll, a.d_row, a.bias, a.scale, a.bias_part, a.N, a.V,
-                                             a.vc0, a.vc0 + a.vc_len, a.vc_ld, a.logit_scale, a.split.se, a.split.sc,
-                                             a.topk};
-  return rows_gemm<false, false, kSplit>(m, rs, epi, bf16, ceil_div(a.N, BM) * num_n, s);
+  if (kSplit && !make_tmap_out(&m.C2, a.dl_lo, dt, a.vc_len, a.N, a.vc_ld)) return cudaErrorInvalidValue;
+  const RowsSched rs = ec_sched(a);
+  const DlogitsEpi2<T, TB, kTopk, kSplit> epi{a.R.targets, a.lse, a.up, a.R.row_of, a.A, a.bias, a.scale, a.bias_part,
+                                             a.N, a.V, a.vc0, a.vc0 + a.vc_len, a.vc_ld, a.scale_z, a.se, a.sc, a.topk};
+  return rows_gemm<false, false, kSplit>(m, rs, epi, dt == CCE_BF16, ceil_div(a.N, BM) * rs.num_n, s);
 }
 
 template <typename TB, bool kTopk>
-cudaError_t dlogits2_types(const BwdChunkArgs& a, cudaStream_t s) {
-  if (a.split.e_hi) return dlogits2_launch<__half, TB, kTopk, true>(a, s);
-  if (a.dtype == CCE_BF16) return dlogits2_launch<__nv_bfloat16, TB, kTopk, false>(a, s);
-  if (a.dtype == CCE_F16) return dlogits2_launch<__half, TB, kTopk, false>(a, s);
+cudaError_t dlogits2_types(const RowsGemmArgs& a, cudaStream_t s) {
+  switch (a.dtype) {
+    case CCE_F32: return dlogits2_launch<__half, TB, kTopk, true>(a, s);
+    case CCE_F16: return dlogits2_launch<__half, TB, kTopk, false>(a, s);
+    case CCE_BF16: return dlogits2_launch<__nv_bfloat16, TB, kTopk, false>(a, s);
+  }
   return cudaErrorNotSupported;
 }
 
 template <typename TB>
-cudaError_t dlogits2_dispatch(const BwdChunkArgs& a, cudaStream_t s) {
+cudaError_t dlogits2_dispatch(const RowsGemmArgs& a, cudaStream_t s) {
   return a.topk.sid ? dlogits2_types<TB, true>(a, s) : dlogits2_types<TB, false>(a, s);
 }
 
-// float32 [z][rows][D] output, written in (16 x 32 x 1) boxes
-bool make_tmap_f32(CUtensorMap* tm, const float* out, int64_t D, int64_t rows, int64_t slabs) {
+// float32 [z][rows][ld] output of D columns, written in (16 x 32 x 1) boxes
+bool make_tmap_f32(CUtensorMap* tm, const float* out, int64_t D, int64_t ld, int64_t rows, int64_t slabs) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)slabs};
-  cuuint64_t strides[2] = {(cuuint64_t)(D * 4), (cuuint64_t)(rows * D * 4)};
+  cuuint64_t strides[2] = {(cuuint64_t)(ld * 4), (cuuint64_t)(rows * ld * 4)};
   cuuint32_t box[3] = {16, 32, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   return fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(out), dims, strides, box, estr,
@@ -580,38 +612,53 @@ bool make_tmap_f32(CUtensorMap* tm, const float* out, int64_t D, int64_t rows, i
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-cudaError_t grad_e_split(const BwdChunkArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
-  const SplitView& sp = a.split;
+template <bool kSplit>
+cudaError_t grad_e_rows(const RowsGemmArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
+  const bool bf16 = a.dtype == CCE_BF16;
+  const int64_t off = a.vc0 * a.Dk;
   RowsMaps m;
-  const uint16_t* ch = static_cast<const uint16_t*>(sp.c_hi) + a.vc0 * sp.Dp;
-  const uint16_t* cl = static_cast<const uint16_t*>(sp.c_lo) + a.vc0 * sp.Dp;
-  if (!make_tmap(&m.A, a.dlogits, false, a.vc_len, a.N, a.vc_ld, BK, BM) ||
-      !make_tmap(&m.A2, a.dlogits_lo, false, a.vc_len, a.N, a.vc_ld, BK, BM) ||
-      !make_tmap_mn3d(&m.B, ch, false, sp.Dp, a.vc_len, sp.Dp, BK, BN / 64) ||
-      !make_tmap_mn3d(&m.B2, cl, false, sp.Dp, a.vc_len, sp.Dp, BK, BN / 64) ||
-      !make_tmap_f32(&m.C, slabs, a.D, a.N, num_slabs))
-    return cudaErrorInvalidValue;
-  m.C2 = m.C;
-  const int num_n = (int)ceil_div(a.D, BN);
-  const RowsSched rs{a.rows, a.N, 1, 0, 0, num_n, (int)ceil_div(a.vc_len, BK), num_slabs, 1,
-                     raster_group(a.N * a.vc_len * 2)};
-  const OutEpi epi{a.scale, sp.sc + 1, accumulate ? 1 : 0, a.N, a.D, 2};
-  return rows_gemm<false, true, true>(m, rs, epi, false, ceil_div(a.N, BM) * num_n * num_slabs, s);
+  int b3d = 0;
+  bool ok = make_tmap(&m.A, a.dl, bf16, a.vc_len, a.N, a.vc_ld, BK, BM) &&
+            make_tmap_mn(&m.B, static_cast<const uint16_t*>(a.c) + off, bf16, a.Dk, a.vc_len, a.Dk, BN / 64, &b3d) &&
+            make_tmap_f32(&m.C, slabs, a.Dout, a.Dout, a.N, num_slabs);
+  m.A2 = m.A, m.B2 = m.B, m.C2 = m.C;
+  if (kSplit)
+    ok = ok && make_tmap(&m.A2, a.dl_lo, bf16, a.vc_len, a.N, a.vc_ld, BK, BM) &&
+         make_tmap_mn(&m.B2, static_cast<const uint16_t*>(a.c_lo) + off, bf16, a.Dk, a.vc_len, a.Dk, BN / 64, &b3d);
+  if (!ok) return cudaErrorInvalidValue;
+  const int num_n = (int)ceil_div(a.Dout, BN);
+  const RowsSched rs{a.R.count, a.N, 1, 0, 0, num_n, (int)ceil_div(a.vc_len, BK), num_slabs, 1,
+                     raster_group(a.N * a.vc_len * 2), b3d};
+  const OutEpi epi{a.scale, kSplit ? a.sc + 1 : nullptr, accumulate ? 1 : 0, a.N, a.Dout, 2};
+  return rows_gemm<false, true, kSplit>(m, rs, epi, bf16, ceil_div(a.N, BM) * num_n * num_slabs, s);
 }
 
-cudaError_t grad_c_split(const BwdChunkArgs& a, float* grad_c, cudaStream_t s) {
-  const SplitView& sp = a.split;
+// grad_c rows of the chunk.  T: the output's type (float with split operands)
+template <typename T, bool kSplit>
+cudaError_t grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t s) {
+  const bool bf16 = a.dtype == CCE_BF16;
+  T* out = static_cast<T*>(grad_c) + a.vc0 * a.Dout;
+  const int64_t cols = round_up(a.vc_len, 64);  // (rows of grad_c behind the chunk are clipped by the output's map)
   RowsMaps m;
-  const int64_t cols = round_up(a.vc_len, 64);  // (rows behind the chunk are clipped by the output's map)
-  if (!make_tmap_mn3d(&m.A, a.dlogits, false, cols, a.N, a.vc_ld, BK, BM / 64) ||
-      !make_tmap_mn3d(&m.A2, a.dlogits_lo, false, cols, a.N, a.vc_ld, BK, BM / 64) ||
-      !make_tmap_mn3d(&m.B, sp.e_hi, false, sp.Dp, a.N, sp.Dp, BK, BN / 64) ||
-      !make_tmap_mn3d(&m.B2, sp.e_lo, false, sp.Dp, a.N, sp.Dp, BK, BN / 64) ||
-      !make_tmap_f32(&m.C, grad_c + a.vc0 * a.D, a.D, a.vc_len, 1))
-    return cudaErrorInvalidValue;
+  int b3d = 0;
+  bool ok = make_tmap_mn3d(&m.A, a.dl, bf16, cols, a.N, a.vc_ld, BK, BM / 64) &&
+            make_tmap_mn(&m.B, a.e, bf16, a.Dk, a.N, a.Dk, BN / 64, &b3d);
+  m.A2 = m.A, m.B2 = m.B;
+  if constexpr (kSplit)
+    ok = ok && make_tmap_mn3d(&m.A2, a.dl_lo, bf16, cols, a.N, a.vc_ld, BK, BM / 64) &&
+         make_tmap_mn(&m.B2, a.e_lo, bf16, a.Dk, a.N, a.Dk, BN / 64, &b3d) &&
+         make_tmap_f32(&m.C, out, a.Dout, a.Dout, a.vc_len, 1);
+  else
+    ok = ok && make_tmap_out(&m.C, out, a.dtype, a.Dout, a.vc_len, a.Dout);
+  if (!ok) return cudaErrorInvalidValue;
   m.C2 = m.C;
-  const int num_m = (int)ceil_div(a.vc_len, BM), num_n = (int)ceil_div(a.D, BN);
-  const RowsSched rs{a.rows, a.N, 0, 1, num_m, num_n, 0, 1, 0, raster_group(a.N * a.D * 2)};
-  const OutEpi epi{a.scale, sp.se + 1, 0, a.vc_len, a.D, 3};
-  return rows_gemm<true, true, true>(m, rs, epi, false, (int64_t)num_m * num_n, s);
+  const int num_m = (int)ceil_div(a.vc_len, BM), num_n = (int)ceil_div(a.Dout, BN);
+  const RowsSched rs{a.R.count, a.N, 0, 1, num_m, num_n, 0, 1, 0, raster_group(a.N * a.Dk * 2), b3d};
+  if constexpr (kSplit) {
+    const OutEpi epi{a.scale, a.se + 1, 0, a.vc_len, a.Dout, 3};
+    return rows_gemm<true, true, true>(m, rs, epi, bf16, (int64_t)num_m * num_n, s);
+  } else {
+    const Out16Epi<T> epi{a.scale, a.vc_len, a.Dout};
+    return rows_gemm<true, true, false>(m, rs, epi, bf16, (int64_t)num_m * num_n, s);
+  }
 }

@@ -198,7 +198,10 @@ def _head(what, e, c, bias, rows_shape):
             raise ValueError(f"[{what}] {name} must be a CUDA tensor (no CPU implementation exists)")
         if t.device != e.device:
             raise ValueError(f"[{what}] {name} is on {t.device}, expected {e.device}")
-    return (e.reshape(-1, e.shape[-1]).contiguous(), c.contiguous(), None if bias is None else bias.contiguous())
+    c = c.contiguous()
+    if c.data_ptr() % 16:  # (a view at an odd element: the kernels' copies start on 16-byte boundaries)
+        c = c.clone()
+    return e.reshape(-1, e.shape[-1]).contiguous(), c, None if bias is None else bias.contiguous()
 
 
 def _ids(what, name, t, dev):

@@ -94,12 +94,14 @@ def test_saved_and_workspace_sizes():
     assert d >= N * D * 2 + N * K * 8 + N * (V // 256) * 2 and d < 2 * b
     assert lib.cce_logp_forward_workspace_bytes(N, D, V, _ext.CCE_BF16) < N * V // 8   # never [N, V]
     flags = _ext.CCE_NEED_DE | _ext.CCE_NEED_DC
-    plain = lib.cce_backward_workspace_bytes(N, D, V, _ext.CCE_BF16, flags)
-    # the same chunk buffers (without the filter's lists of live tiles) and a few values per row
+    # a bounded chunk of the dlogits (never [N, V]) and fp32 slabs of grad_e
     rows = lib.cce_logp_backward_workspace_bytes(N, D, V, _ext.CCE_BF16, flags)
-    assert plain - (1 << 20) < rows < plain + 64 * N
-    # float32: both parts of c, and a bounded chunk of the dlogits' parts
+    assert N * D * 4 <= rows < N * V * 2 / 2 + (256 << 20)
+    # float32: both parts of c as well
     f32 = lib.cce_logp_backward_workspace_bytes(N, D, V, _ext.CCE_F32, flags)
     assert V * D * 4 < f32 < V * D * 4 + 3 * (1 << 29)
+    # odd widths: padded copies of c and grad_c
+    odd = lib.cce_logp_backward_workspace_bytes(64, 71, 1000, _ext.CCE_BF16, flags)
+    assert odd > 2 * 1000 * 72 * 2 + lib.cce_logp_backward_workspace_bytes(64, 72, 1000, _ext.CCE_BF16, flags) - 4096
     assert lib.cce_distill_saved_bytes(N, D, V, 1025, _ext.CCE_BF16) == 0
     assert lib.cce_logp_saved_bytes(-1, D, V, _ext.CCE_BF16) == 0

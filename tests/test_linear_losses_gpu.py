@@ -4,19 +4,22 @@ Tolerances are bounds of the arithmetic, element by element, with u = 2^-24 (hal
 a float32 step), h half a step of the input type, and B = max over the logits of
 sum_k |e_k c_k|:
 
-* a logit of 16-bit inputs: tensor cores add products of 16 at a time rounding
-  towards zero (2u), 16 such steps per segment, then one float32 addition per
-  256 products: dz = (16 * 2u + ceil(D / 256) u) B; of float32 inputs: one
-  rounding per product, dz = D u B; the bias and the temperature 2u |z| more;
+* a logit: tensor cores add products of 16 at a time rounding towards zero (2u);
+  of 16-bit inputs 16 such steps per segment, then one float32 addition per 256
+  products: dz = (16 * 2u + ceil(D / 256) u) B; of float32 inputs, each the sum of
+  two float16 parts to 2^-22 (4u) and the parts' smallest product left out (4u),
+  8 steps per segment and three additions per 128 columns: dz = (8 * 2u +
+  3 * (ceil(D / 128) + 1) u + 12u) B; the bias and the temperature 2u |z| more;
 * a log-probability: the target's logit and the log-sum-exp move by dz each;
   exp2 and its argument (|z - max| < 40) and the logarithm: within 2^-18;
 * a dlogit w, a difference of softmax and teacher values times the row's
   cotangent d: those values carry 2 dz + 2^-18 relative each; w is rounded to the
-  input type (h; float16 holds it over the largest d's power of two: 2^-25 of
-  that more below its normal range); float32 inputs keep it in float32 (u);
+  input type (h; float32 inputs: to two float16 parts, as e and c, h = 12u);
+  float16 parts are in units of 2^-14 of the largest d's power of two, so half
+  their smallest step is 2^-39 of it;
 * a gradient sum_v w_v c_v: those relative errors times sum_v |w_v c_v|, and the
-  accumulation's: 2u per 16 terms (u per term for float32), u per chunk added;
-  the result is rounded to the input type (h).
+  accumulation's: 2u per 16 terms, u per segment, chunk and K split added;
+  the result is rounded to the input type (eps / 2).
 """
 
 import math
@@ -49,19 +52,15 @@ class Bounds:
     """The bounds above for one head."""
 
     def __init__(self, e, c, b, T=1.0):
-        self.dt = e.dtype
         N, D = e.shape
-        self.V = c.shape[0]
         big = float((e.double().abs() @ c.double().abs().t()).max()) if N else 0.0
-        steps = (16 * 2 + math.ceil(D / 256)) if self.tc(D) else D
+        f32 = e.dtype == torch.float32
+        steps = 8 * 2 + 3 * (math.ceil(D / 128) + 1) + 12 if f32 else 16 * 2 + math.ceil(D / 256)
         z = big + (0.0 if b is None else float(b.double().abs().max()))
         self.dz = (steps * U * big + 2 * U * z) / T
         self.dlogp = 2 * self.dz + 2.0 ** -18
-        self.h = torch.finfo(self.dt).eps / 2 if self.dt != torch.float32 else U
-        self.tensor = self.tc(D)
-
-    def tc(self, D):
-        return self.dt != torch.float32 and D % 8 == 0
+        self.h = 12 * U if f32 else torch.finfo(e.dtype).eps / 2
+        self.tiny = 0.0 if e.dtype == torch.bfloat16 else 2.0 ** -39
 
 
 def leaves(e, c, b):
@@ -79,11 +78,8 @@ def check_grads(B, grads, e, c, b, w, mag, d):
             (grads[0], w @ c64, wa, c64, extra @ c64.abs(), "grad_e"),
             (grads[1], w.t() @ e64, wa.t(), e64, extra.t() @ e64.abs(), "grad_c")):
         got = got.cpu()
-        M = left.shape[1]
-        acc = (M / 16 + 64) * 2 * U if B.tensor else (M + 64) * U
-        tol = add + (left @ other.abs()) * ((B.h if B.tensor else U) + acc)
-        if B.dt == torch.float16 and B.tensor:
-            tol = tol + 2.0 ** math.ceil(math.log2(max(float(d.max()), 1e-30))) * 2.0 ** -25 * other.abs().sum(0)
+        tol = add + (left @ other.abs()) * (B.h + (left.shape[1] / 16 + 64) * 2 * U)
+        tol = tol + 2.0 ** math.ceil(math.log2(max(float(d.max()), 1e-30))) * B.tiny * other.abs().sum(0)
         if got.dtype != torch.float32:
             tol = tol + R.half_steps(got.dtype, want.abs() + tol)
         bad = (got.double() - want).abs() > tol + 1e-37
