@@ -87,15 +87,16 @@ def _sequences(what, shape, cu_seqlens, dev):
                      f"got {tuple(shape)}")
 
 
-def _like(what, name, t, logp):
+def _per_token(what, name, t, tokens, dtype=torch.float32):
+    """t as a constant of the tokens' shape and the given dtype."""
     if t is None:
         return None
-    if t.shape != logp.shape:
-        raise ValueError(f"[{what}] {name} must have logp's shape {tuple(logp.shape)}, got {tuple(t.shape)}")
-    if t.dtype != logp.dtype:
-        raise ValueError(f"[{what}] {name} must have logp's dtype {logp.dtype}, got {t.dtype}")
-    if t.device != logp.device:
-        raise ValueError(f"[{what}] {name} is on {t.device}, expected {logp.device}")
+    if t.shape != tokens.shape:
+        raise ValueError(f"[{what}] {name} must have the tokens' shape {tuple(tokens.shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"[{what}] {name} must be {dtype} (the log-probabilities' dtype), got {t.dtype}")
+    if t.device != tokens.device:
+        raise ValueError(f"[{what}] {name} is on {t.device}, expected {tokens.device}")
     return _constant(t)
 
 
@@ -220,17 +221,17 @@ def _distill_params(what, temperature, tail, reduction):
     return _ext.CceDistillParams(temperature, int(bool(tail)), PREFERENCE_REDUCTIONS[reduction])
 
 
-def _reference(what, ref_logp, logp, S):
+def _reference(what, ref_logp, tokens, dtype, S):
     """(per-token reference or None, per-sequence sums or None)"""
     if ref_logp is None:
         return None, None
-    if ref_logp.shape == logp.shape:
-        return _like(what, "ref_logp", ref_logp, logp), None
+    if ref_logp.shape == tokens.shape:
+        return _per_token(what, "ref_logp", ref_logp, tokens, dtype), None
     if ref_logp.shape != (S,):
-        raise ValueError(f"[{what}] ref_logp must be per token {tuple(logp.shape)} or per sequence ({S},), "
+        raise ValueError(f"[{what}] ref_logp must be per token {tuple(tokens.shape)} or per sequence ({S},), "
                          f"got {tuple(ref_logp.shape)}")
-    if not ref_logp.is_floating_point() or ref_logp.device != logp.device:
-        raise ValueError(f"[{what}] ref_logp must be floating point on {logp.device}")
+    if not ref_logp.is_floating_point() or ref_logp.device != tokens.device:
+        raise ValueError(f"[{what}] ref_logp must be floating point on {tokens.device}")
     return None, _constant(ref_logp.to(torch.float32))
 
 
@@ -291,25 +292,70 @@ class PreferenceLossFunction(torch.autograd.Function):
         return (_ext.preference_backward(state, g, reduction, mask, cu, N, pairs, shape, dtype),) + (None,) * 6
 
 
+def _head_grads(grads, bias):
+    ge, gc, gb = grads
+    return ge, gc, gb if gb is None or gb.dtype == bias.dtype else gb.to(bias.dtype)
+
+
 class LogProbsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, e, c, bias, targets, ignore_index):
-        logp, mask, saved = _ext.logp_forward(e, c, bias, targets, ignore_index)
+        logp, saved = _ext.logp_forward(e, c, bias, targets, ignore_index)
         ctx.save_for_backward(c, bias, saved)
         ctx.meta = (e.shape[0], e.dtype)
-        ctx.mark_non_differentiable(mask)
-        ctx.set_materialize_grads(False)
-        return logp, mask
+        return logp
 
     @staticmethod
     @_first_order
-    def backward(ctx, grad_logp, _grad_mask):
-        need = ctx.needs_input_grad
-        if grad_logp is None or not any(need[:3]):
-            return (None,) * 5
+    def backward(ctx, grad_logp):
         c, bias, saved = ctx.saved_tensors
-        ge, gc, gb = _ext.logp_backward(saved, c, bias, grad_logp.to(torch.float32).contiguous(), *ctx.meta, *need[:3])
-        return ge, gc, None if gb is None else gb.to(bias.dtype), None, None
+        g = grad_logp.to(torch.float32).contiguous()
+        return _head_grads(_ext.logp_backward(saved, c, bias, g, *ctx.meta, *ctx.needs_input_grad[:3]), bias) + (None,) * 2
+
+
+class LinearPolicyLossFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, e, c, bias, targets, ignore_index, old, ref, adv, cu, S, params):
+        loss, stats, state = _ext.linear_policy_forward(e, c, bias, targets, ignore_index, old, ref, adv, cu, S, params)
+        ctx.save_for_backward(c, bias, state, cu)
+        ctx.meta = (e.shape[0], e.dtype, params.reduction), S
+        ctx.mark_non_differentiable(stats)
+        ctx.set_materialize_grads(False)
+        return loss, stats
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, grad_loss, _grad_stats):
+        if grad_loss is None:
+            return (None,) * 11
+        c, bias, state, cu = ctx.saved_tensors
+        meta, S = ctx.meta
+        g = grad_loss.to(torch.float32).contiguous()
+        grads = _ext.linear_policy_backward(state, c, bias, g, *meta, cu, S, *ctx.needs_input_grad[:3])
+        return _head_grads(grads, bias) + (None,) * 8
+
+
+class LinearPreferenceLossFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, e, c, bias, targets, ignore_index, ref, ref_sums, cu, pairs, params):
+        loss, rewards, state = _ext.linear_preference_forward(e, c, bias, targets, ignore_index, ref, ref_sums, cu,
+                                                              pairs, params)
+        ctx.save_for_backward(c, bias, state, cu)
+        ctx.meta = (e.shape[0], e.dtype, params.reduction), pairs
+        ctx.mark_non_differentiable(rewards)
+        ctx.set_materialize_grads(False)
+        return loss, rewards
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, grad_loss, _grad_rewards):
+        if grad_loss is None:
+            return (None,) * 10
+        c, bias, state, cu = ctx.saved_tensors
+        meta, pairs = ctx.meta
+        g = grad_loss.to(torch.float32).contiguous()
+        grads = _ext.linear_preference_backward(state, c, bias, g, *meta, cu, pairs, *ctx.needs_input_grad[:3])
+        return _head_grads(grads, bias) + (None,) * 7
 
 
 class DistillationFunction(torch.autograd.Function):
@@ -323,13 +369,9 @@ class DistillationFunction(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, grad_loss):
-        need = ctx.needs_input_grad
-        if not any(need[:3]):
-            return (None,) * 7
         c, bias, saved = ctx.saved_tensors
         g = grad_loss.to(torch.float32).contiguous()
-        ge, gc, gb = _ext.distill_backward(saved, c, bias, g, *ctx.meta, *need[:3])
-        return (ge, gc, None if gb is None else gb.to(bias.dtype)) + (None,) * 4
+        return _head_grads(_ext.distill_backward(saved, c, bias, g, *ctx.meta, *ctx.needs_input_grad[:3]), bias) + (None,) * 4
 
 
 # ---------------------------------------------------------------------------
@@ -368,8 +410,8 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seql
     S, cu = _sequences(what, logp.shape, cu_seqlens, logp.device)
     adv, per_token = _advantages(what, advantages, logp.shape, S, logp.device)
     params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
-    loss, stats = PolicyLossFunction.apply(logp, _like(what, "old_logp", old_logp, logp),
-                                           _like(what, "ref_logp", ref_logp, logp), adv,
+    loss, stats = PolicyLossFunction.apply(logp, _per_token(what, "old_logp", old_logp, logp, logp.dtype),
+                                           _per_token(what, "ref_logp", ref_logp, logp, logp.dtype), adv,
                                            _mask(what, mask, logp.shape, logp.device), cu, S, params)
     return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
 
@@ -404,18 +446,10 @@ def preference_loss(logp, ref_logp=None, *, mask=None, cu_seqlens=None, beta=0.1
     logp = _logp(what, logp)
     pairs, cu = _pairs(what, logp.shape, cu_seqlens, logp.device)
     params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
-    ref, sums = _reference(what, ref_logp, logp, 2 * pairs)
+    ref, sums = _reference(what, ref_logp, logp, logp.dtype, 2 * pairs)
     loss, rewards = PreferenceLossFunction.apply(logp, ref, sums, _mask(what, mask, logp.shape, logp.device), cu,
                                                  pairs, params)
     return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
-
-
-def _log_probs(what, e, c, targets, bias, ignore_index):
-    """(logp, mask) in the targets' shape."""
-    e2, c, bias = _head(what, e, c, bias, targets.shape)
-    targets = _ids(what, "targets", targets, e.device)
-    logp, mask = LogProbsFunction.apply(e2, c, bias, targets.reshape(-1), ignore_index)
-    return logp.view(targets.shape), mask.view(targets.shape)
 
 
 def linear_log_probs(e, c, targets, bias=None, *, ignore_index=-100):
@@ -432,7 +466,10 @@ def linear_log_probs(e, c, targets, bias=None, *, ignore_index=-100):
         float32 also for 16-bit inputs (``linear_cross_entropy`` is to 1e-3),
         differentiable with respect to e, c and bias.
     """
-    return _log_probs("linear_log_probs", e, c, targets, bias, ignore_index)[0]
+    what = "linear_log_probs"
+    e, c, bias = _head(what, e, c, bias, targets.shape)
+    logp = LogProbsFunction.apply(e, c, bias, _ids(what, "targets", targets, e.device), ignore_index)
+    return logp.view(targets.shape)
 
 
 def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_logp=None, cu_seqlens=None, clip=0.2,
@@ -449,9 +486,13 @@ def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_lo
     S, cu = _sequences(what, targets.shape, cu_seqlens, targets.device)
     adv, per_token = _advantages(what, advantages, targets.shape, S, targets.device)
     params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
-    logp, mask = _log_probs(what, e, c, targets, bias, ignore_index)
-    loss, stats = PolicyLossFunction.apply(logp, _like(what, "old_logp", old_logp, logp),
-                                           _like(what, "ref_logp", ref_logp, logp), adv, mask, cu, S, params)
+    e, c, bias = _head(what, e, c, bias, targets.shape)
+    targets = _ids(what, "targets", targets, e.device)
+    loss, stats = LinearPolicyLossFunction.apply(e, c, bias, targets, ignore_index,
+                                                 _per_token(what, "old_logp", old_logp, targets),
+                                                 _per_token(what, "ref_logp", ref_logp, targets), adv, cu, S, params)
+    if reduction == "none":
+        loss = loss.view(targets.shape)
     return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
 
 
@@ -469,9 +510,10 @@ def linear_preference_loss(e, c, targets, ref_logp=None, bias=None, *, cu_seqlen
     what = "linear_preference_loss"
     pairs, cu = _pairs(what, targets.shape, cu_seqlens, targets.device)
     params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
-    logp, mask = _log_probs(what, e, c, targets, bias, ignore_index)
-    ref, sums = _reference(what, ref_logp, logp, 2 * pairs)
-    loss, rewards = PreferenceLossFunction.apply(logp, ref, sums, mask, cu, pairs, params)
+    e, c, bias = _head(what, e, c, bias, targets.shape)
+    targets = _ids(what, "targets", targets, e.device)
+    ref, sums = _reference(what, ref_logp, targets, torch.float32, 2 * pairs)
+    loss, rewards = LinearPreferenceLossFunction.apply(e, c, bias, targets, ignore_index, ref, sums, cu, pairs, params)
     return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
 
 

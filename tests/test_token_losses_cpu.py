@@ -65,15 +65,15 @@ def test_shapes():
     assert losses._advantages("t", torch.zeros(4), (4, 8), 4, dev)[1] is False
     assert losses._advantages("t", torch.zeros(4, 8).half(), (4, 8), 4, dev)[0].dtype == torch.float32
     with pytest.raises(ValueError, match="shape"):
-        losses._like("t", "old_logp", torch.zeros(8), x)
+        losses._per_token("t", "old_logp", torch.zeros(8), x)
     with pytest.raises(ValueError, match="dtype"):
-        losses._like("t", "old_logp", x.half(), x)
+        losses._per_token("t", "old_logp", x.half(), x)
     with pytest.raises(ValueError, match="bool"):
         losses._mask("t", x, x.shape, dev)
     with pytest.raises(ValueError, match="shape"):
         losses._mask("t", x[0] > 0, x.shape, dev)
     with pytest.raises(ValueError, match="per sequence"):
-        losses._reference("t", torch.zeros(3), x, 4)
+        losses._reference("t", torch.zeros(3), x, x.dtype, 4)
 
 
 def test_abi_refusals():
