@@ -34,7 +34,7 @@ struct RowsView {
 // Per packed row up to K listed columns: sid[row][K] sorted and distinct,
 // start[row][tiles1] the first entry of every kTopkTile-column tile (the last:
 // the number of entries), z[row][K] a value per entry.
-constexpr int kTopkTile = 256;
+constexpr int kTopkTile = 128;
 struct TopkView {
   const int32_t* sid = nullptr;
   const uint16_t* start = nullptr;

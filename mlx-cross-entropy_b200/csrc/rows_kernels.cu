@@ -200,7 +200,7 @@ constexpr int kPrepWarps = 4;
 
 // A warp per packed row: the teacher's entries sorted by column, entries of the
 // same column joined, absent ones (a column outside of [0, V)) dropped; their
-// probabilities; and where each 256-column tile's entries begin.
+// probabilities; and where each 128-column tile's entries begin.
 template <typename TI>
 __global__ void __launch_bounds__(kPrepWarps * 32)
 topk_prep_kernel(const TI* __restrict__ ids, const float* __restrict__ logp, int K, int K2, int64_t N, int64_t V,

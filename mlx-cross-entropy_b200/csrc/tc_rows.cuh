@@ -16,7 +16,7 @@
 // accumulator rounding towards zero: a logit of 14 after 144 such steps is
 // about 1e-5 too small, always in the same direction, and sums of
 // log-probabilities over a sequence add that up.  Here an accumulator holds
-// only kSegKb K-blocks (256 products); the epilogue warps add each of those
+// only a segment of K; the epilogue warps add each of those
 // partial logits to the total in their registers (128 per thread, round to
 // nearest).  The two TMEM accumulators take the segments in turn, so the MMAs
 // never wait for the adds: a segment's 16 MMAs take about 2000 cycles, its add
@@ -50,9 +50,6 @@
 
 constexpr int kRgWarps = 8;                   // epilogue warps: two per TMEM lane quarter, a column half each
 constexpr int kRgThreads = 64 + 32 * kRgWarps;
-// K-blocks per accumulator segment: 4 for logits, 2 for split operands (accuracy is
-// what they are for), 16 for gradients that are rounded to 16 bits.
-__host__ __device__ constexpr int seg_kb(bool split, bool grad) { return split ? 2 : grad ? 16 : 4; }
 constexpr size_t kRgSmem = 1024 + STAGES * (size_t)STAGE_BYTES + kRgWarps * 4096 + 256;
 
 struct RowsSched {
@@ -88,24 +85,38 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// z (accumulated in units of the split operands) += bias, -inf behind column V
+// v += bias[cb, cb + 32), nothing behind column V.  Whole chunks come in 16-byte
+// loads (the same for all lanes) where the bias is aligned.
 template <typename TB>
 __device__ __forceinline__ void add_bias(const void* bias, int64_t cb, int64_t V, float* v) {
   if constexpr (!std::is_void<TB>::value) {
-    float b[32];
-    load_bias32<TB>(bias, cb, V, b);
+    constexpr int kPer = 16 / (int)sizeof(TB);
+    const TB* p = static_cast<const TB*>(bias) + cb;
+    if (cb + 32 <= V && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += b[j];
+      for (int i = 0; i < 32 / kPer; ++i) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        const TB* b = reinterpret_cast<const TB*>(&x);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[i * kPer + j] += to_f32(b[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (cb + j < V) v[j] += to_f32(__ldg(p + j));
+    }
   }
 }
 
 // 1 / (s_a s_b) of split operands, 1 for whole ones: s[1] = 1 / s[0]
 __device__ __forceinline__ float unscale(const float* a, const float* b) { return a ? a[1] * b[1] : 1.f; }
 
+struct NoCursor {};
+
 template <typename TB, bool kTopk>
 struct LogitsEpi {
   static constexpr int kKind = 0;
-  static constexpr bool kStores = false;
+  static constexpr bool kStores = false, kExact = true;
   const int32_t* targets;  // [N]
   const void* bias;
   float* part_m;           // [ceil(V / 128)][N]
@@ -116,14 +127,20 @@ struct LogitsEpi {
   const float *se, *sc;    // split operands' scales
   TopkView topk;           // kTopk: the listed columns
 
-  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager&, const CUtensorMap*) const {
+  struct State {
+    int64_t tl;  // the target's place in this half
+    typename std::conditional<kTopk, TopkCursor, NoCursor>::type cur;
+  };
+  __device__ __forceinline__ void begin(State& st, const TileAt& t) const {
     const bool live = t.row < t.rows;
-    const int64_t tl = (!kTopk && live) ? (int64_t)targets[t.row] - t.col0 : -1;  // the target's place in this half
-    TopkCursor cur;
-    if constexpr (kTopk) {
-      cur.open(topk, t.row, live, t.nb);
-      cur.skip_to(t.col0);
-    }
+    st.tl = -1;
+    if constexpr (kTopk) st.cur.open(topk, t.row, live, t.col0 / kTopkTile);
+    else if (live) st.tl = (int64_t)targets[t.row] - t.col0;
+  }
+
+  __device__ __forceinline__ void finish(State& st, float (&z)[128], const TileAt& t, Stager&, const CUtensorMap*) const {
+    const bool live = t.row < t.rows;
+    const int64_t tl = st.tl;
     // The maximum is kept of the unscaled values; exponents are differences to
     // it first, exact next to the maximum, then one product with scale log2 e.
     float m = -INFINITY, sum = 0.f, tz = 0.f;
@@ -145,14 +162,19 @@ struct LogitsEpi {
       }
       if constexpr (kTopk) {
         int p;
-        const uint32_t bits = cur.take(cb, p);
+        const uint32_t bits = st.cur.take(cb, p);
         if (__any_sync(0xffffffffu, bits != 0u)) {
-          float* zo = topk.z + t.row * topk.K;
+          float* zo = topk.z + t.row * topk.K + p;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if ((bits >> j) & 1u) {
-              zo[p + __popc(bits & ((1u << j) - 1u))] = v[j] * scale;
-              v[j] = -INFINITY;
+          for (int g = 0; g < 32; g += 8) {
+            if (__any_sync(0xffffffffu, (bits >> g) & 0xffu)) {
+#pragma unroll
+              for (int j = g; j < g + 8; ++j) {
+                if ((bits >> j) & 1u) {
+                  zo[__popc(bits & ((1u << j) - 1u))] = v[j] * scale;
+                  v[j] = -INFINITY;
+                }
+              }
             }
           }
         }
@@ -195,7 +217,7 @@ struct LogitsEpi {
 template <typename T, typename TB, bool kTopk, bool kSplit>
 struct DlogitsEpi2 {
   static constexpr int kKind = 1;
-  static constexpr bool kStores = true;
+  static constexpr bool kStores = true, kExact = false;
   const int32_t* targets;
   const float* lse;
   Cotangent up;           // d of a row
@@ -209,21 +231,33 @@ struct DlogitsEpi2 {
   const float *se, *sc;
   TopkView topk;
 
-  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap* tm_lo) const {
+  struct State {
+    int64_t tl;      // the target's place in this half
+    float G, L, dr;  // dlogits are G e^(z - L); dr: d
+    typename std::conditional<kTopk, TopkCursor, NoCursor>::type cur;
+  };
+  __device__ __forceinline__ void begin(State& st, const TileAt& t) const {
     const bool live = t.row < t.rows;
-    const float inv = scale ? scale[1] : 1.f;
+    const int64_t v0 = vc0 + t.col0;
     const float d = live ? up.of(t.row, row_of) : 0.f;
-    const float L = live ? lse[t.row] : INFINITY;
-    const float dr = d * inv;
-    // (a row that gets no gradient: 0 whatever its coefficient)
-    const float G = kTopk ? (live && d != 0.f ? A[t.row] * dr : 0.f) : dr;
-    const int64_t v0 = vc0 + t.col0;  // vocabulary id of column 0
-    const int64_t tl = (!kTopk && live) ? (int64_t)targets[t.row] - v0 : -1;
-    TopkCursor cur;
+    st.L = live ? lse[t.row] : INFINITY;
+    st.dr = d * (scale ? scale[1] : 1.f);
+    st.tl = -1;
     if constexpr (kTopk) {
-      cur.open(topk, t.row, live, (vc0 + (int64_t)t.nb * BN) / kTopkTile);
-      cur.skip_to(v0);
+      // (a row that gets no gradient: 0 whatever its coefficient)
+      st.G = live && d != 0.f ? A[t.row] * st.dr : 0.f;
+      st.cur.open(topk, t.row, live, v0 / kTopkTile);
+    } else {
+      st.G = st.dr;
+      if (live) st.tl = (int64_t)targets[t.row] - v0;
     }
+  }
+
+  __device__ __forceinline__ void finish(State& st, float (&z)[128], const TileAt& t, Stager& sg,
+                                         const CUtensorMap* tm_lo) const {
+    const float G = st.G, L = st.L, dr = st.dr;
+    const int64_t v0 = vc0 + t.col0;  // vocabulary id of column 0
+    const int64_t tl = st.tl;
     const float us = unscale(se, sc);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -238,12 +272,17 @@ struct DlogitsEpi2 {
       for (int j = 0; j < 32; ++j) v[j] = G * ex2((v[j] * scale_z - L) * kLog2e);
       if constexpr (kTopk) {
         int p;
-        const uint32_t bits = cur.take(cb, p);
+        const uint32_t bits = st.cur.take(cb, p);
         if (__any_sync(0xffffffffu, bits != 0u)) {
           const float* x = topk.z + t.row * topk.K + p;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if ((bits >> j) & 1u) v[j] = dr * __ldg(x + __popc(bits & ((1u << j) - 1u)));
+          for (int g = 0; g < 32; g += 8) {
+            if (__any_sync(0xffffffffu, (bits >> g) & 0xffu)) {
+#pragma unroll
+              for (int j = g; j < g + 8; ++j)
+                if ((bits >> j) & 1u) v[j] = dr * __ldg(x + __popc(bits & ((1u << j) - 1u)));
+            }
+          }
         }
       } else {
         const int64_t at = tl - c * 32;
@@ -285,11 +324,13 @@ struct DlogitsEpi2 {
 template <typename T>
 struct Out16Epi {
   static constexpr int kKind = 3;
-  static constexpr bool kStores = true;
+  static constexpr bool kStores = true, kExact = false;
   const float* f;  // {s, 1 / s} of float16 dlogits, or nullptr
   int64_t M, D;
 
-  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
+  struct State {};
+  __device__ __forceinline__ void begin(State&, const TileAt&) const {}
+  __device__ __forceinline__ void finish(State&, float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
     const float s = f ? *f : 1.f;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -305,14 +346,16 @@ struct Out16Epi {
 
 // out[ks][row][col] (+)= f1 f2 (A B), float32
 struct OutEpi {
-  static constexpr bool kStores = true;
+  static constexpr bool kStores = true, kExact = false;
   const float *f1, *f2;
   int add;
   int64_t M, D;
   int kind;  // slot in g_mma_cols
   static constexpr int kKind = -1;  // (that of `kind`)
 
-  __device__ __forceinline__ void finish(float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
+  struct State {};
+  __device__ __forceinline__ void begin(State&, const TileAt&) const {}
+  __device__ __forceinline__ void finish(State&, float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
     const float f = (f1 ? *f1 : 1.f) * (f2 ? *f2 : 1.f);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -331,8 +374,7 @@ __global__ void __launch_bounds__(kRgThreads, 1)
 rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA2,
                  const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmB2,
                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmC2, const RowsSched rs,
-                 const Epi epi, const uint32_t idesc, const float untruncate) {
-  constexpr int kSegKb = seg_kb(kSplit, B_MN);
+                 const Epi epi, const uint32_t idesc, const int seg_kb, const float untruncate) {
   constexpr int kPasses = kSplit ? 3 : 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
@@ -426,11 +468,11 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         sched.coords(u, mb, nb, ks);
         sched.krange(ks, kb0, kb1);
         const int n = (kb1 - kb0) * kPasses;
-        for (int k0 = 0; ok && k0 < n; k0 += kSegKb) {
+        for (int k0 = 0; ok && k0 < n; k0 += seg_kb) {
           if (!mbar_wait(tempty + acc, acc_phase ^ 1u, 12)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-          const int k1 = min(n, k0 + kSegKb);
+          const int k1 = min(n, k0 + seg_kb);
           uint32_t fresh = 1;
           for (int k = k0; k < k1; ++k) {
             if (!mbar_wait(full + stage, phase, 13)) { ok = false; break; }
@@ -473,11 +515,15 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       sched.coords(u, mb, nb, ks);
       sched.krange(ks, kb0, kb1);
       const int n = (kb1 - kb0) * kPasses;
+      const int y0 = mb * BM + q * 32;
+      const TileAt t{(int64_t)y0 + lane, (int64_t)nb * BN + h * 128, rows, y0, ks, nb};
+      typename Epi::State st;
+      epi.begin(st, t);
       float z[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) z[j] = 0.f;
 #pragma unroll 1
-      for (int k0 = 0; k0 < n; k0 += kSegKb) {
+      for (int k0 = 0; k0 < n; k0 += seg_kb) {
         // (one verdict for the warp: the TMEM reads below need all of its lanes)
         ok = __all_sync(0xffffffffu, mbar_wait(tfull + acc, acc_phase, 14));
         if (!ok) break;
@@ -495,9 +541,7 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (acc == 0) acc_phase ^= 1u;
       }
       if (!ok) break;
-      const int y0 = mb * BM + q * 32;
-      const TileAt t{(int64_t)y0 + lane, (int64_t)nb * BN + h * 128, rows, y0, ks, nb};
-      epi.finish(z, t, sg, &tmC2);
+      epi.finish(st, z, t, sg, &tmC2);
     }
     if constexpr (Epi::kStores) sg.drain();  // output boxes written before the kernel ends
   }
@@ -516,8 +560,19 @@ struct RowsMaps {
   CUtensorMap A, A2, B, B2, C, C2;
 };
 
-// What a partial product is multiplied by (see the top of this file).
-float untruncate_of(bool split, bool bf16) { return 1.f + (split || bf16 ? 2.f : 3.f) * 1.1920929e-7f; }
+// K-blocks (64 columns) per accumulator segment, and what its partial products are
+// multiplied by (see the top of this file).  `exact`: row statistics.
+struct Segments {
+  int kb;
+  float untruncate;
+};
+
+Segments segments(bool exact, bool split, bool bf16, int64_t num_kb) {
+  const int kb = split ? 2 : !exact ? 16 : bf16 ? 8 : 4;
+  const float steps = 4.f * (float)(num_kb < kb ? num_kb : kb);
+  const float units = roundf(steps * (split ? 1.f / 4 : bf16 ? 1.f / 8 : 3.f / 16));
+  return Segments{kb, 1.f + units * 1.1920929e-7f};
+}
 
 template <bool A_MN, bool B_MN, bool kSplit, class Epi>
 cudaError_t rows_gemm(const RowsMaps& m, const RowsSched& rs, const Epi& epi, bool bf16, int64_t max_units,
@@ -528,8 +583,9 @@ cudaError_t rows_gemm(const RowsMaps& m, const RowsSched& rs, const Epi& epi, bo
   if (err != cudaSuccess) return err;
   if (max_units <= 0) return cudaSuccess;
   const int grid = max_units < num_sms() ? (int)max_units : num_sms();
+  const Segments sg = segments(Epi::kExact, kSplit, bf16, rs.k_rows ? ceil_div(rs.N, BK) : rs.num_kb);
   kern<<<grid, kRgThreads, kRgSmem, s>>>(m.A, m.A2, m.B, m.B2, m.C, m.C2, rs, epi, instr_desc(BM, BN, bf16, A_MN, B_MN),
-                                           untruncate_of(kSplit, bf16));
+                                         sg.kb, sg.untruncate);
   return launched();
 }
 
