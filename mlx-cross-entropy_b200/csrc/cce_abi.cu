@@ -1125,9 +1125,14 @@ struct Parts {
 };
 
 // Widths of the GEMMs' operands and outputs: rows start on 16-byte boundaries
-// (TMA), float16 parts of float32 fill whole 64-column blocks.  Other widths
-// run on padded copies.
-int64_t rows_dk(int64_t D, int dtype) { return cce::round_up(D, dtype == CCE_F32 ? 64 : 8); }
+// (TMA), float16 parts of float32 fill whole 64-column blocks.  Other widths run
+// on padded copies; so do many rows of a width whose rows straddle 128-byte
+// lines (D = 1032, V = 50021, bfloat16: a copy of c costs 60 us and saves 30 at
+// 1024 rows and more above, at 512 rows it loses 15).
+constexpr int64_t kPadRows = 1024;
+int64_t rows_dk(int64_t N, int64_t D, int dtype) {
+  return cce::round_up(D, dtype == CCE_F32 || N >= kPadRows ? 64 : 8);
+}
 int64_t rows_dout(int64_t D, int dtype) { return cce::round_up(D, dtype == CCE_F32 ? 4 : 8); }
 
 // What the forward calls leave for the backward calls.
@@ -1159,7 +1164,7 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
     r.topk.start = p.take<uint16_t>((size_t)N * r.topk.tiles1);
     r.topk.z = p.take<float>((size_t)N * K);
   }
-  const size_t n = (size_t)N * rows_dk(D, dtype);
+  const size_t n = (size_t)N * rows_dk(N, D, dtype);
   r.e = p.take<uint16_t>(n);
   if (dtype == CCE_F32) {
     r.e_lo = p.take<uint16_t>(n);
@@ -1176,15 +1181,15 @@ struct RowsC {
   uint32_t* words;  // largest values of c and e
 };
 
-RowsC rows_c(Parts& p, int64_t D, int64_t V, int dtype) {
+RowsC rows_c(Parts& p, int64_t N, int64_t D, int64_t V, int dtype) {
   RowsC w{};
-  const size_t n = (size_t)V * rows_dk(D, dtype);
+  const size_t n = (size_t)V * rows_dk(N, D, dtype);
   if (dtype == CCE_F32) {
     w.words = p.take<uint32_t>(2);
     w.sc = p.take<float>(2);
     w.c = p.take<uint16_t>(n);
     w.c_lo = p.take<uint16_t>(n);
-  } else if (D % 8 != 0) {
+  } else if (rows_dk(N, D, dtype) != D) {
     w.c = p.take<uint16_t>(n);
   }
   return w;
@@ -1231,7 +1236,7 @@ RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t D, int64_t V, int64_t K, in
     w.rest = p.take<float>(N);
     w.sums = p.take<cce::DistillSum>(cce::distill_blocks(N));
   }
-  w.c = rows_c(p, D, V, dtype);
+  w.c = rows_c(p, N, D, V, dtype);
   w.bytes = p.used;
   return w;
 }
@@ -1287,7 +1292,7 @@ RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, in
   RowsBwdWs w{};
   const RowsPlan pl = rows_plan(N, D, V, dtype);
   const int64_t dout = rows_dout(D, dtype);
-  w.c = rows_c(p, D, V, dtype);
+  w.c = rows_c(p, N, D, V, dtype);
   w.dl = p.take<uint16_t>((size_t)N * pl.vc);
   if (dtype == CCE_F32) w.dl_lo = p.take<uint16_t>((size_t)N * pl.vc);
   if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)pl.slabs * N * dout);
@@ -1319,11 +1324,11 @@ int check_distill(const CceDistillParams* p, const char* what) {
 }
 
 // The device and what the operands' TMA loads ask of c.
-int check_rows_device(const void* c, int64_t D, int dtype, const char* what) {
+int check_rows_device(const void* c, int64_t N, int64_t D, int dtype, const char* what) {
   int rc = check_arch();
   if (rc) return rc;
   if (!cce::tc_available()) return fail(CCE_ERR_CUDA, "%s: the driver's tensor-map encoder is unavailable", what);
-  if (dtype != CCE_F32 && D % 8 == 0 && !aligned16(c))
+  if (dtype != CCE_F32 && rows_dk(N, D, dtype) == D && !aligned16(c))
     return fail(CCE_ERR_ALIGN, "%s: c must start on a 16-byte boundary", what);
   return CCE_OK;
 }
@@ -1410,7 +1415,7 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
 cce::RowsGemmArgs rows_args(const void* bias, int bias_dtype, int64_t N, int64_t D, int64_t V, int dtype) {
   cce::RowsGemmArgs a{};
   a.bias = bias, a.bias_dtype = bias_dtype, a.dtype = dtype;
-  a.N = N, a.V = V, a.Dk = rows_dk(D, dtype), a.Dout = rows_dout(D, dtype);
+  a.N = N, a.V = V, a.Dk = rows_dk(N, D, dtype), a.Dout = rows_dout(D, dtype);
   a.vc_len = V, a.scale_z = 1.f;
   return a;
 }
@@ -1463,7 +1468,7 @@ int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dt
   const RowsSaved v = rows_saved(saved, N, D, V, 0, dtype);
   const RowsFwdWs w = rows_fwd_ws(workspace, N, D, V, 0, dtype);
   rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
-  if (!rc) rc = check_rows_device(c, D, dtype, what);
+  if (!rc) rc = check_rows_device(c, N, D, dtype, what);
   if (rc) return rc;
   cudaStream_t s = (cudaStream_t)stream;
   CCE_CUDA_CHECK(cce::launch_rows_pack(N, targets, target_bytes, ignore_index, has_ignore, nullptr, v.R, mask, logp, w.tgt, s),
@@ -1492,7 +1497,7 @@ int cce_logp_backward(const void* c, const void* bias, int bias_dtype, const flo
   const RowsSaved v = rows_saved(const_cast<void*>(saved), N, D, V, 0, dtype);
   const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags);
   rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
-  if (!rc) rc = check_rows_device(c, D, dtype, what);
+  if (!rc) rc = check_rows_device(c, N, D, dtype, what);
   if (rc) return rc;
   cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
   // d logp / dz = onehot - softmax: the negative of what the dlogits are
@@ -1540,7 +1545,7 @@ int cce_distill_forward(const void* e, const void* c, const void* bias, int bias
   const RowsSaved v = rows_saved(saved, N, D, V, K, dtype);
   const RowsFwdWs w = rows_fwd_ws(workspace, N, D, V, K, dtype);
   rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
-  if (!rc) rc = check_rows_device(c, D, dtype, what);
+  if (!rc) rc = check_rows_device(c, N, D, dtype, what);
   if (rc) return rc;
   CCE_CUDA_CHECK(cce::launch_rows_pack(N, nullptr, 0, 0, 0, mask, v.R, nullptr, red == CCE_REDUCE_NONE ? loss : nullptr,
                                        nullptr, s),
@@ -1579,7 +1584,7 @@ int cce_distill_backward(const void* c, const void* bias, int bias_dtype, const 
   const RowsSaved v = rows_saved(const_cast<void*>(saved), N, D, V, K, dtype);
   const RowsBwdWs w = rows_bwd_ws(workspace, N, D, V, dtype, flags);
   rc = check_space(saved, saved_bytes, v.bytes, workspace, workspace_bytes, w.bytes, what);
-  if (!rc) rc = check_rows_device(c, D, dtype, what);
+  if (!rc) rc = check_rows_device(c, N, D, dtype, what);
   if (rc) return rc;
   cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
   a.scale_z = (float)(1.0 / params->temperature);

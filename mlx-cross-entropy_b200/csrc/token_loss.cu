@@ -9,9 +9,9 @@
 // Policy loss of a token with d = logp - old, r = e^d, advantage A:
 //     l = -min(r A, clip(r, 1 - lo, 1 + hi) A) + beta (e^q - 1 - q),  q = ref - logp
 //     dl/dlogp = -r A (where the minimum is not the clipped side) - beta (e^q - 1)
-// Which side is taken is decided on d in 64 bits against log(1 - lo) and
-// log(1 + hi): r rounded to 32 bits next to the border would give some token
-// of a large batch the other side's gradient.
+// Which side is taken is decided on d against log(1 - lo) and log(1 + hi), in 64
+// bits next to them: r rounded to 32 bits would give some token of a large batch
+// the other side's gradient.
 //
 // Preference loss of a pair with D_s = sum over tokens of (logp - ref):
 //     gap = D_chosen - D_rejected, h = beta gap - margin;
@@ -20,7 +20,7 @@
 //
 // Both are bound by reading their inputs once (17 bytes per token for a float32
 // policy loss with a KL term) and, below a few 100,000 tokens, by launches.
-// One pass reads the tokens in chunks of kChunk; per-sequence sums are joined
+// One pass reads the tokens in chunks of 1024 or 4096; per-sequence sums are joined
 // from the chunks' pieces in a fixed order by a second launch (the same launch
 // when there is one chunk), so results do not depend on scheduling.  Sums are
 // held in 64 bits from the first join on.
@@ -31,7 +31,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPer = 4;                    // consecutive tokens of a thread: one 16-byte load of float32
-constexpr int kChunk = kThreads * kPer;    // tokens of a block
+constexpr int kStep = kThreads * kPer;     // tokens of a block at a time
+// A block takes one step, or kMany of a large batch: finding its sequences and
+// adding its sums up (microseconds of latency) then cost a quarter of a token's
+// share; 64 k tokens in 16 blocks would leave most SMs idle.
+constexpr int kMany = 4;
+constexpr int64_t kManyFrom = 2ll * 148 * 8 * kStep;  // tokens: two waves of 8 blocks an SM
+constexpr int kCached = 64;                // sequence offsets of a block's tokens kept in shared memory
 constexpr int kWarps = kThreads / 32;
 constexpr int kGroup = 8;                  // lanes that join the pieces of one sequence
 constexpr int kFinalSeqs = kThreads / kGroup;  // sequences (pairs) a block of the second launch takes at a time
@@ -42,6 +48,7 @@ constexpr int kFinalBlocks = 148;
 struct Seqs {
   const int32_t* cu;  // [S + 1], nullptr: rows of `len` tokens
   int64_t S, len, N;
+  int64_t chunk;      // tokens of a block
   __device__ __forceinline__ int64_t bound(int64_t s) const {
     if (cu == nullptr) return s * len;
     const int64_t b = __ldg(cu + s);
@@ -149,34 +156,57 @@ __device__ __forceinline__ X warp_sum(X v) {
   return v;
 }
 
-// The sequences of the chunk [c0, c1): lo and hi hold those of its first and last token.
-__device__ __forceinline__ void chunk_seqs(const Seqs& q, int64_t c0, int64_t c1, int64_t* sh) {
-  const int warp = threadIdx.x >> 5;
-  if (warp < 2) {
-    const int64_t s = q.find_warp(warp == 0 ? c0 : c1 - 1);
-    if ((threadIdx.x & 31) == 0) sh[warp] = s;
+// The sequences lo .. hi that a block's tokens [c0, c1) lie in, their offsets in
+// shared memory unless they are many (most blocks hold a piece of one or two).
+struct ChunkSeqs {
+  int64_t lo, hi;
+  int32_t cut[kCached];
+  __device__ __forceinline__ int64_t bound(const Seqs& q, int64_t s) const {
+    return hi - lo + 2 <= kCached ? (int64_t)cut[s - lo] : q.bound(s);
   }
-  __syncthreads();
-}
+  // All threads of the block; ends with a barrier.
+  __device__ __forceinline__ void load(const Seqs& q, int64_t c0, int64_t c1) {
+    const int warp = threadIdx.x >> 5;
+    if (warp < 2) {
+      const int64_t s = q.find_warp(warp == 0 ? c0 : c1 - 1);
+      if ((threadIdx.x & 31) == 0) (warp == 0 ? lo : hi) = s;
+    }
+    __syncthreads();
+    if (hi < lo) {  // (offsets that decrease)
+      __syncthreads();
+      if (threadIdx.x == 0) hi = lo;
+      __syncthreads();
+    }
+    if (hi - lo + 2 <= kCached) {
+      if (threadIdx.x <= hi - lo + 1) cut[threadIdx.x] = lo + threadIdx.x <= q.S ? (int32_t)q.bound(lo + threadIdx.x) : 0;
+      __syncthreads();
+    }
+  }
+};
 
-// Sequence of each of the thread's tokens (-1: none), from the chunk's range.
-__device__ __forceinline__ void token_seqs(const Seqs& q, int64_t i, int64_t lo, int64_t hi, int64_t (&s)[kPer]) {
-  int64_t cur = lo == hi ? lo : q.find(lo, hi, i);
+// Sequence of each of the thread's tokens (-1: none).
+__device__ __forceinline__ void token_seqs(const Seqs& q, const ChunkSeqs& cs, int64_t i, int64_t (&s)[kPer]) {
+  int64_t cur = cs.lo, end = cs.hi;
+  while (cur < end) {  // first sequence that ends behind token i
+    const int64_t mid = (cur + end) >> 1;
+    if (cs.bound(q, mid + 1) <= i) cur = mid + 1;
+    else end = mid;
+  }
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    while (cur < hi && q.bound(cur + 1) <= i + j) ++cur;
-    s[j] = cur < q.S && q.bound(cur) <= i + j ? cur : -1;
+    while (cur < cs.hi && cs.bound(q, cur + 1) <= i + j) ++cur;
+    s[j] = cur < q.S && cs.bound(q, cur) <= i + j && i + j < cs.bound(q, cur + 1) ? cur : -1;
   }
 }
 
 // Sums of val (0 and off for tokens that do not count) over the pieces that
-// the chunk's sequences have in it, a warp per sequence.
-__device__ __forceinline__ void piece_sums(const Seqs& q, int64_t c0, int64_t c1, int64_t lo, int64_t hi,
-                                           const float* val, const uint8_t* on, const Pieces& out) {
+// the block's sequences have in its tokens, a warp per sequence.
+__device__ __forceinline__ void piece_sums(const Seqs& q, const ChunkSeqs& cs, int64_t c0, int64_t c1, const float* val,
+                                           const uint8_t* on, const Pieces& out) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (hi >= q.S) hi = q.S - 1;
-  for (int64_t s = lo + warp; s <= hi; s += kWarps) {
-    const int64_t a = q.bound(s), b = q.bound(s + 1);
+  const int64_t hi = cs.hi < q.S ? cs.hi : q.S - 1;
+  for (int64_t s = cs.lo + warp; s <= hi; s += kWarps) {
+    const int64_t a = cs.bound(q, s), b = cs.bound(q, s + 1);
     const int t0 = (int)((a > c0 ? a : c0) - c0), t1 = (int)((b < c1 ? b : c1) - c0);
     if (t1 <= t0) continue;
     double v = 0.0;
@@ -192,8 +222,8 @@ __device__ __forceinline__ void piece_sums(const Seqs& q, int64_t c0, int64_t c1
         out.begin[s] = v;
         out.begin_n[s] = n;
       } else {
-        out.head[c0 / kChunk] = v;
-        out.head_n[c0 / kChunk] = n;
+        out.head[c0 / q.chunk] = v;
+        out.head_n[c0 / q.chunk] = n;
       }
     }
   }
@@ -206,7 +236,7 @@ __device__ __forceinline__ void join(const Seqs& q, const Pieces& p, int64_t s, 
   const int g = threadIdx.x & (kGroup - 1);
   const int64_t a = s < q.S ? q.bound(s) : 0, b = s < q.S ? q.bound(s + 1) : 0;
   if (b > a) {
-    const int64_t b0 = a / kChunk, b1 = (b - 1) / kChunk;
+    const int64_t b0 = a / q.chunk, b1 = (b - 1) / q.chunk;
     if (g == 0) {
       v = p.begin[s];
       n = p.begin_n[s];
@@ -286,32 +316,47 @@ struct TokenOut {
   bool clipped;
 };
 
-// e^q - 1 - q without the cancellation near 0: its series to q^10 below 1/2
-// (the next term is 1e-10 of the first there).
-__device__ __forceinline__ float kl3(float q, float em1) {
-  if (fabsf(q) >= 0.5f) return em1 - q;
-  float p = 1.f / 3628800.f;
-  p = fmaf(p, q, 1.f / 362880.f);
-  p = fmaf(p, q, 1.f / 40320.f);
-  p = fmaf(p, q, 1.f / 5040.f);
-  p = fmaf(p, q, 1.f / 720.f);
-  p = fmaf(p, q, 1.f / 120.f);
-  p = fmaf(p, q, 1.f / 24.f);
-  p = fmaf(p, q, 1.f / 6.f);
-  p = fmaf(p, q, 0.5f);
-  return q * q * p;
+// e^q - 1 - q and e^q - 1.  Below |q| = 1 the first from its series to q^11 (the
+// next term is 4e-9 of it): the difference would cancel.
+__device__ __forceinline__ void kl3(float q, float& kl, float& em1) {
+  if (fabsf(q) < 1.f) {
+    float p = 1.f / 39916800.f;
+    p = fmaf(p, q, 1.f / 3628800.f);
+    p = fmaf(p, q, 1.f / 362880.f);
+    p = fmaf(p, q, 1.f / 40320.f);
+    p = fmaf(p, q, 1.f / 5040.f);
+    p = fmaf(p, q, 1.f / 720.f);
+    p = fmaf(p, q, 1.f / 120.f);
+    p = fmaf(p, q, 1.f / 24.f);
+    p = fmaf(p, q, 1.f / 6.f);
+    p = fmaf(p, q, 0.5f);
+    kl = q * q * p;
+    em1 = q + kl;
+  } else {
+    em1 = expf(q) - 1.f;
+    kl = em1 - q;
+  }
+}
+
+// Whether the exact difference x - old lies above `border`; d is the difference
+// rounded to float32, so only next to the border are 64 bits needed.
+__device__ __forceinline__ bool above(float d, float x, float old, double border) {
+  const float gap = d - (float)border;
+  if (fabsf(gap) > 1e-6f * (1.f + fabsf(d))) return gap > 0.f;
+  return (double)x - (double)old > border;
 }
 
 __device__ __forceinline__ TokenOut policy_token(const Policy& P, float x, float old, float ref, float A) {
-  const double d = P.old ? (double)x - (double)old : 0.0;
-  const float r = P.old ? expf((float)d) : 1.f;
+  const float d = P.old ? x - old : 0.f;
+  const float r = P.old ? expf(d) : 1.f;
   bool open = true;
   float b = r;
+  if (!P.old) old = x;
   if (A > 0.f) {
-    if (d > P.log_hi) open = false, b = P.hi;
+    if (above(d, x, old, P.log_hi)) open = false, b = P.hi;
   } else if (A < 0.f) {
-    if (d < P.log_lo) open = false, b = P.lo;
-    if (P.dual > 0.f && d > P.log_dual) open = false, b = P.dual;
+    if (above(-d, old, x, -P.log_lo)) open = false, b = P.lo;
+    if (P.dual > 0.f && above(d, x, old, P.log_dual)) open = false, b = P.dual;
   }
   TokenOut o;
   o.loss = -(b * A);
@@ -319,9 +364,8 @@ __device__ __forceinline__ TokenOut policy_token(const Policy& P, float x, float
   o.clipped = !open;
   o.kl = 0.f;
   if (P.ref) {
-    const float k = (float)((double)ref - (double)x);
-    const float em1 = expm1f(k);
-    o.kl = kl3(k, em1);
+    float em1;
+    kl3(ref - x, o.kl, em1);
     o.loss = fmaf(P.beta, o.kl, o.loss);
     o.g = fmaf(-P.beta, em1, o.g);
   }
@@ -369,6 +413,7 @@ __device__ void policy_final(const Policy& P) {
   }
   // totals over the chunks (the last or only block)
   double loss = 0.0, kl = 0.0, n = 0.0, clipped = 0.0;
+#pragma unroll 4
   for (int b = threadIdx.x; b < P.chunks; b += kThreads) {
     const BlockSums x = P.blk[b];
     loss += x.loss;
@@ -402,72 +447,79 @@ __device__ void policy_final(const Policy& P) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) policy_forward_kernel(const Policy P) {
-  __shared__ float val[kChunk];
-  __shared__ uint8_t on_sh[kChunk];
-  __shared__ int64_t range[2];
+  __shared__ float val[kMany * kStep];
+  __shared__ uint8_t on_sh[kMany * kStep];
+  __shared__ ChunkSeqs cs;
   __shared__ double shd[kWarps];
   __shared__ int shi[kWarps];
   const int64_t N = P.q.N;
-  const int64_t c0 = (int64_t)blockIdx.x * kChunk;
-  const int64_t c1 = c0 + kChunk < N ? c0 + kChunk : N;
-  const int64_t i = c0 + (int64_t)threadIdx.x * kPer;
+  const int64_t c0 = (int64_t)blockIdx.x * P.q.chunk;
+  const int64_t c1 = c0 + P.q.chunk < N ? c0 + P.q.chunk : N;
   const bool by_seq = P.reduction == CCE_REDUCE_SEQUENCE;
+  const bool search = by_seq || !P.adv_token;
   const bool vec = P.vec != 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) *P.counter = 0u;
-
-  float x[kPer], old[kPer], ref[kPer], A[kPer];
-  bool on[kPer];
-  load4(static_cast<const T*>(P.logp), i, N, vec, x);
-  load_mask4(P.mask, i, N, vec, on);
-  if (P.old) load4(static_cast<const T*>(P.old), i, N, vec, old);
-  if (P.ref) load4(static_cast<const T*>(P.ref), i, N, vec, ref);
-  if (P.adv_token) load4(P.adv, i, N, vec, A);
-  if (by_seq || !P.adv_token) {
-    chunk_seqs(P.q, c0, c1, range);
-    int64_t s[kPer];
-    token_seqs(P.q, i, range[0], range[1], s);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      on[j] = on[j] && s[j] >= 0;
-      if (!P.adv_token) A[j] = on[j] ? __ldg(P.adv + s[j]) : 0.f;
-    }
-  } else if (P.q.cu != nullptr) {  // tokens before the first and behind the last sequence
-    const int64_t b0 = P.q.S > 0 ? P.q.bound(0) : N, b1 = P.q.S > 0 ? P.q.bound(P.q.S) : N;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) on[j] = on[j] && i + j >= b0 && i + j < b1;
+  int64_t b0 = 0, b1 = N;  // tokens before the first and behind the last sequence
+  if (search) {
+    cs.load(P.q, c0, c1);
+  } else if (P.q.cu != nullptr) {
+    b0 = P.q.S > 0 ? P.q.bound(0) : N;
+    b1 = P.q.S > 0 ? P.q.bound(P.q.S) : N;
   }
-  float l[kPer], g[kPer];
-  double loss = 0.0, kl = 0.0;
+  float loss = 0.f, kl = 0.f;  // of the thread's few tokens
   int n = 0, clipped = 0;
+#pragma unroll 1
+  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
+    float x[kPer], old[kPer], ref[kPer], A[kPer];
+    bool on[kPer];
+    load4(static_cast<const T*>(P.logp), i, N, vec, x);
+    load_mask4(P.mask, i, N, vec, on);
+    if (P.old) load4(static_cast<const T*>(P.old), i, N, vec, old);
+    if (P.ref) load4(static_cast<const T*>(P.ref), i, N, vec, ref);
+    if (P.adv_token) load4(P.adv, i, N, vec, A);
+    if (search) {
+      int64_t s[kPer];
+      token_seqs(P.q, cs, i, s);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    l[j] = g[j] = 0.f;
-    if (on[j]) {
-      const TokenOut o = policy_token(P, x[j], old[j], ref[j], A[j]);
-      l[j] = o.loss;
-      g[j] = o.g;
-      loss += (double)o.loss;
-      kl += (double)o.kl;
-      ++n;
-      clipped += o.clipped;
+      for (int j = 0; j < kPer; ++j) {
+        on[j] = on[j] && s[j] >= 0;
+        if (!P.adv_token) A[j] = on[j] ? __ldg(P.adv + s[j]) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) on[j] = on[j] && i + j >= b0 && i + j < b1;
     }
-  }
-  store4(P.coef, i, N, vec, g);
-  if (P.reduction == CCE_REDUCE_NONE) store4(P.loss, i, N, vec, l);
-  if (by_seq) {
+    float l[kPer], g[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      val[threadIdx.x * kPer + j] = l[j];
-      on_sh[threadIdx.x * kPer + j] = on[j] ? 1 : 0;
+      l[j] = g[j] = 0.f;
+      if (on[j]) {
+        const TokenOut o = policy_token(P, x[j], old[j], ref[j], A[j]);
+        l[j] = o.loss;
+        g[j] = o.g;
+        loss += o.loss;
+        kl += o.kl;
+        ++n;
+        clipped += o.clipped;
+      }
     }
-    __syncthreads();
-    piece_sums(P.q, c0, c1, range[0], range[1], val, on_sh, P.pc);
+    store4(P.coef, i, N, vec, g);
+    if (P.reduction == CCE_REDUCE_NONE) store4(P.loss, i, N, vec, l);
+    if (by_seq) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        val[i - c0 + j] = l[j];
+        on_sh[i - c0 + j] = on[j] ? 1 : 0;
+      }
+    }
   }
-  loss = block_sum(loss, shd);
-  kl = block_sum(kl, shd);
-  n = block_sum(n, shi);
-  clipped = block_sum(clipped, shi);
-  if (threadIdx.x == 0) P.blk[blockIdx.x] = BlockSums{loss, kl, n, clipped};
+  if (by_seq) {
+    __syncthreads();
+    piece_sums(P.q, cs, c0, c1, val, on_sh, P.pc);
+  }
+  const double loss_sum = block_sum((double)loss, shd), kl_sum = block_sum((double)kl, shd);
+  n = block_sum(n | clipped << 16, shi);  // (at most 4096 tokens a block)
+  if (threadIdx.x == 0) P.blk[blockIdx.x] = BlockSums{loss_sum, kl_sum, n & 0xffff, n >> 16};
   if (gridDim.x == 1) {
     __syncthreads();
     policy_final(P);
@@ -481,25 +533,27 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 policy_backward_kernel(const float* __restrict__ coef, const float* __restrict__ weight, const float* __restrict__ up,
                        int up_token, int by_seq, const Seqs q, int vec, T* __restrict__ grad) {
-  __shared__ int64_t range[2];
-  const int64_t c0 = (int64_t)blockIdx.x * kChunk;
-  const int64_t c1 = c0 + kChunk < q.N ? c0 + kChunk : q.N;
-  const int64_t i = c0 + (int64_t)threadIdx.x * kPer;
-  float g[kPer], u[kPer];
-  load4(coef, i, q.N, vec != 0, g);
-  if (up_token) load4(up, i, q.N, vec != 0, u);
+  __shared__ ChunkSeqs cs;
+  const int64_t c0 = (int64_t)blockIdx.x * q.chunk;
+  const int64_t c1 = c0 + q.chunk < q.N ? c0 + q.chunk : q.N;
   const float w = (up_token ? 1.f : __ldg(up)) * __ldg(weight);
-  if (by_seq) {
-    chunk_seqs(q, c0, c1, range);
-    int64_t s[kPer];
-    token_seqs(q, i, range[0], range[1], s);
+  if (by_seq) cs.load(q, c0, c1);
+#pragma unroll 1
+  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
+    float g[kPer], u[kPer];
+    load4(coef, i, q.N, vec != 0, g);
+    if (up_token) load4(up, i, q.N, vec != 0, u);
+    if (by_seq) {
+      int64_t s[kPer];
+      token_seqs(q, cs, i, s);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) g[j] = s[j] >= 0 && g[j] != 0.f ? g[j] * __ldg(weight + 1 + s[j]) : 0.f;
+      for (int j = 0; j < kPer; ++j) g[j] = s[j] >= 0 && g[j] != 0.f ? g[j] * __ldg(weight + 1 + s[j]) : 0.f;
+    }
+    // (a token that does not count has coef 0: an infinite upstream must not make it NaN)
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) g[j] = g[j] == 0.f ? 0.f : g[j] * w * (up_token ? u[j] : 1.f);
+    store4(grad, i, q.N, vec != 0, g);
   }
-  // (a token that does not count has coef 0: an infinite upstream must not make it NaN)
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) g[j] = g[j] == 0.f ? 0.f : g[j] * w * (up_token ? u[j] : 1.f);
-  store4(grad, i, q.N, vec != 0, g);
 }
 
 // ---------------------------------------------------------------------------
@@ -583,27 +637,29 @@ __device__ void preference_final(const Preference& P) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) preference_forward_kernel(const Preference P) {
-  __shared__ float val[kChunk];
-  __shared__ uint8_t on_sh[kChunk];
-  __shared__ int64_t range[2];
+  __shared__ float val[kMany * kStep];
+  __shared__ uint8_t on_sh[kMany * kStep];
+  __shared__ ChunkSeqs cs;
   const int64_t N = P.q.N;
-  const int64_t c0 = (int64_t)blockIdx.x * kChunk;
-  const int64_t c1 = c0 + kChunk < N ? c0 + kChunk : N;
-  const int64_t i = c0 + (int64_t)threadIdx.x * kPer;
+  const int64_t c0 = (int64_t)blockIdx.x * P.q.chunk;
+  const int64_t c1 = c0 + P.q.chunk < N ? c0 + P.q.chunk : N;
   const bool vec = P.vec != 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) *P.counter = 0u;
-  float x[kPer], ref[kPer];
-  bool on[kPer];
-  load4(static_cast<const T*>(P.logp), i, N, vec, x);
-  load_mask4(P.mask, i, N, vec, on);
-  if (P.ref) load4(static_cast<const T*>(P.ref), i, N, vec, ref);
+#pragma unroll 2
+  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
+    float x[kPer], ref[kPer];
+    bool on[kPer];
+    load4(static_cast<const T*>(P.logp), i, N, vec, x);
+    load_mask4(P.mask, i, N, vec, on);
+    if (P.ref) load4(static_cast<const T*>(P.ref), i, N, vec, ref);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    val[threadIdx.x * kPer + j] = on[j] ? (P.ref ? x[j] - ref[j] : x[j]) : 0.f;
-    on_sh[threadIdx.x * kPer + j] = on[j] ? 1 : 0;
+    for (int j = 0; j < kPer; ++j) {
+      val[i - c0 + j] = on[j] ? (P.ref ? x[j] - ref[j] : x[j]) : 0.f;
+      on_sh[i - c0 + j] = on[j] ? 1 : 0;
+    }
   }
-  chunk_seqs(P.q, c0, c1, range);  // (ends with a barrier: val and on_sh are complete)
-  piece_sums(P.q, c0, c1, range[0], range[1], val, on_sh, P.pc);
+  cs.load(P.q, c0, c1);  // (ends with a barrier: val and on_sh are complete)
+  piece_sums(P.q, cs, c0, c1, val, on_sh, P.pc);
   if (gridDim.x == 1) {
     __syncthreads();
     preference_final(P);
@@ -616,25 +672,27 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 preference_backward_kernel(const float* __restrict__ coef, const float* __restrict__ up, int up_pair, int64_t pairs,
                            const uint8_t* __restrict__ mask, const Seqs q, int vec, T* __restrict__ grad) {
-  __shared__ int64_t range[2];
-  const int64_t c0 = (int64_t)blockIdx.x * kChunk;
-  const int64_t c1 = c0 + kChunk < q.N ? c0 + kChunk : q.N;
-  const int64_t i = c0 + (int64_t)threadIdx.x * kPer;
-  bool on[kPer];
-  load_mask4(mask, i, q.N, vec != 0, on);
-  chunk_seqs(q, c0, c1, range);
-  int64_t s[kPer];
-  token_seqs(q, i, range[0], range[1], s);
-  float g[kPer];
+  __shared__ ChunkSeqs cs;
+  const int64_t c0 = (int64_t)blockIdx.x * q.chunk;
+  const int64_t c1 = c0 + q.chunk < q.N ? c0 + q.chunk : q.N;
+  cs.load(q, c0, c1);
+#pragma unroll 1
+  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
+    bool on[kPer];
+    load_mask4(mask, i, q.N, vec != 0, on);
+    int64_t s[kPer];
+    token_seqs(q, cs, i, s);
+    float g[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    g[j] = 0.f;
-    if (on[j] && s[j] >= 0) {
-      const int64_t p = s[j] < pairs ? s[j] : s[j] - pairs;
-      g[j] = __ldg(coef + s[j]) * __ldg(up + (up_pair ? p : 0));
+    for (int j = 0; j < kPer; ++j) {
+      g[j] = 0.f;
+      if (on[j] && s[j] >= 0) {
+        const int64_t p = s[j] < pairs ? s[j] : s[j] - pairs;
+        g[j] = __ldg(coef + s[j]) * __ldg(up + (up_pair ? p : 0));
+      }
     }
+    store4(grad, i, q.N, vec != 0, g);
   }
-  store4(grad, i, q.N, vec != 0, g);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -675,8 +733,21 @@ int final_blocks(int64_t items) {
 
 }  // namespace
 
+static int64_t chunk_of(int64_t N) { return N >= kManyFrom ? kMany * kStep : kStep; }
 // (an empty batch still has a chunk: it zeroes the second launch's counter)
-static int64_t chunks_of(int64_t N) { return N > 0 ? ceil_div(N, kChunk) : 1; }
+static int64_t chunks_of(int64_t N) { return N > 0 ? ceil_div(N, chunk_of(N)) : 1; }
+
+// Runs launch(type tag) for a dtype.
+template <typename F>
+static cudaError_t by_type(int dtype, F launch) {
+  switch (dtype) {
+    case CCE_F32: launch(float()); break;
+    case CCE_F16: launch(__half()); break;
+    case CCE_BF16: launch(__nv_bfloat16()); break;
+    default: return cudaErrorInvalidValue;
+  }
+  return launched();
+}
 
 size_t token_loss_workspace_bytes(int64_t N, int64_t S) {
   const int64_t chunks = chunks_of(N);
@@ -687,7 +758,7 @@ size_t token_loss_workspace_bytes(int64_t N, int64_t S) {
 cudaError_t policy_forward(const PolicyArgs& a, void* ws, cudaStream_t s) {
   Policy P{};
   P.logp = a.logp, P.old = a.old, P.ref = a.ref, P.adv = a.adv, P.mask = a.mask;
-  P.q = Seqs{a.cu, a.S, a.S > 0 ? a.N / a.S : 0, a.N};
+  P.q = Seqs{a.cu, a.S, a.S > 0 ? a.N / a.S : 0, a.N, chunk_of(a.N)};
   P.adv_token = a.adv_token, P.reduction = a.reduction;
   P.lo = (float)(1.0 - a.clip_low), P.hi = (float)(1.0 + a.clip_high), P.dual = (float)a.dual_clip;
   P.beta = (float)a.kl_coef;
@@ -698,13 +769,9 @@ cudaError_t policy_forward(const PolicyArgs& a, void* ws, cudaStream_t s) {
   P.blk = c.blk, P.pc = c.pc, P.part = c.part, P.counter = c.counter;
   P.vec = aligned16(a.logp) && aligned16(a.old) && aligned16(a.ref) && aligned16(a.mask) && aligned16(a.coef) &&
           (!a.adv_token || aligned16(a.adv)) && (a.reduction != CCE_REDUCE_NONE || aligned16(a.loss));
-  switch (a.dtype) {
-    case CCE_F32: policy_forward_kernel<float><<<P.chunks, kThreads, 0, s>>>(P); break;
-    case CCE_F16: policy_forward_kernel<__half><<<P.chunks, kThreads, 0, s>>>(P); break;
-    case CCE_BF16: policy_forward_kernel<__nv_bfloat16><<<P.chunks, kThreads, 0, s>>>(P); break;
-    default: return cudaErrorInvalidValue;
-  }
-  cudaError_t err = launched();
+  cudaError_t err = by_type(a.dtype, [&](auto t) {
+    policy_forward_kernel<decltype(t)><<<P.chunks, kThreads, 0, s>>>(P);
+  });
   if (err != cudaSuccess || P.chunks == 1) return err;
   policy_final_kernel<<<a.reduction == CCE_REDUCE_SEQUENCE ? final_blocks(a.S) : 1, kThreads, 0, s>>>(P);
   return launched();
@@ -712,31 +779,20 @@ cudaError_t policy_forward(const PolicyArgs& a, void* ws, cudaStream_t s) {
 
 cudaError_t policy_backward(const float* coef, const float* weight, const float* up, int up_token, int reduction,
                             const int32_t* cu, int64_t N, int64_t S, int dtype, void* grad, cudaStream_t s) {
-  const Seqs q{cu, S, S > 0 ? N / S : 0, N};
-  const int chunks = (int)ceil_div(N, kChunk);
+  const Seqs q{cu, S, S > 0 ? N / S : 0, N, chunk_of(N)};
   const int by_seq = reduction == CCE_REDUCE_SEQUENCE;
   const int vec = aligned16(coef) && aligned16(grad) && (!up_token || aligned16(up));
-  switch (dtype) {
-    case CCE_F32:
-      policy_backward_kernel<float><<<chunks, kThreads, 0, s>>>(coef, weight, up, up_token, by_seq, q, vec, (float*)grad);
-      break;
-    case CCE_F16:
-      policy_backward_kernel<__half><<<chunks, kThreads, 0, s>>>(coef, weight, up, up_token, by_seq, q, vec, (__half*)grad);
-      break;
-    case CCE_BF16:
-      policy_backward_kernel<__nv_bfloat16><<<chunks, kThreads, 0, s>>>(coef, weight, up, up_token, by_seq, q, vec,
-                                                                        (__nv_bfloat16*)grad);
-      break;
-    default: return cudaErrorInvalidValue;
-  }
-  return launched();
+  return by_type(dtype, [&](auto t) {
+    policy_backward_kernel<decltype(t)><<<(int)chunks_of(N), kThreads, 0, s>>>(
+        coef, weight, up, up_token, by_seq, q, vec, static_cast<decltype(t)*>(grad));
+  });
 }
 
 cudaError_t preference_forward(const PreferenceArgs& a, void* ws, cudaStream_t s) {
   Preference P{};
   const int64_t S = 2 * a.pairs;
   P.logp = a.logp, P.ref = a.ref, P.ref_seq = a.ref_seq, P.mask = a.mask;
-  P.q = Seqs{a.cu, S, S > 0 ? a.N / S : 0, a.N};
+  P.q = Seqs{a.cu, S, S > 0 ? a.N / S : 0, a.N, chunk_of(a.N)};
   P.pairs = a.pairs, P.kind = a.kind, P.reduction = a.reduction, P.by_length = a.by_length;
   P.beta = a.beta, P.margin = a.margin, P.smoothing = a.smoothing;
   P.loss = a.loss, P.rewards = a.rewards, P.coef = a.coef;
@@ -744,13 +800,9 @@ cudaError_t preference_forward(const PreferenceArgs& a, void* ws, cudaStream_t s
   const Carve c = carve(ws, S, chunks);
   P.pc = c.pc, P.part = c.part, P.counter = c.counter;
   P.vec = aligned16(a.logp) && aligned16(a.ref) && aligned16(a.mask);
-  switch (a.dtype) {
-    case CCE_F32: preference_forward_kernel<float><<<chunks, kThreads, 0, s>>>(P); break;
-    case CCE_F16: preference_forward_kernel<__half><<<chunks, kThreads, 0, s>>>(P); break;
-    case CCE_BF16: preference_forward_kernel<__nv_bfloat16><<<chunks, kThreads, 0, s>>>(P); break;
-    default: return cudaErrorInvalidValue;
-  }
-  cudaError_t err = launched();
+  cudaError_t err = by_type(a.dtype, [&](auto t) {
+    preference_forward_kernel<decltype(t)><<<chunks, kThreads, 0, s>>>(P);
+  });
   if (err != cudaSuccess || chunks == 1) return err;
   preference_final_kernel<<<final_blocks(a.pairs), kThreads, 0, s>>>(P);
   return launched();
@@ -758,23 +810,12 @@ cudaError_t preference_forward(const PreferenceArgs& a, void* ws, cudaStream_t s
 
 cudaError_t preference_backward(const float* coef, const float* up, int up_pair, const uint8_t* mask, const int32_t* cu,
                                 int64_t N, int64_t pairs, int dtype, void* grad, cudaStream_t s) {
-  const Seqs q{cu, 2 * pairs, pairs > 0 ? N / (2 * pairs) : 0, N};
-  const int chunks = (int)ceil_div(N, kChunk);
+  const Seqs q{cu, 2 * pairs, pairs > 0 ? N / (2 * pairs) : 0, N, chunk_of(N)};
   const int vec = aligned16(mask) && aligned16(grad);
-  switch (dtype) {
-    case CCE_F32:
-      preference_backward_kernel<float><<<chunks, kThreads, 0, s>>>(coef, up, up_pair, pairs, mask, q, vec, (float*)grad);
-      break;
-    case CCE_F16:
-      preference_backward_kernel<__half><<<chunks, kThreads, 0, s>>>(coef, up, up_pair, pairs, mask, q, vec, (__half*)grad);
-      break;
-    case CCE_BF16:
-      preference_backward_kernel<__nv_bfloat16><<<chunks, kThreads, 0, s>>>(coef, up, up_pair, pairs, mask, q, vec,
-                                                                            (__nv_bfloat16*)grad);
-      break;
-    default: return cudaErrorInvalidValue;
-  }
-  return launched();
+  return by_type(dtype, [&](auto t) {
+    preference_backward_kernel<decltype(t)><<<(int)chunks_of(N), kThreads, 0, s>>>(
+        coef, up, up_pair, pairs, mask, q, vec, static_cast<decltype(t)*>(grad));
+  });
 }
 
 }  // namespace cce

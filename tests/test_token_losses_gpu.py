@@ -79,6 +79,17 @@ def test_policy_sizes(n, S, packed, reduction):
     check_policy(b, adv, go, kl_coef=0.05, reduction=reduction)
 
 
+@pytest.mark.parametrize("reduction", REDUCTIONS)
+def test_policy_large_batch(reduction):
+    """Enough tokens for blocks of four steps; sequences longer and shorter than a block."""
+    n = 2 * 148 * 8 * 1024 + 1500
+    b = batch(n, 37, seed=77, first=3, last=5000)
+    b["cu"][5] = b["cu"][4] + 1 if b["cu"][4] + 1 <= b["cu"][6] else b["cu"][5]
+    adv = torch.randn(37, generator=b["g"])
+    go = torch.randn(b["shape"], generator=b["g"]) if reduction == "none" else None
+    check_policy(b, adv, go, kl_coef=0.05, reduction=reduction)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", REDUCTIONS)
 def test_policy_types_and_token_advantages(dtype, reduction):
@@ -262,6 +273,12 @@ def check_preference(b, ref, grad_out=None, **kw):
 def test_preference_sizes(n, pairs, packed, loss_type):
     b = batch(n, 2 * pairs, seed=n + pairs, packed=packed)
     check_preference(b, b["ref"], loss_type=loss_type)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_preference_large_batch(dtype):
+    b = batch(2 * 148 * 8 * 1024 + 1500, 2 * 301, seed=78, dtype=dtype, first=9, last=4000)
+    check_preference(b, b["ref"], loss_type="ipo", beta=0.01)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
