@@ -3,8 +3,8 @@
 //
 // Tokens lie in one array of N; sequence s holds the tokens [cu[s], cu[s+1])
 // (packed) or [s L, (s+1) L) (padded rows).  Tokens that the mask or the
-// offsets leave out add nothing and get a zero gradient; what they hold
-// (infinities, NaN) is never used in arithmetic.
+// offsets leave out add nothing and get a zero gradient, whatever they hold
+// (infinities, NaN): values are taken or left, never multiplied by the mask.
 //
 // Policy loss of a token with d = logp - old, r = e^d, advantage A:
 //     l = -min(r A, clip(r, 1 - lo, 1 + hi) A) + beta (e^q - 1 - q),  q = ref - logp
@@ -100,7 +100,7 @@ struct BlockSums {  // a chunk's totals
 };
 
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec, float (&v)[kPer]) {
+__device__ __forceinline__ void load4(const T* p, int i, int n, bool vec, float (&v)[kPer]) {
   if (vec && i + kPer <= n) {
     if constexpr (sizeof(T) == 4) {
       const float4 x = __ldg(reinterpret_cast<const float4*>(p + i));
@@ -118,7 +118,7 @@ __device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec
 }
 
 template <typename T>
-__device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, const float (&v)[kPer]) {
+__device__ __forceinline__ void store4(T* p, int i, int n, bool vec, const float (&v)[kPer]) {
   if (vec && i + kPer <= n) {
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(p + i) = make_float4(v[0], v[1], v[2], v[3]);
@@ -136,7 +136,7 @@ __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, con
   }
 }
 
-__device__ __forceinline__ void load_mask4(const uint8_t* m, int64_t i, int64_t n, bool vec, bool (&on)[kPer]) {
+__device__ __forceinline__ void load_mask4(const uint8_t* m, int i, int n, bool vec, bool (&on)[kPer]) {
   if (m == nullptr) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) on[j] = i + j < n;
@@ -156,14 +156,12 @@ __device__ __forceinline__ X warp_sum(X v) {
   return v;
 }
 
-// The sequences lo .. hi that a block's tokens [c0, c1) lie in, their offsets in
-// shared memory unless they are many (most blocks hold a piece of one or two).
+// The sequences lo .. hi that a block's tokens [c0, c1) lie in, and (unless they
+// are many: most blocks hold a piece of one or two) where each begins in them.
 struct ChunkSeqs {
   int64_t lo, hi;
-  int32_t cut[kCached];
-  __device__ __forceinline__ int64_t bound(const Seqs& q, int64_t s) const {
-    return hi - lo + 2 <= kCached ? (int64_t)cut[s - lo] : q.bound(s);
-  }
+  int cut[kCached];  // begin of sequence lo + k, from c0, clamped to [0, c1 - c0]
+  __device__ __forceinline__ bool cached() const { return hi - lo + 2 <= kCached; }
   // All threads of the block; ends with a barrier.
   __device__ __forceinline__ void load(const Seqs& q, int64_t c0, int64_t c1) {
     const int warp = threadIdx.x >> 5;
@@ -177,48 +175,100 @@ struct ChunkSeqs {
       if (threadIdx.x == 0) hi = lo;
       __syncthreads();
     }
-    if (hi - lo + 2 <= kCached) {
-      if (threadIdx.x <= hi - lo + 1) cut[threadIdx.x] = lo + threadIdx.x <= q.S ? (int32_t)q.bound(lo + threadIdx.x) : 0;
+    if (cached()) {
+      if (threadIdx.x <= hi - lo + 1) {
+        const int64_t b = lo + threadIdx.x <= q.S ? q.bound(lo + threadIdx.x) : c0;
+        cut[threadIdx.x] = (int)(b < c0 ? 0 : b > c1 ? c1 - c0 : b - c0);
+      }
       __syncthreads();
     }
   }
 };
 
-// Sequence of each of the thread's tokens (-1: none).
-__device__ __forceinline__ void token_seqs(const Seqs& q, const ChunkSeqs& cs, int64_t i, int64_t (&s)[kPer]) {
-  int64_t cur = cs.lo, end = cs.hi;
-  while (cur < end) {  // first sequence that ends behind token i
-    const int64_t mid = (cur + end) >> 1;
-    if (cs.bound(q, mid + 1) <= i) cur = mid + 1;
-    else end = mid;
+// Sequences of the thread's tokens t .. t + 3 of the block (-1: none); true when
+// all four lie in one, s[0].
+__device__ __forceinline__ bool token_seqs(const Seqs& q, const ChunkSeqs& cs, int64_t c0, int t, int64_t (&s)[kPer]) {
+  if (cs.cached()) {
+    const int n = (int)(cs.hi - cs.lo);
+    int k = 0, end = n;
+    while (k < end) {  // first sequence that ends behind token t
+      const int mid = (k + end) >> 1;
+      if (cs.cut[mid + 1] <= t) k = mid + 1;
+      else end = mid;
+    }
+    const bool some = cs.lo + k < q.S;
+    if (some && cs.cut[k] <= t && t + kPer <= cs.cut[k + 1]) {
+      s[0] = cs.lo + k;
+      return true;
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      while (k < n && cs.cut[k + 1] <= t + j) ++k;
+      s[j] = cs.lo + k < q.S && cs.cut[k] <= t + j && t + j < cs.cut[k + 1] ? cs.lo + k : -1;
+    }
+    return false;
   }
+  int64_t cur = q.find(cs.lo, cs.hi, c0 + t);
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    while (cur < cs.hi && cs.bound(q, cur + 1) <= i + j) ++cur;
-    s[j] = cur < q.S && cs.bound(q, cur) <= i + j && i + j < cs.bound(q, cur + 1) ? cur : -1;
+    while (cur < cs.hi && q.bound(cur + 1) <= c0 + t + j) ++cur;
+    s[j] = cur < q.S && q.bound(cur) <= c0 + t + j && c0 + t + j < q.bound(cur + 1) ? cur : -1;
   }
+  return false;
 }
 
 // Sums of val (0 and off for tokens that do not count) over the pieces that
-// the block's sequences have in its tokens, a warp per sequence.
+// the block's sequences have in its tokens: a warp per sequence, or where they
+// are few several warps a sequence, each a part of the piece.  All threads of
+// the block; `sh` holds kWarps of each.
 __device__ __forceinline__ void piece_sums(const Seqs& q, const ChunkSeqs& cs, int64_t c0, int64_t c1, const float* val,
-                                           const uint8_t* on, const Pieces& out) {
+                                           const uint8_t* on, double* shd, int* shi, const Pieces& out) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t hi = cs.hi < q.S ? cs.hi : q.S - 1;
-  for (int64_t s = cs.lo + warp; s <= hi; s += kWarps) {
-    const int64_t a = cs.bound(q, s), b = cs.bound(q, s + 1);
-    const int t0 = (int)((a > c0 ? a : c0) - c0), t1 = (int)((b < c1 ? b : c1) - c0);
-    if (t1 <= t0) continue;
+  const int64_t num = hi - cs.lo + 1;
+  const int parts = num <= 1 ? kWarps : num <= 2 ? kWarps / 2 : num <= 4 ? kWarps / 4 : 1;
+  const int part = warp % parts;
+  for (int64_t s0 = cs.lo; s0 <= hi; s0 += kWarps / parts) {
+    const int64_t s = s0 + warp / parts;
     double v = 0.0;
     int n = 0;
-    for (int t = t0 + lane; t < t1; t += 32) {
-      v += (double)val[t];
-      n += on[t];
+    bool some = false, begins = false;
+    if (s <= hi) {
+      const int64_t a = q.bound(s), b = q.bound(s + 1);
+      const int t0 = (int)((a > c0 ? a : c0) - c0), t1 = (int)((b < c1 ? b : c1) - c0);
+      some = t1 > t0;
+      begins = a >= c0;
+      // a lane's values in float32 by 4, then in 64 bits
+      for (int t = t0 + part * 32 + lane; t < t1; t += 4 * 32 * parts) {
+        float x = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (t + 32 * parts * u < t1) {
+            x += val[t + 32 * parts * u];
+            n += on[t + 32 * parts * u];
+          }
+        }
+        v += (double)x;
+      }
+      v = warp_sum(v);
+      n = warp_sum(n);
     }
-    v = warp_sum(v);
-    n = warp_sum(n);
-    if (lane == 0) {
-      if (a >= c0) {
+    if (parts > 1) {
+      __syncthreads();
+      if (lane == 0) {
+        shd[warp] = v;
+        shi[warp] = n;
+      }
+      __syncthreads();
+      if (lane == 0 && part == 0) {
+        for (int k = 1; k < parts; ++k) {
+          v += shd[warp + k];
+          n += shi[warp + k];
+        }
+      }
+    }
+    if (lane == 0 && part == 0 && some) {
+      if (begins) {
         out.begin[s] = v;
         out.begin_n[s] = n;
       } else {
@@ -317,51 +367,54 @@ struct TokenOut {
 };
 
 // e^q - 1 - q and e^q - 1.  Below |q| = 1 the first from its series to q^11 (the
-// next term is 4e-9 of it): the difference would cancel.
+// next term is 4e-9 of it): the difference would cancel.  Both are computed and
+// one is taken: in a warp of tokens some are always far from the reference.
 __device__ __forceinline__ void kl3(float q, float& kl, float& em1) {
-  if (fabsf(q) < 1.f) {
-    float p = 1.f / 39916800.f;
-    p = fmaf(p, q, 1.f / 3628800.f);
-    p = fmaf(p, q, 1.f / 362880.f);
-    p = fmaf(p, q, 1.f / 40320.f);
-    p = fmaf(p, q, 1.f / 5040.f);
-    p = fmaf(p, q, 1.f / 720.f);
-    p = fmaf(p, q, 1.f / 120.f);
-    p = fmaf(p, q, 1.f / 24.f);
-    p = fmaf(p, q, 1.f / 6.f);
-    p = fmaf(p, q, 0.5f);
-    kl = q * q * p;
-    em1 = q + kl;
-  } else {
-    em1 = expf(q) - 1.f;
-    kl = em1 - q;
-  }
+  float p = 1.f / 39916800.f;
+  p = fmaf(p, q, 1.f / 3628800.f);
+  p = fmaf(p, q, 1.f / 362880.f);
+  p = fmaf(p, q, 1.f / 40320.f);
+  p = fmaf(p, q, 1.f / 5040.f);
+  p = fmaf(p, q, 1.f / 720.f);
+  p = fmaf(p, q, 1.f / 120.f);
+  p = fmaf(p, q, 1.f / 24.f);
+  p = fmaf(p, q, 1.f / 6.f);
+  p = fmaf(p, q, 0.5f);
+  const float near = q * q * p, far = expf(q) - 1.f;
+  const bool small = fabsf(q) < 1.f;
+  kl = small ? near : far - q;
+  em1 = small ? q + near : far;
 }
 
-// Whether the exact difference x - old lies above `border`; d is the difference
-// rounded to float32, so only next to the border are 64 bits needed.
-__device__ __forceinline__ bool above(float d, float x, float old, double border) {
-  const float gap = d - (float)border;
-  if (fabsf(gap) > 1e-6f * (1.f + fabsf(d))) return gap > 0.f;
-  return (double)x - (double)old > border;
+// Whether d = x - old lies above the borders, decided on the exact difference:
+// d is rounded to float32, so only next to a border are 64 bits needed.
+struct Beyond {
+  bool hi, lo, dual;
+};
+__device__ __forceinline__ Beyond beyond(const Policy& P, float d, float x, float old) {
+  const float hi = (float)P.log_hi, lo = (float)P.log_lo, dual = (float)P.log_dual;
+  Beyond b{d > hi, d < lo, d > dual};
+  const float near = 1e-6f * (1.f + fabsf(d));
+  if (fabsf(d - hi) <= near || fabsf(d - lo) <= near || fabsf(d - dual) <= near) {
+    const double e = (double)x - (double)old;
+    b = Beyond{e > P.log_hi, e < P.log_lo, e > P.log_dual};
+  }
+  return b;
 }
 
 __device__ __forceinline__ TokenOut policy_token(const Policy& P, float x, float old, float ref, float A) {
   const float d = P.old ? x - old : 0.f;
   const float r = P.old ? expf(d) : 1.f;
-  bool open = true;
-  float b = r;
-  if (!P.old) old = x;
-  if (A > 0.f) {
-    if (above(d, x, old, P.log_hi)) open = false, b = P.hi;
-  } else if (A < 0.f) {
-    if (above(-d, old, x, -P.log_lo)) open = false, b = P.lo;
-    if (P.dual > 0.f && above(d, x, old, P.log_dual)) open = false, b = P.dual;
-  }
+  const Beyond b = beyond(P, d, x, P.old ? old : x);
+  const bool pos = A > 0.f, neg = A < 0.f;
+  float bounded = r;
+  bounded = pos && b.hi ? P.hi : bounded;
+  bounded = neg && b.lo ? P.lo : bounded;
+  bounded = neg && P.dual > 0.f && b.dual ? P.dual : bounded;
   TokenOut o;
-  o.loss = -(b * A);
-  o.g = open ? -(r * A) : 0.f;
-  o.clipped = !open;
+  o.clipped = (pos && b.hi) || (neg && (b.lo || (P.dual > 0.f && b.dual)));
+  o.loss = -(bounded * A);
+  o.g = o.clipped ? 0.f : -(r * A);
   o.kl = 0.f;
   if (P.ref) {
     float em1;
@@ -447,8 +500,8 @@ __device__ void policy_final(const Policy& P) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) policy_forward_kernel(const Policy P) {
-  __shared__ float val[kMany * kStep];
-  __shared__ uint8_t on_sh[kMany * kStep];
+  __shared__ __align__(16) float val[kMany * kStep];
+  __shared__ __align__(4) uint8_t on_sh[kMany * kStep];
   __shared__ ChunkSeqs cs;
   __shared__ double shd[kWarps];
   __shared__ int shi[kWarps];
@@ -468,54 +521,56 @@ __global__ void __launch_bounds__(kThreads) policy_forward_kernel(const Policy P
   }
   float loss = 0.f, kl = 0.f;  // of the thread's few tokens
   int n = 0, clipped = 0;
+  const int len = (int)(c1 - c0);
+  const T* logp = static_cast<const T*>(P.logp) + c0;
+  const T* oldp = static_cast<const T*>(P.old) + c0;
+  const T* refp = static_cast<const T*>(P.ref) + c0;
 #pragma unroll 1
-  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
-    float x[kPer], old[kPer], ref[kPer], A[kPer];
+  for (int i = threadIdx.x * kPer; i < len; i += kStep) {
+    float x[kPer], old[kPer] = {}, ref[kPer] = {}, A[kPer] = {};
     bool on[kPer];
-    load4(static_cast<const T*>(P.logp), i, N, vec, x);
-    load_mask4(P.mask, i, N, vec, on);
-    if (P.old) load4(static_cast<const T*>(P.old), i, N, vec, old);
-    if (P.ref) load4(static_cast<const T*>(P.ref), i, N, vec, ref);
-    if (P.adv_token) load4(P.adv, i, N, vec, A);
+    load4(logp, i, len, vec, x);
+    load_mask4(P.mask ? P.mask + c0 : nullptr, i, len, vec, on);
+    if (P.old) load4(oldp, i, len, vec, old);
+    if (P.ref) load4(refp, i, len, vec, ref);
+    if (P.adv_token) load4(P.adv + c0, i, len, vec, A);
     if (search) {
       int64_t s[kPer];
-      token_seqs(P.q, cs, i, s);
+      if (token_seqs(P.q, cs, c0, i, s)) {
+        if (!P.adv_token) A[0] = A[1] = A[2] = A[3] = __ldg(P.adv + s[0]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        on[j] = on[j] && s[j] >= 0;
-        if (!P.adv_token) A[j] = on[j] ? __ldg(P.adv + s[j]) : 0.f;
+        for (int j = 0; j < kPer; ++j) {
+          on[j] = on[j] && s[j] >= 0;
+          if (!P.adv_token) A[j] = on[j] ? __ldg(P.adv + s[j]) : 0.f;
+        }
       }
-    } else {
+    } else if (P.q.cu != nullptr) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) on[j] = on[j] && i + j >= b0 && i + j < b1;
+      for (int j = 0; j < kPer; ++j) on[j] = on[j] && c0 + i + j >= b0 && c0 + i + j < b1;
     }
     float l[kPer], g[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      l[j] = g[j] = 0.f;
-      if (on[j]) {
-        const TokenOut o = policy_token(P, x[j], old[j], ref[j], A[j]);
-        l[j] = o.loss;
-        g[j] = o.g;
-        loss += o.loss;
-        kl += o.kl;
-        ++n;
-        clipped += o.clipped;
-      }
+      // (computed for every token, taken where it counts: what a masked one holds goes nowhere)
+      const TokenOut o = policy_token(P, x[j], old[j], ref[j], A[j]);
+      l[j] = on[j] ? o.loss : 0.f;
+      g[j] = on[j] ? o.g : 0.f;
+      loss += l[j];
+      kl += on[j] ? o.kl : 0.f;
+      n += on[j];
+      clipped += on[j] && o.clipped;
     }
-    store4(P.coef, i, N, vec, g);
-    if (P.reduction == CCE_REDUCE_NONE) store4(P.loss, i, N, vec, l);
+    store4(P.coef + c0, i, len, vec, g);
+    if (P.reduction == CCE_REDUCE_NONE) store4(P.loss + c0, i, len, vec, l);
     if (by_seq) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        val[i - c0 + j] = l[j];
-        on_sh[i - c0 + j] = on[j] ? 1 : 0;
-      }
+      *reinterpret_cast<float4*>(val + i) = make_float4(l[0], l[1], l[2], l[3]);
+      *reinterpret_cast<uchar4*>(on_sh + i) = make_uchar4(on[0], on[1], on[2], on[3]);
     }
   }
   if (by_seq) {
     __syncthreads();
-    piece_sums(P.q, cs, c0, c1, val, on_sh, P.pc);
+    piece_sums(P.q, cs, c0, c1, val, on_sh, shd, shi, P.pc);
   }
   const double loss_sum = block_sum((double)loss, shd), kl_sum = block_sum((double)kl, shd);
   n = block_sum(n | clipped << 16, shi);  // (at most 4096 tokens a block)
@@ -538,21 +593,27 @@ policy_backward_kernel(const float* __restrict__ coef, const float* __restrict__
   const int64_t c1 = c0 + q.chunk < q.N ? c0 + q.chunk : q.N;
   const float w = (up_token ? 1.f : __ldg(up)) * __ldg(weight);
   if (by_seq) cs.load(q, c0, c1);
+  const int len = (int)(c1 - c0);
 #pragma unroll 1
-  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
+  for (int i = threadIdx.x * kPer; i < len; i += kStep) {
     float g[kPer], u[kPer];
-    load4(coef, i, q.N, vec != 0, g);
-    if (up_token) load4(up, i, q.N, vec != 0, u);
+    load4(coef + c0, i, len, vec != 0, g);
+    if (up_token) load4(up + c0, i, len, vec != 0, u);
     if (by_seq) {
       int64_t s[kPer];
-      token_seqs(q, cs, i, s);
+      if (token_seqs(q, cs, c0, i, s)) {
+        const float ws = __ldg(weight + 1 + s[0]);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) g[j] = s[j] >= 0 && g[j] != 0.f ? g[j] * __ldg(weight + 1 + s[j]) : 0.f;
+        for (int j = 0; j < kPer; ++j) g[j] = g[j] != 0.f ? g[j] * ws : 0.f;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) g[j] = s[j] >= 0 && g[j] != 0.f ? g[j] * __ldg(weight + 1 + s[j]) : 0.f;
+      }
     }
     // (a token that does not count has coef 0: an infinite upstream must not make it NaN)
 #pragma unroll
     for (int j = 0; j < kPer; ++j) g[j] = g[j] == 0.f ? 0.f : g[j] * w * (up_token ? u[j] : 1.f);
-    store4(grad, i, q.N, vec != 0, g);
+    store4(grad + c0, i, len, vec != 0, g);
   }
 }
 
@@ -637,29 +698,34 @@ __device__ void preference_final(const Preference& P) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) preference_forward_kernel(const Preference P) {
-  __shared__ float val[kMany * kStep];
-  __shared__ uint8_t on_sh[kMany * kStep];
+  __shared__ __align__(16) float val[kMany * kStep];
+  __shared__ __align__(4) uint8_t on_sh[kMany * kStep];
   __shared__ ChunkSeqs cs;
+  __shared__ double shd[kWarps];
+  __shared__ int shi[kWarps];
   const int64_t N = P.q.N;
   const int64_t c0 = (int64_t)blockIdx.x * P.q.chunk;
   const int64_t c1 = c0 + P.q.chunk < N ? c0 + P.q.chunk : N;
   const bool vec = P.vec != 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) *P.counter = 0u;
+  const int len = (int)(c1 - c0);
+  const T* logp = static_cast<const T*>(P.logp) + c0;
+  const T* refp = static_cast<const T*>(P.ref) + c0;
 #pragma unroll 2
-  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
+  for (int i = threadIdx.x * kPer; i < len; i += kStep) {
     float x[kPer], ref[kPer];
     bool on[kPer];
-    load4(static_cast<const T*>(P.logp), i, N, vec, x);
-    load_mask4(P.mask, i, N, vec, on);
-    if (P.ref) load4(static_cast<const T*>(P.ref), i, N, vec, ref);
+    load4(logp, i, len, vec, x);
+    load_mask4(P.mask ? P.mask + c0 : nullptr, i, len, vec, on);
+    if (P.ref) load4(refp, i, len, vec, ref);
+    float d[kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      val[i - c0 + j] = on[j] ? (P.ref ? x[j] - ref[j] : x[j]) : 0.f;
-      on_sh[i - c0 + j] = on[j] ? 1 : 0;
-    }
+    for (int j = 0; j < kPer; ++j) d[j] = on[j] ? (P.ref ? x[j] - ref[j] : x[j]) : 0.f;
+    *reinterpret_cast<float4*>(val + i) = make_float4(d[0], d[1], d[2], d[3]);
+    *reinterpret_cast<uchar4*>(on_sh + i) = make_uchar4(on[0], on[1], on[2], on[3]);
   }
   cs.load(P.q, c0, c1);  // (ends with a barrier: val and on_sh are complete)
-  piece_sums(P.q, cs, c0, c1, val, on_sh, P.pc);
+  piece_sums(P.q, cs, c0, c1, val, on_sh, shd, shi, P.pc);
   if (gridDim.x == 1) {
     __syncthreads();
     preference_final(P);
@@ -676,22 +742,23 @@ preference_backward_kernel(const float* __restrict__ coef, const float* __restri
   const int64_t c0 = (int64_t)blockIdx.x * q.chunk;
   const int64_t c1 = c0 + q.chunk < q.N ? c0 + q.chunk : q.N;
   cs.load(q, c0, c1);
+  const int len = (int)(c1 - c0);
+  auto slope = [&](int64_t s) { return __ldg(coef + s) * __ldg(up + (up_pair ? (s < pairs ? s : s - pairs) : 0)); };
 #pragma unroll 1
-  for (int64_t i = c0 + (int64_t)threadIdx.x * kPer; i < c1; i += kStep) {
+  for (int i = threadIdx.x * kPer; i < len; i += kStep) {
     bool on[kPer];
-    load_mask4(mask, i, q.N, vec != 0, on);
+    load_mask4(mask ? mask + c0 : nullptr, i, len, vec != 0, on);
     int64_t s[kPer];
-    token_seqs(q, cs, i, s);
     float g[kPer];
+    if (token_seqs(q, cs, c0, i, s)) {
+      const float x = slope(s[0]);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      g[j] = 0.f;
-      if (on[j] && s[j] >= 0) {
-        const int64_t p = s[j] < pairs ? s[j] : s[j] - pairs;
-        g[j] = __ldg(coef + s[j]) * __ldg(up + (up_pair ? p : 0));
-      }
+      for (int j = 0; j < kPer; ++j) g[j] = on[j] ? x : 0.f;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) g[j] = on[j] && s[j] >= 0 ? slope(s[j]) : 0.f;
     }
-    store4(grad, i, q.N, vec != 0, g);
+    store4(grad + c0, i, len, vec != 0, g);
   }
 }
 
