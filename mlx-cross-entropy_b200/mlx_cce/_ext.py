@@ -207,6 +207,22 @@ def _load():
 lib = _load()
 
 
+def _load_torch_ops():
+    """The torch operators of the losses on log-probabilities (csrc/torch_ops.cpp), calling ``lib``."""
+    path = Path(__file__).resolve().parent / "libcce_torch.so"
+    if not path.exists():
+        raise ImportError(
+            f"{path} is missing: build it with `python mlx-cross-entropy_b200/mlx_cce/build.py` "
+            "(there is no fallback implementation)")
+    torch.ops.load_library(str(path))
+    ops = torch.ops.cce_b200
+    ops.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ops.functions()])
+    return ops
+
+
+torch_ops = _load_torch_ops()
+
+
 def version() -> int:
     return lib.cce_version()
 
@@ -559,295 +575,6 @@ def dequantize(wq, scales, biases, group_size: int, bits: int, dtype, out=None, 
                             int(group_size), int(bits), dtype_code(dtype, what), _ptr(out), _stream(stream))
     _check(rc, what)
     return out
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _pad(n):
-    """Bytes up to the next multiple of 256."""
-    return (n + 255) & -256
-
-
-# The raw handle of a device's current stream, without a Stream object around it
-# (a few microseconds of a call whose kernels take less).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
-    (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _on_its_device(call):
-    """Runs a call of this module, whose first argument is a CUDA tensor, with that tensor's device current."""
-    def wrapped(t, *args):
-        if t.device.index == torch.cuda.current_device():
-            return call(t, *args)
-        with torch.cuda.device(t.device):
-            return call(t, *args)
-    return wrapped
-
-
-@_on_its_device
-def policy_forward(logp, old, ref, adv, mask, cu, S, params):
-    """``cce_policy_loss_forward`` on checked contiguous tensors.
-
-    Returns (loss, stats [2], state): state holds the per-token coefficients and
-    the weights for ``policy_backward``, and behind them the call's workspace.
-    """
-    dev, N = logp.device, logp.numel()
-    loss = torch.empty(logp.shape if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-    stats = torch.empty((2,), dtype=torch.float32, device=dev)
-    at_weight = _pad(4 * N)
-    at_ws = at_weight + _pad(4 * (1 + S))
-    ws_bytes = lib.cce_token_loss_workspace_bytes(N, S)
-    state = torch.empty((at_ws + ws_bytes,), dtype=torch.uint8, device=dev)
-    p = state.data_ptr()
-    rc = lib.cce_policy_loss_forward(logp.data_ptr(), _addr(old), _addr(ref), _DTYPE_CODE[logp.dtype], adv.data_ptr(),
-                                     _addr(mask), _addr(cu), N, S, params, loss.data_ptr(), stats.data_ptr(), p,
-                                     p + at_weight, p + at_ws, ws_bytes, _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_policy_loss_forward")
-    return loss, stats, state
-
-
-@_on_its_device
-def policy_backward(state, grad_loss, reduction, cu, N, S, shape, dtype):
-    """``cce_policy_loss_backward``: the gradient with respect to logp."""
-    dev = state.device
-    grad = torch.empty(shape, dtype=dtype, device=dev)
-    p = state.data_ptr()
-    rc = lib.cce_policy_loss_backward(p, p + _pad(4 * N), grad_loss.data_ptr(), reduction, _addr(cu), N, S,
-                                      _DTYPE_CODE[dtype], grad.data_ptr(), _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_policy_loss_backward")
-    return grad
-
-
-@_on_its_device
-def preference_forward(logp, ref, ref_sums, mask, cu, pairs, params):
-    """``cce_preference_loss_forward`` on checked contiguous tensors.
-
-    Returns (loss, rewards [2 pairs], state): state holds the per-sequence
-    coefficients for ``preference_backward``, and behind them the call's workspace.
-    """
-    dev, N = logp.device, logp.numel()
-    loss = torch.empty((pairs,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-    rewards = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
-    at_ws = _pad(8 * pairs)
-    ws_bytes = lib.cce_token_loss_workspace_bytes(N, 2 * pairs)
-    state = torch.empty((at_ws + ws_bytes,), dtype=torch.uint8, device=dev)
-    p = state.data_ptr()
-    rc = lib.cce_preference_loss_forward(logp.data_ptr(), _addr(ref), _DTYPE_CODE[logp.dtype], _addr(ref_sums),
-                                         _addr(mask), _addr(cu), N, pairs, params, loss.data_ptr(),
-                                         rewards.data_ptr(), p, p + at_ws, ws_bytes, _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_preference_loss_forward")
-    return loss, rewards, state
-
-
-@_on_its_device
-def preference_backward(state, grad_loss, reduction, mask, cu, N, pairs, shape, dtype):
-    """``cce_preference_loss_backward``: the gradient with respect to logp."""
-    dev = state.device
-    grad = torch.empty(shape, dtype=dtype, device=dev)
-    rc = lib.cce_preference_loss_backward(state.data_ptr(), grad_loss.data_ptr(), reduction, _addr(mask), _addr(cu), N,
-                                          pairs, _DTYPE_CODE[dtype], grad.data_ptr(), _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_preference_loss_backward")
-    return grad
-
-
-def _bias_code(bias):
-    return 0 if bias is None else _DTYPE_CODE[bias.dtype]
-
-
-def _bytes(n, dev):
-    return torch.empty((max(n, 1),), dtype=torch.uint8, device=dev)
-
-
-def _logp_forward(e, c, bias, targets, ignore_index, logp, mask, saved, saved_bytes, ws, ws_bytes):
-    """``cce_logp_forward`` with outputs and buffers by address."""
-    (N, D), V = e.shape, c.shape[0]
-    rc = lib.cce_logp_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), targets.data_ptr(),
-                              targets.element_size(), 0 if ignore_index is None else ignore_index,
-                              ignore_index is not None, N, D, V, _DTYPE_CODE[e.dtype], logp, mask, saved, saved_bytes,
-                              ws, ws_bytes, _raw_stream(e.device.index))
-    if rc:
-        _check(rc, "cce_logp_forward")
-
-
-def _logp_sizes(e, c):
-    (N, D), V, dt = e.shape, c.shape[0], _DTYPE_CODE[e.dtype]
-    return _pad(lib.cce_logp_saved_bytes(N, D, V, dt)), _pad(lib.cce_logp_forward_workspace_bytes(N, D, V, dt))
-
-
-@_on_its_device
-def logp_forward(e, c, bias, targets, ignore_index):
-    """``cce_logp_forward`` on checked contiguous tensors: (logp [N], saved)."""
-    dev, N = e.device, e.shape[0]
-    logp = torch.empty((N,), dtype=torch.float32, device=dev)
-    saved_bytes, ws_bytes = _logp_sizes(e, c)
-    saved = torch.empty((saved_bytes + 256,), dtype=torch.uint8, device=dev)
-    ws = torch.empty((_pad(N) + ws_bytes + 256,), dtype=torch.uint8, device=dev)
-    p = ws.data_ptr()
-    _logp_forward(e, c, bias, targets, ignore_index, logp.data_ptr(), p, saved.data_ptr(), saved_bytes, p + _pad(N),
-                  ws_bytes)
-    return logp, saved
-
-
-def _rows_grads(c, N, dtype, need_e, need_c, need_bias):
-    """Outputs and flags of the backward calls on packed rows."""
-    dev, (V, D) = c.device, c.shape
-    ge = torch.empty((N, D), dtype=dtype, device=dev) if need_e else None
-    gc = torch.empty((V, D), dtype=c.dtype, device=dev) if need_c else None
-    gb = torch.empty((V,), dtype=torch.float32, device=dev) if need_bias else None
-    flags = (CCE_NEED_DE if need_e else 0) | (CCE_NEED_DC if need_c else 0) | (CCE_NEED_DBIAS if need_bias else 0)
-    return ge, gc, gb, flags
-
-
-def _logp_backward(saved, saved_bytes, c, bias, grad_logp, N, dtype, need, extra=0):
-    """``cce_logp_backward``: (grad_e, grad_c, grad_bias fp32), absent ones None.
-
-    ``grad_logp`` is an address, or a function of the address of ``extra`` bytes
-    in front of the workspace that computes it there.
-    """
-    dev, (V, D), dt = c.device, c.shape, _DTYPE_CODE[dtype]
-    ge, gc, gb, flags = _rows_grads(c, N, dtype, *need)
-    ws_bytes = lib.cce_logp_backward_workspace_bytes(N, D, V, dt, flags)
-    extra = _pad(extra)
-    ws = torch.empty((extra + ws_bytes + 256,), dtype=torch.uint8, device=dev)
-    p = ws.data_ptr()
-    if callable(grad_logp):
-        grad_logp(p)
-        grad_logp = p
-    rc = lib.cce_logp_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_logp, N, D, V, dt, flags, saved,
-                               saved_bytes, _addr(ge), _addr(gc), _addr(gb), p + extra, ws_bytes,
-                               _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_logp_backward")
-    return ge, gc, gb
-
-
-@_on_its_device
-def logp_backward(saved, c, bias, grad_logp, N, dtype, *need):
-    """``cce_logp_backward``: (grad_e, grad_c, grad_bias fp32); absent ones are None."""
-    return _logp_backward(saved.data_ptr(), saved.numel(), c, bias, grad_logp.data_ptr(), N, dtype, need)
-
-
-@_on_its_device
-def linear_policy_forward(e, c, bias, targets, ignore_index, old, ref, adv, cu, S, params):
-    """``cce_logp_forward``, then ``cce_policy_loss_forward`` on its log-probabilities.
-
-    Returns (loss, stats [2], state): state holds what the two backward calls read
-    (``linear_policy_backward``).
-    """
-    dev, N = e.device, e.shape[0]
-    loss = torch.empty((N,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-    stats = torch.empty((2,), dtype=torch.float32, device=dev)
-    saved_bytes, ws_bytes = _logp_sizes(e, c)
-    at_weight = _pad(4 * N)
-    at_saved = at_weight + _pad(4 * (1 + S))
-    state = torch.empty((at_saved + saved_bytes + 256,), dtype=torch.uint8, device=dev)
-    loss_bytes = lib.cce_token_loss_workspace_bytes(N, S)
-    at_mask = _pad(4 * N)
-    at_ws = at_mask + _pad(N)
-    ws = torch.empty((at_ws + max(ws_bytes, loss_bytes) + 256,), dtype=torch.uint8, device=dev)
-    p, w = state.data_ptr(), ws.data_ptr()
-    _logp_forward(e, c, bias, targets, ignore_index, w, w + at_mask, p + at_saved, saved_bytes, w + at_ws, ws_bytes)
-    # (in stream order behind the log-probabilities, so the workspace is free again)
-    rc = lib.cce_policy_loss_forward(w, _addr(old), _addr(ref), CCE_F32, adv.data_ptr(), w + at_mask, _addr(cu), N, S,
-                                     params, loss.data_ptr(), stats.data_ptr(), p, p + at_weight, w + at_ws,
-                                     loss_bytes, _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_policy_loss_forward")
-    return loss, stats, state
-
-
-@_on_its_device
-def linear_policy_backward(state, c, bias, grad_loss, N, dtype, reduction, cu, S, *need):
-    """(grad_e, grad_c, grad_bias fp32) of ``linear_policy_forward``; absent ones are None."""
-    p = state.data_ptr()
-    at_weight = _pad(4 * N)
-    at_saved = at_weight + _pad(4 * (1 + S))
-
-    def grad_logp(out):
-        rc = lib.cce_policy_loss_backward(p, p + at_weight, grad_loss.data_ptr(), reduction, _addr(cu), N, S, CCE_F32,
-                                          out, _raw_stream(state.device.index))
-        if rc:
-            _check(rc, "cce_policy_loss_backward")
-
-    return _logp_backward(p + at_saved, state.numel() - at_saved, c, bias, grad_logp, N, dtype, need, extra=4 * N)
-
-
-@_on_its_device
-def linear_preference_forward(e, c, bias, targets, ignore_index, ref, ref_sums, cu, pairs, params):
-    """``cce_logp_forward``, then ``cce_preference_loss_forward`` on its log-probabilities.
-
-    Returns (loss, rewards [2 pairs], state) as ``linear_policy_forward``.
-    """
-    dev, N = e.device, e.shape[0]
-    loss = torch.empty((pairs,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-    rewards = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
-    saved_bytes, ws_bytes = _logp_sizes(e, c)
-    at_mask = _pad(8 * pairs)
-    at_saved = at_mask + _pad(N)
-    state = torch.empty((at_saved + saved_bytes + 256,), dtype=torch.uint8, device=dev)
-    loss_bytes = lib.cce_token_loss_workspace_bytes(N, 2 * pairs)
-    at_ws = _pad(4 * N)
-    ws = torch.empty((at_ws + max(ws_bytes, loss_bytes) + 256,), dtype=torch.uint8, device=dev)
-    p, w = state.data_ptr(), ws.data_ptr()
-    _logp_forward(e, c, bias, targets, ignore_index, w, p + at_mask, p + at_saved, saved_bytes, w + at_ws, ws_bytes)
-    rc = lib.cce_preference_loss_forward(w, _addr(ref), CCE_F32, _addr(ref_sums), p + at_mask, _addr(cu), N, pairs,
-                                         params, loss.data_ptr(), rewards.data_ptr(), p, w + at_ws, loss_bytes,
-                                         _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_preference_loss_forward")
-    return loss, rewards, state
-
-
-@_on_its_device
-def linear_preference_backward(state, c, bias, grad_loss, N, dtype, reduction, cu, pairs, *need):
-    """(grad_e, grad_c, grad_bias fp32) of ``linear_preference_forward``; absent ones are None."""
-    p = state.data_ptr()
-    at_mask = _pad(8 * pairs)
-    at_saved = at_mask + _pad(N)
-
-    def grad_logp(out):
-        rc = lib.cce_preference_loss_backward(p, grad_loss.data_ptr(), reduction, p + at_mask, _addr(cu), N, pairs,
-                                              CCE_F32, out, _raw_stream(state.device.index))
-        if rc:
-            _check(rc, "cce_preference_loss_backward")
-
-    return _logp_backward(p + at_saved, state.numel() - at_saved, c, bias, grad_logp, N, dtype, need, extra=4 * N)
-
-
-@_on_its_device
-def distill_forward(e, c, bias, ids, teacher, mask, params):
-    """``cce_distill_forward`` on checked contiguous tensors: (loss, saved)."""
-    dev, (N, D), V, K, dt = e.device, e.shape, c.shape[0], ids.shape[1], _DTYPE_CODE[e.dtype]
-    loss = torch.empty((N,) if params.reduction == CCE_REDUCE_NONE else (), dtype=torch.float32, device=dev)
-    saved = _bytes(lib.cce_distill_saved_bytes(N, D, V, K, dt), dev)
-    ws = _bytes(lib.cce_distill_forward_workspace_bytes(N, D, V, K, dt), dev)
-    rc = lib.cce_distill_forward(e.data_ptr(), c.data_ptr(), _addr(bias), _bias_code(bias), ids.data_ptr(),
-                                 ids.element_size(), teacher.data_ptr(), _addr(mask), N, D, V, K, dt, params,
-                                 loss.data_ptr(), saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
-                                 _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_distill_forward")
-    return loss, saved
-
-
-@_on_its_device
-def distill_backward(saved, c, bias, grad_loss, N, K, dtype, params, need_e, need_c, need_bias):
-    """``cce_distill_backward``: (grad_e, grad_c, grad_bias fp32); absent ones are None."""
-    dev, (V, D), dt = c.device, c.shape, _DTYPE_CODE[dtype]
-    ge, gc, gb, flags = _rows_grads(c, N, dtype, need_e, need_c, need_bias)
-    ws = _bytes(lib.cce_distill_backward_workspace_bytes(N, D, V, dt, flags), dev)
-    rc = lib.cce_distill_backward(c.data_ptr(), _addr(bias), _bias_code(bias), grad_loss.data_ptr(), N, D, V, K,
-                                  dt, params, flags, saved.data_ptr(), saved.numel(), _addr(ge), _addr(gc),
-                                  _addr(gb), ws.data_ptr(), ws.numel(), _raw_stream(dev.index))
-    if rc:
-        _check(rc, "cce_distill_backward")
-    return ge, gc, gb
 
 
 # ---------------------------------------------------------------------------

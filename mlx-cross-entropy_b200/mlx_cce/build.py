@@ -1,9 +1,11 @@
-"""Compile the CUDA sources of this package into ``libcce_b200.so`` (in-tree).
+"""Compile the sources of this package in-tree: ``libcce_b200.so`` (CUDA) and
+``libcce_torch.so`` (the torch operators that call it).
 
 The library is built for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``)
 with nvcc; it links the CUDA runtime statically and resolves the driver's
 tensor-map encoder at run time, so it loads on a machine without a GPU and
-needs nothing at run time but the NVIDIA driver.
+needs nothing at run time but the NVIDIA driver.  The torch operators are host
+code (g++, torch's own headers) and belong to the torch they were built with.
 
     python mlx-cross-entropy_b200/mlx_cce/build.py           # rebuild if stale
     python mlx-cross-entropy_b200/mlx_cce/build.py --force
@@ -26,6 +28,8 @@ REPO = ROOT.parent
 INCLUDE = REPO / "include"
 LIB_NAME = "libcce_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+TORCH_SOURCE = CSRC / "torch_ops.cpp"
+TORCH_LIB_PATH = PKG_DIR / "libcce_torch.so"
 
 SOURCES = ["cce_abi.cu", "aux_kernels.cu", "simt_kernels.cu", "tc_kernels.cu", "noalloc.cu", "peer.cu",
            "token_loss.cu", "rows_kernels.cu"]
@@ -53,26 +57,51 @@ def _deps():
     return deps
 
 
-def needs_build() -> bool:
-    if not LIB_PATH.exists():
+def _stale(lib: Path, deps) -> bool:
+    if not lib.exists():
         return True
-    t = LIB_PATH.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in _deps())
+    t = lib.stat().st_mtime
+    return any(p.stat().st_mtime > t for p in deps)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the shared library if missing or stale; return its path."""
-    if not force and not needs_build():
-        return LIB_PATH
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-o", str(tmp)]
-    cmd += [str(CSRC / s) for s in SOURCES]
+def needs_build() -> bool:
+    return _stale(LIB_PATH, _deps())
+
+
+def _run(cmd, what, verbose):
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, LIB_PATH)
+        raise RuntimeError(f"{what} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the torch operators if missing or stale; return their path."""
+    if not force and not _stale(TORCH_LIB_PATH, [TORCH_SOURCE, *INCLUDE.glob("*.h")]):
+        return TORCH_LIB_PATH
+    import torch
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    tmp = TORCH_LIB_PATH.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}", f"-I{home / 'include'}",
+           f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{cuda / 'include'}", str(TORCH_SOURCE),
+           "-o", str(tmp), f"-L{home / 'lib'}", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    _run(cmd, "g++", verbose)
+    os.replace(tmp, TORCH_LIB_PATH)
+    return TORCH_LIB_PATH
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the shared libraries if missing or stale; return the CUDA library's path."""
+    if force or needs_build():
+        tmp = LIB_PATH.with_suffix(".so.tmp")
+        cmd = [nvcc_path(), *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-o", str(tmp)]
+        cmd += [str(CSRC / s) for s in SOURCES]
+        _run(cmd, "nvcc", verbose)
+        os.replace(tmp, LIB_PATH)
+    build_torch_ops(force, verbose)
     return LIB_PATH
 
 

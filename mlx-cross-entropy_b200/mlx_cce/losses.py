@@ -29,9 +29,16 @@ import math
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ext
+
+# The operators (csrc/torch_ops.cpp), called without the overload lookup.
+_POLICY = _ext.torch_ops.policy_loss.default
+_PREFERENCE = _ext.torch_ops.preference_loss.default
+_LOG_PROBS = _ext.torch_ops.log_probs.default
+_LINEAR_POLICY = _ext.torch_ops.linear_policy_loss.default
+_LINEAR_PREFERENCE = _ext.torch_ops.linear_preference_loss.default
+_DISTILLATION = _ext.torch_ops.distillation.default
 
 POLICY_REDUCTIONS = {"mean": _ext.CCE_REDUCE_MEAN, "sum": _ext.CCE_REDUCE_SUM,
                      "sequence": _ext.CCE_REDUCE_SEQUENCE, "none": _ext.CCE_REDUCE_NONE}
@@ -129,7 +136,7 @@ def _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_tok
         raise ValueError(f"[{what}] dual_clip must be above 1, got {dual_clip}")
     if not math.isfinite(kl_coef):
         raise ValueError(f"[{what}] kl_coef must be finite, got {kl_coef}")
-    return _ext.CcePolicyParams(clip, high, dual_clip or 0.0, kl_coef, POLICY_REDUCTIONS[reduction], int(per_token))
+    return [float(clip), float(high), float(dual_clip or 0.0), float(kl_coef)], POLICY_REDUCTIONS[reduction], per_token
 
 
 def _advantages(what, advantages, shape, S, dev):
@@ -161,8 +168,8 @@ def _preference_params(what, beta, margin, loss_type, label_smoothing, length_no
         raise ValueError(f"[{what}] label_smoothing belongs to the sigmoid loss")
     if loss_type == "ipo" and margin:
         raise ValueError(f"[{what}] margin does not apply to the ipo loss")
-    return _ext.CcePreferenceParams(beta, margin, label_smoothing, PREFERENCE_LOSSES[loss_type],
-                                    PREFERENCE_REDUCTIONS[reduction], int(bool(length_normalize)))
+    return ([float(beta), float(margin), float(label_smoothing)], PREFERENCE_LOSSES[loss_type],
+            PREFERENCE_REDUCTIONS[reduction], bool(length_normalize))
 
 
 def _pairs(what, shape, cu_seqlens, dev):
@@ -218,7 +225,7 @@ def _distill_params(what, temperature, tail, reduction):
         raise ValueError(f"[{what}] Unknown reduction: {reduction}")
     if not (temperature > 0 and math.isfinite(temperature)):
         raise ValueError(f"[{what}] temperature must be positive, got {temperature}")
-    return _ext.CceDistillParams(temperature, int(bool(tail)), PREFERENCE_REDUCTIONS[reduction])
+    return float(temperature), bool(tail), PREFERENCE_REDUCTIONS[reduction]
 
 
 def _reference(what, ref_logp, tokens, dtype, S):
@@ -233,145 +240,6 @@ def _reference(what, ref_logp, tokens, dtype, S):
     if not ref_logp.is_floating_point() or ref_logp.device != tokens.device:
         raise ValueError(f"[{what}] ref_logp must be floating point on {tokens.device}")
     return None, _constant(ref_logp.to(torch.float32))
-
-
-# ---------------------------------------------------------------------------
-# autograd
-# ---------------------------------------------------------------------------
-
-def _first_order(backward):
-    """once_differentiable (a second derivative is an error, not a wrong zero), which
-    only costs its wrapping where a graph of the backward pass is recorded."""
-    recorded = once_differentiable(backward)
-
-    def wrapped(ctx, *grads):
-        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
-
-    return wrapped
-
-
-class PolicyLossFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logp, old, ref, adv, mask, cu, S, params):
-        loss, stats, state = _ext.policy_forward(logp, old, ref, adv, mask, cu, S, params)
-        ctx.save_for_backward(state, cu)
-        ctx.meta = (params.reduction, logp.numel(), S, logp.shape, logp.dtype)
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)
-        return loss, stats
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, grad_loss, _grad_stats):
-        if grad_loss is None:
-            return (None,) * 8
-        state, cu = ctx.saved_tensors
-        reduction, N, S, shape, dtype = ctx.meta
-        g = grad_loss.to(torch.float32).contiguous()
-        return (_ext.policy_backward(state, g, reduction, cu, N, S, shape, dtype),) + (None,) * 7
-
-
-class PreferenceLossFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logp, ref, ref_sums, mask, cu, pairs, params):
-        loss, rewards, state = _ext.preference_forward(logp, ref, ref_sums, mask, cu, pairs, params)
-        ctx.save_for_backward(state, mask, cu)
-        ctx.meta = (params.reduction, logp.numel(), pairs, logp.shape, logp.dtype)
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, grad_loss, _grad_rewards):
-        if grad_loss is None:
-            return (None,) * 7
-        state, mask, cu = ctx.saved_tensors
-        reduction, N, pairs, shape, dtype = ctx.meta
-        g = grad_loss.to(torch.float32).contiguous()
-        return (_ext.preference_backward(state, g, reduction, mask, cu, N, pairs, shape, dtype),) + (None,) * 6
-
-
-def _head_grads(grads, bias):
-    ge, gc, gb = grads
-    return ge, gc, gb if gb is None or gb.dtype == bias.dtype else gb.to(bias.dtype)
-
-
-class LogProbsFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, e, c, bias, targets, ignore_index):
-        logp, saved = _ext.logp_forward(e, c, bias, targets, ignore_index)
-        ctx.save_for_backward(c, bias, saved)
-        ctx.meta = (e.shape[0], e.dtype)
-        return logp
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, grad_logp):
-        c, bias, saved = ctx.saved_tensors
-        g = grad_logp.to(torch.float32).contiguous()
-        return _head_grads(_ext.logp_backward(saved, c, bias, g, *ctx.meta, *ctx.needs_input_grad[:3]), bias) + (None,) * 2
-
-
-class LinearPolicyLossFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, e, c, bias, targets, ignore_index, old, ref, adv, cu, S, params):
-        loss, stats, state = _ext.linear_policy_forward(e, c, bias, targets, ignore_index, old, ref, adv, cu, S, params)
-        ctx.save_for_backward(c, bias, state, cu)
-        ctx.meta = (e.shape[0], e.dtype, params.reduction), S
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)
-        return loss, stats
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, grad_loss, _grad_stats):
-        if grad_loss is None:
-            return (None,) * 11
-        c, bias, state, cu = ctx.saved_tensors
-        meta, S = ctx.meta
-        g = grad_loss.to(torch.float32).contiguous()
-        grads = _ext.linear_policy_backward(state, c, bias, g, *meta, cu, S, *ctx.needs_input_grad[:3])
-        return _head_grads(grads, bias) + (None,) * 8
-
-
-class LinearPreferenceLossFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, e, c, bias, targets, ignore_index, ref, ref_sums, cu, pairs, params):
-        loss, rewards, state = _ext.linear_preference_forward(e, c, bias, targets, ignore_index, ref, ref_sums, cu,
-                                                              pairs, params)
-        ctx.save_for_backward(c, bias, state, cu)
-        ctx.meta = (e.shape[0], e.dtype, params.reduction), pairs
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, grad_loss, _grad_rewards):
-        if grad_loss is None:
-            return (None,) * 10
-        c, bias, state, cu = ctx.saved_tensors
-        meta, pairs = ctx.meta
-        g = grad_loss.to(torch.float32).contiguous()
-        grads = _ext.linear_preference_backward(state, c, bias, g, *meta, cu, pairs, *ctx.needs_input_grad[:3])
-        return _head_grads(grads, bias) + (None,) * 7
-
-
-class DistillationFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, e, c, bias, ids, teacher, mask, params):
-        loss, saved = _ext.distill_forward(e, c, bias, ids, teacher, mask, params)
-        ctx.save_for_backward(c, bias, saved)
-        ctx.meta = (e.shape[0], ids.shape[1], e.dtype, params)
-        return loss
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, grad_loss):
-        c, bias, saved = ctx.saved_tensors
-        g = grad_loss.to(torch.float32).contiguous()
-        return _head_grads(_ext.distill_backward(saved, c, bias, g, *ctx.meta, *ctx.needs_input_grad[:3]), bias) + (None,) * 4
 
 
 # ---------------------------------------------------------------------------
@@ -410,9 +278,9 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seql
     S, cu = _sequences(what, logp.shape, cu_seqlens, logp.device)
     adv, per_token = _advantages(what, advantages, logp.shape, S, logp.device)
     params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
-    loss, stats = PolicyLossFunction.apply(logp, _per_token(what, "old_logp", old_logp, logp, logp.dtype),
-                                           _per_token(what, "ref_logp", ref_logp, logp, logp.dtype), adv,
-                                           _mask(what, mask, logp.shape, logp.device), cu, S, params)
+    loss, stats = _POLICY(logp, _per_token(what, "old_logp", old_logp, logp, logp.dtype),
+                          _per_token(what, "ref_logp", ref_logp, logp, logp.dtype), adv,
+                          _mask(what, mask, logp.shape, logp.device), cu, S, *params)
     return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
 
 
@@ -447,8 +315,7 @@ def preference_loss(logp, ref_logp=None, *, mask=None, cu_seqlens=None, beta=0.1
     pairs, cu = _pairs(what, logp.shape, cu_seqlens, logp.device)
     params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
     ref, sums = _reference(what, ref_logp, logp, logp.dtype, 2 * pairs)
-    loss, rewards = PreferenceLossFunction.apply(logp, ref, sums, _mask(what, mask, logp.shape, logp.device), cu,
-                                                 pairs, params)
+    loss, rewards = _PREFERENCE(logp, ref, sums, _mask(what, mask, logp.shape, logp.device), cu, pairs, *params)
     return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
 
 
@@ -468,7 +335,7 @@ def linear_log_probs(e, c, targets, bias=None, *, ignore_index=-100):
     """
     what = "linear_log_probs"
     e, c, bias = _head(what, e, c, bias, targets.shape)
-    logp = LogProbsFunction.apply(e, c, bias, _ids(what, "targets", targets, e.device), ignore_index)
+    logp = _LOG_PROBS(e, c, bias, _ids(what, "targets", targets, e.device), ignore_index)
     return logp.view(targets.shape)
 
 
@@ -488,9 +355,8 @@ def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_lo
     params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
     e, c, bias = _head(what, e, c, bias, targets.shape)
     targets = _ids(what, "targets", targets, e.device)
-    loss, stats = LinearPolicyLossFunction.apply(e, c, bias, targets, ignore_index,
-                                                 _per_token(what, "old_logp", old_logp, targets),
-                                                 _per_token(what, "ref_logp", ref_logp, targets), adv, cu, S, params)
+    loss, stats = _LINEAR_POLICY(e, c, bias, targets, ignore_index, _per_token(what, "old_logp", old_logp, targets),
+                                 _per_token(what, "ref_logp", ref_logp, targets), adv, cu, S, *params)
     if reduction == "none":
         loss = loss.view(targets.shape)
     return (loss, PolicyStats(*stats.unbind())) if return_stats else loss
@@ -513,7 +379,7 @@ def linear_preference_loss(e, c, targets, ref_logp=None, bias=None, *, cu_seqlen
     e, c, bias = _head(what, e, c, bias, targets.shape)
     targets = _ids(what, "targets", targets, e.device)
     ref, sums = _reference(what, ref_logp, targets, torch.float32, 2 * pairs)
-    loss, rewards = LinearPreferenceLossFunction.apply(e, c, bias, targets, ignore_index, ref, sums, cu, pairs, params)
+    loss, rewards = _LINEAR_PREFERENCE(e, c, bias, targets, ignore_index, ref, sums, cu, pairs, *params)
     return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
 
 
@@ -556,5 +422,5 @@ def linear_distillation_loss(e, c, teacher_ids, teacher_logprobs, bias=None, *, 
     if not teacher_logprobs.is_floating_point() or teacher_logprobs.device != e.device:
         raise ValueError(f"[{what}] teacher_logprobs must be floating point on {e.device}")
     teacher = _constant(teacher_logprobs.to(torch.float32))
-    loss = DistillationFunction.apply(e2, c, bias, ids, teacher, _mask(what, mask, rows, e.device), params)
+    loss = _DISTILLATION(e2, c, bias, ids, teacher, _mask(what, mask, rows, e.device), *params)
     return loss.view(rows) if reduction == "none" else loss

@@ -105,3 +105,10 @@ def test_saved_and_workspace_sizes():
     assert odd > 2 * 1000 * 72 * 2 + lib.cce_logp_backward_workspace_bytes(64, 72, 1000, _ext.CCE_BF16, flags) - 4096
     assert lib.cce_distill_saved_bytes(N, D, V, 1025, _ext.CCE_BF16) == 0
     assert lib.cce_logp_saved_bytes(-1, D, V, _ext.CCE_BF16) == 0
+
+
+def test_torch_operators_call_the_declared_functions():
+    names = torch.ops.cce_b200.functions()
+    assert set(names) <= set(_ext.EXPORTED_SYMBOLS)
+    with pytest.raises(RuntimeError, match="no address"):
+        torch.ops.cce_b200.bind([1])

@@ -445,6 +445,23 @@ def test_gradients_against_differences():
         assert abs(diff - float((grads[k] * d).sum())) <= h * h * reach ** 3 * mean + 2.0 ** -18 / h
 
 
+def test_second_derivatives_are_an_error_and_changed_weights_are_noticed():
+    e, c, b, t, g = head(40, 64, 300, torch.bfloat16, 51)
+    tlp, ids = teacher(e, c, b, 4, g)
+    xs = leaves(e, c, None)
+    for fn in (lambda: mlx_cce.linear_distillation_loss(xs[0], xs[1], ids.cuda(), tlp.cuda()),
+               lambda: mlx_cce.linear_log_probs(xs[0], xs[1], t.cuda()).sum(),
+               lambda: mlx_cce.linear_preference_loss(xs[0].view(4, 10, 64), xs[1], t.view(4, 10).cuda())):
+        ge, gc = torch.autograd.grad(fn(), xs, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            ge.float().sum().backward()
+        loss = fn()
+        with torch.no_grad():
+            xs[1].mul_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
 def test_results_do_not_change_between_runs():
     e, c, b, t, g = head(700, 128, 3000, torch.bfloat16, 49, bias=torch.float32)
     tlp, ids = teacher(e, c, b, 16, g)

@@ -418,3 +418,36 @@ def test_linear_cross_entropy_feeds_both_losses():
     # log-probabilities carry about 1e-6 (float32 logits of magnitude 5); no ratio lies so near to a border
     assert abs(float(loss) - float(p["loss"] + q["loss"])) < 1e-5
     assert torch.all((ec.grad.cpu().double() - want).abs() <= 1e-5 * want.abs().max())
+
+
+def test_second_derivatives_are_an_error():
+    b = batch(200, 4, seed=90)
+    x = b["logp"].cuda().requires_grad_(True)
+    adv = torch.ones(4, device="cuda")
+    for loss in (mlx_cce.policy_loss(x, b["old"].cuda(), adv, cu_seqlens=cuda_cu(b["cu"])),
+                 mlx_cce.preference_loss(x, cu_seqlens=cuda_cu(b["cu"]))):
+        (plain,) = torch.autograd.grad(loss, [x], retain_graph=True)
+        (grad,) = torch.autograd.grad(loss, [x], create_graph=True)
+        assert torch.equal(grad.detach(), plain)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            grad.sum().backward()
+
+
+def test_backward_twice_and_accumulation():
+    """A graph kept for a second pass gives the same gradient; .grad adds up; an
+    upstream gradient that is expanded, strided or of another type is taken as it is."""
+    b = batch(3000, 6, seed=91)
+    x = b["logp"].cuda().requires_grad_(True)
+    old, adv, mask, cu = b["old"].cuda(), torch.randn(3000, generator=b["g"]).cuda(), b["mask"].cuda(), cuda_cu(b["cu"])
+    loss = mlx_cce.policy_loss(x, old, adv, mask=mask, cu_seqlens=cu)
+    loss.backward(retain_graph=True)
+    first = x.grad.clone()
+    loss.backward()
+    assert torch.equal(x.grad, first * 2)
+    each = mlx_cce.policy_loss(x, old, adv, mask=mask, cu_seqlens=cu, reduction="none")
+    (a,) = torch.autograd.grad(each.sum(), [x], retain_graph=True)   # an expanded scalar
+    (c,) = torch.autograd.grad(each, [x], torch.ones(3000, 2, device="cuda")[:, 0], retain_graph=True)
+    assert torch.equal(a, c)
+    with torch.no_grad():
+        again = mlx_cce.policy_loss(x, old, adv, mask=mask, cu_seqlens=cu)
+    assert not again.requires_grad and torch.equal(again, loss.detach())
