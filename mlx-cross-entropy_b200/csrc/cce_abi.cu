@@ -1143,6 +1143,7 @@ struct RowsSaved {
   float* weight;    // distillation [1]
   cce::TopkView topk;
   float* se;        // float32: scale of e's parts
+  uint32_t* words;  // float32: largest values of c and e
   void *e, *e_lo;   // packed rows [N][Dk]
   size_t bytes;
 };
@@ -1169,6 +1170,7 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
   if (dtype == CCE_F32) {
     r.e_lo = p.take<uint16_t>(n);
     r.se = p.take<float>(2);
+    r.words = p.take<uint32_t>(2);
   }
   r.bytes = p.used;
   return r;
@@ -1178,14 +1180,12 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
 struct RowsC {
   void *c, *c_lo;
   float* sc;
-  uint32_t* words;  // largest values of c and e
 };
 
 RowsC rows_c(Parts& p, int64_t N, int64_t D, int64_t V, int dtype) {
   RowsC w{};
   const size_t n = (size_t)V * rows_dk(N, D, dtype);
   if (dtype == CCE_F32) {
-    w.words = p.take<uint32_t>(2);
     w.sc = p.take<float>(2);
     w.c = p.take<uint16_t>(n);
     w.c_lo = p.take<uint16_t>(n);
@@ -1203,14 +1203,14 @@ cudaError_t rows_operands(cce::RowsGemmArgs& a, const RowsSaved& v, const RowsC&
   a.c = w.c ? w.c : c, a.c_lo = w.c_lo, a.sc = w.sc;
   cudaError_t err = cudaSuccess;
   if (a.dtype == CCE_F32) {
-    if ((err = cudaMemsetAsync(w.words, 0, 2 * sizeof(uint32_t), s)) != cudaSuccess) return err;
     if (e) {
-      if ((err = cce::launch_absmax((const float*)e, a.N, D, &v.R, w.words + 1, s)) != cudaSuccess) return err;
-      if ((err = cce::launch_split((const float*)e, a.N, D, a.Dk, &v.R, w.words + 1, v.se, v.e, v.e_lo, s)) != cudaSuccess)
+      if ((err = cudaMemsetAsync(v.words, 0, 2 * sizeof(uint32_t), s)) != cudaSuccess) return err;
+      if ((err = cce::launch_absmax((const float*)c, a.V, D, nullptr, v.words, s)) != cudaSuccess) return err;
+      if ((err = cce::launch_absmax((const float*)e, a.N, D, &v.R, v.words + 1, s)) != cudaSuccess) return err;
+      if ((err = cce::launch_split((const float*)e, a.N, D, a.Dk, &v.R, v.words + 1, v.se, v.e, v.e_lo, s)) != cudaSuccess)
         return err;
     }
-    if ((err = cce::launch_absmax((const float*)c, a.V, D, nullptr, w.words, s)) != cudaSuccess) return err;
-    return cce::launch_split((const float*)c, a.V, D, a.Dk, nullptr, w.words, w.sc, w.c, w.c_lo, s);
+    return cce::launch_split((const float*)c, a.V, D, a.Dk, nullptr, v.words, w.sc, w.c, w.c_lo, s);
   }
   if (e && (err = cce::launch_rows_copy(e, a.N, D, D, &v.R, v.e, a.Dk, s)) != cudaSuccess) return err;
   return w.c ? cce::launch_rows_copy(c, a.V, D, D, nullptr, w.c, a.Dk, s) : cudaSuccess;
@@ -1248,6 +1248,28 @@ struct RowsPlan {
   int slabs;
 };
 
+// K splits of grad_e over a chunk of vc vocabulary rows, the one whose estimate is
+// least: whole waves of (128 rows, 256 columns, K / splits) units over 148 SMs, at
+// 0.27 us per 64-row K-block and pass and 4 us for a unit's start and output, and
+// 8 bytes of slab traffic per value at 4 TB/s.  331 x 1024 x 32000: 12 tiles in
+// one split are 135 us, in 12 splits 16 us and 4 us of slabs.
+int rows_slabs(int64_t N, int64_t D, int64_t vc, int dtype) {
+  const int64_t tiles = cce::ceil_div(N, 128) * cce::ceil_div(D, 256);
+  const int64_t kb = cce::ceil_div(vc, 64), passes = dtype == CCE_F32 ? 3 : 1;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 32; ++s) {
+    if (s > 1 && (s * N * D * 4 > (256ll << 20) || kb < 2 * s)) break;
+    const double waves = (double)cce::ceil_div(tiles * s, 148);
+    const double us = waves * (0.27 * (double)(cce::ceil_div(kb, s) * passes) + 4.0) + (double)(s * N * D) * 8.0 / 4e6;
+    if (us < 0.97 * least) {
+      least = us;
+      best = s;
+    }
+  }
+  return best;
+}
+
 RowsPlan rows_plan(int64_t N, int64_t D, int64_t V, int dtype) {
   const int64_t n = N > 0 ? N : 1, elt = dtype == CCE_F32 ? 4 : 2;
   const int64_t target = target_chunk_rows();
@@ -1266,16 +1288,7 @@ RowsPlan rows_plan(int64_t N, int64_t D, int64_t V, int dtype) {
   }
   const int64_t vmax = cce::round_up(V, 256);
   if (p.vc > vmax) p.vc = vmax;
-  // enough units of (128 rows, 256 columns, at least kMinK of K) for every SM to
-  // have two, within 256 MiB of fp32 slabs
-  constexpr int64_t kMinK = 512;
-  const int64_t tiles = cce::ceil_div(n, 128) * cce::ceil_div(D, 256);
-  int64_t sl = cce::ceil_div(2 * 148, tiles);
-  const int64_t fit = (256ll << 20) / (n * D * 4);
-  if (sl > fit) sl = fit;
-  if (sl > p.vc / kMinK) sl = p.vc / kMinK;
-  if (sl > 32) sl = 32;
-  p.slabs = sl < 1 ? 1 : (int)sl;
+  p.slabs = rows_slabs(n, D, p.vc, dtype);
   return p;
 }
 

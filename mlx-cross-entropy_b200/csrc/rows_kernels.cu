@@ -509,6 +509,7 @@ absmax_kernel(const float* __restrict__ x, int64_t rows, int64_t D, const int32_
   for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
     const float* p = x + (row_of ? row_of[r] : r) * D;
     if (vec) {
+#pragma unroll 8
       for (int64_t k = 4 * lane; k < D; k += 128) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + k));
         m = max(m, max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu)));
@@ -690,6 +691,10 @@ cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, int64_t ld, c
 }
 
 cudaError_t launch_absmax(const float* x, int64_t rows, int64_t D, const RowsView* R, uint32_t* word, cudaStream_t s) {
+  if (R == nullptr && rows * D % 4096 == 0) {  // contiguous: rows of a width that keeps many loads in flight
+    rows = rows * D / 4096;
+    D = 4096;
+  }
   absmax_kernel<<<warps_grid(rows), 256, 0, s>>>(x, rows, D, R ? R->row_of : nullptr, R ? R->count : nullptr,
                                                  D % 4 == 0 && aligned16(x), word);
   return launched();
