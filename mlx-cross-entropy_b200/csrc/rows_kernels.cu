@@ -424,15 +424,22 @@ distill_final_kernel(const DistillSum* __restrict__ sums, int blocks, int reduct
 // backward
 // ---------------------------------------------------------------------------
 
-// One block: the largest |d| of the rows that count, as a power of two s (1 when
-// all are zero) times 2^-14: dlogits are at most d in magnitude, so w / s stays
+// Bits of |x| as an order of values, 0 for infinities and NaN: a row that holds one
+// must not take the scale away from the others.
+__device__ __forceinline__ uint32_t finite_bits(uint32_t x) {
+  x &= 0x7fffffffu;
+  return x < 0x7f800000u ? x : 0u;
+}
+
+// One block: the largest finite |d| of the rows that count, as a power of two s (1
+// when all are zero) times 2^-14: dlogits are at most d in magnitude, so w / s stays
 // below 2^14 in float16 and a softmax value of 2^-28 is still a normal number.
 __global__ void __launch_bounds__(1024) rows_scale_kernel(const Cotangent up, const RowsView R, float* __restrict__ out) {
   __shared__ float red[32];
   const int count = *R.count;
   float m = 0.f;
   for (int i = threadIdx.x; i < (up.per_row ? count : min(count, 1)); i += blockDim.x)
-    m = fmaxf(m, fabsf(up.of(i, R.row_of)));
+    m = fmaxf(m, __uint_as_float(finite_bits(__float_as_uint(up.of(i, R.row_of)))));
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
@@ -440,7 +447,7 @@ __global__ void __launch_bounds__(1024) rows_scale_kernel(const Cotangent up, co
   if (threadIdx.x == 0) {
     for (int w = 1; w < 32; ++w) m = fmaxf(m, red[w]);
     int ex = 0;
-    if (m > 0.f && isfinite(m)) {
+    if (m > 0.f) {
       const float f = frexpf(m, &ex);  // m = f * 2^ex, f in [0.5, 1)
       if (f == 0.5f) --ex;
     }
@@ -498,8 +505,7 @@ rows_scatter_kernel(const float* __restrict__ slabs, int num, int64_t ld, const 
 // float32 operands as two float16 parts
 // ---------------------------------------------------------------------------
 
-// The largest |x| as the bits of a float (their order is that of the values; NaN
-// and infinity come out on top), whatever order the blocks run in.
+// The largest finite |x| as the bits of a float, whatever order the blocks run in.
 __global__ void __launch_bounds__(256)
 absmax_kernel(const float* __restrict__ x, int64_t rows, int64_t D, const int32_t* __restrict__ row_of,
               const int32_t* __restrict__ count, int vec, uint32_t* __restrict__ word) {
@@ -512,10 +518,10 @@ absmax_kernel(const float* __restrict__ x, int64_t rows, int64_t D, const int32_
 #pragma unroll 8
       for (int64_t k = 4 * lane; k < D; k += 128) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + k));
-        m = max(m, max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu)));
+        m = max(m, max(max(finite_bits(v.x), finite_bits(v.y)), max(finite_bits(v.z), finite_bits(v.w))));
       }
     } else {
-      for (int64_t k = lane; k < D; k += 32) m = max(m, __float_as_uint(p[k]) & 0x7fffffffu);
+      for (int64_t k = lane; k < D; k += 32) m = max(m, finite_bits(__float_as_uint(p[k])));
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
@@ -532,7 +538,7 @@ split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, c
   const int lane = threadIdx.x & 31;
   const float big = __uint_as_float(*word);
   float s = 1.f;
-  if (big > 0.f && isfinite(big)) {
+  if (big > 0.f) {
     int ex;
     frexpf(big, &ex);
     s = ldexpf(1.f, min(110, max(-110, 14 - ex)));

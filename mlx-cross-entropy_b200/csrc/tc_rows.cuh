@@ -16,10 +16,10 @@
 // accumulator rounding towards zero: a logit of 14 after 144 such steps is
 // about 1e-5 too small, always in the same direction, and sums of
 // log-probabilities over a sequence add that up.  Here an accumulator holds
-// only a segment of K; the epilogue warps add each of those
-// partial logits to the total in their registers (128 per thread, round to
-// nearest).  The two TMEM accumulators take the segments in turn, so the MMAs
-// never wait for the adds: a segment's 16 MMAs take about 2000 cycles, its add
+// only a segment of K; the epilogue warps add each of those partial logits to
+// the total in their registers (128 per thread, round to nearest).  The two TMEM
+// accumulators take the segments in turn, so the MMAs run on while the adds are
+// made.  A segment of 4 K-blocks is 16 MMAs, about 2000 cycles; its add takes
 // about 500 of the issue slots of the 8 epilogue warps.
 //
 // What is left of the drift is added back in expectation.  A step that rounds
@@ -28,22 +28,26 @@
 // steps of a partial logit p that grows in a straight line 6 * 2^-24 |p|.  The
 // noise on the way makes it less, float16 products (22 bits, cut to the
 // accumulator's) make it more.  The partials are multiplied by 1 + k 2^-23 in the
-// same fused multiply-add, k (untruncate_of) from the root mean square error of
-// log-probabilities of 2048 peaked rows, V = 32000, in units of 1e-6 for
-// k = 0, 1, 2, 3, 4 (in brackets a library's float32 product):
+// same fused multiply-add, k (segments() below: a share of the segment's MMA
+// steps) from the root mean square error of log-probabilities of 2048 peaked
+// rows, V = 32000, in units of 1e-6 for k = 0, 1, 2, 3, 4 at segments of 16 steps
+// (float32: 8), in brackets a library's float32 product:
 //   bfloat16, D = 2304     1.00 0.68 0.55 0.68 0.98   (5.1)
 //   bfloat16, D = 512      1.15 0.80 0.60 0.65 0.92   (2.2)
 //   float16, D = 2304      1.31 0.96 0.73 0.64 0.80   (6.5)
 //   float16, D = 512       2.30 1.94 1.63 1.37 1.20   (3.1)
 //   float32, D = 2304      1.69 1.60 1.63 1.73 1.92   (6.7)
 //   float32, D = 512       1.29 1.03 0.93 1.00 1.23   (3.0)
-// With one accumulator for all of K a bfloat16 D = 2304 head has 5.7.
+// bfloat16 runs on segments of 32 steps with k = 4: 0.68 (D = 2304), 0.75 (4096),
+// 1.08 (512), for half the adds.  With one accumulator for all of K a bfloat16
+// D = 2304 head has 5.7.  Gradients and dlogits, which are rounded to 16 bits or
+// summed over far smaller terms, take segments of 64 steps.
 //
 // Float32 inputs.  x = (hi + lo) / s with hi, lo float16 and s a power of two that
 // puts the tensor's largest value below 2^14: hi holds 11 bits and lo the next 11.
 // A product runs as three passes over K, hi hi + hi lo + lo hi (lo lo is 2^-22 of
 // it), each on the tensor cores: 3 times the 16-bit work, where FFMA is 20 times
-// slower.  512 x 512 x 32000, loss and gradients: 2.75 ms on the CUDA cores.
+// slower.  512 x 512 x 32000, loss and gradients: 0.38 ms, 2.75 ms on the CUDA cores.
 //
 // Rows are counted on the device (the batch without its masked rows), so row
 // tiles behind the count cost nothing.

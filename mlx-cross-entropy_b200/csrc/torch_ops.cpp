@@ -9,11 +9,15 @@
 // library's functions come as addresses (bind), so that whichever build of it is
 // loaded is the one that is called.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
+
+#include <unordered_set>
 
 #include "cce_b200.h"
 
@@ -111,6 +115,29 @@ variable_list first_order(variable_list grads) {
   return (*error)(std::move(grads));
 }
 
+// A backward pass that is being captured must not add into a leaf whose gradient
+// node an eager graph made on the default stream and still holds (a loss that was
+// not deleted): the engine would wait on that stream, which no capture may, and
+// the process would end.  Every such node below is looked for, once per capture.
+void check_capture() {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const c10::Stream eager = c10::cuda::getDefaultCUDAStream().unwrap();
+  std::vector<torch::autograd::Node*> todo{torch::autograd::get_current_node().get()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    torch::autograd::Node* n = todo.back();
+    todo.pop_back();
+    if (n == nullptr || !seen.insert(n).second) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(n)) {
+      const auto at = n->stream();
+      TORCH_CHECK(!at || *at != eager,
+                  "a backward pass is captured into a CUDA graph while an eager graph of the same leaves, made on the "
+                  "default stream, is alive: delete its loss first (or run it on another stream)");
+    }
+    for (const auto& edge : n->next_edges()) todo.push_back(edge.function.get());
+  }
+}
+
 // ---- losses on given log-probabilities ----
 
 struct PolicyArgs {
@@ -150,6 +177,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const auto shape = ctx->saved_data["shape"].toIntVector();
     const Tensor& state = saved[0];
     c10::cuda::CUDAGuard guard(state.device());
+    check_capture();
     const auto type = static_cast<at::ScalarType>(m[2]);
     Tensor grad = at::empty(shape, state.options().dtype(type));
     const int64_t N = grad.numel();
@@ -196,6 +224,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const auto m = ctx->saved_data["m"].toIntVector();
     const auto shape = ctx->saved_data["shape"].toIntVector();
     c10::cuda::CUDAGuard guard(saved[0].device());
+    check_capture();
     const auto type = static_cast<at::ScalarType>(m[2]);
     Tensor grad = at::empty(shape, saved[0].options().dtype(type));
     const Tensor g = upstream(grads[0]);
@@ -289,6 +318,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
     const auto saved = ctx->get_saved_variables();
     const auto m = ctx->saved_data["m"].toIntVector();
     c10::cuda::CUDAGuard guard(saved[0].device());
+    check_capture();
     const Tensor g = upstream(grads[0]);
     return logp_backward(ctx, saved[0], saved[1], ptr(saved[2]), saved[2].numel(), m[0],
                          static_cast<at::ScalarType>(m[1]), [&](float*) { return ptr<const float>(g); });
@@ -329,6 +359,7 @@ struct LinearPolicyLoss : torch::autograd::Function<LinearPolicyLoss> {
     const auto saved = ctx->get_saved_variables();
     const auto m = ctx->saved_data["m"].toIntVector();
     c10::cuda::CUDAGuard guard(saved[0].device());
+    check_capture();
     const Tensor g = upstream(grads[0]);
     const int64_t N = m[0];
     char* p = ptr<char>(saved[2]);
@@ -375,6 +406,7 @@ struct LinearPreferenceLoss : torch::autograd::Function<LinearPreferenceLoss> {
     const auto saved = ctx->get_saved_variables();
     const auto m = ctx->saved_data["m"].toIntVector();
     c10::cuda::CUDAGuard guard(saved[0].device());
+    check_capture();
     const Tensor g = upstream(grads[0]);
     const int64_t N = m[0];
     char* p = ptr<char>(saved[2]);
@@ -420,6 +452,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
     const auto m = ctx->saved_data["m"].toIntVector();
     const Tensor &c = saved[0], &bias = saved[1];
     c10::cuda::CUDAGuard guard(c.device());
+    check_capture();
     const auto type = static_cast<at::ScalarType>(m[1]);
     const CceDistillParams params{ctx->saved_data["T"].toDouble(), (int32_t)m[3], (int32_t)m[4]};
     const Tensor up = upstream(grads[0]);

@@ -10,7 +10,7 @@ after pre-training.  ``linear_log_probs`` is the head's part of the first two
 ``policy_loss`` and ``preference_loss`` take log-probabilities.  Hidden states,
 classifier, bias and log-probabilities are differentiable, the other tensors
 are constants.  Kernels: ``csrc/token_loss.cu``, ``csrc/rows_kernels.cu`` and
-the GEMMs of ``csrc/tc_kernels.cu`` / ``csrc/simt_kernels.cu``.
+the GEMMs of ``csrc/tc_rows.cuh``.
 
 The linear forms differ from ``linear_cross_entropy`` in two ways: gradients
 are exact (the filter of small softmax values is not applied: a policy

@@ -22,6 +22,7 @@ sum_k |e_k c_k|:
   the result is rounded to the input type (eps / 2).
 """
 
+import gc
 import math
 
 import pytest
@@ -546,6 +547,54 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for _, out in graphs:
             assert all(torch.equal(x.detach(), y) for x, y in zip(out, want))
+
+
+def test_capture_beside_a_live_eager_graph_is_refused():
+    """Refused before anything of the backward pass runs; without the eager graph the
+    same capture works."""
+    args = _mixed_inputs(71)
+    e, c = (x.detach().requires_grad_(True) for x in args[:2])
+    eager = _mixed(e, c, *args[2:])
+    gr = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="delete its loss first"):
+        with torch.cuda.graph(gr):
+            _mixed(e, c, *args[2:]).backward()
+    eager.backward()
+    want = [e.grad.clone(), c.grad.clone()]
+    del eager, gr
+    gc.collect()  # (the refused call's frames hold its loss)
+    e.grad = c.grad = None
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        loss = _mixed(e, c, *args[2:])
+        loss.backward()
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(e.grad, want[0]) and torch.equal(c.grad, want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_are_not_finite_stay_alone(dtype):
+    """A NaN or infinite row that counts, or an infinite upstream gradient, costs its own
+    row: the others get the bits they get beside a row of zeros."""
+    e, c, b, t, g = head(150, 64, 700, dtype, 90)
+    up = torch.randn(150, generator=g).cuda()
+    def run(bad, g3):
+        e1 = e.clone()
+        e1[3] = 0
+        e1[3, 5:7] = bad
+        e1 = e1.cuda().requires_grad_(True)
+        logp = mlx_cce.linear_log_probs(e1, c.cuda(), t.cuda())
+        u = up.clone()
+        u[3] = g3
+        return logp.detach(), torch.autograd.grad(logp, [e1], u)[0]
+    rest = torch.arange(150, device="cuda") != 3
+    want = run(0.0, 0.0)
+    assert torch.isfinite(want[1]).all()
+    for bad, g3 in ((float("nan"), 1.0), (float("inf"), 1.0), (0.0, float("inf")), (0.0, float("nan"))):
+        got = run(bad, g3)
+        assert torch.equal(got[0][rest], want[0][rest]) and torch.equal(got[1][rest], want[1][rest])
+        assert not torch.isfinite(got[1][3]).any() or bad == 0.0
 
 
 def test_a_run_of_all_operators_together():

@@ -451,3 +451,27 @@ def test_backward_twice_and_accumulation():
     with torch.no_grad():
         again = mlx_cce.policy_loss(x, old, adv, mask=mask, cu_seqlens=cu)
     assert not again.requires_grad and torch.equal(again, loss.detach())
+
+
+def test_tokens_that_are_not_finite_stay_in_their_sequence():
+    b = batch(9000, 8, seed=92)
+    adv = torch.ones(8, device="cuda")
+    cu = cuda_cu(b["cu"])
+    first, last = b["cu"][2], b["cu"][3]
+    assert last - first > 3
+    def run(bad):
+        x = b["logp"].clone()
+        x[first + 1] = bad
+        x = x.cuda().requires_grad_(True)
+        p = mlx_cce.policy_loss(x, b["old"].cuda(), adv, ref_logp=b["ref"].cuda(), cu_seqlens=cu, kl_coef=0.1,
+                                reduction="none")
+        q = mlx_cce.preference_loss(x, b["ref"].cuda(), cu_seqlens=cu, reduction="none")
+        return p.detach(), q.detach(), *torch.autograd.grad(p.sum() + q.sum(), [x])
+    want, got = run(-1.0), run(float("nan"))
+    at = torch.arange(9000, device="cuda")
+    other_tokens, other_pairs = at != first + 1, torch.arange(4, device="cuda") != 2
+    outside = (at < first) | (at >= last)
+    outside &= (at < b["cu"][6]) | (at >= b["cu"][7])   # (the rejected sequence of the same pair)
+    assert torch.equal(got[0][other_tokens], want[0][other_tokens]) and torch.isnan(got[0][first + 1])
+    assert torch.equal(got[1][other_pairs], want[1][other_pairs]) and torch.isnan(got[1][2])
+    assert torch.equal(got[2][outside], want[2][outside])
