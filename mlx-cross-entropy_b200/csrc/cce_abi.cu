@@ -1245,29 +1245,22 @@ RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t D, int64_t V, int64_t K, in
 // bounds) and K splits of grad_e.
 struct RowsPlan {
   int64_t vc;
-  int slabs;
+  cce::SlabPlan slabs;
 };
 
-// K splits of grad_e over a chunk of vc vocabulary rows, the one whose estimate is
-// least: whole waves of (128 rows, 256 columns, K / splits) units over 148 SMs, at
-// 0.27 us per 64-row K-block and pass and 4 us for a unit's start and output, and
-// 8 bytes of slab traffic per value at 4 TB/s.  331 x 1024 x 32000: 12 tiles in
-// one split are 135 us, in 12 splits 16 us and 4 us of slabs.
-int rows_slabs(int64_t N, int64_t D, int64_t vc, int dtype) {
-  const int64_t tiles = cce::ceil_div(N, 128) * cce::ceil_div(D, 256);
-  const int64_t kb = cce::ceil_div(vc, 64), passes = dtype == CCE_F32 ? 3 : 1;
-  int best = 1;
-  double least = 1e30;
-  for (int s = 1; s <= 32; ++s) {
-    if (s > 1 && (s * N * D * 4 > (256ll << 20) || kb < 2 * s)) break;
-    const double waves = (double)cce::ceil_div(tiles * s, 148);
-    const double us = waves * (0.27 * (double)(cce::ceil_div(kb, s) * passes) + 4.0) + (double)(s * N * D) * 8.0 / 4e6;
-    if (us < 0.97 * least) {
-      least = us;
-      best = s;
-    }
-  }
-  return best;
+// Room for up to 8 waves of units (a fixed 155 MB), 32 splits of a small batch's rows.
+cce::SlabPlan slab_plan(int64_t N, int64_t D, int64_t vc, int dtype) {
+  const int64_t tiles = cce::ceil_div(N, 128), kb = cce::ceil_div(vc, 64);
+  cce::SlabPlan p{};
+  p.num_n = (int)cce::ceil_div(D, 256);
+  p.kb = (int)kb;
+  p.passes = dtype == CCE_F32 ? 3 : 1;
+  p.cols = D;
+  const int64_t most = tiles * (kb / 2 < 1 ? 1 : kb / 2 < cce::SlabPlan::kMost ? kb / 2 : cce::SlabPlan::kMost);
+  int64_t cap = 8 * 148 / p.num_n;
+  if (cap > most) cap = most;
+  p.cap = (int)(cap < tiles ? tiles : cap);
+  return p;
 }
 
 RowsPlan rows_plan(int64_t N, int64_t D, int64_t V, int dtype) {
@@ -1288,7 +1281,7 @@ RowsPlan rows_plan(int64_t N, int64_t D, int64_t V, int dtype) {
   }
   const int64_t vmax = cce::round_up(V, 256);
   if (p.vc > vmax) p.vc = vmax;
-  p.slabs = rows_slabs(n, D, p.vc, dtype);
+  p.slabs = slab_plan(n, D, p.vc, dtype);
   return p;
 }
 
@@ -1308,7 +1301,7 @@ RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, in
   w.c = rows_c(p, N, D, V, dtype);
   w.dl = p.take<uint16_t>((size_t)N * pl.vc);
   if (dtype == CCE_F32) w.dl_lo = p.take<uint16_t>((size_t)N * pl.vc);
-  if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)pl.slabs * N * dout);
+  if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)pl.slabs.cap * 128 * dout);
   if (dtype != CCE_BF16) w.scale = p.take<float>(2);
   if (flags & CCE_NEED_DBIAS) w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * pl.vc);
   if ((flags & CCE_NEED_DC) && dout != D) w.grad_c = p.take<char>((size_t)V * dout * dtype_size(dtype));
@@ -1401,7 +1394,7 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
     if (need_de) {
       CCE_CUDA_CHECK(cce::tc_grad_e_rows(a, w.slabs, pl.slabs, a.vc0 > 0, se), what);
       if (a.vc0 + pl.vc >= a.V)
-        CCE_CUDA_CHECK(cce::launch_rows_scatter(w.slabs, pl.slabs, a.Dout, v.R.pos, a.N, D, a.dtype, grad_e, se), what);
+        CCE_CUDA_CHECK(cce::launch_rows_scatter(w.slabs, pl.slabs, a.Dout, v.R, a.N, D, a.dtype, grad_e, se), what);
     }
     if (need_dc) {
       CCE_CUDA_CHECK(cce::tc_grad_c_rows(a, gc, sc), what);

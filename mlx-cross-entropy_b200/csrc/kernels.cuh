@@ -5,8 +5,11 @@
 
 #include "common.cuh"
 #include "peer.cuh"
+#include "schedule.cuh"
 
 namespace cce {
+
+using tc::SlabPlan;
 
 // Counts one kernel launch (cce_launch_count) and returns cudaGetLastError().
 cudaError_t launched();
@@ -169,9 +172,9 @@ cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_
                                 const RowsView& R, const TopkView& topk, const float* p, const float* rest,
                                 int reduction, float* lse_rest, float* A, DistillSum* sums, float* loss, float* weight,
                                 cudaStream_t stream);
-// out[n] = sum over the slabs [N][ld] of row pos[n], in order; 0 where pos[n] < 0
-cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, int64_t ld, const int32_t* pos, int64_t N, int64_t D,
-                                int dtype, void* out, cudaStream_t stream);
+// out[n] = sum over the K splits' slabs (rows of ld values) of row pos[n], in order; 0 where pos[n] < 0
+cudaError_t launch_rows_scatter(const float* slabs, const SlabPlan& plan, int64_t ld, const RowsView& R, int64_t N,
+                                int64_t D, int dtype, void* out, cudaStream_t stream);
 // out = {s, 1 / s}, s the power of two >= the largest |d| of the rows, times 2^-14
 cudaError_t launch_rows_scale(const Cotangent& up, const RowsView& R, float* out, cudaStream_t stream);
 // largest |x| of the rows (those of R, if given) as the bits of a float, into *word (zeroed)
@@ -236,8 +239,9 @@ cudaError_t tc_selftest_wait(uint64_t limit_ns, int code, cudaStream_t stream);
 bool tc_available();  // the driver's tensor-map encoder was found
 cudaError_t tc_logits(const RowsGemmArgs& a, cudaStream_t stream);
 cudaError_t tc_dlogits_rows(const RowsGemmArgs& a, cudaStream_t stream);
-// slabs[num_slabs][N][Dout] (+)= the K splits of dl c (fp32)
-cudaError_t tc_grad_e_rows(const RowsGemmArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t stream);
+// slabs[plan.cap 128][Dout] (+)= the K splits of dl c (fp32)
+cudaError_t tc_grad_e_rows(const RowsGemmArgs& a, float* slabs, const SlabPlan& plan, bool accumulate,
+                           cudaStream_t stream);
 // grad_c rows [vc0, vc0 + vc_len) = dl^T e, row stride Dout
 cudaError_t tc_grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t stream);
 

@@ -457,14 +457,16 @@ __global__ void __launch_bounds__(1024) rows_scale_kernel(const Cotangent up, co
   }
 }
 
-// grad_e row n = the slabs' rows pos[n] added in order, 0 for rows that do not
+// grad_e row n = row pos[n] of each K split's slab added in order, 0 for rows that do not
 // count; a warp per row and 128 columns (few rows with many slabs need the width).
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(256)
-rows_scatter_kernel(const float* __restrict__ slabs, int num, int64_t ld, const int32_t* __restrict__ pos, int64_t N,
+rows_scatter_kernel(const float* __restrict__ slabs, const SlabPlan plan, int64_t ld, const RowsView R, int64_t N,
                     int64_t D, T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
-  const int64_t stride = N * ld;
+  const int32_t* pos = R.pos;
+  const int64_t tiles = ceil_div(*R.count, 128), stride = tiles * 128 * ld;
+  const int num = plan.warp_splits((int)tiles);
   const int64_t pieces = ceil_div(D, 128), items = N * pieces;
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < items; i += (int64_t)gridDim.x * 8) {
     const int64_t n = i / pieces, k0 = (i - n * pieces) * 128;
@@ -676,22 +678,22 @@ cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_
 }
 
 template <typename T>
-static cudaError_t scatter(const float* slabs, int num, int64_t ld, const int32_t* pos, int64_t N, int64_t D, void* out,
-                           cudaStream_t s) {
+static cudaError_t scatter(const float* slabs, const SlabPlan& plan, int64_t ld, const RowsView& R, int64_t N, int64_t D,
+                           void* out, cudaStream_t s) {
   const unsigned grid = warps_grid(N * ceil_div(D, 128));
   if (D % 4 == 0 && ld % 4 == 0 && aligned16(slabs) && aligned16(out))
-    rows_scatter_kernel<T, true><<<grid, 256, 0, s>>>(slabs, num, ld, pos, N, D, static_cast<T*>(out));
+    rows_scatter_kernel<T, true><<<grid, 256, 0, s>>>(slabs, plan, ld, R, N, D, static_cast<T*>(out));
   else
-    rows_scatter_kernel<T, false><<<grid, 256, 0, s>>>(slabs, num, ld, pos, N, D, static_cast<T*>(out));
+    rows_scatter_kernel<T, false><<<grid, 256, 0, s>>>(slabs, plan, ld, R, N, D, static_cast<T*>(out));
   return launched();
 }
 
-cudaError_t launch_rows_scatter(const float* slabs, int num_slabs, int64_t ld, const int32_t* pos, int64_t N, int64_t D,
-                                int dtype, void* out, cudaStream_t s) {
+cudaError_t launch_rows_scatter(const float* slabs, const SlabPlan& plan, int64_t ld, const RowsView& R, int64_t N,
+                                int64_t D, int dtype, void* out, cudaStream_t s) {
   switch (dtype) {
-    case CCE_F32: return scatter<float>(slabs, num_slabs, ld, pos, N, D, out, s);
-    case CCE_F16: return scatter<__half>(slabs, num_slabs, ld, pos, N, D, out, s);
-    case CCE_BF16: return scatter<__nv_bfloat16>(slabs, num_slabs, ld, pos, N, D, out, s);
+    case CCE_F32: return scatter<float>(slabs, plan, ld, R, N, D, out, s);
+    case CCE_F16: return scatter<__half>(slabs, plan, ld, R, N, D, out, s);
+    case CCE_BF16: return scatter<__nv_bfloat16>(slabs, plan, ld, R, N, D, out, s);
   }
   return cudaErrorInvalidValue;
 }

@@ -63,6 +63,39 @@ struct Sched {
   }
 };
 
+// K splits of grad_e over a batch's packed rows, whose number t of 128-row tiles
+// only the device knows: the s with the least estimate, in ns.  Whole waves of
+// (128 rows, 256 columns, K / s) units over 148 SMs, 270 ns per 64-row K-block and
+// pass and 4 us for a unit's start and output; 8 bytes of slab traffic per value
+// at 4 TB/s.  331 x 1024 x 32000: 12 tiles in one split are 135 us, in 12 splits
+// 16 us and 4 us of slabs.  Split z of tile row m is the slabs' tile row z t + m.
+struct SlabPlan {
+  int cap;       // 128-row tiles the slabs hold
+  int num_n;     // 256-column tiles
+  int kb;        // 64-row K-blocks of a chunk
+  int passes;
+  int64_t cols;
+  static constexpr int kMost = 32;
+  __host__ __device__ __forceinline__ unsigned long long cost(int s, int t) const {
+    if (s > 1 && ((int64_t)s * t > cap || kb < 2 * s)) return ~0ull >> 6;
+    const int64_t waves = ((int64_t)t * num_n * s + 147) / 148;
+    return (unsigned long long)(waves * (270ll * passes * ((kb + s - 1) / s) + 4000) + (int64_t)s * t * cols * 128 / 500);
+  }
+#ifdef __CUDACC__
+  // The best s, by a whole warp.
+  __device__ __forceinline__ int warp_splits(int t) const {
+    const unsigned lane = threadIdx.x & 31u;
+    unsigned long long x = cost((int)lane + 1, t) << 5 | lane;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, o);
+      x = y < x ? y : x;
+    }
+    return (int)(x & 31u) + 1;
+  }
+#endif
+};
+
 // Fast-dimension group size: all blocks when that operand fits comfortably in
 // L2 (it is then read from DRAM once however the tiles are ordered), else 16.
 __host__ __device__ inline int raster_group(int64_t fast_operand_bytes) {

@@ -1590,9 +1590,9 @@ cudaError_t tc_dlogits_rows(const RowsGemmArgs& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-cudaError_t tc_grad_e_rows(const RowsGemmArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
-  return a.dtype == CCE_F32 ? grad_e_rows<true>(a, slabs, num_slabs, accumulate, s)
-                            : grad_e_rows<false>(a, slabs, num_slabs, accumulate, s);
+cudaError_t tc_grad_e_rows(const RowsGemmArgs& a, float* slabs, const SlabPlan& plan, bool accumulate, cudaStream_t s) {
+  return a.dtype == CCE_F32 ? grad_e_rows<true>(a, slabs, plan, accumulate, s)
+                            : grad_e_rows<false>(a, slabs, plan, accumulate, s);
 }
 
 cudaError_t tc_grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t s) {

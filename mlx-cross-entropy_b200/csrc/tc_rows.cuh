@@ -62,13 +62,14 @@ struct RowsSched {
   int m_rows, k_rows;    // M / K runs over the rows
   int num_m, num_n, num_kb, ksplit, m_fast, group;
   int b3d = 1;           // MN-major B as one 3-D box (else one 2-D box per 64 columns)
+  SlabPlan slabs{};      // cap > 0: K splits by the rows that count
   __device__ __forceinline__ Sched get(int64_t& count) const {
     count = min((int64_t)__ldg(rows), N);
     Sched s{};
     s.num_m = m_rows ? (int)ceil_div(count, BM) : num_m;
     s.num_n = num_n;
     s.num_kb = k_rows ? (int)ceil_div(count, BK) : num_kb;
-    s.ksplit = ksplit;
+    s.ksplit = slabs.cap > 0 ? slabs.warp_splits(s.num_m) : ksplit;
     s.m_fast = m_fast;
     s.group = group;
     return s;
@@ -348,7 +349,7 @@ struct Out16Epi {
   }
 };
 
-// out[ks][row][col] (+)= f1 f2 (A B), float32
+// out[row][col] (+)= f1 f2 (A B), float32; K split ks behind ks times the row tiles
 struct OutEpi {
   static constexpr bool kStores = true, kExact = false;
   const float *f1, *f2;
@@ -361,6 +362,7 @@ struct OutEpi {
   __device__ __forceinline__ void begin(State&, const TileAt&) const {}
   __device__ __forceinline__ void finish(State&, float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
     const float f = (f1 ? *f1 : 1.f) * (f2 ? *f2 : 1.f);
+    const int y = t.ks * (int)round_up(t.rows, BM) + t.y0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t col = t.col0 + c * 32;
@@ -368,7 +370,7 @@ struct OutEpi {
       float(&v)[32] = *reinterpret_cast<float(*)[32]>(z + c * 32);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= f;
-      sg.store_f32(v, (int)col, t.y0, t.ks, add != 0);
+      sg.store_f32(v, (int)col, y, 0, add != 0);
     }
   }
 };
@@ -659,11 +661,11 @@ cudaError_t dlogits2_dispatch(const RowsGemmArgs& a, cudaStream_t s) {
   return a.topk.sid ? dlogits2_types<TB, true>(a, s) : dlogits2_types<TB, false>(a, s);
 }
 
-// float32 [z][rows][ld] output of D columns, written in (16 x 32 x 1) boxes
-bool make_tmap_f32(CUtensorMap* tm, const float* out, int64_t D, int64_t ld, int64_t rows, int64_t slabs) {
+// float32 [rows][ld] output of D columns, written in (16 x 32 x 1) boxes
+bool make_tmap_f32(CUtensorMap* tm, const float* out, int64_t D, int64_t ld, int64_t rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)slabs};
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)rows, 1};
   cuuint64_t strides[2] = {(cuuint64_t)(ld * 4), (cuuint64_t)(rows * ld * 4)};
   cuuint32_t box[3] = {16, 32, 1};
   cuuint32_t estr[3] = {1, 1, 1};
@@ -673,24 +675,23 @@ bool make_tmap_f32(CUtensorMap* tm, const float* out, int64_t D, int64_t ld, int
 }
 
 template <bool kSplit>
-cudaError_t grad_e_rows(const RowsGemmArgs& a, float* slabs, int num_slabs, bool accumulate, cudaStream_t s) {
+cudaError_t grad_e_rows(const RowsGemmArgs& a, float* slabs, const SlabPlan& plan, bool accumulate, cudaStream_t s) {
   const bool bf16 = a.dtype == CCE_BF16;
   const int64_t off = a.vc0 * a.Dk;
   RowsMaps m;
   int b3d = 0;
   bool ok = make_tmap(&m.A, a.dl, bf16, a.vc_len, a.N, a.vc_ld, BK, BM) &&
             make_tmap_mn(&m.B, static_cast<const uint16_t*>(a.c) + off, bf16, a.Dk, a.vc_len, a.Dk, BN / 64, &b3d) &&
-            make_tmap_f32(&m.C, slabs, a.Dout, a.Dout, a.N, num_slabs);
+            make_tmap_f32(&m.C, slabs, a.Dout, a.Dout, (int64_t)plan.cap * BM);
   m.A2 = m.A, m.B2 = m.B, m.C2 = m.C;
   if (kSplit)
     ok = ok && make_tmap(&m.A2, a.dl_lo, bf16, a.vc_len, a.N, a.vc_ld, BK, BM) &&
          make_tmap_mn(&m.B2, static_cast<const uint16_t*>(a.c_lo) + off, bf16, a.Dk, a.vc_len, a.Dk, BN / 64, &b3d);
   if (!ok) return cudaErrorInvalidValue;
-  const int num_n = (int)ceil_div(a.Dout, BN);
-  const RowsSched rs{a.R.count, a.N, 1, 0, 0, num_n, (int)ceil_div(a.vc_len, BK), num_slabs, 1,
-                     raster_group(a.N * a.vc_len * 2), b3d};
+  const RowsSched rs{a.R.count, a.N, 1, 0, 0, plan.num_n, (int)ceil_div(a.vc_len, BK), 1, 1,
+                     raster_group(a.N * a.vc_len * 2), b3d, plan};
   const OutEpi epi{a.scale, kSplit ? a.sc + 1 : nullptr, accumulate ? 1 : 0, a.N, a.Dout, 2};
-  return rows_gemm<false, true, kSplit>(m, rs, epi, bf16, ceil_div(a.N, BM) * num_n * num_slabs, s);
+  return rows_gemm<false, true, kSplit>(m, rs, epi, bf16, (int64_t)plan.cap * plan.num_n, s);
 }
 
 // grad_c rows of the chunk.  T: the output's type (float with split operands)
@@ -707,7 +708,7 @@ cudaError_t grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t s) {
   if constexpr (kSplit)
     ok = ok && make_tmap_mn3d(&m.A2, a.dl_lo, bf16, cols, a.N, a.vc_ld, BK, BM / 64) &&
          make_tmap_mn(&m.B2, a.e_lo, bf16, a.Dk, a.N, a.Dk, BN / 64, &b3d) &&
-         make_tmap_f32(&m.C, out, a.Dout, a.Dout, a.vc_len, 1);
+         make_tmap_f32(&m.C, out, a.Dout, a.Dout, a.vc_len);
   else
     ok = ok && make_tmap_out(&m.C, out, a.dtype, a.Dout, a.vc_len, a.Dout);
   if (!ok) return cudaErrorInvalidValue;
