@@ -424,7 +424,9 @@ CCE_API int cce_preference_loss_backward(const float* coef, const float* grad_lo
  * two levels to float32 accuracy, and the gradients are exact (no filter).
  *
  * A forward call fills `saved` (cce_*_saved_bytes), which the backward call of
- * the same sizes reads; c and bias must not have changed in between.
+ * the same sizes reads; c and bias must not have changed in between.  It holds the
+ * packed rows of e and, for float32 and for widths that the tensor cores cannot
+ * read in place, a converted copy of c.
  * --------------------------------------------------------------------------- */
 
 CCE_API size_t cce_logp_saved_bytes(int64_t N, int64_t D, int64_t V, int dtype);

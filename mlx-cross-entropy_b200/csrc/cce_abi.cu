@@ -1126,14 +1126,21 @@ struct Parts {
 
 // Widths of the GEMMs' operands and outputs: rows start on 16-byte boundaries
 // (TMA), float16 parts of float32 fill whole 64-column blocks.  Other widths run
-// on padded copies; so do many rows of a width whose rows straddle 128-byte
-// lines (D = 1032, V = 50021, bfloat16: a copy of c costs 60 us and saves 30 at
-// 1024 rows and more above, at 512 rows it loses 15).
-constexpr int64_t kPadRows = 1024;
+// on padded copies, made once by the forward call; so do batches of kPadRows and
+// more of a width whose rows straddle 128-byte lines, which double the L2 requests
+// of a load (D = 1032, V = 50021, bfloat16, forward and backward without / with the
+// copy: 227 / 248 us at 256 rows, 350 / 330 at 512, 606 / 541 at 1024).
+constexpr int64_t kPadRows = 384;
 int64_t rows_dk(int64_t N, int64_t D, int dtype) {
   return cce::round_up(D, dtype == CCE_F32 || N >= kPadRows ? 64 : 8);
 }
 int64_t rows_dout(int64_t D, int dtype) { return cce::round_up(D, dtype == CCE_F32 ? 4 : 8); }
+
+// c as an operand: itself, a padded copy, or float16 parts with their scale.
+struct RowsC {
+  void *c, *c_lo;
+  float* sc;
+};
 
 // What the forward calls leave for the backward calls.
 struct RowsSaved {
@@ -1145,6 +1152,7 @@ struct RowsSaved {
   float* se;        // float32: scale of e's parts
   uint32_t* words;  // float32: largest values of c and e
   void *e, *e_lo;   // packed rows [N][Dk]
+  RowsC c;          // [V][Dk], where c itself is not the operand
   size_t bytes;
 };
 
@@ -1171,55 +1179,41 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
     r.e_lo = p.take<uint16_t>(n);
     r.se = p.take<float>(2);
     r.words = p.take<uint32_t>(2);
+    r.c.sc = p.take<float>(2);
   }
+  const size_t nc = (size_t)V * rows_dk(N, D, dtype);
+  if (dtype == CCE_F32 || rows_dk(N, D, dtype) != D) r.c.c = p.take<uint16_t>(nc);
+  if (dtype == CCE_F32) r.c.c_lo = p.take<uint16_t>(nc);
   r.bytes = p.used;
   return r;
 }
 
-// c as an operand: itself, a padded copy, or float16 parts with their scale.
-struct RowsC {
-  void *c, *c_lo;
-  float* sc;
-};
-
-RowsC rows_c(Parts& p, int64_t N, int64_t D, int64_t V, int dtype) {
-  RowsC w{};
-  const size_t n = (size_t)V * rows_dk(N, D, dtype);
-  if (dtype == CCE_F32) {
-    w.sc = p.take<float>(2);
-    w.c = p.take<uint16_t>(n);
-    w.c_lo = p.take<uint16_t>(n);
-  } else if (rows_dk(N, D, dtype) != D) {
-    w.c = p.take<uint16_t>(n);
-  }
-  return w;
+// The operands' part of the GEMM arguments.
+void rows_operands(cce::RowsGemmArgs& a, const RowsSaved& v, const void* c) {
+  a.e = v.e, a.e_lo = v.e_lo, a.se = v.se;
+  a.c = v.c.c ? v.c.c : c, a.c_lo = v.c.c_lo, a.sc = v.c.sc;
 }
 
-// The operands' part of the GEMM arguments.  e != nullptr (the forward call):
-// its packed rows go to the saved copy first.
-cudaError_t rows_operands(cce::RowsGemmArgs& a, const RowsSaved& v, const RowsC& w, const void* e, const void* c,
-                          int64_t D, cudaStream_t s) {
-  a.e = v.e, a.e_lo = v.e_lo, a.se = v.se;
-  a.c = w.c ? w.c : c, a.c_lo = w.c_lo, a.sc = w.sc;
+// The forward call's copies: the packed rows of e, and c where it is not an operand.
+cudaError_t rows_copies(const RowsSaved& v, const void* e, const void* c, int64_t N, int64_t D, int64_t V, int dtype,
+                        cudaStream_t s) {
+  const int64_t Dk = rows_dk(N, D, dtype);
   cudaError_t err = cudaSuccess;
-  if (a.dtype == CCE_F32) {
-    if (e) {
-      if ((err = cudaMemsetAsync(v.words, 0, 2 * sizeof(uint32_t), s)) != cudaSuccess) return err;
-      if ((err = cce::launch_absmax((const float*)c, a.V, D, nullptr, v.words, s)) != cudaSuccess) return err;
-      if ((err = cce::launch_absmax((const float*)e, a.N, D, &v.R, v.words + 1, s)) != cudaSuccess) return err;
-      if ((err = cce::launch_split((const float*)e, a.N, D, a.Dk, &v.R, v.words + 1, v.se, v.e, v.e_lo, s)) != cudaSuccess)
-        return err;
-    }
-    return cce::launch_split((const float*)c, a.V, D, a.Dk, nullptr, v.words, w.sc, w.c, w.c_lo, s);
+  if (dtype != CCE_F32) {
+    if ((err = cce::launch_rows_copy(e, N, D, D, &v.R, v.e, Dk, s)) != cudaSuccess) return err;
+    return v.c.c ? cce::launch_rows_copy(c, V, D, D, nullptr, v.c.c, Dk, s) : cudaSuccess;
   }
-  if (e && (err = cce::launch_rows_copy(e, a.N, D, D, &v.R, v.e, a.Dk, s)) != cudaSuccess) return err;
-  return w.c ? cce::launch_rows_copy(c, a.V, D, D, nullptr, w.c, a.Dk, s) : cudaSuccess;
+  if ((err = cudaMemsetAsync(v.words, 0, 2 * sizeof(uint32_t), s)) != cudaSuccess) return err;
+  if ((err = cce::launch_absmax((const float*)c, V, D, nullptr, v.words, s)) != cudaSuccess) return err;
+  if ((err = cce::launch_absmax((const float*)e, N, D, &v.R, v.words + 1, s)) != cudaSuccess) return err;
+  if ((err = cce::launch_split((const float*)e, N, D, Dk, &v.R, v.words + 1, v.se, v.e, v.e_lo, s)) != cudaSuccess)
+    return err;
+  return cce::launch_split((const float*)c, V, D, Dk, nullptr, v.words, v.c.sc, v.c.c, v.c.c_lo, s);
 }
 
 struct RowsFwdWs {
   float *part_m, *part_s, *tgt, *p, *rest;
   cce::DistillSum* sums;
-  RowsC c;
   size_t bytes;
 };
 
@@ -1236,7 +1230,6 @@ RowsFwdWs rows_fwd_ws(void* base, int64_t N, int64_t D, int64_t V, int64_t K, in
     w.rest = p.take<float>(N);
     w.sums = p.take<cce::DistillSum>(cce::distill_blocks(N));
   }
-  w.c = rows_c(p, N, D, V, dtype);
   w.bytes = p.used;
   return w;
 }
@@ -1286,7 +1279,6 @@ RowsPlan rows_plan(int64_t N, int64_t D, int64_t V, int dtype) {
 }
 
 struct RowsBwdWs {
-  RowsC c;
   void *dl, *dl_lo;
   float *slabs, *scale, *bias_part;
   void* grad_c;  // padded rows
@@ -1298,7 +1290,6 @@ RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, in
   RowsBwdWs w{};
   const RowsPlan pl = rows_plan(N, D, V, dtype);
   const int64_t dout = rows_dout(D, dtype);
-  w.c = rows_c(p, N, D, V, dtype);
   w.dl = p.take<uint16_t>((size_t)N * pl.vc);
   if (dtype == CCE_F32) w.dl_lo = p.take<uint16_t>((size_t)N * pl.vc);
   if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)pl.slabs.cap * 128 * dout);
@@ -1361,7 +1352,7 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
   const bool need_de = flags & CCE_NEED_DE, need_dc = flags & CCE_NEED_DC, need_db = flags & CCE_NEED_DBIAS;
   if (!need_de && !need_dc && !need_db) return CCE_OK;
   const RowsPlan pl = rows_plan(a.N, D, a.V, a.dtype);
-  CCE_CUDA_CHECK(rows_operands(a, v, w.c, nullptr, c, D, s), what);
+  rows_operands(a, v, c);
   a.R = v.R, a.topk = v.topk, a.lse = v.lse, a.A = v.A;
   a.dl = w.dl, a.dl_lo = w.dl_lo, a.vc_ld = pl.vc, a.scale = w.scale;
   a.bias_part = need_db ? w.bias_part : nullptr;
@@ -1481,7 +1472,8 @@ int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dt
                  what);
   cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
   a.R = v.R, a.part_m = w.part_m, a.part_s = w.part_s, a.tgt = w.tgt;
-  CCE_CUDA_CHECK(rows_operands(a, v, w.c, e, c, D, s), what);
+  CCE_CUDA_CHECK(rows_copies(v, e, c, N, D, V, dtype, s), what);
+  rows_operands(a, v, c);
   CCE_CUDA_CHECK(cce::tc_logits(a, s), what);
   CCE_CUDA_CHECK(cce::launch_rows_logp(w.part_m, w.part_s, cce::ceil_div(V, 128), N, v.R, w.tgt, v.lse, logp, s), what);
   return CCE_OK;
@@ -1562,7 +1554,8 @@ int cce_distill_forward(const void* e, const void* c, const void* bias, int bias
   cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
   a.R = v.R, a.topk = v.topk, a.part_m = w.part_m, a.part_s = w.part_s;
   a.scale_z = (float)(1.0 / params->temperature);
-  CCE_CUDA_CHECK(rows_operands(a, v, w.c, e, c, D, s), what);
+  CCE_CUDA_CHECK(rows_copies(v, e, c, N, D, V, dtype, s), what);
+  rows_operands(a, v, c);
   CCE_CUDA_CHECK(cce::tc_logits(a, s), what);
   CCE_CUDA_CHECK(cce::launch_distill_rows(w.part_m, w.part_s, cce::ceil_div(V, 128), N, V, v.R, v.topk, w.p, w.rest,
                                           red, v.lse, v.A, w.sums, loss, v.weight, s),

@@ -90,28 +90,44 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// v += bias[cb, cb + 32), nothing behind column V.  Whole chunks come in 16-byte
-// loads (the same for all lanes) where the bias is aligned.
-template <typename TB>
-__device__ __forceinline__ void add_bias(const void* bias, int64_t cb, int64_t V, float* v) {
-  if constexpr (!std::is_void<TB>::value) {
-    constexpr int kPer = 16 / (int)sizeof(TB);
-    const TB* p = static_cast<const TB*>(bias) + cb;
-    if (cb + 32 <= V && (reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+// The bias of a warp's 128 columns: four of them per lane, loaded before the tile's
+// products are waited for, and added through the warp's staging area (reads of one
+// address by all lanes); with loads beside the adds the logits took 85 instead of
+// 80 us, the dlogits 93 instead of 91 (900 rows, D = 1088, V = 50021).
+struct Bias128 {
+  float b[4];
+  template <typename TB>
+  __device__ __forceinline__ void load(const void* bias, int64_t col0, int64_t V) {
+    if constexpr (!std::is_void<TB>::value) {
+      const TB* p = static_cast<const TB*>(bias);
+      const int64_t c = col0 + 4 * (threadIdx.x & 31);
 #pragma unroll
-      for (int i = 0; i < 32 / kPer; ++i) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        const TB* b = reinterpret_cast<const TB*>(&x);
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) v[i * kPer + j] += to_f32(b[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (cb + j < V) v[j] += to_f32(__ldg(p + j));
+      for (int j = 0; j < 4; ++j) b[j] = c + j < V ? to_f32(__ldg(p + c + j)) : 0.f;
     }
   }
-}
+  // z = us z + bias
+  template <typename TB, bool kScaled>
+  __device__ __forceinline__ void add(float (&z)[128], float us, const Stager& sg) const {
+    if constexpr (!std::is_void<TB>::value) {
+      sg.acquire<0>();
+      float4* buf = reinterpret_cast<float4*>(sg.buf);
+      buf[threadIdx.x & 31] = make_float4(b[0], b[1], b[2], b[3]);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float4 x = buf[j];
+        z[4 * j] = (kScaled ? z[4 * j] * us : z[4 * j]) + x.x;
+        z[4 * j + 1] = (kScaled ? z[4 * j + 1] * us : z[4 * j + 1]) + x.y;
+        z[4 * j + 2] = (kScaled ? z[4 * j + 2] * us : z[4 * j + 2]) + x.z;
+        z[4 * j + 3] = (kScaled ? z[4 * j + 3] * us : z[4 * j + 3]) + x.w;
+      }
+      __syncwarp();
+    } else if constexpr (kScaled) {
+#pragma unroll
+      for (int j = 0; j < 128; ++j) z[j] *= us;
+    }
+  }
+};
 
 // 1 / (s_a s_b) of split operands, 1 for whole ones: s[1] = 1 / s[0]
 __device__ __forceinline__ float unscale(const float* a, const float* b) { return a ? a[1] * b[1] : 1.f; }
@@ -134,32 +150,30 @@ struct LogitsEpi {
 
   struct State {
     int64_t tl;  // the target's place in this half
+    Bias128 bias;
     typename std::conditional<kTopk, TopkCursor, NoCursor>::type cur;
   };
   __device__ __forceinline__ void begin(State& st, const TileAt& t) const {
     const bool live = t.row < t.rows;
+    st.bias.template load<TB>(bias, t.col0, V);
     st.tl = -1;
     if constexpr (kTopk) st.cur.open(topk, t.row, live, t.col0 / kTopkTile);
     else if (live) st.tl = (int64_t)targets[t.row] - t.col0;
   }
 
-  __device__ __forceinline__ void finish(State& st, float (&z)[128], const TileAt& t, Stager&, const CUtensorMap*) const {
+  __device__ __forceinline__ void finish(State& st, float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
     const bool live = t.row < t.rows;
     const int64_t tl = st.tl;
     // The maximum is kept of the unscaled values; exponents are differences to
     // it first, exact next to the maximum, then one product with scale log2 e.
     float m = -INFINITY, sum = 0.f, tz = 0.f;
     const float cexp = scale * kLog2e;
-    const float us = unscale(se, sc);
+    if (se) st.bias.template add<TB, true>(z, unscale(se, sc), sg);
+    else st.bias.template add<TB, false>(z, 1.f, sg);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t cb = t.col0 + c * 32;
       float* v = z + c * 32;
-      if (se) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= us;
-      }
-      add_bias<TB>(bias, cb, V, v);
       if (cb + 32 > V) {
         const int left = (int)(V - cb);
 #pragma unroll
@@ -239,12 +253,14 @@ struct DlogitsEpi2 {
   struct State {
     int64_t tl;      // the target's place in this half
     float G, L, dr;  // dlogits are G e^(z - L); dr: d
+    Bias128 bias;
     typename std::conditional<kTopk, TopkCursor, NoCursor>::type cur;
   };
   __device__ __forceinline__ void begin(State& st, const TileAt& t) const {
     const bool live = t.row < t.rows;
     const int64_t v0 = vc0 + t.col0;
     const float d = live ? up.of(t.row, row_of) : 0.f;
+    st.bias.template load<TB>(bias, v0, vc_end);
     st.L = live ? lse[t.row] : INFINITY;
     st.dr = d * (scale ? scale[1] : 1.f);
     st.tl = -1;
@@ -263,16 +279,11 @@ struct DlogitsEpi2 {
     const float G = st.G, L = st.L, dr = st.dr;
     const int64_t v0 = vc0 + t.col0;  // vocabulary id of column 0
     const int64_t tl = st.tl;
-    const float us = unscale(se, sc);
+    st.bias.template add<TB, kSplit>(z, kSplit ? unscale(se, sc) : 1.f, sg);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t cb = v0 + c * 32;
       float(&v)[32] = *reinterpret_cast<float(*)[32]>(z + c * 32);
-      if constexpr (kSplit) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= us;
-      }
-      add_bias<TB>(bias, cb, vc_end, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = G * ex2((v[j] * scale_z - L) * kLog2e);
       if constexpr (kTopk) {

@@ -97,9 +97,12 @@ def test_saved_and_workspace_sizes():
     # a bounded chunk of the dlogits (never [N, V]) and fp32 slabs of grad_e
     rows = lib.cce_logp_backward_workspace_bytes(N, D, V, _ext.CCE_BF16, flags)
     assert N * D * 4 <= rows < N * V * 2 / 2 + (256 << 20)
-    # float32: both parts of c as well
-    f32 = lib.cce_logp_backward_workspace_bytes(N, D, V, _ext.CCE_F32, flags)
-    assert V * D * 4 < f32 < V * D * 4 + 3 * (1 << 29)
+    # float32: both parts of e and c, made once by the forward call
+    f32 = lib.cce_logp_saved_bytes(N, D, V, _ext.CCE_F32)
+    assert (V + N) * D * 4 < f32 < (V + N) * D * 4 + 64 * N + 4096
+    # ... as is the padded copy of c of a width whose rows straddle 128-byte lines
+    pad = lib.cce_logp_saved_bytes(N, D + 8, V, _ext.CCE_BF16)
+    assert (V + N) * (D + 64) * 2 < pad < (V + N) * (D + 64) * 2 + 64 * N + 4096
     # odd widths: padded copies of c and grad_c
     odd = lib.cce_logp_backward_workspace_bytes(64, 71, 1000, _ext.CCE_BF16, flags)
     assert odd > 2 * 1000 * 72 * 2 + lib.cce_logp_backward_workspace_bytes(64, 72, 1000, _ext.CCE_BF16, flags) - 4096
