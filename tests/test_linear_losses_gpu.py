@@ -6,7 +6,8 @@ sum_k |e_k c_k|:
 
 * a logit: tensor cores add products of 16 at a time rounding towards zero (2u);
   of 16-bit inputs 16 such steps per segment, then one float32 addition per 256
-  products: dz = (16 * 2u + ceil(D / 256) u) B; of float32 inputs, each the sum of
+  products: dz = (16 * 2u + ceil(D / 256) u) B (bfloat16 runs 32 steps per segment
+  and is held to the same bound but for long vocabularies); of float32 inputs, each the sum of
   two float16 parts to 2^-22 (4u) and the parts' smallest product left out (4u),
   8 steps per segment and three additions per 128 columns: dz = (8 * 2u +
   3 * (ceil(D / 128) + 1) u + 12u) B; the bias and the temperature 2u |z| more;
@@ -623,3 +624,69 @@ def test_a_run_of_all_operators_together():
     assert abs(float(loss) - float(q["loss"] + dl)) < 2e-5
     for got, want in zip(grads, (w @ c.double(), w.t() @ e.double(), w.sum(0))):
         assert torch.all((got.cpu().double() - want).abs() <= 2e-5 * want.abs().max())
+
+
+def _free(gib):
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of free device memory")
+
+
+def test_offsets_past_32_bits_rows():
+    """N D and N V beyond 2^31: the last rows are those of a call of their own."""
+    _free(60)
+    N, D, V = 540_001, 4096, 4200
+    g = torch.Generator(device="cuda").manual_seed(100)
+    e = torch.randn(N, D, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    c = (torch.randn(V, D, generator=g, device="cuda") * 0.03).bfloat16()
+    t = torch.randint(0, V, (N,), generator=g, device="cuda")
+    t[5:-300] = torch.where(torch.rand(N - 305, generator=g, device="cuda") < 0.1, -100, t[5:-300])
+    logp = mlx_cce.linear_log_probs(e, c, t)
+    up = torch.ones(N, device="cuda")
+    (grad,) = torch.autograd.grad(logp, [e], up)
+    tail = e.detach()[-300:].clone().requires_grad_(True)
+    want = mlx_cce.linear_log_probs(tail, c, t[-300:])
+    assert torch.equal(logp.detach()[-300:], want.detach())
+    (gt,) = torch.autograd.grad(want, [tail], up[:300])
+    # the K splits differ with the number of rows: float32 sums in another order, then one rounding each
+    w = torch.softmax(tail.detach().float() @ c.float().t(), 1)
+    w[torch.arange(300, device="cuda"), t[-300:]] -= 1
+    tol = (w.abs() @ c.float().abs()) * ((V / 16 + 64) * 2 * U) + R.half_steps(torch.bfloat16, gt.float()).float() * 2
+    assert torch.all((grad[-300:].float() - gt.float()).abs() <= tol * 1.01)
+    assert (grad[5:-300][t[5:-300] == -100] == 0).all()
+    _ext.device_status()
+
+
+@pytest.mark.parametrize("D", [4096, 4104])
+def test_offsets_past_32_bits_vocabulary(D):
+    """V D beyond 2^31, in place and on the padded copy of c: against 64 bits."""
+    _free(60)
+    N, V = 400, 530_001
+    g = torch.Generator(device="cuda").manual_seed(101)
+    e = torch.randn(N, D, generator=g, device="cuda").bfloat16()
+    c = torch.empty(V, D, dtype=torch.bfloat16, device="cuda")
+    for v in range(0, V, 1 << 16):
+        c[v:v + (1 << 16)] = torch.randn(min(1 << 16, V - v), D, generator=g, device="cuda") * 0.03
+    t = torch.randint(V - 200, V, (N,), generator=g, device="cuda")
+    c.requires_grad_(True)
+    logp = mlx_cce.linear_log_probs(e, c, t)
+    (grad,) = torch.autograd.grad(logp, [c], torch.ones(N, device="cuda"))
+    e64, last = e.double(), c.detach()[-200:].double()
+    lse = torch.full((N,), -math.inf, dtype=torch.float64, device="cuda")
+    big = 0.0
+    for v in range(0, V, 20_000):
+        part = c.detach()[v:v + 20_000].double()
+        lse = torch.logaddexp(lse, torch.logsumexp(e64 @ part.t(), 1))
+        big = max(big, float((e64.abs() @ part.abs().t()).max()))
+    lq = e64 @ last.t() - lse[:, None]
+    dz = ((32 * 2 + math.ceil(D / 512)) * U) * big   # bfloat16: 32 steps a segment
+    want = lq.gather(1, (t - (V - 200))[:, None])[:, 0]
+    assert torch.all((logp.detach().double() - want).abs() <= 2 * dz + 2.0 ** -18)
+    w = -lq.exp()
+    extra = w.abs() * (2 * dz + 2.0 ** -18)
+    w[torch.arange(N, device="cuda"), t - (V - 200)] += 1
+    wa = w.abs() + extra
+    want = w.t() @ e64
+    tol = extra.t() @ e64.abs() + (wa.t() @ e64.abs()) * (2.0 ** -8 + (N / 16 + 64) * 2 * U)
+    tol = tol + R.half_steps(torch.bfloat16, want.abs().cpu() + tol.cpu()).to("cuda")
+    assert torch.all((grad[-200:].double() - want).abs() <= tol)
+    _ext.device_status()

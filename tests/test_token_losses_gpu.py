@@ -475,3 +475,24 @@ def test_tokens_that_are_not_finite_stay_in_their_sequence():
     assert torch.equal(got[0][other_tokens], want[0][other_tokens]) and torch.isnan(got[0][first + 1])
     assert torch.equal(got[1][other_pairs], want[1][other_pairs]) and torch.isnan(got[1][2])
     assert torch.equal(got[2][outside], want[2][outside])
+
+
+def test_as_many_tokens_as_offsets_can_count():
+    """2^31 - 8 tokens in two sequences: every gradient, and the sum."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GiB of free device memory")
+    n, last = 2 ** 31 - 8, 92
+    x = torch.zeros(n, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    cu = torch.tensor([0, n - last, n], dtype=torch.int32, device="cuda")
+    adv = torch.tensor([1.0, -2.0], device="cuda")
+    loss = mlx_cce.policy_loss(x, None, adv, cu_seqlens=cu, reduction="sum")
+    (grad,) = torch.autograd.grad(loss, [x])
+    assert float(loss) == float(torch.tensor(-float(n - last) + 2.0 * last))   # ratios of 1: exact in 64 bits
+    assert (grad[n - last:] == 2).all()
+    assert all((grad[a:min(a + (1 << 29), n - last)] == -1).all() for a in range(0, n - last, 1 << 29))
+    loss = mlx_cce.preference_loss(x, cu_seqlens=cu, loss_type="hinge", beta=0.5)
+    (grad,) = torch.autograd.grad(loss, [x])
+    assert float(loss) == 1.0 and (grad[n - last:] == 0.5).all()
+    assert all((grad[a:min(a + (1 << 29), n - last)] == -0.5).all() for a in range(0, n - last, 1 << 29))
+    with pytest.raises(ValueError, match="bad sizes"):
+        mlx_cce.policy_loss(torch.zeros(2 ** 31, dtype=torch.bfloat16, device="cuda"), None, adv[:1])
