@@ -47,7 +47,7 @@
 // puts the tensor's largest value below 2^14: hi holds 11 bits and lo the next 11.
 // A product runs as three passes over K, hi hi + hi lo + lo hi (lo lo is 2^-22 of
 // it), each on the tensor cores: 3 times the 16-bit work, where FFMA is 20 times
-// slower.  512 x 512 x 32000, loss and gradients: 0.38 ms, 2.75 ms on the CUDA cores.
+// slower.  512 x 512 x 32000, loss and gradients: 0.37 ms, 2.75 ms on the CUDA cores.
 //
 // Rows are counted on the device (the batch without its masked rows), so row
 // tiles behind the count cost nothing.

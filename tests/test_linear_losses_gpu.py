@@ -550,6 +550,37 @@ def test_captured_and_replayed():
             assert all(torch.equal(x.detach(), y) for x, y in zip(out, want))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_captured_with_other_rows_than_replayed(dtype):
+    """The rows that count, and so the row tiles and K splits, are the replay's."""
+    e, c, b, t, g = head(700, 64, 3000, dtype, 95, bias=torch.float32)
+    tlp, ids = teacher(e, c, b, 8, g)
+    tlp, ids = tlp.cuda(), ids.cuda()
+    xs = leaves(e, c, b)
+    targets, mask = t.cuda(), torch.ones(700, dtype=torch.bool, device="cuda")
+
+    def step():
+        logp = mlx_cce.linear_log_probs(xs[0], xs[1], targets, xs[2])
+        loss = mlx_cce.linear_distillation_loss(xs[0], xs[1], ids, tlp, xs[2], mask=mask)
+        return [logp, loss, *torch.autograd.grad(logp.sum() + loss, xs)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = step()
+    for keep in (700, 0, 1, 130, 700):
+        targets.copy_(torch.where(torch.arange(700) < keep, t, torch.full_like(t, -100)))
+        mask.copy_(torch.arange(700) >= 700 - keep)
+        want = [x.detach().clone() for x in step()]
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x.detach(), y) for x, y in zip(out, want))
+
+
 def test_capture_beside_a_live_eager_graph_is_refused():
     """Refused before anything of the backward pass runs; without the eager graph the
     same capture works."""
