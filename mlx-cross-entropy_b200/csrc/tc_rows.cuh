@@ -233,6 +233,10 @@ struct LogitsEpi {
 // w = d (softmax - onehot).  Distillation: A d e^(z - L) with the coefficient and
 // log-sum-exp of the columns outside of the row's list, d x for the listed ones.
 // float16 holds w / s (`scale` = {s, 1 / s}); split: hi + lo.
+// 16-bit inputs: w is rounded to their type, as an operand of the gradient products
+// must be; half a step beside the result's own half step (bfloat16 gradients are
+// 0.0023 to 0.0025 off, 0.0017 with one rounding).  Two parts would double those
+// products.
 template <typename T, typename TB, bool kTopk, bool kSplit>
 struct DlogitsEpi2 {
   static constexpr int kKind = 1;
