@@ -407,8 +407,9 @@ __device__ __forceinline__ Beyond beyond(const Policy& P, float d, float x, floa
 }
 
 __device__ __forceinline__ TokenOut policy_token(const Policy& P, float x, float old, float ref, float A) {
-  const float d = P.old ? x - old : 0.f;
-  const float r = P.old ? expf(d) : 1.f;
+  // (without old the ratio is 1; a NaN log-probability stays one)
+  const float d = P.old ? x - old : (x == x ? 0.f : x);
+  const float r = P.old ? expf(d) : 1.f + d;
   const Beyond b = beyond(P, d, x, P.old ? old : x);
   const bool pos = A > 0.f, neg = A < 0.f;
   float bounded = r;
