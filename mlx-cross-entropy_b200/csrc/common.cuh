@@ -34,4 +34,13 @@ __host__ __device__ __forceinline__ int64_t round_up(int64_t a, int64_t b) { ret
 // log2(e), the base change used with exp2f (exp(x) = 2^(x * log2(e))).
 constexpr float kLog2e = 1.4426950408889634f;
 
+// The larger of two values, NaN if either is one.  Running maxima of logits keep a
+// NaN: fmaxf drops it, and where nothing but NaN and -infinity had come so far the
+// sum would be passed over as one of nothing.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 }  // namespace cce

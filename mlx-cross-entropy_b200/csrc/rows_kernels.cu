@@ -137,8 +137,9 @@ rows_copy_kernel(const uint16_t* __restrict__ src, int64_t rows, int64_t cols, i
 constexpr int kStRows = 8;
 constexpr int kStSlices = 64;
 
+// (A row with a NaN logit has a NaN maximum, here and below.)
 __device__ __forceinline__ void fold(float& m, float& s, float mp, float sp) {
-  const float M = fmaxf(m, mp);
+  const float M = fmax_nan(m, mp);
   if (M == -INFINITY) return;
   s = s * exp2f((m - M) * kLog2e) + sp * exp2f((mp - M) * kLog2e);
   m = M;
@@ -341,12 +342,12 @@ distill_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ 
     const float mr = sm[0][w], sr = ss[0][w];
     float mx = mr, mass = 0.f;
     for (int k = lane; k < n; k += 32) {
-      mx = fmaxf(mx, zr[k]);
+      mx = fmax_nan(mx, zr[k]);
       mass += pr[k];
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       mass += __shfl_xor_sync(0xffffffffu, mass, o);
     }
     float top = 0.f;

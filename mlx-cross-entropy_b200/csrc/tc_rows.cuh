@@ -207,8 +207,8 @@ struct LogitsEpi {
       }
       float mc = v[0];
 #pragma unroll
-      for (int j = 1; j < 32; ++j) mc = fmaxf(mc, v[j]);
-      const float nm = fmaxf(m, mc);
+      for (int j = 1; j < 32; ++j) mc = fmax_nan(mc, v[j]);
+      const float nm = fmax_nan(m, mc);
       if (nm != -INFINITY) {
         float part = 0.f;
 #pragma unroll
