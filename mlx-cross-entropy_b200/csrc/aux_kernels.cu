@@ -17,9 +17,10 @@ namespace {
 constexpr int kCombRows = 32;    // rows per block (threadIdx.x): a warp reads 128 contiguous bytes
 constexpr int kCombSlices = 32;  // partial slices per row (threadIdx.y)
 
-// Fold (mp, sp) into the running (m, s): s * 2^(m - M) + sp * 2^(mp - M), M = max.
+// Fold (mp, sp) into the running (m, s): s * 2^(m - M) + sp * 2^(mp - M), M = max
+// (NaN where a logit is one).
 __device__ __forceinline__ void fold(float& m, float& s, float mp, float sp) {
-  const float M = fmaxf(m, mp);
+  const float M = fmax_nan(m, mp);
   if (M == -INFINITY) return;
   s = s * exp2f((m - M) * kLog2e) + sp * exp2f((mp - M) * kLog2e);
   m = M;
@@ -46,7 +47,7 @@ lse_combine_kernel(const float* __restrict__ part_max, const float* __restrict__
         sp[u] = part_sum ? part_sum[q] : 1.0f;
         if (part_tgt) t += part_tgt[q];
       }
-      const float M = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), m);
+      const float M = fmax_nan(fmax_nan(fmax_nan(mp[0], mp[1]), fmax_nan(mp[2], mp[3])), m);
       if (M != -INFINITY) {
         float acc = s * exp2f((m - M) * kLog2e);
 #pragma unroll

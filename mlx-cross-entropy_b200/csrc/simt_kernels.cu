@@ -112,12 +112,12 @@ simt_fwd_kernel(const T* __restrict__ e, const T* __restrict__ c, const void* __
     for (int j = 0; j < 8; ++j) {
       const int64_t v = v0 + tx + 16 * j;
       x[j] = (v < V) ? acc[i][j] + bv[j] : -INFINITY;
-      m[gof(j)] = fmaxf(m[gof(j)], x[j]);
+      m[gof(j)] = fmax_nan(m[gof(j)], x[j]);
     }
 #pragma unroll
     for (int g = 0; g < SG; ++g)
 #pragma unroll
-      for (int o = 8; o >= 1; o >>= 1) m[g] = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], o));
+      for (int o = 8; o >= 1; o >>= 1) m[g] = fmax_nan(m[g], __shfl_xor_sync(0xffffffffu, m[g], o));
     float s[SG];
 #pragma unroll
     for (int g = 0; g < SG; ++g) s[g] = 0.f;
@@ -136,7 +136,7 @@ simt_fwd_kernel(const T* __restrict__ e, const T* __restrict__ c, const void* __
         // the tile's LSE partial: fold the statistics tiles' (max, sum-exp)
         float M = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < SG; ++g) M = fmaxf(M, m[g]);
+        for (int g = 0; g < SG; ++g) M = fmax_nan(M, m[g]);
         float S = 0.f;
 #pragma unroll
         for (int g = 0; g < SG; ++g)

@@ -270,10 +270,10 @@ struct FwdEpi {
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       v[j] = (cb + j < V) ? v[j] + b[j] : -INFINITY;
-      mc = fmaxf(mc, v[j]);
+      mc = fmax_nan(mc, v[j]);  // (a NaN logit must reach the sum)
       if (cb + j == st.tl && cb + j < V) tgt[st.row] = v[j];
     }
-    const float nm = fmaxf(st.m, mc);
+    const float nm = fmax_nan(st.m, mc);
     if (nm != -INFINITY) {
       const float nml = nm * kLog2e;
       float acc = 0.f;

@@ -71,3 +71,13 @@ def test_columns_of_minus_infinity_are_still_no_columns(dtype):
     at = torch.searchsorted(left, t)
     got = mlx_cce.linear_log_probs(e.cuda(), c.cuda(), t.cuda(), torch.where(gone, -INF, b).cuda())
     assert torch.all((got.cpu().double() - want.gather(1, at[:, None])[:, 0]).abs() <= Bounds(e, c, b).dlogp)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("where", ["c", "bias"])
+@pytest.mark.parametrize("V,cols", NAN_COLUMNS)
+def test_a_nan_column_is_in_the_cross_entropy(V, cols, where, dtype):
+    e, c, b, t, _ = _nan_head(V, cols, where, dtype)
+    assert torch.isnan(mlx_cce.linear_cross_entropy(e, c, t, b, reduction="none")).all()
+    assert torch.isnan(mlx_cce.linear_cross_entropy(e, c, t, torch.where(torch.isnan(b), b, -INF))).all() or where == "c"
+    _ext.device_status()
