@@ -1147,6 +1147,7 @@ struct RowsSaved {
   cce::RowsView R;
   float* lse;       // distillation: over the columns outside of the list
   float* A;         // distillation
+  float* whole;     // distillation: the row's p and what they leave over, added up
   float* weight;    // distillation [1]
   cce::TopkView topk;
   float* se;        // float32: scale of e's parts
@@ -1166,6 +1167,7 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
   r.lse = p.take<float>(N);
   if (K > 0) {
     r.A = p.take<float>(N);
+    r.whole = p.take<float>(N);
     r.weight = p.take<float>(1);
     r.topk.K = (int)K;
     r.topk.tiles1 = (int)cce::ceil_div(V, cce::kTopkTile) + 1;
@@ -1280,7 +1282,10 @@ RowsPlan rows_plan(int64_t N, int64_t D, int64_t V, int dtype) {
 
 struct RowsBwdWs {
   void *dl, *dl_lo;
-  float *slabs, *scale, *bias_part;
+  float *slabs, *scale, *max_s, *bias_part;
+  void *ec, *ec_lo;  // e with the rows' scales folded in
+  float* sec;
+  uint32_t* word;
   void* grad_c;  // padded rows
   size_t bytes;
 };
@@ -1293,7 +1298,16 @@ RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, in
   w.dl = p.take<uint16_t>((size_t)N * pl.vc);
   if (dtype == CCE_F32) w.dl_lo = p.take<uint16_t>((size_t)N * pl.vc);
   if (flags & CCE_NEED_DE) w.slabs = p.take<float>((size_t)pl.slabs.cap * 128 * dout);
-  if (dtype != CCE_BF16) w.scale = p.take<float>(2);
+  if (dtype != CCE_BF16) {
+    w.scale = p.take<float>(N);
+    w.max_s = p.take<float>(1);
+    if (flags & CCE_NEED_DC) {
+      const size_t n = (size_t)N * rows_dk(N, D, dtype);
+      w.ec = p.take<uint16_t>(n);
+      if (dtype == CCE_F32) w.ec_lo = p.take<uint16_t>(n);
+      else w.sec = p.take<float>(2), w.word = p.take<uint32_t>(1);
+    }
+  }
   if (flags & CCE_NEED_DBIAS) w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * pl.vc);
   if ((flags & CCE_NEED_DC) && dout != D) w.grad_c = p.take<char>((size_t)V * dout * dtype_size(dtype));
   w.bytes = p.used;
@@ -1354,9 +1368,16 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
   const RowsPlan pl = rows_plan(a.N, D, a.V, a.dtype);
   rows_operands(a, v, c);
   a.R = v.R, a.topk = v.topk, a.lse = v.lse, a.A = v.A;
-  a.dl = w.dl, a.dl_lo = w.dl_lo, a.vc_ld = pl.vc, a.scale = w.scale;
+  a.dl = w.dl, a.dl_lo = w.dl_lo, a.vc_ld = pl.vc;
   a.bias_part = need_db ? w.bias_part : nullptr;
-  if (w.scale) CCE_CUDA_CHECK(cce::launch_rows_scale(a.up, v.R, w.scale, s), what);
+  // Rows of one cotangent share a scale; else grad_c's e takes the rows' own.
+  const bool fold = w.ec && a.up.per_row;
+  if (w.max_s) {
+    a.scale = cce::RowScale{a.up.per_row ? w.scale : w.max_s, a.up.per_row};
+    a.max_s = w.max_s;
+    if (fold) a.ec = w.ec, a.ec_lo = w.ec_lo, a.sec = w.sec;
+    CCE_CUDA_CHECK(cce::launch_rows_scale(a.up, v.whole, v.R, w.scale, w.max_s, s), what);
+  }
   const bool fork = need_de && need_dc;
   SideStreams* ss = nullptr;
   cudaStream_t se = s, sc = s;
@@ -1379,8 +1400,7 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
       CCE_CUDA_CHECK(cudaStreamWaitEvent(sc, ss->ev_l, 0), what);
     }
     if (need_db)
-      CCE_CUDA_CHECK(cce::launch_bias_sum(w.bias_part, cce::ceil_div(a.N, 32), v.R, pl.vc, a.vc_len, w.scale,
-                                          grad_bias + a.vc0, s),
+      CCE_CUDA_CHECK(cce::launch_bias_sum(w.bias_part, cce::ceil_div(a.N, 32), v.R, pl.vc, a.vc_len, grad_bias + a.vc0, s),
                      what);
     if (need_de) {
       CCE_CUDA_CHECK(cce::tc_grad_e_rows(a, w.slabs, pl.slabs, a.vc0 > 0, se), what);
@@ -1388,6 +1408,11 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
         CCE_CUDA_CHECK(cce::launch_rows_scatter(w.slabs, pl.slabs, a.Dout, v.R, a.N, D, a.dtype, grad_e, se), what);
     }
     if (need_dc) {
+      if (fold && a.vc0 == 0) {
+        if (w.word) CCE_CUDA_CHECK(cudaMemsetAsync(w.word, 0, sizeof(uint32_t), sc), what);
+        CCE_CUDA_CHECK(cce::launch_rows_fold(v.e, v.e_lo, a.N, a.Dk, v.R, w.scale, w.max_s, w.word, w.sec, w.ec, w.ec_lo, sc),
+                       what);
+      }
       CCE_CUDA_CHECK(cce::tc_grad_c_rows(a, gc, sc), what);
       if (w.grad_c) {  // (16-bit units: two per float32)
         const int64_t u = (int64_t)dtype_size(a.dtype) / 2;
@@ -1558,7 +1583,7 @@ int cce_distill_forward(const void* e, const void* c, const void* bias, int bias
   rows_operands(a, v, c);
   CCE_CUDA_CHECK(cce::tc_logits(a, s), what);
   CCE_CUDA_CHECK(cce::launch_distill_rows(w.part_m, w.part_s, cce::ceil_div(V, 128), N, V, v.R, v.topk, w.p, w.rest,
-                                          red, v.lse, v.A, w.sums, loss, v.weight, s),
+                                          red, v.lse, v.A, v.whole, w.sums, loss, v.weight, s),
                  what);
   return CCE_OK;
 }

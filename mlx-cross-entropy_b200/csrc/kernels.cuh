@@ -59,6 +59,15 @@ struct Cotangent {
 #endif
 };
 
+// The power of two that a packed row's float16 dlogits are in units of.
+struct RowScale {
+  const float* s;  // [N], or one for all; nullptr: 1
+  int per_row;
+#ifdef __CUDACC__
+  __device__ __forceinline__ float of(int64_t packed) const { return s ? s[per_row ? packed : 0] : 1.f; }
+#endif
+};
+
 // GEMMs over a batch's packed rows (tc_rows.cuh), 16-bit operands; dtype CCE_F32:
 // float32 operands as two float16 parts, x = (hi + lo) / s[0] (e, c and e_lo,
 // c_lo; se, sc: {s, 1 / s} on the device).
@@ -79,10 +88,14 @@ struct RowsGemmArgs {
   // dlogits and gradients
   const float *lse, *A;          // A: distillation
   Cotangent up;
-  const float* scale;            // {s, 1 / s}: float16 dlogits hold w / s (nullptr: 1)
+  RowScale scale;                // float16 dlogits hold w / s of their row
+  // grad_c: e with the rows' scales folded in, in units of max_s (the largest of them); se: its scale
+  const void *ec, *ec_lo;
+  const float *max_s, *sec;
   void *dl, *dl_lo;              // [N][vc_ld] 16-bit
   int64_t vc_ld;
-  float* bias_part;              // [ceil(N / 32)][vc_ld] zeroed: column sums of dlogits, or nullptr
+  float* bias_part;              // [ceil(N / 32)][vc_ld] column sums of dlogits (those of the row tiles that
+                                 // count are written and read), or nullptr
 };
 
 struct FwdArgs {
@@ -170,22 +183,29 @@ cudaError_t launch_topk_prep(const void* ids, int id_bytes, const float* logp, i
 int64_t distill_blocks(int64_t N);  // entries of `sums`
 cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_t P, int64_t N, int64_t V,
                                 const RowsView& R, const TopkView& topk, const float* p, const float* rest,
-                                int reduction, float* lse_rest, float* A, DistillSum* sums, float* loss, float* weight,
-                                cudaStream_t stream);
+                                int reduction, float* lse_rest, float* A, float* whole, DistillSum* sums, float* loss,
+                                float* weight, cudaStream_t stream);
 // out[n] = sum over the K splits' slabs (rows of ld values) of row pos[n], in order; 0 where pos[n] < 0
 cudaError_t launch_rows_scatter(const float* slabs, const SlabPlan& plan, int64_t ld, const RowsView& R, int64_t N,
                                 int64_t D, int dtype, void* out, cudaStream_t stream);
-// out = {s, 1 / s}, s the power of two >= the largest |d| of the rows, times 2^-14
-cudaError_t launch_rows_scale(const Cotangent& up, const RowsView& R, float* out, cudaStream_t stream);
+// A row's scale: the power of two >= |d| whole (whole nullptr: 1; below 1: 1) times 2^-14, into
+// rows[N] where the cotangents are per row; max_s: the largest (and every row's, where they are not).
+cudaError_t launch_rows_scale(const Cotangent& up, const float* whole, const RowsView& R, float* rows, float* max_s,
+                              cudaStream_t stream);
+// e's packed rows times rows / max_s, as one float16 value (lo nullptr; scale = {s, 1 / s} of the result, *word:
+// zeroed) or two parts (in their own scale): what grad_c multiplies float16 dlogits of several scales by.
+cudaError_t launch_rows_fold(const void* e, const void* e_lo, int64_t N, int64_t Dk, const RowsView& R,
+                             const float* rows, const float* max_s, uint32_t* word, float* scale, void* out,
+                             void* out_lo, cudaStream_t stream);
 // largest |x| of the rows (those of R, if given) as the bits of a float, into *word (zeroed)
 cudaError_t launch_absmax(const float* x, int64_t rows, int64_t D, const RowsView* R, uint32_t* word,
                           cudaStream_t stream);
 // x -> hi, lo [rows][Dp] and scale = {s, 1 / s}; R: the packed rows of x, zeros behind their count
 cudaError_t launch_split(const float* x, int64_t rows, int64_t D, int64_t Dp, const RowsView* R, const uint32_t* word,
                          float* scale, void* hi, void* lo, cudaStream_t stream);
-// column sums part[parts][ld] of 32 packed rows each -> out[cols], times scale[0]
-cudaError_t launch_bias_sum(const float* part, int64_t parts, const RowsView& R, int64_t ld, int64_t cols,
-                            const float* scale, float* out, cudaStream_t stream);
+// column sums part[parts][ld] of 32 packed rows each -> out[cols]
+cudaError_t launch_bias_sum(const float* part, int64_t parts, const RowsView& R, int64_t ld, int64_t cols, float* out,
+                            cudaStream_t stream);
 
 // ---- SIMT kernels (simt_kernels.cu): any dtype, any shape ----
 cudaError_t simt_forward(const FwdArgs& a, cudaStream_t stream);

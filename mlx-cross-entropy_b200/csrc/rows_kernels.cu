@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kStRows * kStSlices)
 distill_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ part_s, int64_t P, int64_t N, int64_t V,
                     const RowsView R, const TopkView T, const float* __restrict__ p_in,
                     const float* __restrict__ rest_in, float* __restrict__ lse_rest, float* __restrict__ A,
-                    float* __restrict__ loss_row, DistillSum* __restrict__ sums) {
+                    float* __restrict__ whole_out, float* __restrict__ loss_row, DistillSum* __restrict__ sums) {
   __shared__ float sm[kStSlices][kStRows], ss[kStSlices][kStRows];
   __shared__ double tot[kStRows];
   __shared__ int has[kStRows];
@@ -373,11 +373,13 @@ distill_rows_kernel(const float* __restrict__ part_m, const float* __restrict__ 
         loss += others ? (double)(rest * (logf(rest) - ((mr - mx) + logf(sr) - logS))) : (double)INFINITY;
       A[i] = ok && others ? whole * (sr_mx / S) - rest : 0.f;
       lse_rest[i] = others ? mr + logf(sr) : INFINITY;
+      whole_out[i] = whole;
       if (loss_row) loss_row[R.row_of[i]] = (float)loss;
     }
   } else if (i < N && lane == 0) {
     A[i] = 0.f;
     lse_rest[i] = INFINITY;
+    whole_out[i] = 0.f;
   }
   if (w < kStRows && lane == 0) {
     tot[w] = loss;
@@ -438,29 +440,40 @@ __device__ __forceinline__ uint32_t finite_bits(uint32_t x) {
   return x < 0x7f800000u ? x : 0u;
 }
 
-// One block: the largest finite |d| of the rows that count, as a power of two s (1
-// when all are zero) times 2^-14: dlogits are at most d in magnitude, so w / s stays
-// below 2^14 in float16 and a softmax value of 2^-28 is still a normal number.
-__global__ void __launch_bounds__(1024) rows_scale_kernel(const Cotangent up, const RowsView R, float* __restrict__ out) {
+// The power of two >= m (2^-100 below that) times 2^-14.
+__device__ __forceinline__ float scale_of(float m) {
+  int ex = -100;
+  if (m > 0.f) {
+    const float f = frexpf(m, &ex);  // m = f * 2^ex, f in [0.5, 1)
+    if (f == 0.5f) --ex;
+  }
+  return ldexpf(1.f, max(ex, -100) - 14);
+}
+
+// One block: per row the power of two above its largest dlogit's bound, |d| (times
+// the sum of a teacher's probabilities, where that is above 1), times 2^-14: w / s
+// stays below 2^14 in float16, and a softmax value of 2^-28 is still a normal
+// number whatever the cotangents of the other rows are.  A row whose bound is not
+// finite takes 2^-14 and leaves the largest scale to the others.
+__global__ void __launch_bounds__(1024)
+rows_scale_kernel(const Cotangent up, const float* __restrict__ whole, const RowsView R, float* __restrict__ rows,
+                  float* __restrict__ max_s) {
   __shared__ float red[32];
   const int count = *R.count;
   float m = 0.f;
-  for (int i = threadIdx.x; i < (up.per_row ? count : min(count, 1)); i += blockDim.x)
-    m = fmaxf(m, __uint_as_float(finite_bits(__float_as_uint(up.of(i, R.row_of)))));
+  for (int i = threadIdx.x; i < (up.per_row || whole ? count : min(count, 1)); i += blockDim.x) {
+    const float b = fabsf(up.of(i, R.row_of)) * (whole ? fmaxf(whole[i], 1.f) : 1.f);
+    const bool finite = b < INFINITY;
+    if (finite) m = fmaxf(m, b);
+    if (up.per_row) rows[i] = scale_of(finite ? b : 1.f);
+  }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 32; ++w) m = fmaxf(m, red[w]);
-    int ex = 0;
-    if (m > 0.f) {
-      const float f = frexpf(m, &ex);  // m = f * 2^ex, f in [0.5, 1)
-      if (f == 0.5f) --ex;
-    }
-    const float s = ldexpf(1.f, max(ex, -100) - 14);
-    out[0] = s;
-    out[1] = 1.f / s;
+    max_s[0] = scale_of(m);
   }
 }
 
@@ -583,11 +596,77 @@ split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, c
   }
 }
 
+// The largest finite |x| of 16-bit rows as float16 bits.
+__global__ void __launch_bounds__(256)
+absmax_half_kernel(const uint16_t* __restrict__ x, int64_t Dk, const int32_t* __restrict__ count,
+                   uint32_t* __restrict__ word) {
+  const int64_t n = *count * Dk / 8;  // (rows are a multiple of 8 wide)
+  uint32_t m = 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(x) + i);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = w[j] & 0x7fffu, b = (w[j] >> 16) & 0x7fffu;
+      m = max(m, max(a < 0x7c00u ? a : 0u, b < 0x7c00u ? b : 0u));
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(word, m);
+}
+
+// grad_c sums s_i (w / s_i) e_i over rows of different scales s_i: e_i takes s_i / S, S the
+// largest.  float16: the largest value goes to [2^13, 2^14), so a row 2^20 below the
+// largest scale still has normal numbers (e alone would leave 4 bits of them); two
+// parts are there already and are split anew.  A warp per row; zeros behind the count.
+template <bool kSplit>
+__global__ void __launch_bounds__(256)
+rows_fold_kernel(const __half* __restrict__ e, const __half* __restrict__ e_lo, int64_t N, int64_t Dk,
+                 const int32_t* __restrict__ count, const float* __restrict__ rows, const float* __restrict__ max_s,
+                 const uint32_t* __restrict__ word, float* __restrict__ scale, __half* __restrict__ out,
+                 __half* __restrict__ out_lo) {
+  const int lane = threadIdx.x & 31;
+  float k = 1.f;
+  if constexpr (!kSplit) {
+    const float big = __half2float(__ushort_as_half((unsigned short)*word));
+    if (big > 0.f) {
+      int ex;
+      frexpf(big, &ex);
+      k = ldexpf(1.f, 14 - ex);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      scale[0] = k;
+      scale[1] = 1.f / k;
+    }
+  }
+  const int64_t live = *count;
+  const float inv = 1.f / max_s[0];
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < N; r += (int64_t)gridDim.x * 8) {
+    // (at most 1: a row that is not finite may have a scale above the others')
+    const float f = r < live ? fminf(rows[r] * inv, 1.f) * k : 0.f;
+    for (int64_t c = 4 * lane; c < Dk; c += 128) {
+      __half h[4] = {}, l[4] = {};
+      if (r < live) {
+        *reinterpret_cast<uint2*>(h) = __ldg(reinterpret_cast<const uint2*>(e + r * Dk + c));
+        if constexpr (kSplit) *reinterpret_cast<uint2*>(l) = __ldg(reinterpret_cast<const uint2*>(e_lo + r * Dk + c));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float y = (kSplit ? __half2float(h[j]) + __half2float(l[j]) : __half2float(h[j])) * f;
+          h[j] = __float2half_rn(y);
+          if constexpr (kSplit) l[j] = __float2half_rn(y - __half2float(h[j]));
+        }
+      }
+      *reinterpret_cast<uint2*>(out + r * Dk + c) = *reinterpret_cast<uint2*>(h);
+      if constexpr (kSplit) *reinterpret_cast<uint2*>(out_lo + r * Dk + c) = *reinterpret_cast<uint2*>(l);
+    }
+  }
+}
+
 // grad_bias of a vocabulary chunk from the column sums of 32 rows each, in order:
 // the same result every time, where atomics would add in any order.
 __global__ void __launch_bounds__(256)
 bias_sum_kernel(const float* __restrict__ part, int64_t parts, const int32_t* __restrict__ count, int64_t ld,
-                int64_t cols, const float* __restrict__ scale, float* __restrict__ out) {
+                int64_t cols, float* __restrict__ out) {
   __shared__ float sh[8][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
@@ -600,7 +679,7 @@ bias_sum_kernel(const float* __restrict__ part, int64_t parts, const int32_t* __
   if (w == 0 && c < cols) {
 #pragma unroll
     for (int k = 1; k < 8; ++k) s += sh[k][lane];
-    out[c] = s * (scale ? scale[0] : 1.f);
+    out[c] = s;
   }
 }
 
@@ -641,8 +720,26 @@ cudaError_t launch_rows_copy(const void* src, int64_t rows, int64_t cols, int64_
   return launched();
 }
 
-cudaError_t launch_rows_scale(const Cotangent& up, const RowsView& R, float* out, cudaStream_t s) {
-  rows_scale_kernel<<<1, 1024, 0, s>>>(up, R, out);
+cudaError_t launch_rows_scale(const Cotangent& up, const float* whole, const RowsView& R, float* rows, float* max_s,
+                              cudaStream_t s) {
+  rows_scale_kernel<<<1, 1024, 0, s>>>(up, whole, R, rows, max_s);
+  return launched();
+}
+
+cudaError_t launch_rows_fold(const void* e, const void* e_lo, int64_t N, int64_t Dk, const RowsView& R,
+                             const float* rows, const float* max_s, uint32_t* word, float* scale, void* out,
+                             void* out_lo, cudaStream_t s) {
+  const __half *h = static_cast<const __half*>(e), *l = static_cast<const __half*>(e_lo);
+  if (e_lo) {
+    rows_fold_kernel<true><<<warps_grid(N), 256, 0, s>>>(h, l, N, Dk, R.count, rows, max_s, word, scale,
+                                                         static_cast<__half*>(out), static_cast<__half*>(out_lo));
+    return launched();
+  }
+  absmax_half_kernel<<<warps_grid(ceil_div(N * Dk, 256)), 256, 0, s>>>(static_cast<const uint16_t*>(e), Dk, R.count, word);
+  cudaError_t err = launched();
+  if (err != cudaSuccess) return err;
+  rows_fold_kernel<false><<<warps_grid(N), 256, 0, s>>>(h, nullptr, N, Dk, R.count, rows, max_s, word, scale,
+                                                        static_cast<__half*>(out), nullptr);
   return launched();
 }
 
@@ -673,11 +770,12 @@ int64_t distill_blocks(int64_t N) { return ceil_div(N, kStRows); }
 
 cudaError_t launch_distill_rows(const float* part_m, const float* part_s, int64_t P, int64_t N, int64_t V,
                                 const RowsView& R, const TopkView& topk, const float* p, const float* rest,
-                                int reduction, float* lse_rest, float* A, DistillSum* sums, float* loss, float* weight,
-                                cudaStream_t s) {
+                                int reduction, float* lse_rest, float* A, float* whole, DistillSum* sums, float* loss,
+                                float* weight, cudaStream_t s) {
   const int blocks = (int)distill_blocks(N);
   distill_rows_kernel<<<blocks, dim3(kStRows, kStSlices), 0, s>>>(
-      part_m, part_s, P, N, V, R, topk, p, rest, lse_rest, A, reduction == CCE_REDUCE_NONE ? loss : nullptr, sums);
+      part_m, part_s, P, N, V, R, topk, p, rest, lse_rest, A, whole, reduction == CCE_REDUCE_NONE ? loss : nullptr,
+      sums);
   cudaError_t err = launched();
   if (err != cudaSuccess) return err;
   distill_final_kernel<<<1, 256, 0, s>>>(sums, blocks, reduction, loss, weight);
@@ -723,9 +821,9 @@ cudaError_t launch_split(const float* x, int64_t rows, int64_t D, int64_t Dp, co
   return launched();
 }
 
-cudaError_t launch_bias_sum(const float* part, int64_t parts, const RowsView& R, int64_t ld, int64_t cols,
-                            const float* scale, float* out, cudaStream_t s) {
-  bias_sum_kernel<<<(unsigned)ceil_div(cols, 32), 256, 0, s>>>(part, parts, R.count, ld, cols, scale, out);
+cudaError_t launch_bias_sum(const float* part, int64_t parts, const RowsView& R, int64_t ld, int64_t cols, float* out,
+                            cudaStream_t s) {
+  bias_sum_kernel<<<(unsigned)ceil_div(cols, 32), 256, 0, s>>>(part, parts, R.count, ld, cols, out);
   return launched();
 }
 

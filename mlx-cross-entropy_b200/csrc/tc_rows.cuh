@@ -232,7 +232,7 @@ struct LogitsEpi {
 // dlogits of one vocabulary chunk (columns relative to it).  Log-probabilities:
 // w = d (softmax - onehot).  Distillation: A d e^(z - L) with the coefficient and
 // log-sum-exp of the columns outside of the row's list, d x for the listed ones.
-// float16 holds w / s (`scale` = {s, 1 / s}); split: hi + lo.
+// float16 holds w / s, s the row's scale; split: hi + lo.
 // 16-bit inputs: w is rounded to their type, as an operand of the gradient products
 // must be; half a step beside the result's own half step (bfloat16 gradients are
 // 0.0023 to 0.0025 off, 0.0017 with one rounding).  Two parts would double those
@@ -247,7 +247,7 @@ struct DlogitsEpi2 {
   const int32_t* row_of;
   const float* A;         // [N] kTopk: coefficient over d
   const void* bias;       // of column 0 of the whole vocabulary
-  const float* scale;
+  RowScale scale;
   float* bias_part;       // [ceil(N / 32)][ld] column sums of w, or nullptr
   int64_t N, V, vc0, vc_end, ld;
   float scale_z;
@@ -256,7 +256,8 @@ struct DlogitsEpi2 {
 
   struct State {
     int64_t tl;      // the target's place in this half
-    float G, L, dr;  // dlogits are G e^(z - L); dr: d
+    float G, L, dr;  // dlogits are G e^(z - L); dr: d; both over s
+    float s;
     Bias128 bias;
     typename std::conditional<kTopk, TopkCursor, NoCursor>::type cur;
   };
@@ -266,7 +267,8 @@ struct DlogitsEpi2 {
     const float d = live ? up.of(t.row, row_of) : 0.f;
     st.bias.template load<TB>(bias, v0, vc_end);
     st.L = live ? lse[t.row] : INFINITY;
-    st.dr = d * (scale ? scale[1] : 1.f);
+    st.s = live ? scale.of(t.row) : 1.f;
+    st.dr = d * (1.f / st.s);  // (exact: s is a power of two)
     st.tl = -1;
     if constexpr (kTopk) {
       // (a row that gets no gradient: 0 whatever its coefficient)
@@ -321,7 +323,7 @@ struct DlogitsEpi2 {
         if (bias_part != nullptr) {
           float x[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = v[j];
+          for (int j = 0; j < 32; ++j) x[j] = v[j] * st.s;
           const int lane = threadIdx.x & 31;
           const float colsum = warp_transpose_sum32(x);
           if (cb + lane < vc_end) bias_part[(int64_t)(t.y0 / 32) * ld + (cb - vc0) + lane] = colsum;
@@ -340,18 +342,18 @@ struct DlogitsEpi2 {
   }
 };
 
-// out[row][col] = f (A B) in T
+// out[row][col] = f1 f2 (A B) in T
 template <typename T>
 struct Out16Epi {
   static constexpr int kKind = 3;
   static constexpr bool kStores = true, kExact = false;
-  const float* f;  // {s, 1 / s} of float16 dlogits, or nullptr
+  const float *f1, *f2;
   int64_t M, D;
 
   struct State {};
   __device__ __forceinline__ void begin(State&, const TileAt&) const {}
   __device__ __forceinline__ void finish(State&, float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
-    const float s = f ? *f : 1.f;
+    const float s = (f1 ? *f1 : 1.f) * (f2 ? *f2 : 1.f);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int64_t col = t.col0 + c * 32;
@@ -364,10 +366,11 @@ struct Out16Epi {
   }
 };
 
-// out[row][col] (+)= f1 f2 (A B), float32; K split ks behind ks times the row tiles
+// out[row][col] (+)= f1 f2 (A B), float32, f1 by row; K split ks behind ks times the row tiles
 struct OutEpi {
   static constexpr bool kStores = true, kExact = false;
-  const float *f1, *f2;
+  RowScale f1;
+  const float* f2;
   int add;
   int64_t M, D;
   int kind;  // slot in g_mma_cols
@@ -376,7 +379,7 @@ struct OutEpi {
   struct State {};
   __device__ __forceinline__ void begin(State&, const TileAt&) const {}
   __device__ __forceinline__ void finish(State&, float (&z)[128], const TileAt& t, Stager& sg, const CUtensorMap*) const {
-    const float f = (f1 ? *f1 : 1.f) * (f2 ? *f2 : 1.f);
+    const float f = (t.row < t.rows || !f1.per_row ? f1.of(t.row) : 1.f) * (f2 ? *f2 : 1.f);
     const int y = t.ks * (int)round_up(t.rows, BM) + t.y0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -717,12 +720,13 @@ cudaError_t grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t s) {
   const int64_t cols = round_up(a.vc_len, 64);  // (rows of grad_c behind the chunk are clipped by the output's map)
   RowsMaps m;
   int b3d = 0;
+  const void *e = a.ec ? a.ec : a.e, *e_lo = a.ec ? a.ec_lo : a.e_lo;
   bool ok = make_tmap_mn3d(&m.A, a.dl, bf16, cols, a.N, a.vc_ld, BK, BM / 64) &&
-            make_tmap_mn(&m.B, a.e, bf16, a.Dk, a.N, a.Dk, BN / 64, &b3d);
+            make_tmap_mn(&m.B, e, bf16, a.Dk, a.N, a.Dk, BN / 64, &b3d);
   m.A2 = m.A, m.B2 = m.B;
   if constexpr (kSplit)
     ok = ok && make_tmap_mn3d(&m.A2, a.dl_lo, bf16, cols, a.N, a.vc_ld, BK, BM / 64) &&
-         make_tmap_mn(&m.B2, a.e_lo, bf16, a.Dk, a.N, a.Dk, BN / 64, &b3d) &&
+         make_tmap_mn(&m.B2, e_lo, bf16, a.Dk, a.N, a.Dk, BN / 64, &b3d) &&
          make_tmap_f32(&m.C, out, a.Dout, a.Dout, a.vc_len);
   else
     ok = ok && make_tmap_out(&m.C, out, a.dtype, a.Dout, a.vc_len, a.Dout);
@@ -731,10 +735,10 @@ cudaError_t grad_c_rows(const RowsGemmArgs& a, void* grad_c, cudaStream_t s) {
   const int num_m = (int)ceil_div(a.vc_len, BM), num_n = (int)ceil_div(a.Dout, BN);
   const RowsSched rs{a.R.count, a.N, 0, 1, num_m, num_n, 0, 1, 0, raster_group(a.N * a.Dk * 2), b3d};
   if constexpr (kSplit) {
-    const OutEpi epi{a.scale, a.se + 1, 0, a.vc_len, a.Dout, 3};
+    const OutEpi epi{RowScale{a.max_s, 0}, a.se + 1, 0, a.vc_len, a.Dout, 3};
     return rows_gemm<true, true, true>(m, rs, epi, bf16, (int64_t)num_m * num_n, s);
   } else {
-    const Out16Epi<T> epi{a.scale, a.vc_len, a.Dout};
+    const Out16Epi<T> epi{a.max_s, a.sec ? a.sec + 1 : nullptr, a.vc_len, a.Dout};
     return rows_gemm<true, true, false>(m, rs, epi, bf16, (int64_t)num_m * num_n, s);
   }
 }

@@ -81,3 +81,104 @@ def test_a_nan_column_is_in_the_cross_entropy(V, cols, where, dtype):
     assert torch.isnan(mlx_cce.linear_cross_entropy(e, c, t, b, reduction="none")).all()
     assert torch.isnan(mlx_cce.linear_cross_entropy(e, c, t, torch.where(torch.isnan(b), b, -INF))).all() or where == "c"
     _ext.device_status()
+
+
+# ---------------------------------------------------------------------------
+# rows of very different cotangents
+# ---------------------------------------------------------------------------
+
+def _check_rows_apart(grads, e, c, b, w, mag, d, B, floor):
+    """As check_grads, but each row's floor is its own: a dlogit of row i is held to
+    ``floor`` dd_i (dd: the power of two above its cotangent's bound) beside its
+    relative error.  grad_c takes row i's e in units of the largest dd: what that
+    leaves of e_i is 2 floor max|e| D / dd_i, weighted by the row's dlogits."""
+    extra = mag * d[:, None] * (2 * B.dz + 2.0 ** -18)
+    wa = w.abs() + extra
+    dd = 2.0 ** torch.ceil(torch.log2((d * mag.max(1).values.clamp(min=1)).clamp(min=1e-300)))
+    e64, c64 = e.double(), c.double()
+    N, V = w.shape
+    half = R.half_steps if e.dtype != torch.float32 else lambda t, x: 0.0
+
+    def off(got, want, tol):
+        """Errors; 0 for an infinity of the right sign where the value may round to one
+        (float16: from 65520, half a step above its largest number)."""
+        err = (got.cpu().double() - want).abs()
+        if e.dtype == torch.float16:
+            err = torch.where((want.abs() + tol >= 65520) & torch.isinf(got.cpu()) & (got.cpu() * want > 0), 0.0, err)
+        return err
+
+    want = w @ c64
+    tol = extra @ c64.abs() + (wa @ c64.abs()) * (B.h + (V / 16 + 64) * 2 * U) + floor * dd[:, None] * c64.abs().sum(0)
+    tol = tol + half(e.dtype, want.abs() + tol)
+    err = off(grads[0], want, tol)
+    assert torch.all(err <= tol), ("grad_e", (err / tol).max())
+    want = w.t() @ e64
+    tol = extra.t() @ e64.abs() + (wa.t() @ e64.abs()) * (2 * B.h + (N / 16 + 64) * 2 * U)
+    tol = tol + floor * (dd[:, None] * e64.abs()).sum(0)
+    tol = tol + (wa / dd[:, None]).sum(0)[:, None] * 2 * floor * e64.abs().max() * dd.max()
+    tol = tol + half(c.dtype, want.abs() + tol)
+    err = off(grads[1], want, tol)
+    assert torch.all(err <= tol), ("grad_c", (err / tol).max())
+    if b is not None:
+        tol = extra.sum(0) + wa.sum(0) * (N + 64) * U
+        assert torch.all((grads[2].cpu().double() - w.sum(0)).abs() <= tol), "grad_bias"
+
+
+FLOORS = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 2.0 ** -39}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("chunks", [1, 6])
+def test_one_cotangent_far_above_the_others(dtype, chunks, monkeypatch):
+    """An unbounded policy ratio: one row's cotangent 2^30 times the others'.  The other
+    rows keep their gradients, tails included."""
+    if chunks > 1:
+        monkeypatch.setenv("CCE_BWD_CHUNK_ROWS", "512")
+    e, c, b, t, g = head(200, 64, 3000, dtype, 11, bias=torch.float32)
+    e = (e.float() * 0.5).to(dtype)
+    go = torch.randn(200, generator=g) * 2.0 ** -14
+    go[7] = 2.0 ** 16
+    go[8] = 0.0
+    go[9] = 1e-30
+    xs = leaves(e, c, b)
+    logp = mlx_cce.linear_log_probs(xs[0], xs[1], t.cuda(), xs[2])
+    grads = torch.autograd.grad(logp, xs, go.cuda())
+    lq = torch.log_softmax(e.double() @ c.double().t() + b.double(), 1)
+    w = -lq.exp()
+    w[torch.arange(200), t] += 1
+    d = go.double()
+    B = Bounds(e, c, b)
+    _check_rows_apart(grads, e, c, b, w * d[:, None], lq.exp(), d.abs(), B, FLOORS[dtype])
+    assert torch.all(grads[0][8] == 0)
+    _ext.device_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_teacher_probabilities_above_one(dtype, reduction):
+    """With a tail the teacher's values are used as they are: a sum of 40 must not
+    overflow the float16 dlogits."""
+    e, c, b, t, g = head(60, 64, 900, dtype, 12)
+    tlp, ids = teacher(e, c, b, 8, g)
+    tlp = tlp - torch.logsumexp(tlp, 1, keepdim=True)
+    tlp[::2] += math.log(40.0)
+    tlp[1::2] += math.log(0.6)
+    go = torch.randn(60, generator=g) * 2.0 ** 10 if reduction == "none" else torch.tensor(2.0 ** 16)
+    xs = leaves(e, c, b)
+    loss = mlx_cce.linear_distillation_loss(xs[0], xs[1], ids.cuda(), tlp.cuda(), tail=True, reduction=reduction)
+    grads = torch.autograd.grad(loss, xs, go.cuda())
+    want, size, w, on = distill64(e, c, b, ids, tlp, tail=True, reduction=reduction, go=go)
+    assert torch.all((loss.detach().cpu().double() - want).abs() <= 1e-4 * want.abs() + 1e-4 * size.max())
+    q = torch.log_softmax(e.double() @ c.double().t(), 1).exp()
+    p = torch.zeros_like(q).scatter_add(1, ids, tlp.double().exp())
+    whole = p.sum(1).clamp(min=1)[:, None]
+    d = (go.double().abs() if reduction == "none" else go.double().abs().expand(60) / 60).clone()
+    if reduction == "mean":  # (one scale for all rows, that of the largest sum)
+        d64 = torch.full_like(d, float(d[0]))
+        floor = FLOORS[dtype] * float(whole.max())
+    else:
+        d64, floor = d, FLOORS[dtype]
+    B = Bounds(e, c, b)
+    # the tail's coefficient is a difference: whole q_r - r, errors of both
+    _check_rows_apart(grads, e, c, b, w, whole * q + p + 1, d64, B, floor)
+    _ext.device_status()
