@@ -69,8 +69,9 @@ struct RowScale {
 };
 
 // GEMMs over a batch's packed rows (tc_rows.cuh), 16-bit operands; dtype CCE_F32:
-// float32 operands as two float16 parts, x = (hi + lo) / s[0] (e, c and e_lo,
-// c_lo; se, sc: {s, 1 / s} on the device).
+// float32 operands as two float16 parts, x = (hi + lo / kLoUnits) / s[0] (e, c and
+// e_lo, c_lo; se, sc: {s, 1 / s} on the device).
+constexpr float kLoUnits = 2048.f;
 struct RowsGemmArgs {
   const void *e, *e_lo;          // [N][Dk] packed rows, zeros behind the count
   const void *c, *c_lo;          // [V][Dk]

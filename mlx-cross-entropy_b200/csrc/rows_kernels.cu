@@ -550,9 +550,15 @@ absmax_kernel(const float* __restrict__ x, int64_t rows, int64_t D, const int32_
   if (lane == 0 && m) atomicMax(word, m);
 }
 
-// s puts the largest value into [2^13, 2^14): hi = fp16(s x), lo = fp16(s x - hi)
-// together hold 22 bits of values down to 2^-14 of the largest, 2^-25 absolute
-// (in units of 1 / s) below.
+// s puts the largest value into [2^13, 2^14): hi = fp16(s x), lo = fp16(2^11 (s x - hi)).
+// hi has 11 bits down to 2^-14, so of values down to 2^-28 of the largest 22 bits are
+// held, and 2^-36 absolute (in units of 1 / s), 2^-50 of the largest, below.  (In hi's
+// own units lo would run out at 2^-25, and one row 2^20 above the others would leave
+// them 17 bits.)  |s x - hi| <= 4, so lo stays below 2^13.
+__device__ __forceinline__ void split_parts(float y, __half& hi, __half& lo) {
+  hi = __float2half_rn(y);
+  lo = __float2half_rn((y - __half2float(hi)) * kLoUnits);
+}
 __global__ void __launch_bounds__(256)
 split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, const int32_t* __restrict__ row_of,
              const int32_t* __restrict__ count, int vec, const uint32_t* __restrict__ word, float* __restrict__ scale,
@@ -586,9 +592,7 @@ split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, c
       __half h[4], l[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float y = v[j] * s;
-        h[j] = __float2half_rn(y);
-        l[j] = __float2half_rn(y - __half2float(h[j]));
+        split_parts(v[j] * s, h[j], l[j]);
       }
       *reinterpret_cast<uint2*>(hi + r * Dp + k) = *reinterpret_cast<uint2*>(h);
       *reinterpret_cast<uint2*>(lo + r * Dp + k) = *reinterpret_cast<uint2*>(l);
@@ -651,9 +655,8 @@ rows_fold_kernel(const __half* __restrict__ e, const __half* __restrict__ e_lo, 
         if constexpr (kSplit) *reinterpret_cast<uint2*>(l) = __ldg(reinterpret_cast<const uint2*>(e_lo + r * Dk + c));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float y = (kSplit ? __half2float(h[j]) + __half2float(l[j]) : __half2float(h[j])) * f;
-          h[j] = __float2half_rn(y);
-          if constexpr (kSplit) l[j] = __float2half_rn(y - __half2float(h[j]));
+          if constexpr (kSplit) split_parts((__half2float(h[j]) + __half2float(l[j]) / kLoUnits) * f, h[j], l[j]);
+          else h[j] = __float2half_rn(__half2float(h[j]) * f);
         }
       }
       *reinterpret_cast<uint2*>(out + r * Dk + c) = *reinterpret_cast<uint2*>(h);

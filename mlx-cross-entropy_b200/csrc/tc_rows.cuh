@@ -43,8 +43,9 @@
 // D = 2304 head has 5.7.  Gradients and dlogits, which are rounded to 16 bits or
 // summed over far smaller terms, take segments of 64 steps.
 //
-// Float32 inputs.  x = (hi + lo) / s with hi, lo float16 and s a power of two that
-// puts the tensor's largest value below 2^14: hi holds 11 bits and lo the next 11.
+// Float32 inputs.  x = (hi + 2^-11 lo) / s with hi, lo float16 and s a power of two that
+// puts the tensor's largest value below 2^14: hi holds 11 bits and lo the next 11, of
+// values down to 2^-28 of the largest; lo's units are 2^-11 of hi's.
 // A product runs as three passes over K, hi hi + hi lo + lo hi (lo lo is 2^-22 of
 // it), each on the tensor cores: 3 times the 16-bit work, where FFMA is 20 times
 // slower.  512 x 512 x 32000, loss and gradients: 0.37 ms, 2.75 ms on the CUDA cores.
@@ -131,6 +132,15 @@ struct Bias128 {
 
 // 1 / (s_a s_b) of split operands, 1 for whole ones: s[1] = 1 / s[0]
 __device__ __forceinline__ float unscale(const float* a, const float* b) { return a ? a[1] * b[1] : 1.f; }
+
+// The K-blocks that one accumulator holds, of a unit of kb K-blocks walked in
+// `passes` passes; no segment spans the first pass, hi hi, and the others, whose
+// products are in units of 1 / kLoUnits.
+struct Segment {
+  int kb, passes, len;
+  __device__ __forceinline__ int n() const { return kb * passes; }
+  __device__ __forceinline__ int end(int k0) const { return min(k0 < kb ? kb : n(), k0 + len); }
+};
 
 struct NoCursor {};
 
@@ -331,7 +341,7 @@ struct DlogitsEpi2 {
         sg.template store16<T>(v, (int)(cb - vc0), t.y0);
         if constexpr (kSplit) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] -= to_f32(from_f32<T>(v[j]));
+          for (int j = 0; j < 32; ++j) v[j] = (v[j] - to_f32(from_f32<T>(v[j]))) * kLoUnits;
           const CUtensorMap* tm_hi = sg.tm;
           sg.tm = tm_lo;
           sg.template store16<T>(v, (int)(cb - vc0), t.y0);
@@ -491,12 +501,12 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         int mb, nb, ks, kb0, kb1;
         sched.coords(u, mb, nb, ks);
         sched.krange(ks, kb0, kb1);
-        const int n = (kb1 - kb0) * kPasses;
-        for (int k0 = 0; ok && k0 < n; k0 += seg_kb) {
+        const Segment seg{kb1 - kb0, kPasses, seg_kb};
+        for (int k0 = 0, k1; ok && k0 < seg.n(); k0 = k1) {
+          k1 = seg.end(k0);
           if (!mbar_wait(tempty + acc, acc_phase ^ 1u, 12)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem_base + (uint32_t)(acc * BN);
-          const int k1 = min(n, k0 + seg_kb);
           uint32_t fresh = 1;
           for (int k = k0; k < k1; ++k) {
             if (!mbar_wait(full + stage, phase, 13)) { ok = false; break; }
@@ -538,7 +548,7 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       int mb, nb, ks, kb0, kb1;
       sched.coords(u, mb, nb, ks);
       sched.krange(ks, kb0, kb1);
-      const int n = (kb1 - kb0) * kPasses;
+      const Segment seg{kb1 - kb0, kPasses, seg_kb};
       const int y0 = mb * BM + q * 32;
       const TileAt t{(int64_t)y0 + lane, (int64_t)nb * BN + h * 128, rows, y0, ks, nb};
       typename Epi::State st;
@@ -547,17 +557,18 @@ rows_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
       for (int j = 0; j < 128; ++j) z[j] = 0.f;
 #pragma unroll 1
-      for (int k0 = 0; k0 < n; k0 += seg_kb) {
+      for (int k0 = 0; k0 < seg.n(); k0 = seg.end(k0)) {
         // (one verdict for the warp: the TMEM reads below need all of its lanes)
         ok = __all_sync(0xffffffffu, mbar_wait(tfull + acc, acc_phase, 14));
         if (!ok) break;
         tc_fence_after();
+        const float f = kSplit && k0 >= seg.kb ? untruncate / kLoUnits : untruncate;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float v[32];
           tmem_ld32(tbase + (uint32_t)(acc * BN + c * 32), v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[c * 32 + j] = fmaf(v[j], untruncate, z[c * 32 + j]);
+          for (int j = 0; j < 32; ++j) z[c * 32 + j] = fmaf(v[j], f, z[c * 32 + j]);
         }
         tc_fence_before();
         mbar_arrive(tempty + acc);

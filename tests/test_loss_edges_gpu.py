@@ -124,7 +124,9 @@ def _check_rows_apart(grads, e, c, b, w, mag, d, B, floor):
         assert torch.all((grads[2].cpu().double() - w.sum(0)).abs() <= tol), "grad_bias"
 
 
-FLOORS = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 2.0 ** -39}
+# half the smallest step of a float16 part, 2^-25, in units of 2^-14 of dd; float32's
+# second part is in units of 2^-11 of the first's
+FLOORS = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 2.0 ** -50}
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -181,4 +183,61 @@ def test_teacher_probabilities_above_one(dtype, reduction):
     B = Bounds(e, c, b)
     # the tail's coefficient is a difference: whole q_r - r, errors of both
     _check_rows_apart(grads, e, c, b, w, whole * q + p + 1, d64, B, floor)
+    _ext.device_status()
+
+
+def _log_probs_of_rest(e, c, b, t, go, row, col):
+    """Log-probabilities and gradients of all rows but one, whose e is far above the
+    others' and whose cotangent is 0; the classifier's column ``col`` is as far above
+    and masked.  What 22-bit parts with a common scale leave of the other values
+    besides is 2^-50 of the tensor's largest (2^-49: the scale is within a factor 2)."""
+    rest = torch.arange(e.shape[0]) != row
+    cols = torch.arange(c.shape[0]) != col
+    xs = leaves(e, c, b)
+    logp = mlx_cce.linear_log_probs(xs[0], xs[1], t.cuda(), xs[2])
+    grads = torch.autograd.grad(logp, xs, go.cuda())
+    e1, c1, b1, t1 = e[rest], c[cols], b[cols], t[rest] - (t[rest] > col).long()
+    lq = torch.log_softmax(e1.double() @ c1.double().t() + b1.double(), 1)
+    B = Bounds(e1, c1, b1)
+    floor = 2.0 ** -49 if e.dtype == torch.float32 else 0.0
+    lost = floor * float(e.abs().max() * c1.abs().sum(1).max() + c.abs().max() * e1.abs().sum(1).max())
+    B.dz += lost
+    B.dlogp += 2 * lost
+    n = e1.shape[0]
+    want = lq.gather(1, t1[:, None])[:, 0]
+    assert torch.all((logp.detach().cpu().double()[rest] - want).abs() <= B.dlogp)
+    w = -lq.exp()
+    w[torch.arange(n), t1] += 1
+    d = go[rest].double()
+    w = w * d[:, None]
+    mag = lq.exp()
+    extra = mag * d.abs()[:, None] * (2 * B.dz + 2.0 ** -18)
+    wa = w.abs() + extra
+    h = R.half_steps if e.dtype != torch.float32 else lambda dt, x: 0.0
+    for got, left, other, add, big in ((grads[0].cpu()[rest], w, c1.double(), extra @ c1.double().abs(), float(c.abs().max())),
+                                       (grads[1].cpu()[cols], w.t(), e1.double(), extra.t() @ e1.double().abs(),
+                                        float(e.abs().max()))):
+        want = left @ other
+        la = wa if left is w else wa.t()
+        tol = add + (la @ other.abs()) * (2 * B.h + (left.shape[1] / 16 + 64) * 2 * U)
+        tol = tol + floor * big * la.sum(1, keepdim=True)
+        tol = tol + FLOORS[e.dtype] * 2 * float(d.abs().max()) * other.abs().sum(0)
+        tol = tol + h(e.dtype, want.abs() + tol)
+        err = (got.double() - want).abs()
+        assert torch.all(err <= tol), (err / tol).max()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 192])
+def test_values_far_above_the_others(dtype, D):
+    """One row of e and one masked column of c 2^24 above the rest of the tensors: the
+    other rows keep their digits."""
+    e, c, b, t, g = head(200, D, 1500, dtype, 13, bias=torch.float32)
+    t = torch.where(t == 5, torch.full_like(t, 6), t)
+    e[11] *= 2.0 ** 24
+    c[5] *= 2.0 ** 24
+    b[5] = -INF
+    go = torch.randn(200, generator=g)
+    go[11] = 0.0
+    _log_probs_of_rest(e, c, b, t, go, 11, 5)
     _ext.device_status()
