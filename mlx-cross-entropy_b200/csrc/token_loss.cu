@@ -418,8 +418,10 @@ __device__ __forceinline__ TokenOut policy_token(const Policy& P, float x, float
   bounded = neg && P.dual > 0.f && b.dual ? P.dual : bounded;
   TokenOut o;
   o.clipped = (pos && b.hi) || (neg && (b.lo || (P.dual > 0.f && b.dual)));
-  o.loss = -(bounded * A);
-  o.g = o.clipped ? 0.f : -(r * A);
+  // (an advantage of 0 asks nothing of a ratio past float32's range, e^88.7; NaN stays)
+  const bool idle = A == 0.f && d == d;
+  o.loss = idle ? 0.f : -(bounded * A);
+  o.g = o.clipped || idle ? 0.f : -(r * A);
   o.kl = 0.f;
   if (P.ref) {
     float em1;

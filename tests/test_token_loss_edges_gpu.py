@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import mlx_cce
-from test_token_losses_gpu import DTYPES, batch, check_policy
+import token_loss_ref as R
+from test_token_losses_gpu import DTYPES, EPS, batch, run_policy
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +26,31 @@ def test_a_nan_log_probability_without_old_is_not_hidden(dtype):
     assert torch.isnan(mlx_cce.policy_loss(x, None, adv, cu_seqlens=cu))
     mask = ~torch.isnan(x)
     assert torch.isfinite(mlx_cce.policy_loss(x, None, adv, mask=mask, cu_seqlens=cu))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sequence", "sum", "none"])
+def test_an_advantage_of_zero_with_any_ratio(reduction):
+    """Ratios of e^100 and e^700, past float32: a group whose rewards are all the same has
+    advantages of 0, and 0 of any ratio is 0."""
+    b = batch(2000, 4, seed=21)
+    b["old"][::7] = b["logp"][::7] - 100.0
+    b["old"][3::7] = b["logp"][3::7] - 700.0
+    adv = torch.randn(b["shape"], generator=b["g"])
+    adv[::7] = adv[3::7] = 0.0
+    go = torch.randn(b["shape"], generator=b["g"]) if reduction == "none" else None
+    kw = dict(kl_coef=0.1, reduction=reduction)
+    loss, grad, _, _ = run_policy(b, adv, go, **kw)
+    r = R.policy(b["logp"], b["old"], adv, b["ref"], b["mask"], b["cu"], grad_out=go, **kw)
+    assert torch.all((loss - r["loss"]).abs() <= EPS * r["lsize"])
+    # check_policy's tolerance, and where only the KL term is left the definition's own rounding:
+    # its autograd forms the slope e^q - 1 as (expm1(q) + 1) - 1, off by 2^-53 in 64 bits, times
+    # kl_coef and a token's weight
+    n = torch.tensor([int(b["mask"][lo:hi].sum()) for lo, hi in zip(b["cu"], b["cu"][1:])])
+    n = n[n > 0]
+    weight = {"mean": 1 / int(n.sum()), "sequence": 1 / (len(n) * int(n.min())), "sum": 1.0}.get(reduction)
+    weight = weight or float(go.abs().max())
+    assert torch.all((grad.double() - r["grad"]).abs() <= EPS * r["gsize"] + 2.0 ** -52 * 0.1 * weight)
+    x = b["logp"].cuda()
+    x[14] = float("nan")  # (not hidden by the advantage)
+    mask = torch.ones_like(b["mask"]).cuda()
+    assert torch.isnan(mlx_cce.policy_loss(x, b["old"].cuda(), adv.cuda(), mask=mask))
