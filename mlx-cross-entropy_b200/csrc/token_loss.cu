@@ -426,8 +426,10 @@ __device__ __forceinline__ TokenOut policy_token(const Policy& P, float x, float
   if (P.ref) {
     float em1;
     kl3(ref - x, o.kl, em1);
-    o.loss = fmaf(P.beta, o.kl, o.loss);
-    o.g = fmaf(-P.beta, em1, o.g);
+    if (P.beta != 0.f) {  // (0: the term is only measured, and may pass float32's range)
+      o.loss = fmaf(P.beta, o.kl, o.loss);
+      o.g = fmaf(-P.beta, em1, o.g);
+    }
   }
   return o;
 }

@@ -265,7 +265,7 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seql
         clip, clip_high: the ratio is clipped to ``[1 - clip, 1 + clip_high]``
             (clip_high defaults to clip; ``inf`` leaves that side open)
         dual_clip: bounds a negative advantage's loss by ``-dual_clip * A``
-        kl_coef: weight of the KL term
+        kl_coef: weight of the KL term (0: it is measured for the statistics alone)
         reduction: "mean" over tokens, "sequence" (mean over the sequences that
             have a token of their tokens' means), "sum" or "none" (per token)
         return_stats: also return ``PolicyStats(kl, clip_fraction)``

@@ -54,3 +54,25 @@ def test_an_advantage_of_zero_with_any_ratio(reduction):
     x[14] = float("nan")  # (not hidden by the advantage)
     mask = torch.ones_like(b["mask"]).cuda()
     assert torch.isnan(mlx_cce.policy_loss(x, b["old"].cuda(), adv.cuda(), mask=mask))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sequence", "sum", "none"])
+def test_a_kl_term_of_weight_zero_is_only_measured(reduction):
+    """ref - logp of 100: e^100 is past float32, 0 times it is 0 all the same."""
+    b = batch(2000, 4, seed=22)
+    b["mask"][:] = True
+    far = b["logp"] - 100.0
+    near = b["ref"].clone()
+    adv = torch.randn(4, generator=b["g"])
+    cu = torch.tensor(b["cu"], dtype=torch.int32, device="cuda")
+    out = []
+    for x, ref in ((b["logp"], near), (far, b["logp"])):
+        x = x.cuda().requires_grad_(True)
+        old = x.detach() + 0.01
+        loss, stats = mlx_cce.policy_loss(x, old, adv.cuda(), ref_logp=ref.cuda(), cu_seqlens=cu, reduction=reduction,
+                                          return_stats=True)
+        bare = mlx_cce.policy_loss(x, old, adv.cuda(), cu_seqlens=cu, reduction=reduction)
+        grads = [torch.autograd.grad(l.sum(), [x])[0] for l in (loss, bare)]
+        assert torch.isfinite(loss).all() and torch.equal(loss, bare) and torch.equal(*grads)
+        out.append(stats.kl.item())
+    assert 0 < out[0] < 10 and out[1] == float("inf")
