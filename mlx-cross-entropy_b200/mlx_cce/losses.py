@@ -18,7 +18,11 @@ gradient pushes the unlikely tokens too), and rows that do not count are taken
 out before the GEMMs.
 
 Tokens come as padded rows ``[S, T]`` (a row is a sequence) or packed in one
-dimension with ``cu_seqlens`` (int32 offsets ``[S + 1]``).  Tokens that
+dimension with ``cu_seqlens`` (int32 offsets ``[S + 1]``).  Advantages and
+reference log-probabilities come per token or per sequence, told apart by their
+shape; a packed batch of as many tokens as sequences fits both and is read per
+token, with a warning, unless ``advantages_per_token`` or ``ref_per_token`` says
+which it is.  Tokens that
 ``mask`` leaves out, and packed tokens of no sequence, add nothing and get a
 zero gradient, whatever they hold.
 """
@@ -26,6 +30,7 @@ zero gradient, whatever they hold.
 from __future__ import annotations
 
 import math
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -139,15 +144,25 @@ def _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_tok
     return [float(clip), float(high), float(dual_clip or 0.0), float(kl_coef)], POLICY_REDUCTIONS[reduction], per_token
 
 
-def _advantages(what, advantages, shape, S, dev):
+def _is_per_token(what, name, got, shape, S, per_token, argument):
+    """Whether values of shape ``got`` are one per token, not one per sequence."""
+    fits = {True: got == tuple(shape), False: got == (S,)}
+    if per_token is not None:
+        if not fits[bool(per_token)]:
+            raise ValueError(f"[{what}] {name} must be {tuple(shape) if per_token else (S,)} with {argument}="
+                             f"{bool(per_token)}, got {got}")
+        return bool(per_token)
+    if not any(fits.values()):
+        raise ValueError(f"[{what}] {name} must be per token {tuple(shape)} or per sequence ({S},), got {got}")
+    if all(fits.values()) and S > 1:
+        warnings.warn(f"[{what}] {name} of shape {got} could be one per token or one per sequence and are read per "
+                      f"token: say {argument}=True or False", stacklevel=4)
+    return fits[True]
+
+
+def _advantages(what, advantages, shape, S, dev, per_token=None):
     """(float32 advantages, one per token?)"""
-    if advantages.shape == shape:
-        per_token = True
-    elif advantages.shape == (S,):
-        per_token = False
-    else:
-        raise ValueError(f"[{what}] advantages must be per token {tuple(shape)} or per sequence ({S},), "
-                         f"got {tuple(advantages.shape)}")
+    per_token = _is_per_token(what, "advantages", tuple(advantages.shape), shape, S, per_token, "advantages_per_token")
     if not advantages.is_floating_point():
         raise ValueError(f"[{what}] advantages must be floating point, got {advantages.dtype}")
     if advantages.device != dev:
@@ -228,15 +243,12 @@ def _distill_params(what, temperature, tail, reduction):
     return float(temperature), bool(tail), PREFERENCE_REDUCTIONS[reduction]
 
 
-def _reference(what, ref_logp, tokens, dtype, S):
+def _reference(what, ref_logp, tokens, dtype, S, per_token=None):
     """(per-token reference or None, per-sequence sums or None)"""
     if ref_logp is None:
         return None, None
-    if ref_logp.shape == tokens.shape:
+    if _is_per_token(what, "ref_logp", tuple(ref_logp.shape), tokens.shape, S, per_token, "ref_per_token"):
         return _per_token(what, "ref_logp", ref_logp, tokens, dtype), None
-    if ref_logp.shape != (S,):
-        raise ValueError(f"[{what}] ref_logp must be per token {tuple(tokens.shape)} or per sequence ({S},), "
-                         f"got {tuple(ref_logp.shape)}")
     if not ref_logp.is_floating_point() or ref_logp.device != tokens.device:
         raise ValueError(f"[{what}] ref_logp must be floating point on {tokens.device}")
     return None, _constant(ref_logp.to(torch.float32))
@@ -247,7 +259,7 @@ def _reference(what, ref_logp, tokens, dtype, S):
 # ---------------------------------------------------------------------------
 
 def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seqlens=None, clip=0.2, clip_high=None,
-                dual_clip=None, kl_coef=0.0, reduction="mean", return_stats=False):
+                dual_clip=None, kl_coef=0.0, reduction="mean", return_stats=False, advantages_per_token=None):
     """Clipped policy loss with a KL term, on per-token log-probabilities.
 
     With ratio ``r = exp(logp - old_logp)`` and advantage ``A`` a token's loss is
@@ -269,6 +281,8 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seql
         reduction: "mean" over tokens, "sequence" (mean over the sequences that
             have a token of their tokens' means), "sum" or "none" (per token)
         return_stats: also return ``PolicyStats(kl, clip_fraction)``
+        advantages_per_token: what advantages of a shape that fits both are (True,
+            False; None: per token, with a warning)
     Returns:
         float32 loss (scalar, or logp's shape for reduction="none"); with
         ``return_stats`` a tuple ``(loss, stats)``.
@@ -276,7 +290,7 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seql
     what = "policy_loss"
     logp = _logp(what, logp)
     S, cu = _sequences(what, logp.shape, cu_seqlens, logp.device)
-    adv, per_token = _advantages(what, advantages, logp.shape, S, logp.device)
+    adv, per_token = _advantages(what, advantages, logp.shape, S, logp.device, advantages_per_token)
     params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
     loss, stats = _POLICY(logp, _per_token(what, "old_logp", old_logp, logp, logp.dtype),
                           _per_token(what, "ref_logp", ref_logp, logp, logp.dtype), adv,
@@ -285,7 +299,8 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seql
 
 
 def preference_loss(logp, ref_logp=None, *, mask=None, cu_seqlens=None, beta=0.1, margin=0.0, loss_type="sigmoid",
-                    label_smoothing=0.0, length_normalize=False, reduction="mean", return_rewards=False):
+                    label_smoothing=0.0, length_normalize=False, reduction="mean", return_rewards=False,
+                    ref_per_token=None):
     """Preference loss of pairs of sequences from the log-ratios of their tokens.
 
     The first half of the sequences is chosen over the second half, in the same
@@ -306,6 +321,8 @@ def preference_loss(logp, ref_logp=None, *, mask=None, cu_seqlens=None, beta=0.1
         length_normalize: divide ``D`` by the sequence's number of tokens
         reduction: "mean", "sum" or "none" over the pairs
         return_rewards: also return ``PreferenceRewards(chosen, rejected)``
+        ref_per_token: what a ref_logp of a shape that fits both is (True, False; None:
+            per token, with a warning)
     Returns:
         float32 loss (scalar, or ``[pairs]`` for reduction="none"); with
         ``return_rewards`` a tuple ``(loss, rewards)``.
@@ -314,7 +331,7 @@ def preference_loss(logp, ref_logp=None, *, mask=None, cu_seqlens=None, beta=0.1
     logp = _logp(what, logp)
     pairs, cu = _pairs(what, logp.shape, cu_seqlens, logp.device)
     params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
-    ref, sums = _reference(what, ref_logp, logp, logp.dtype, 2 * pairs)
+    ref, sums = _reference(what, ref_logp, logp, logp.dtype, 2 * pairs, ref_per_token)
     loss, rewards = _PREFERENCE(logp, ref, sums, _mask(what, mask, logp.shape, logp.device), cu, pairs, *params)
     return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
 
@@ -341,7 +358,7 @@ def linear_log_probs(e, c, targets, bias=None, *, ignore_index=-100):
 
 def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_logp=None, cu_seqlens=None, clip=0.2,
                        clip_high=None, dual_clip=None, kl_coef=0.0, reduction="mean", ignore_index=-100,
-                       return_stats=False):
+                       return_stats=False, advantages_per_token=None):
     """``policy_loss`` of the head's log-probabilities of ``targets``.
 
     e ``[..., D]``, c ``[V, D]`` and bias as in ``linear_log_probs``; targets are the
@@ -351,7 +368,7 @@ def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_lo
     """
     what = "linear_policy_loss"
     S, cu = _sequences(what, targets.shape, cu_seqlens, targets.device)
-    adv, per_token = _advantages(what, advantages, targets.shape, S, targets.device)
+    adv, per_token = _advantages(what, advantages, targets.shape, S, targets.device, advantages_per_token)
     params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
     e, c, bias = _head(what, e, c, bias, targets.shape)
     targets = _ids(what, "targets", targets, e.device)
@@ -364,7 +381,7 @@ def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_lo
 
 def linear_preference_loss(e, c, targets, ref_logp=None, bias=None, *, cu_seqlens=None, beta=0.1, margin=0.0,
                            loss_type="sigmoid", label_smoothing=0.0, length_normalize=False, reduction="mean",
-                           ignore_index=-100, return_rewards=False):
+                           ignore_index=-100, return_rewards=False, ref_per_token=None):
     """``preference_loss`` of the head's log-probabilities of ``targets``.
 
     e ``[..., D]``, c ``[V, D]`` and bias as in ``linear_log_probs``; targets are the
@@ -378,7 +395,7 @@ def linear_preference_loss(e, c, targets, ref_logp=None, bias=None, *, cu_seqlen
     params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
     e, c, bias = _head(what, e, c, bias, targets.shape)
     targets = _ids(what, "targets", targets, e.device)
-    ref, sums = _reference(what, ref_logp, targets, torch.float32, 2 * pairs)
+    ref, sums = _reference(what, ref_logp, targets, torch.float32, 2 * pairs, ref_per_token)
     loss, rewards = _LINEAR_PREFERENCE(e, c, bias, targets, ignore_index, ref, sums, cu, pairs, *params)
     return (loss, PreferenceRewards(rewards[:pairs], rewards[pairs:])) if return_rewards else loss
 

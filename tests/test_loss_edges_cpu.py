@@ -1,0 +1,42 @@
+"""Checks of the losses on log-probabilities at the edges of their range that run without a GPU."""
+
+import warnings
+
+import pytest
+import torch
+
+from mlx_cce import losses
+
+CPU = torch.device("cpu")
+
+
+def test_advantages_that_fit_tokens_and_sequences():
+    """Three packed tokens, three sequences: [0, 2), [2, 2) and [2, 3)."""
+    adv = torch.tensor([1.0, 2.0, 3.0])
+    with pytest.warns(UserWarning, match="advantages_per_token"):
+        assert losses._advantages("t", adv, (3,), 3, CPU)[1] is True
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert losses._advantages("t", adv, (3,), 3, CPU, True)[1] is True
+        assert losses._advantages("t", adv, (3,), 3, CPU, False)[1] is False
+        assert losses._advantages("t", adv[:1], (1,), 1, CPU)[1] is True  # (one token, one sequence: the same)
+        assert losses._advantages("t", adv, (8,), 3, CPU)[1] is False
+        assert losses._advantages("t", adv, (3,), 2, CPU)[1] is True
+    with pytest.raises(ValueError, match="advantages_per_token=True"):
+        losses._advantages("t", adv, (8,), 3, CPU, True)
+    with pytest.raises(ValueError, match="advantages_per_token=False"):
+        losses._advantages("t", adv, (3,), 2, CPU, False)
+
+
+def test_a_reference_that_fits_tokens_and_sequences():
+    x, ref = torch.zeros(4), torch.ones(4)
+    with pytest.warns(UserWarning, match="ref_per_token"):
+        got = losses._reference("t", ref, x, x.dtype, 4)
+    assert got[0] is not None and got[1] is None
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert losses._reference("t", ref, x, x.dtype, 4, True)[1] is None
+        ref, sums = losses._reference("t", ref.double(), x, x.dtype, 4, False)
+        assert ref is None and sums.dtype == torch.float32
+    with pytest.raises(ValueError, match="ref_per_token=False"):
+        losses._reference("t", x[:3], x[:3], x.dtype, 4, False)

@@ -76,3 +76,30 @@ def test_a_kl_term_of_weight_zero_is_only_measured(reduction):
         assert torch.isfinite(loss).all() and torch.equal(loss, bare) and torch.equal(*grads)
         out.append(stats.kl.item())
     assert 0 < out[0] < 10 and out[1] == float("inf")
+
+
+def test_as_many_tokens_as_sequences():
+    """Per sequence when asked: the values of the same batch with one token more, where
+    the shape says it."""
+    g = torch.Generator().manual_seed(31)
+    logp, old = -torch.rand(4, generator=g).cuda(), -torch.rand(4, generator=g).cuda()
+    val = torch.randn(4, generator=g).cuda()
+    cu = torch.tensor([0, 2, 2, 3, 4], device="cuda")
+    more = lambda t: torch.cat([t, t.new_zeros(1)])
+    got = mlx_cce.policy_loss(logp, old, val, cu_seqlens=cu, reduction="none", advantages_per_token=False)
+    want = mlx_cce.policy_loss(more(logp), more(old), val, cu_seqlens=cu, reduction="none")
+    assert torch.equal(got, want[:4])
+    token = mlx_cce.policy_loss(logp, old, val, cu_seqlens=cu, reduction="none", advantages_per_token=True)
+    assert not torch.equal(got, token)
+    with pytest.warns(UserWarning, match="per token"):
+        assert torch.equal(mlx_cce.policy_loss(logp, old, val, cu_seqlens=cu, reduction="none"), token)
+    got = mlx_cce.preference_loss(logp, val, cu_seqlens=cu, reduction="none", ref_per_token=False)
+    want = mlx_cce.preference_loss(more(logp), val, cu_seqlens=cu, reduction="none")
+    assert torch.equal(got, want)
+    e, c = torch.randn(4, 64, generator=g).bfloat16().cuda(), torch.randn(90, 64, generator=g).bfloat16().cuda()
+    t = torch.tensor([3, 50, 7, 89], device="cuda")
+    lp = mlx_cce.linear_log_probs(e, c, t)
+    assert torch.equal(mlx_cce.linear_policy_loss(e, c, t, old, val, cu_seqlens=cu, advantages_per_token=False),
+                       mlx_cce.policy_loss(lp, old, val, cu_seqlens=cu, advantages_per_token=False))
+    assert torch.equal(mlx_cce.linear_preference_loss(e, c, t, val, cu_seqlens=cu, ref_per_token=False),
+                       mlx_cce.preference_loss(lp, val, cu_seqlens=cu, ref_per_token=False))
