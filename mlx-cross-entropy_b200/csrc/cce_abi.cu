@@ -16,6 +16,7 @@
 #include <unordered_map>
 
 #include "kernels.cuh"
+#include "side_join.cuh"
 
 namespace cce {
 
@@ -248,6 +249,15 @@ struct SideStreams {
 };
 
 thread_local SideStreams g_side[64];
+
+struct StreamCalls {
+  using Stream = cudaStream_t;
+  using Event = cudaEvent_t;
+  static bool record(cudaEvent_t ev, cudaStream_t s) { return cudaEventRecord(ev, s) == cudaSuccess; }
+  static bool wait(cudaStream_t s, cudaEvent_t ev) { return cudaStreamWaitEvent(s, ev, 0) == cudaSuccess; }
+  static void synchronize(cudaStream_t s) { cudaStreamSynchronize(s); }
+};
+using Join = cce::SideJoin<StreamCalls>;
 
 int side_streams(SideStreams** out) {
   int dev = 0;
@@ -590,8 +600,10 @@ int cce_forward_q(const void* e, const CceQuantHead* head, const void* bias, int
   rc = side_streams(&ss);
   if (rc) return rc;
   CCE_CUDA_CHECK(cudaMemsetAsync(tgt, 0, (size_t)N * sizeof(float), s), "cce_forward_q memset");
+  Join join(s, ss->start);
   CCE_CUDA_CHECK(cudaEventRecord(ss->start, s), "cce_forward_q fork");
   CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->sq, ss->start, 0), "cce_forward_q fork");
+  join.forked(ss->sq);
   CCE_CUDA_CHECK(dequant_rows(head, 0, vq, D, dtype, cbuf[0], ss->sq), "cce_forward_q dequantise");
   CCE_CUDA_CHECK(cudaEventRecord(ss->ev_q[0], ss->sq), "cce_forward_q record");
   const int64_t nchunks = cce::ceil_div(V, vq);
@@ -619,6 +631,7 @@ int cce_forward_q(const void* e, const CceQuantHead* head, const void* bias, int
       CCE_CUDA_CHECK(cce::simt_forward(a, s), "cce_forward_q simt kernel");
     }
   }
+  join.joined();  // `s` has waited for every chunk
   CCE_CUDA_CHECK(cce::launch_lse_combine(part_m, part_s, nullptr, P, N, N, lse, nullptr, nullptr, s),
                  "cce_forward_q combine");
   return CCE_OK;
@@ -750,14 +763,20 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
   if (p.tc || qh) {
     rc = side_streams(&ss);
     if (rc) return rc;
+  }
+  Join join(s, ss ? ss->start : nullptr);
+  if (ss) {
     // fork: the side streams start after everything enqueued on `s` so far
     CCE_CUDA_CHECK(cudaEventRecord(ss->start, s), "cce_backward fork");
     if (p.tc) {
       CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->se, ss->start, 0), "cce_backward fork");
+      join.forked(ss->se);
       CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->sc, ss->start, 0), "cce_backward fork");
+      join.forked(ss->sc);
     }
     if (qh) {
       CCE_CUDA_CHECK(cudaStreamWaitEvent(ss->sq, ss->start, 0), "cce_backward fork");
+      join.forked(ss->sq);
       const int64_t rows0 = V < p.vc ? V : p.vc;
       CCE_CUDA_CHECK(dequant_rows(qh, 0, rows0, D, dtype, cbuf[0], ss->sq), "cce_backward_q dequantise");
       CCE_CUDA_CHECK(cudaEventRecord(ss->ev_q[0], ss->sq), "cce_backward record");
@@ -826,6 +845,7 @@ static int backward_impl(const void* e, const void* c, const CceQuantHead* qh, c
       }
     }
   }
+  join.joined();  // the last chunk's joins
   return CCE_OK;
 }
 
@@ -1386,6 +1406,7 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
     if (rc) return rc;
     se = ss->se, sc = ss->sc;
   }
+  Join join(s, fork ? ss->start : nullptr);
   void* gc = w.grad_c ? w.grad_c : grad_c;
   for (a.vc0 = 0; a.vc0 < a.V; a.vc0 += pl.vc) {
     a.vc_len = a.V - a.vc0 < pl.vc ? a.V - a.vc0 : pl.vc;
@@ -1397,7 +1418,9 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
     if (fork) {
       CCE_CUDA_CHECK(cudaEventRecord(ss->ev_l, s), what);
       CCE_CUDA_CHECK(cudaStreamWaitEvent(se, ss->ev_l, 0), what);
+      if (a.vc0 == 0) join.forked(se);
       CCE_CUDA_CHECK(cudaStreamWaitEvent(sc, ss->ev_l, 0), what);
+      if (a.vc0 == 0) join.forked(sc);
     }
     if (need_db)
       CCE_CUDA_CHECK(cce::launch_bias_sum(w.bias_part, cce::ceil_div(a.N, 32), v.R, pl.vc, a.vc_len, grad_bias + a.vc0, s),
@@ -1431,6 +1454,7 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
     CCE_CUDA_CHECK(cudaStreamWaitEvent(s, ss->ev_e, 0), what);
     CCE_CUDA_CHECK(cudaStreamWaitEvent(s, ss->ev_c, 0), what);
   }
+  join.joined();
   return CCE_OK;
 }
 

@@ -1,12 +1,16 @@
 """Checks of the losses on log-probabilities at the edges of their range that run without a GPU."""
 
+import shutil
+import subprocess
 import warnings
+from pathlib import Path
 
 import pytest
 import torch
 
 from mlx_cce import losses
 
+REPO = Path(__file__).resolve().parent.parent
 CPU = torch.device("cpu")
 
 
@@ -40,3 +44,19 @@ def test_a_reference_that_fits_tokens_and_sequences():
         assert ref is None and sums.dtype == torch.float32
     with pytest.raises(ValueError, match="ref_per_token=False"):
         losses._reference("t", x[:3], x[:3], x.dtype, 4, False)
+
+
+def test_side_streams_are_joined_when_a_call_fails(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = tmp_path / "side_join_check"
+    csrc = REPO / "mlx-cross-entropy_b200" / "csrc"
+    res = subprocess.run([gxx, "-std=c++17", "-O1", "-I", str(csrc), "-o", str(exe), str(REPO / "tests" / "side_join_check.cpp")],
+                         capture_output=True, text=True, timeout=120)
+    assert res.returncode == 0, res.stderr[-3000:]
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and "SIDE_JOIN_OK" in run.stdout, run.stdout
+    # every call that takes side streams holds the guard
+    abi = (csrc / "cce_abi.cu").read_text()
+    assert abi.count("side_streams(&ss)") == abi.count("Join join(") == abi.count("join.joined();") == 3
