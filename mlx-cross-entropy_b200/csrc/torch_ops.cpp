@@ -21,6 +21,9 @@
 
 #include "cce_b200.h"
 
+// Read from the file before it is loaded: another torch would fail on a symbol.
+__attribute__((used)) static const char built_for[] = CCE_BUILT_FOR;
+
 namespace {
 
 using at::Tensor;

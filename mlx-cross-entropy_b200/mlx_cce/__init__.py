@@ -17,6 +17,7 @@ and ``linear_cross_entropy_quantized`` for an affine group-quantised head
 
 Kernels: hand-written sm_100a CUDA in ``libcce_b200.so`` (tcgen05 / TMEM / TMA
 for 16-bit inputs, CUDA-core FFMA for float32), called through its C ABI.
+``losses`` (loaded on first use) has what a head is trained with afterwards.
 """
 
 from __future__ import annotations
@@ -133,5 +134,21 @@ class LinearCrossEntropy(torch.nn.Module):
 
 
 from .quantized import QuantizedClassifier, linear_cross_entropy_quantized  # noqa: E402
-from .losses import (PolicyStats, PreferenceRewards, linear_distillation_loss,  # noqa: E402
-                     linear_log_probs, linear_policy_loss, linear_preference_loss, policy_loss, preference_loss)
+
+# The losses on log-probabilities, imported when one is first used: their torch
+# operators (libcce_torch.so) belong to one torch, which the rest does not ask for.
+_LOSSES = ("policy_loss", "PolicyStats", "preference_loss", "PreferenceRewards", "linear_log_probs",
+           "linear_policy_loss", "linear_preference_loss", "linear_distillation_loss")
+
+
+def __getattr__(name):
+    if name not in _LOSSES and name != "losses":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    import importlib
+    losses = importlib.import_module(".losses", __name__)
+    globals().update({n: getattr(losses, n) for n in _LOSSES})
+    return globals()[name]
+
+
+def __dir__():
+    return sorted({*globals(), *_LOSSES, "losses"})

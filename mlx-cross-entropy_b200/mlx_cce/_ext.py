@@ -17,11 +17,14 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 import os
 from pathlib import Path
 
 import torch
+
+from . import build
 
 # CCE_LIB_PATH may point at another build of the same library (A/B timing).
 _LIB_PATH = Path(os.environ.get("CCE_LIB_PATH") or Path(__file__).resolve().parent / "libcce_b200.so")
@@ -207,20 +210,20 @@ def _load():
 lib = _load()
 
 
-def _load_torch_ops():
+@functools.cache
+def torch_ops():
     """The torch operators of the losses on log-probabilities (csrc/torch_ops.cpp), calling ``lib``."""
-    path = Path(__file__).resolve().parent / "libcce_torch.so"
+    path = build.TORCH_LIB_PATH
+    how = "build it with `python mlx-cross-entropy_b200/mlx_cce/build.py` (there is no fallback implementation)"
     if not path.exists():
-        raise ImportError(
-            f"{path} is missing: build it with `python mlx-cross-entropy_b200/mlx_cce/build.py` "
-            "(there is no fallback implementation)")
+        raise ImportError(f"{path} is missing: {how}")
+    made_for = build.torch_built_for(path)
+    if made_for != torch.__version__:
+        raise ImportError(f"{path} was built for torch {made_for}, this is torch {torch.__version__}: {how}")
     torch.ops.load_library(str(path))
     ops = torch.ops.cce_b200
     ops.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ops.functions()])
     return ops
-
-
-torch_ops = _load_torch_ops()
 
 
 def version() -> int:

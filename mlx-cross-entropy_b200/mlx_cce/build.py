@@ -76,16 +76,29 @@ def _run(cmd, what, verbose):
         raise RuntimeError(f"{what} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
 
 
+# Text in the torch operators' library, followed by the version of the torch that it was built for.
+_BUILT_FOR = b"cce_b200 operators for torch "
+
+
+def torch_built_for(path: Path = TORCH_LIB_PATH):
+    """The version of torch that the operators at ``path`` were built for (None: it does not say)."""
+    data = path.read_bytes()
+    at = data.find(_BUILT_FOR)
+    return None if at < 0 else data[at + len(_BUILT_FOR):data.index(b"\0", at)].decode()
+
+
 def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the torch operators if missing or stale; return their path."""
-    if not force and not _stale(TORCH_LIB_PATH, [TORCH_SOURCE, *INCLUDE.glob("*.h")]):
-        return TORCH_LIB_PATH
+    """Compile the torch operators if missing, stale or of another torch; return their path."""
     import torch
+    if not force and not _stale(TORCH_LIB_PATH, [TORCH_SOURCE, *INCLUDE.glob("*.h")]) \
+            and torch_built_for() == torch.__version__:
+        return TORCH_LIB_PATH
     home = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc_path()).resolve().parent.parent
     tmp = TORCH_LIB_PATH.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}", f"-I{home / 'include'}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f'-DCCE_BUILT_FOR="{_BUILT_FOR.decode()}{torch.__version__}"', f"-I{INCLUDE}", f"-I{home / 'include'}",
            f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{cuda / 'include'}", str(TORCH_SOURCE),
            "-o", str(tmp), f"-L{home / 'lib'}", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     _run(cmd, "g++", verbose)

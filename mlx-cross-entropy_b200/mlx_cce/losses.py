@@ -38,12 +38,13 @@ import torch
 from . import _ext
 
 # The operators (csrc/torch_ops.cpp), called without the overload lookup.
-_POLICY = _ext.torch_ops.policy_loss.default
-_PREFERENCE = _ext.torch_ops.preference_loss.default
-_LOG_PROBS = _ext.torch_ops.log_probs.default
-_LINEAR_POLICY = _ext.torch_ops.linear_policy_loss.default
-_LINEAR_PREFERENCE = _ext.torch_ops.linear_preference_loss.default
-_DISTILLATION = _ext.torch_ops.distillation.default
+_OPS = _ext.torch_ops()
+_POLICY = _OPS.policy_loss.default
+_PREFERENCE = _OPS.preference_loss.default
+_LOG_PROBS = _OPS.log_probs.default
+_LINEAR_POLICY = _OPS.linear_policy_loss.default
+_LINEAR_PREFERENCE = _OPS.linear_preference_loss.default
+_DISTILLATION = _OPS.distillation.default
 
 POLICY_REDUCTIONS = {"mean": _ext.CCE_REDUCE_MEAN, "sum": _ext.CCE_REDUCE_SUM,
                      "sequence": _ext.CCE_REDUCE_SEQUENCE, "none": _ext.CCE_REDUCE_NONE}

@@ -1,14 +1,16 @@
 """Checks of the losses on log-probabilities at the edges of their range that run without a GPU."""
 
+import os
 import shutil
 import subprocess
+import sys
 import warnings
 from pathlib import Path
 
 import pytest
 import torch
 
-from mlx_cce import losses
+from mlx_cce import build, losses
 
 REPO = Path(__file__).resolve().parent.parent
 CPU = torch.device("cpu")
@@ -60,3 +62,35 @@ def test_side_streams_are_joined_when_a_call_fails(tmp_path):
     # every call that takes side streams holds the guard
     abi = (csrc / "cce_abi.cu").read_text()
     assert abi.count("side_streams(&ss)") == abi.count("Join join(") == abi.count("join.joined();") == 3
+
+
+def _python(code, package):
+    env = dict(os.environ, PYTHONPATH=str(package))
+    return subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env, cwd=package)
+
+
+def test_the_cross_entropy_does_not_need_the_torch_operators(tmp_path):
+    """Without libcce_torch.so, and with one of another torch: the package imports, and the
+    losses on log-probabilities say what is wrong when one is first asked for."""
+    src = REPO / "mlx-cross-entropy_b200" / "mlx_cce"
+    pkg = tmp_path / "mlx_cce"
+    pkg.mkdir()
+    for f in src.glob("*.py"):
+        shutil.copy(f, pkg)
+    (pkg / "libcce_b200.so").symlink_to(src / "libcce_b200.so")
+    use = "import mlx_cce; mlx_cce.linear_cross_entropy; print('imported'); mlx_cce.{}; print('loaded')"
+    for name in ("policy_loss", "losses"):
+        run = _python(use.format(name), tmp_path)
+        assert run.stdout == "imported\n" and "ImportError" in run.stderr and "is missing" in run.stderr, run.stderr
+    data = (src / "libcce_torch.so").read_bytes()
+    here = ("torch " + torch.__version__).encode()
+    assert data.count(here) >= 1 and build.torch_built_for() == torch.__version__
+    other = ("torch " + "0" * len(torch.__version__)).encode()
+    (pkg / "libcce_torch.so").write_bytes(data.replace(here, other))
+    run = _python(use.format("linear_log_probs"), tmp_path)
+    assert run.stdout == "imported\n" and "ImportError" in run.stderr and "built for torch 000" in run.stderr, run.stderr
+    shutil.copy(src / "libcce_torch.so", pkg)
+    run = _python(use.format("PolicyStats") + "; assert set(mlx_cce.__all__) <= set(dir(mlx_cce))", tmp_path)
+    assert run.stdout == "imported\nloaded\n", run.stderr
+    run = _python("import mlx_cce; mlx_cce.nothing", tmp_path)
+    assert "AttributeError" in run.stderr
