@@ -9,6 +9,7 @@
 // library's functions come as addresses (bind), so that whichever build of it is
 // loaded is the one that is called.
 #include <ATen/ATen.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -105,7 +106,20 @@ Tensor bytes(size_t n, const Tensor& like) {
 }
 Tensor f32(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, like.options().dtype(at::kFloat)); }
 
-Tensor upstream(const Tensor& g) { return g.to(at::kFloat).contiguous(); }
+// The operators read and write memory that torch's tracers do not see: a trace of one
+// would hold its buffers and none of its kernels.
+void plain(const Tensor& t) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  TORCH_CHECK(!t.key_set().has(c10::DispatchKey::Python) && !Modes::get_mode(Key::PROXY) && !Modes::get_mode(Key::FAKE),
+              "the losses on log-probabilities run on plain CUDA tensors and cannot be traced or given tensor "
+              "subclasses: call them outside of the traced function (torch.compiler.disable)");
+}
+
+Tensor upstream(const Tensor& g) {
+  TORCH_CHECK(g.has_storage(), "the losses on log-probabilities take one gradient at a time (not is_grads_batched)");
+  return g.to(at::kFloat).contiguous();
+}
 
 // Gradients for a backward pass that is itself recorded: a second derivative is
 // an error, not a wrong zero.
@@ -486,6 +500,7 @@ CcePreferenceParams preference_params(at::ArrayRef<double> x, int64_t kind, int6
 std::tuple<Tensor, Tensor> policy_loss(const Tensor& logp, const OptTensor& old, const OptTensor& ref, const Tensor& adv,
                                        const OptTensor& mask, const OptTensor& cu, int64_t S, at::ArrayRef<double> params,
                                        int64_t reduction, bool per_token) {
+  plain(logp);
   auto out = PolicyLoss::apply(logp, PolicyArgs{old, ref, adv, mask, cu, S, policy_params(params, reduction, per_token)});
   return {out[0], out[1]};
 }
@@ -493,6 +508,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logp, const OptTensor& old,
 std::tuple<Tensor, Tensor> preference_loss(const Tensor& logp, const OptTensor& ref, const OptTensor& ref_sums,
                                            const OptTensor& mask, const OptTensor& cu, int64_t pairs,
                                            at::ArrayRef<double> params, int64_t kind, int64_t reduction, bool by_length) {
+  plain(logp);
   auto out = PreferenceLoss::apply(
       logp, PreferenceArgs{ref, ref_sums, mask, cu, pairs, preference_params(params, kind, reduction, by_length)});
   return {out[0], out[1]};
@@ -504,6 +520,7 @@ HeadArgs head_args(const Tensor& targets, std::optional<int64_t> ignore_index) {
 
 Tensor log_probs(const Tensor& e, const Tensor& c, const OptTensor& bias, const Tensor& targets,
                  std::optional<int64_t> ignore_index) {
+  plain(e);
   return LogProbs::apply(e, c, bias, head_args(targets, ignore_index));
 }
 
@@ -512,6 +529,7 @@ std::tuple<Tensor, Tensor> linear_policy_loss(const Tensor& e, const Tensor& c, 
                                               const OptTensor& old, const OptTensor& ref, const Tensor& adv,
                                               const OptTensor& cu, int64_t S, at::ArrayRef<double> params,
                                               int64_t reduction, bool per_token) {
+  plain(e);
   auto out = LinearPolicyLoss::apply(
       e, c, bias, std::make_pair(head_args(targets, ignore_index),
                                  PolicyArgs{old, ref, adv, std::nullopt, cu, S, policy_params(params, reduction, per_token)}));
@@ -523,6 +541,7 @@ std::tuple<Tensor, Tensor> linear_preference_loss(const Tensor& e, const Tensor&
                                                   const OptTensor& ref, const OptTensor& ref_sums, const OptTensor& cu,
                                                   int64_t pairs, at::ArrayRef<double> params, int64_t kind,
                                                   int64_t reduction, bool by_length) {
+  plain(e);
   auto out = LinearPreferenceLoss::apply(
       e, c, bias,
       std::make_pair(head_args(targets, ignore_index),
@@ -533,6 +552,7 @@ std::tuple<Tensor, Tensor> linear_preference_loss(const Tensor& e, const Tensor&
 
 Tensor distillation(const Tensor& e, const Tensor& c, const OptTensor& bias, const Tensor& ids, const Tensor& teacher,
                     const OptTensor& mask, double temperature, bool tail, int64_t reduction) {
+  plain(e);
   return Distillation::apply(e, c, bias,
                              DistillArgs{ids, teacher, mask, CceDistillParams{temperature, tail, (int32_t)reduction}});
 }

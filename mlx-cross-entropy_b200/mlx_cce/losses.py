@@ -68,6 +68,12 @@ class PreferenceRewards(NamedTuple):
 # argument checks
 # ---------------------------------------------------------------------------
 
+def _untraced(what):
+    """torch.compile breaks its graph here: the call runs as it is, between two graphs."""
+    if torch.compiler.is_compiling():
+        raise RuntimeError(f"[{what}] cannot be part of a traced graph")
+
+
 def _constant(t):
     """t as a kernel input: contiguous, cut from the graph."""
     if t.requires_grad:
@@ -289,6 +295,7 @@ def policy_loss(logp, old_logp, advantages, *, ref_logp=None, mask=None, cu_seql
         ``return_stats`` a tuple ``(loss, stats)``.
     """
     what = "policy_loss"
+    _untraced(what)
     logp = _logp(what, logp)
     S, cu = _sequences(what, logp.shape, cu_seqlens, logp.device)
     adv, per_token = _advantages(what, advantages, logp.shape, S, logp.device, advantages_per_token)
@@ -329,6 +336,7 @@ def preference_loss(logp, ref_logp=None, *, mask=None, cu_seqlens=None, beta=0.1
         ``return_rewards`` a tuple ``(loss, rewards)``.
     """
     what = "preference_loss"
+    _untraced(what)
     logp = _logp(what, logp)
     pairs, cu = _pairs(what, logp.shape, cu_seqlens, logp.device)
     params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
@@ -352,6 +360,7 @@ def linear_log_probs(e, c, targets, bias=None, *, ignore_index=-100):
         differentiable with respect to e, c and bias.
     """
     what = "linear_log_probs"
+    _untraced(what)
     e, c, bias = _head(what, e, c, bias, targets.shape)
     logp = _LOG_PROBS(e, c, bias, _ids(what, "targets", targets, e.device), ignore_index)
     return logp.view(targets.shape)
@@ -368,6 +377,7 @@ def linear_policy_loss(e, c, targets, old_logp, advantages, bias=None, *, ref_lo
     targets.  The other arguments and the result are those of ``policy_loss``.
     """
     what = "linear_policy_loss"
+    _untraced(what)
     S, cu = _sequences(what, targets.shape, cu_seqlens, targets.device)
     adv, per_token = _advantages(what, advantages, targets.shape, S, targets.device, advantages_per_token)
     params = _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_token)
@@ -392,6 +402,7 @@ def linear_preference_loss(e, c, targets, ref_logp=None, bias=None, *, cu_seqlen
     result are those of ``preference_loss``.
     """
     what = "linear_preference_loss"
+    _untraced(what)
     pairs, cu = _pairs(what, targets.shape, cu_seqlens, targets.device)
     params = _preference_params(what, beta, margin, loss_type, label_smoothing, length_normalize, reduction)
     e, c, bias = _head(what, e, c, bias, targets.shape)
@@ -428,6 +439,7 @@ def linear_distillation_loss(e, c, teacher_ids, teacher_logprobs, bias=None, *, 
         with respect to e, c and bias.
     """
     what = "linear_distillation_loss"
+    _untraced(what)
     params = _distill_params(what, temperature, tail, reduction)
     if teacher_ids.dim() < 1 or teacher_ids.shape != teacher_logprobs.shape:
         raise ValueError(f"[{what}] teacher_ids and teacher_logprobs must be [..., K] of one shape, got "

@@ -241,3 +241,60 @@ def test_values_far_above_the_others(dtype, D):
     go[11] = 0.0
     _log_probs_of_rest(e, c, b, t, go, 11, 5)
     _ext.device_status()
+
+
+# ---------------------------------------------------------------------------
+# torch's transforms
+# ---------------------------------------------------------------------------
+
+def _transformed():
+    """(name, a function of one tensor around each loss, its argument)"""
+    g = torch.Generator().manual_seed(61)
+    x, old = -torch.rand(4, 50, generator=g).cuda(), -torch.rand(4, 50, generator=g).cuda()
+    adv = torch.randn(4, generator=g).cuda()
+    e, c, _, t, g = head(200, 64, 300, torch.bfloat16, 62)
+    tlp, ids = (v.cuda() for v in teacher(e, c, None, 4, g))
+    e, c, t = e.cuda(), c.cuda(), t.cuda()
+    return [("policy", lambda v: mlx_cce.policy_loss(v * 1.5, old, adv) * 2, x),
+            ("preference", lambda v: mlx_cce.preference_loss(v * 1.5, old) * 2, x),
+            ("log_probs", lambda v: mlx_cce.linear_log_probs(v * 1.5, c, t).sum() * 2, e),
+            ("linear_policy", lambda v: mlx_cce.linear_policy_loss((v * 1.5).view(4, 50, 64), c, t.view(4, 50), old, adv) * 2,
+             e),
+            ("linear_preference", lambda v: mlx_cce.linear_preference_loss((v * 1.5).view(4, 50, 64), c, t.view(4, 50)) * 2,
+             e),
+            ("distillation", lambda v: mlx_cce.linear_distillation_loss(v * 1.5, c, ids, tlp) * 2, e)]
+
+
+@pytest.mark.parametrize("k", range(6))
+def test_compiled_functions_break_their_graph_at_the_losses(k):
+    _, f, x = _transformed()[k]
+    out = []
+    for fn in (f, torch.compile(f, backend="aot_eager")):
+        torch._dynamo.reset()
+        y = x.clone().requires_grad_(True)
+        loss = fn(y)
+        out.append((loss.detach(), torch.autograd.grad(loss, [y])[0]))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    torch._dynamo.reset()
+    with pytest.raises(Exception, match="traced graph|Observed exception"):
+        torch.compile(f, backend="eager", fullgraph=True)(x)
+    torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("k", range(6))
+def test_traces_and_transforms_are_refused_or_right(k):
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    _, f, x = _transformed()[k]
+    with pytest.raises(RuntimeError, match="cannot be traced"):  # (a trace would hold buffers and no kernel)
+        make_fx(f)(x)
+    xs = torch.stack([x, 0.5 * x])
+    assert torch.equal(torch.func.vmap(f)(xs), torch.stack([f(v) for v in xs]))  # (one call for each)
+    with pytest.raises(RuntimeError, match="functorch transforms"):
+        torch.func.grad(f)(x)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="jvp is not implemented"):
+        f(forward_ad.make_dual(x, torch.ones_like(x)))
+    y = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="one gradient at a time"):
+        torch.autograd.grad(f(y), [y], torch.ones(2, device="cuda"), is_grads_batched=True)
+    _ext.device_status()
