@@ -153,23 +153,23 @@ def _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_tok
 
 def _is_per_token(what, name, got, shape, S, per_token, argument):
     """Whether values of shape ``got`` are one per token, not one per sequence."""
-    fits = {True: got == tuple(shape), False: got == (S,)}
+    tokens, seqs = got == shape, got == (S,)
     if per_token is not None:
-        if not fits[bool(per_token)]:
+        if not (tokens if per_token else seqs):
             raise ValueError(f"[{what}] {name} must be {tuple(shape) if per_token else (S,)} with {argument}="
-                             f"{bool(per_token)}, got {got}")
+                             f"{bool(per_token)}, got {tuple(got)}")
         return bool(per_token)
-    if not any(fits.values()):
-        raise ValueError(f"[{what}] {name} must be per token {tuple(shape)} or per sequence ({S},), got {got}")
-    if all(fits.values()) and S > 1:
-        warnings.warn(f"[{what}] {name} of shape {got} could be one per token or one per sequence and are read per "
-                      f"token: say {argument}=True or False", stacklevel=4)
-    return fits[True]
+    if not (tokens or seqs):
+        raise ValueError(f"[{what}] {name} must be per token {tuple(shape)} or per sequence ({S},), got {tuple(got)}")
+    if tokens and seqs and S > 1:
+        warnings.warn(f"[{what}] {name} of shape {tuple(got)} could be one per token or one per sequence and are read "
+                      f"per token: say {argument}=True or False", stacklevel=4)
+    return tokens
 
 
 def _advantages(what, advantages, shape, S, dev, per_token=None):
     """(float32 advantages, one per token?)"""
-    per_token = _is_per_token(what, "advantages", tuple(advantages.shape), shape, S, per_token, "advantages_per_token")
+    per_token = _is_per_token(what, "advantages", advantages.shape, shape, S, per_token, "advantages_per_token")
     if not advantages.is_floating_point():
         raise ValueError(f"[{what}] advantages must be floating point, got {advantages.dtype}")
     if advantages.device != dev:
@@ -254,7 +254,7 @@ def _reference(what, ref_logp, tokens, dtype, S, per_token=None):
     """(per-token reference or None, per-sequence sums or None)"""
     if ref_logp is None:
         return None, None
-    if _is_per_token(what, "ref_logp", tuple(ref_logp.shape), tokens.shape, S, per_token, "ref_per_token"):
+    if _is_per_token(what, "ref_logp", ref_logp.shape, tokens.shape, S, per_token, "ref_per_token"):
         return _per_token(what, "ref_logp", ref_logp, tokens, dtype), None
     if not ref_logp.is_floating_point() or ref_logp.device != tokens.device:
         raise ValueError(f"[{what}] ref_logp must be floating point on {tokens.device}")
