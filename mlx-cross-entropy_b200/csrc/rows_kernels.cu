@@ -145,7 +145,7 @@ __device__ __forceinline__ void fold(float& m, float& s, float mp, float sp) {
   m = M;
 }
 
-// (max, sum) of the block's 32 rows over P partials, into sm[0][..], ss[0][..].
+// (max, sum) of the block's kStRows rows over P partials, into sm[0][..], ss[0][..].
 __device__ __forceinline__ void fold_rows(const float* __restrict__ part_m, const float* __restrict__ part_s, int64_t P,
                                           int64_t N, int64_t row, bool live, float (*sm)[kStRows],
                                           float (*ss)[kStRows]) {

@@ -19,8 +19,9 @@
 // only a segment of K; the epilogue warps add each of those partial logits to
 // the total in their registers (128 per thread, round to nearest).  The two TMEM
 // accumulators take the segments in turn, so the MMAs run on while the adds are
-// made.  A segment of 4 K-blocks is 16 MMAs, about 2000 cycles; its add takes
-// about 500 of the issue slots of the 8 epilogue warps.
+// made.  A segment of 4 K-blocks (float16 row statistics; segments() has the others)
+// is 16 MMAs, about 2000 cycles; its add takes about 500 of the issue slots of the
+// 8 epilogue warps.
 //
 // What is left of the drift is added back in expectation.  A step that rounds
 // an accumulator a towards zero loses on average half a unit in its last place,
@@ -40,8 +41,15 @@
 //   float32, D = 512       1.29 1.03 0.93 1.00 1.23   (3.0)
 // bfloat16 runs on segments of 32 steps with k = 4: 0.68 (D = 2304), 0.75 (4096),
 // 1.08 (512), for half the adds.  With one accumulator for all of K a bfloat16
-// D = 2304 head has 5.7.  Gradients and dlogits, which are rounded to 16 bits or
-// summed over far smaller terms, take segments of 64 steps.
+// D = 2304 head has 5.7.  16-bit gradients and dlogits, which are rounded to 16 bits,
+// take segments of 64 steps; float32 products are all summed in segments of 8.
+//
+// k is a fit to logits that grow steadily.  Where one channel carries a logit alone,
+// the cuts that follow it in its segment decide: all of them when it comes first,
+// one when it comes last, with the same k 2^-23 added back.  So k lies between the
+// two extremes, and what is left is at most 5e-7 of the logit either way: mean errors
+// at a logit of 14, first / last in a segment, in units of 1e-6: bfloat16 4.6 / -6.3,
+// float16 0.7 / -4.7, float32 -0.3 / -2.8 (one accumulator for D = 4096: 74).
 //
 // Float32 inputs.  x = (hi + 2^-11 lo) / s with hi, lo float16 and s a power of two that
 // puts the tensor's largest value below 2^14: hi holds 11 bits and lo the next 11, of

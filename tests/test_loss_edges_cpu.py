@@ -94,3 +94,61 @@ def test_the_cross_entropy_does_not_need_the_torch_operators(tmp_path):
     assert run.stdout == "imported\nloaded\n", run.stderr
     run = _python("import mlx_cce; mlx_cce.nothing", tmp_path)
     assert "AttributeError" in run.stderr
+
+
+# ---------------------------------------------------------------------------
+# the tensor cores' rounding towards zero, restated
+# ---------------------------------------------------------------------------
+
+def drift_inputs(dtype, D=4096, N=256, V=512):
+    """Rows with one logit of about 14 and targets elsewhere: the log-sum-exp takes the
+    large logit's drift, and no drift of the target's own cancels it."""
+    from test_linear_losses_gpu import head
+    e, c, _, t, _ = head(N, D, V, dtype, 5, peak=14.0)
+    return e, c, t, (t + 1) % V
+
+
+def drift_bound(e, c, peak, target, seg, k):
+    """A segment of S accumulating steps whose partial logit p grows steadily loses 0.36 S
+    2^-24 |p| on average, less with noise on the way, and k 2^-23 |p| are added back:
+    what is left is at most k 2^-23 |p| (0.36 S / 2 < 2 k), summed over the segments of both
+    logits.  2^-20 for the exponentials, the logarithm and float32's last places."""
+    size = 0.0
+    for v in (peak, target):
+        size = size + (e.double() * c[v].double()).view(len(e), -1, seg).sum(2).abs().sum(1)
+    return k * 2.0 ** -23 * float(size.mean()) + 2.0 ** -20
+
+
+SEGMENTS = {torch.bfloat16: (512, 4), torch.float16: (256, 3), torch.float32: (128, 2)}  # columns, k
+
+
+def to_zero(x):
+    """64-bit values cut to float32 towards zero."""
+    y = x.float()
+    return torch.where(y.double().abs() > x.abs(), torch.nextafter(y, torch.zeros_like(y)), y).double()
+
+
+def accumulated(a, b, seg, k):
+    """Logits sum_k a b in accumulators of ``seg`` columns, 16 a step, each step cut
+    towards zero; the partials times 1 + k 2^-23 added in float32."""
+    steps = (a.double() * b.double()).view(len(a), -1, 16).sum(2)
+    z = torch.zeros(len(a))
+    for s in range(0, steps.shape[1], seg // 16):
+        acc = torch.zeros(len(a), dtype=torch.float64)
+        for j in range(s, min(s + seg // 16, steps.shape[1])):
+            acc = to_zero(acc + steps[:, j])
+        z = (z.double() + acc * (1 + k * 2.0 ** -23)).float()
+    return z.double()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_drift_bound_tells_one_accumulator_from_several(dtype):
+    e, c, peak, target = drift_inputs(dtype)
+    seg, k = SEGMENTS[dtype]
+    bound = drift_bound(e, c, peak, target, seg, k)
+    exact = [(e.double() * c[v].double()).sum(1) for v in (peak, target)]
+    # the target's logit less the log-sum-exp, of which the large logit is nearly all
+    one, several = ([accumulated(e, c[v], s, f) - x for v, x in zip((peak, target), exact)]
+                    for s, f in ((e.shape[1], 0), (seg, k)))
+    assert float((several[1] - several[0]).mean().abs()) < bound
+    assert float((one[1] - one[0]).mean().abs()) > 4 * bound

@@ -10,6 +10,7 @@ import torch
 import mlx_cce
 import token_loss_ref as R
 from mlx_cce import _ext
+from test_loss_edges_cpu import SEGMENTS, drift_bound, drift_inputs
 from test_linear_losses_gpu import DTYPES, U, Bounds, distill64, head, leaves, teacher
 
 pytestmark = pytest.mark.gpu
@@ -298,3 +299,47 @@ def test_traces_and_transforms_are_refused_or_right(k):
     with pytest.raises(RuntimeError, match="one gradient at a time"):
         torch.autograd.grad(f(y), [y], torch.ones(2, device="cuda"), is_grads_batched=True)
     _ext.device_status()
+
+
+# ---------------------------------------------------------------------------
+# the tensor cores' rounding towards zero
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_drift_of_a_large_logit(dtype):
+    """The mean error of log-probabilities beside a logit of 14, which one accumulator
+    would leave 7e-5 off (test_the_drift_bound_tells_one_accumulator_from_several)."""
+    e, c, peak, target = drift_inputs(dtype)
+    lp = mlx_cce.linear_log_probs(e.cuda(), c.cuda(), target.cuda()).cpu().double()
+    want = torch.log_softmax(e.double() @ c.double().t(), 1).gather(1, target[:, None])[:, 0]
+    err = float((lp - want).mean())
+    assert abs(err) < drift_bound(e, c, peak, target, *SEGMENTS[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("place", ["first", "last"])
+def test_drift_of_a_logit_that_one_channel_carries(place, dtype):
+    """A logit of 14 in the first step of its segment is cut in each of the S steps that
+    follow, half a last place, 2^-21, each on average; in the last step it is cut
+    once.  k 2^-23 of it are added back for both: a mean error in between."""
+    seg, k = SEGMENTS[dtype]
+    steps = seg // 16
+    g = torch.Generator().manual_seed(6)
+    N, D, V = 256, 2048, 512
+    e = torch.randn(N, D, generator=g)
+    c = torch.randn(V, D, generator=g) * D ** -0.5
+    ch = 3 * seg + (0 if place == "first" else seg - 1)
+    c[:, ch] = 0.0
+    e[:, ch], c[0, ch] = 7.0, 2.0
+    e, c = e.to(dtype), c.to(dtype)
+    target = torch.arange(N) % (V - 1) + 1
+    z = e.double() @ c.double().t()
+    e, z = e[z[:, 0] > 8.5], z[z[:, 0] > 8.5]  # (one binade)
+    e, z = e[z[:, 0] < 15.5], z[z[:, 0] < 15.5]
+    target = target[:len(e)]
+    lp = mlx_cce.linear_log_probs(e.cuda(), c.cuda(), target.cuda()).cpu().double()
+    err = float((lp - torch.log_softmax(z, 1).gather(1, target[:, None])[:, 0]).mean())
+    back = k * 2.0 ** -23 * 14
+    # (the error of the log-sum-exp, negated: what was added back and what was cut, to
+    # an eighth, and 2^-20 for everything after the sum)
+    assert -1.125 * back - 2.0 ** -20 <= err <= 1.125 * (steps * 2.0 ** -21 - back) + 2.0 ** -20
