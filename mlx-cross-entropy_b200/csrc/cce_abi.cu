@@ -7,6 +7,8 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <cfloat>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1022,7 +1024,8 @@ int cce_policy_loss_forward(const void* logp, const void* old_logp, const void* 
                 params->clip_low, params->clip_high);
   if (!(params->dual_clip == 0.0 || params->dual_clip > 1.0))
     return fail(CCE_ERR_ARG, "%s: dual_clip must be 0 or above 1, got %g", what, params->dual_clip);
-  if (params->kl_coef != params->kl_coef) return fail(CCE_ERR_ARG, "%s: kl_coef is NaN", what);
+  if (!(fabs(params->kl_coef) <= FLT_MAX))
+    return fail(CCE_ERR_ARG, "%s: kl_coef must be finite in float32, got %g", what, params->kl_coef);
   const int red = params->reduction;
   if (red < CCE_REDUCE_MEAN || red > CCE_REDUCE_NONE) return fail(CCE_ERR_ARG, "%s: reduction code %d", what, red);
   if (!loss && !(red == CCE_REDUCE_NONE && N == 0)) return fail(CCE_ERR_ARG, "%s: NULL loss", what);
@@ -1347,8 +1350,9 @@ int check_rows(int64_t N, int64_t D, int64_t V, int64_t K, int dtype, const char
 
 int check_distill(const CceDistillParams* p, const char* what) {
   if (!p) return fail(CCE_ERR_ARG, "%s: NULL params", what);
-  if (!(p->temperature > 0.0) || p->temperature > 1e30)
-    return fail(CCE_ERR_ARG, "%s: temperature must be positive, got %g", what, p->temperature);
+  // (the kernels hold it and its reciprocal in float32)
+  if (!(p->temperature >= 1e-30 && p->temperature <= 1e30))
+    return fail(CCE_ERR_ARG, "%s: temperature must be in [1e-30, 1e30], got %g", what, p->temperature);
   if (p->reduction != CCE_REDUCE_MEAN && p->reduction != CCE_REDUCE_SUM && p->reduction != CCE_REDUCE_NONE)
     return fail(CCE_ERR_ARG, "%s: reduction code %d", what, p->reduction);
   return CCE_OK;

@@ -146,8 +146,8 @@ def _policy_params(what, clip, clip_high, dual_clip, kl_coef, reduction, per_tok
         raise ValueError(f"[{what}] clip must be in [0, 1] and clip_high >= 0, got {clip} and {clip_high}")
     if dual_clip is not None and not dual_clip > 1:
         raise ValueError(f"[{what}] dual_clip must be above 1, got {dual_clip}")
-    if not math.isfinite(kl_coef):
-        raise ValueError(f"[{what}] kl_coef must be finite, got {kl_coef}")
+    if not abs(kl_coef) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"[{what}] kl_coef must be finite in float32, got {kl_coef}")
     return [float(clip), float(high), float(dual_clip or 0.0), float(kl_coef)], POLICY_REDUCTIONS[reduction], per_token
 
 
@@ -245,8 +245,8 @@ def _ids(what, name, t, dev):
 def _distill_params(what, temperature, tail, reduction):
     if reduction not in PREFERENCE_REDUCTIONS:
         raise ValueError(f"[{what}] Unknown reduction: {reduction}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"[{what}] temperature must be positive, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:  # (held in float32, and its reciprocal)
+        raise ValueError(f"[{what}] temperature must be in [1e-30, 1e30], got {temperature}")
     return float(temperature), bool(tail), PREFERENCE_REDUCTIONS[reduction]
 
 

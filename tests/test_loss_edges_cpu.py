@@ -1,5 +1,6 @@
 """Checks of the losses on log-probabilities at the edges of their range that run without a GPU."""
 
+import ctypes
 import os
 import shutil
 import subprocess
@@ -10,7 +11,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from mlx_cce import build, losses
+from mlx_cce import _ext, build, losses
 
 REPO = Path(__file__).resolve().parent.parent
 CPU = torch.device("cpu")
@@ -62,6 +63,26 @@ def test_side_streams_are_joined_when_a_call_fails(tmp_path):
     # every call that takes side streams holds the guard
     abi = (csrc / "cce_abi.cu").read_text()
     assert abi.count("side_streams(&ss)") == abi.count("Join join(") == abi.count("join.joined();") == 3
+
+
+@pytest.mark.parametrize("bad", [0.0, -1.0, 1e-39, 1e31, float("inf"), float("nan")])
+def test_temperatures_past_float32_are_refused(bad):
+    with pytest.raises(ValueError, match="temperature"):
+        losses._distill_params("t", bad, False, "mean")
+    losses._distill_params("t", 1e-30, False, "mean")
+    one, p = ctypes.c_void_p(256), _ext.CceDistillParams(bad, 0, 0)  # (refused before anything is followed)
+    assert _ext.lib.cce_distill_forward(one, one, None, 0, one, 8, one, None, 4, 8, 16, 3, 2, ctypes.byref(p), one, None, 0,
+                                        None, 0, None) == _ext.CCE_ERR_ARG
+
+
+@pytest.mark.parametrize("bad", [1e39, -1e39, float("inf"), float("nan")])
+def test_kl_weights_past_float32_are_refused(bad):
+    with pytest.raises(ValueError, match="kl_coef"):
+        losses._policy_params("t", 0.2, None, None, bad, "mean", True)
+    losses._policy_params("t", 0.2, None, None, -3e38, "mean", True)
+    one, p = ctypes.c_void_p(256), _ext.CcePolicyParams(0.2, 0.2, 0.0, bad, 0, 1)
+    assert _ext.lib.cce_policy_loss_forward(one, None, None, 0, one, None, None, 8, 2, ctypes.byref(p), one, one, one, one,
+                                            None, 0, None) == _ext.CCE_ERR_ARG
 
 
 def _python(code, package):
