@@ -390,38 +390,36 @@ __device__ __forceinline__ void kl3(float q, float& kl, float& em1) {
   em1 = small ? q + near : far;
 }
 
-// Whether d = x - old lies above the borders, decided on the exact difference:
-// d is rounded to float32, so only next to a border are 64 bits needed.
-struct Beyond {
-  bool hi, lo, dual;
-};
-__device__ __forceinline__ Beyond beyond(const Policy& P, float d, float x, float old) {
-  const float hi = (float)P.log_hi, lo = (float)P.log_lo, dual = (float)P.log_dual;
-  Beyond b{d > hi, d < lo, d > dual};
-  const float near = 1e-6f * (1.f + fabsf(d));
-  if (fabsf(d - hi) <= near || fabsf(d - lo) <= near || fabsf(d - dual) <= near) {
+// Whether d = x - old lies above (below) the border, decided on the exact difference:
+// d is rounded to float32, so only next to the border are 64 bits needed.
+__device__ __forceinline__ bool beyond(bool above, float d, float x, float old, double border) {
+  const float b = (float)border;
+  if (fabsf(d - b) <= 1e-6f * (1.f + fabsf(d))) {
     const double e = (double)x - (double)old;
-    b = Beyond{e > P.log_hi, e < P.log_lo, e > P.log_dual};
+    return above ? e > border : e < border;
   }
-  return b;
+  return above ? d > b : d < b;
 }
 
 __device__ __forceinline__ TokenOut policy_token(const Policy& P, float x, float old, float ref, float A) {
   // (without old the ratio is 1; a NaN log-probability stays one)
   const float d = P.old ? x - old : (x == x ? 0.f : x);
-  const float r = P.old ? expf(d) : 1.f + d;
-  const Beyond b = beyond(P, d, x, P.old ? old : x);
+  if (!P.old) old = x;
+  // (an advantage of 0 asks nothing of a ratio past float32's range, e^88.7: its
+  // product is 0 whatever finite number stands here, and NaN stays)
+  const float r = A == 0.f ? d : expf(d);
   const bool pos = A > 0.f, neg = A < 0.f;
-  float bounded = r;
-  bounded = pos && b.hi ? P.hi : bounded;
-  bounded = neg && b.lo ? P.lo : bounded;
-  bounded = neg && P.dual > 0.f && b.dual ? P.dual : bounded;
   TokenOut o;
-  o.clipped = (pos && b.hi) || (neg && (b.lo || (P.dual > 0.f && b.dual)));
-  // (an advantage of 0 asks nothing of a ratio past float32's range, e^88.7; NaN stays)
-  const bool idle = A == 0.f && d == d;
-  o.loss = idle ? 0.f : -(bounded * A);
-  o.g = o.clipped || idle ? 0.f : -(r * A);
+  // the advantage's sign says which border can be passed
+  o.clipped = (pos || neg) && beyond(pos, d, x, old, pos ? P.log_hi : P.log_lo);
+  float bounded = o.clipped ? (pos ? P.hi : P.lo) : r;
+  if (P.dual > 0.f) {
+    const bool far = neg && beyond(true, d, x, old, P.log_dual);
+    bounded = far ? P.dual : bounded;
+    o.clipped = o.clipped || far;
+  }
+  o.loss = -(bounded * A);
+  o.g = o.clipped ? 0.f : -(r * A);
   o.kl = 0.f;
   if (P.ref) {
     float em1;
