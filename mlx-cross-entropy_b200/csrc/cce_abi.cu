@@ -1174,7 +1174,7 @@ struct RowsSaved {
   float* weight;    // distillation [1]
   cce::TopkView topk;
   float* se;        // float32: scale of e's parts
-  uint32_t* words;  // float32: largest values of c and e
+  uint32_t* words;  // largest values of c (float32) and e (float32, float16)
   void *e, *e_lo;   // packed rows [N][Dk]
   RowsC c;          // [V][Dk], where c itself is not the operand
   size_t bytes;
@@ -1200,10 +1200,10 @@ RowsSaved rows_saved(void* base, int64_t N, int64_t D, int64_t V, int64_t K, int
   }
   const size_t n = (size_t)N * rows_dk(N, D, dtype);
   r.e = p.take<uint16_t>(n);
+  if (dtype != CCE_BF16) r.words = p.take<uint32_t>(2);
   if (dtype == CCE_F32) {
     r.e_lo = p.take<uint16_t>(n);
     r.se = p.take<float>(2);
-    r.words = p.take<uint32_t>(2);
     r.c.sc = p.take<float>(2);
   }
   const size_t nc = (size_t)V * rows_dk(N, D, dtype);
@@ -1225,10 +1225,10 @@ cudaError_t rows_copies(const RowsSaved& v, const void* e, const void* c, int64_
   const int64_t Dk = rows_dk(N, D, dtype);
   cudaError_t err = cudaSuccess;
   if (dtype != CCE_F32) {
-    if ((err = cce::launch_rows_copy(e, N, D, D, &v.R, v.e, Dk, s)) != cudaSuccess) return err;
-    return v.c.c ? cce::launch_rows_copy(c, V, D, D, nullptr, v.c.c, Dk, s) : cudaSuccess;
+    if ((err = cce::launch_rows_copy(e, N, D, D, &v.R, v.e, Dk, v.words ? v.words + 1 : nullptr, s)) != cudaSuccess)
+      return err;
+    return v.c.c ? cce::launch_rows_copy(c, V, D, D, nullptr, v.c.c, Dk, nullptr, s) : cudaSuccess;
   }
-  if ((err = cudaMemsetAsync(v.words, 0, 2 * sizeof(uint32_t), s)) != cudaSuccess) return err;
   if ((err = cce::launch_absmax((const float*)c, V, D, nullptr, v.words, s)) != cudaSuccess) return err;
   if ((err = cce::launch_absmax((const float*)e, N, D, &v.R, v.words + 1, s)) != cudaSuccess) return err;
   if ((err = cce::launch_split((const float*)e, N, D, Dk, &v.R, v.words + 1, v.se, v.e, v.e_lo, s)) != cudaSuccess)
@@ -1308,7 +1308,6 @@ struct RowsBwdWs {
   float *slabs, *scale, *max_s, *bias_part;
   void *ec, *ec_lo;  // e with the rows' scales folded in
   float* sec;
-  uint32_t* word;
   void* grad_c;  // padded rows
   size_t bytes;
 };
@@ -1328,7 +1327,7 @@ RowsBwdWs rows_bwd_ws(void* base, int64_t N, int64_t D, int64_t V, int dtype, in
       const size_t n = (size_t)N * rows_dk(N, D, dtype);
       w.ec = p.take<uint16_t>(n);
       if (dtype == CCE_F32) w.ec_lo = p.take<uint16_t>(n);
-      else w.sec = p.take<float>(2), w.word = p.take<uint32_t>(1);
+      else w.sec = p.take<float>(2);
     }
   }
   if (flags & CCE_NEED_DBIAS) w.bias_part = p.take<float>((size_t)cce::ceil_div(N, 32) * pl.vc);
@@ -1436,8 +1435,8 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
     }
     if (need_dc) {
       if (fold && a.vc0 == 0) {
-        if (w.word) CCE_CUDA_CHECK(cudaMemsetAsync(w.word, 0, sizeof(uint32_t), sc), what);
-        CCE_CUDA_CHECK(cce::launch_rows_fold(v.e, v.e_lo, a.N, a.Dk, v.R, w.scale, w.max_s, w.word, w.sec, w.ec, w.ec_lo, sc),
+        CCE_CUDA_CHECK(cce::launch_rows_fold(v.e, v.e_lo, a.N, a.Dk, v.R, w.scale, w.max_s, v.words + 1, w.sec, w.ec,
+                                             w.ec_lo, sc),
                        what);
       }
       CCE_CUDA_CHECK(cce::tc_grad_c_rows(a, gc, sc), what);
@@ -1445,7 +1444,7 @@ int rows_backward(cce::RowsGemmArgs a, const RowsSaved& v, const RowsBwdWs& w, c
         const int64_t u = (int64_t)dtype_size(a.dtype) / 2;
         const size_t row = dtype_size(a.dtype);
         CCE_CUDA_CHECK(cce::launch_rows_copy((char*)gc + (size_t)a.vc0 * a.Dout * row, a.vc_len, D * u, a.Dout * u, nullptr,
-                                             (char*)grad_c + (size_t)a.vc0 * D * row, D * u, sc),
+                                             (char*)grad_c + (size_t)a.vc0 * D * row, D * u, nullptr, sc),
                        what);
       }
     }
@@ -1521,7 +1520,8 @@ int cce_logp_forward(const void* e, const void* c, const void* bias, int bias_dt
   if (!rc) rc = check_rows_device(c, N, D, dtype, what);
   if (rc) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  CCE_CUDA_CHECK(cce::launch_rows_pack(N, targets, target_bytes, ignore_index, has_ignore, nullptr, v.R, mask, logp, w.tgt, s),
+  CCE_CUDA_CHECK(cce::launch_rows_pack(N, targets, target_bytes, ignore_index, has_ignore, nullptr, v.R, mask, logp, w.tgt,
+                                       v.words, s),
                  what);
   cce::RowsGemmArgs a = rows_args(bias, bias_dtype, N, D, V, dtype);
   a.R = v.R, a.part_m = w.part_m, a.part_s = w.part_s, a.tgt = w.tgt;
@@ -1599,7 +1599,7 @@ int cce_distill_forward(const void* e, const void* c, const void* bias, int bias
   if (!rc) rc = check_rows_device(c, N, D, dtype, what);
   if (rc) return rc;
   CCE_CUDA_CHECK(cce::launch_rows_pack(N, nullptr, 0, 0, 0, mask, v.R, nullptr, red == CCE_REDUCE_NONE ? loss : nullptr,
-                                       nullptr, s),
+                                       nullptr, v.words, s),
                  what);
   CCE_CUDA_CHECK(cce::launch_topk_prep(teacher_ids, id_bytes, teacher_logp, N, V, (int)K, params->temperature,
                                        params->tail, v.R, v.topk, w.p, w.rest, s),

@@ -167,14 +167,14 @@ struct DistillSum {
   int32_t n;
 };
 // Row lists of the batch; mask_out and per_row_out (0 for rows left out) nullable;
-// tgt: a value per packed row, zeroed (with targets).
+// tgt: a value per packed row, zeroed (with targets); words: two, zeroed, nullable.
 cudaError_t launch_rows_pack(int64_t N, const void* targets, int target_bytes, int64_t ignore_index, int has_ignore,
                              const uint8_t* mask, const RowsView& R, uint8_t* mask_out, float* per_row_out, float* tgt,
-                             cudaStream_t stream);
+                             uint32_t* words, cudaStream_t stream);
 // 16-bit rows: dst[i] = src[row_of[i]] (R; zeros behind the count), or src[i] (R == nullptr),
-// `cols` values each, zeros up to dst_ld
+// `cols` values each, zeros up to dst_ld; word (zeroed, nullable): float16 bits of the largest finite |value|
 cudaError_t launch_rows_copy(const void* src, int64_t rows, int64_t cols, int64_t src_ld, const RowsView* R, void* dst,
-                             int64_t dst_ld, cudaStream_t stream);
+                             int64_t dst_ld, uint32_t* word, cudaStream_t stream);
 // lse (packed rows) and logp (batch rows) from P partials
 cudaError_t launch_rows_logp(const float* part_m, const float* part_s, int64_t P, int64_t N, const RowsView& R,
                              const float* tgt, float* lse, float* logp, cudaStream_t stream);
@@ -194,9 +194,9 @@ cudaError_t launch_rows_scatter(const float* slabs, const SlabPlan& plan, int64_
 cudaError_t launch_rows_scale(const Cotangent& up, const float* whole, const RowsView& R, float* rows, float* max_s,
                               cudaStream_t stream);
 // e's packed rows times rows / max_s, as one float16 value (lo nullptr; scale = {s, 1 / s} of the result, *word:
-// zeroed) or two parts (in their own scale): what grad_c multiplies float16 dlogits of several scales by.
+// the largest |e|) or two parts (in their own scale): what grad_c multiplies float16 dlogits of several scales by.
 cudaError_t launch_rows_fold(const void* e, const void* e_lo, int64_t N, int64_t Dk, const RowsView& R,
-                             const float* rows, const float* max_s, uint32_t* word, float* scale, void* out,
+                             const float* rows, const float* max_s, const uint32_t* word, float* scale, void* out,
                              void* out_lo, cudaStream_t stream);
 // largest |x| of the rows (those of R, if given) as the bits of a float, into *word (zeroed)
 cudaError_t launch_absmax(const float* x, int64_t rows, int64_t D, const RowsView* R, uint32_t* word,

@@ -37,11 +37,12 @@ template <typename TT>  // target type; void: rows count by `mask` alone
 __global__ void __launch_bounds__(kPackThreads)
 rows_pack_kernel(const TT* __restrict__ targets, int64_t ignore_index, int has_ignore,
                  const uint8_t* __restrict__ mask, int64_t N, const RowsView R, uint8_t* __restrict__ mask_out,
-                 float* __restrict__ per_row_out, float* __restrict__ tgt) {
+                 float* __restrict__ per_row_out, float* __restrict__ tgt, uint32_t* __restrict__ words) {
   __shared__ int warp_tot[32];
   __shared__ int base_sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) base_sh = 0;
+  if (words && threadIdx.x < 2) words[threadIdx.x] = 0u;
   __syncthreads();
   for (int64_t r0 = 0; r0 < N; r0 += kPackThreads * kPackPer) {
     const int64_t n0 = r0 + (int64_t)threadIdx.x * kPackPer;
@@ -108,23 +109,42 @@ rows_pack_kernel(const TT* __restrict__ targets, int64_t ignore_index, int has_i
 // A warp per row of 16-bit values: dst[i] = src[row_of[i]], zeros behind the
 // count (the grad_c GEMM multiplies those rows by zeros, so they must be
 // numbers), or with no list dst[i] = src[i]; columns behind `cols` are zeros.
-template <bool kVec>
+// kMax: float16, the largest finite |value| as its bits into *word.
+template <bool kVec, bool kMax>
 __global__ void __launch_bounds__(256)
 rows_copy_kernel(const uint16_t* __restrict__ src, int64_t rows, int64_t cols, int64_t src_ld,
                  const int32_t* __restrict__ row_of, const int32_t* __restrict__ count, uint16_t* __restrict__ dst,
-                 int64_t dst_ld) {
+                 int64_t dst_ld, uint32_t* __restrict__ word) {
   const int lane = threadIdx.x & 31;
+  uint32_t m = 0;
+  auto larger = [&](uint32_t x) {
+    x &= 0x7fffu;
+    m = max(m, x < 0x7c00u ? x : 0u);
+  };
   const int64_t live = count ? *count : rows;
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows; i += (int64_t)gridDim.x * 8) {
     const uint16_t* p = i < live ? src + (row_of ? row_of[i] : i) * src_ld : nullptr;
     uint16_t* q = dst + i * dst_ld;
     if constexpr (kVec) {
-      for (int64_t k = lane * 8; k < dst_ld; k += 256)
-        *reinterpret_cast<uint4*>(q + k) =
-            p && k < cols ? __ldg(reinterpret_cast<const uint4*>(p + k)) : make_uint4(0u, 0u, 0u, 0u);
+      for (int64_t k = lane * 8; k < dst_ld; k += 256) {
+        const uint4 v = p && k < cols ? __ldg(reinterpret_cast<const uint4*>(p + k)) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(q + k) = v;
+        if constexpr (kMax) {
+          larger(v.x), larger(v.y), larger(v.z), larger(v.w);
+          larger(v.x >> 16), larger(v.y >> 16), larger(v.z >> 16), larger(v.w >> 16);
+        }
+      }
     } else {
-      for (int64_t k = lane; k < dst_ld; k += 32) q[k] = p && k < cols ? p[k] : (uint16_t)0;
+      for (int64_t k = lane; k < dst_ld; k += 32) {
+        const uint16_t v = p && k < cols ? p[k] : (uint16_t)0;
+        q[k] = v;
+        if constexpr (kMax) larger(v);
+      }
     }
+  }
+  if constexpr (kMax) {
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0 && m) atomicMax(word, m);
   }
 }
 
@@ -600,25 +620,6 @@ split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, c
   }
 }
 
-// The largest finite |x| of 16-bit rows as float16 bits.
-__global__ void __launch_bounds__(256)
-absmax_half_kernel(const uint16_t* __restrict__ x, int64_t Dk, const int32_t* __restrict__ count,
-                   uint32_t* __restrict__ word) {
-  const int64_t n = *count * Dk / 8;  // (rows are a multiple of 8 wide)
-  uint32_t m = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(x) + i);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t a = w[j] & 0x7fffu, b = (w[j] >> 16) & 0x7fffu;
-      m = max(m, max(a < 0x7c00u ? a : 0u, b < 0x7c00u ? b : 0u));
-    }
-  }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0 && m) atomicMax(word, m);
-}
-
 // grad_c sums s_i (w / s_i) e_i over rows of different scales s_i: e_i takes s_i / S, S the
 // largest.  float16: the largest value goes to [2^13, 2^14), so a row 2^20 below the
 // largest scale still has normal numbers (e alone would leave 4 bits of them); two
@@ -697,29 +698,28 @@ unsigned warps_grid(int64_t N) {
 
 cudaError_t launch_rows_pack(int64_t N, const void* targets, int target_bytes, int64_t ignore_index, int has_ignore,
                              const uint8_t* mask, const RowsView& R, uint8_t* mask_out, float* per_row_out, float* tgt,
-                             cudaStream_t s) {
+                             uint32_t* words, cudaStream_t s) {
   if (targets == nullptr)
-    rows_pack_kernel<void><<<1, kPackThreads, 0, s>>>(nullptr, 0, 0, mask, N, R, mask_out, per_row_out, nullptr);
+    rows_pack_kernel<void><<<1, kPackThreads, 0, s>>>(nullptr, 0, 0, mask, N, R, mask_out, per_row_out, nullptr,
+                                                     words);
   else if (target_bytes == 8)
     rows_pack_kernel<int64_t><<<1, kPackThreads, 0, s>>>((const int64_t*)targets, ignore_index, has_ignore, mask, N, R,
-                                                         mask_out, per_row_out, tgt);
+                                                         mask_out, per_row_out, tgt, words);
   else
     rows_pack_kernel<int32_t><<<1, kPackThreads, 0, s>>>((const int32_t*)targets, ignore_index, has_ignore, mask, N, R,
-                                                         mask_out, per_row_out, tgt);
+                                                         mask_out, per_row_out, tgt, words);
   return launched();
 }
 
 cudaError_t launch_rows_copy(const void* src, int64_t rows, int64_t cols, int64_t src_ld, const RowsView* R, void* dst,
-                             int64_t dst_ld, cudaStream_t s) {
+                             int64_t dst_ld, uint32_t* word, cudaStream_t s) {
   const bool vec = ((cols | src_ld | dst_ld) & 7) == 0 && aligned16(src) && aligned16(dst);
   const int32_t* row_of = R ? R->row_of : nullptr;
   const int32_t* count = R ? R->count : nullptr;
-  if (vec)
-    rows_copy_kernel<true><<<warps_grid(rows), 256, 0, s>>>((const uint16_t*)src, rows, cols, src_ld, row_of, count,
-                                                            (uint16_t*)dst, dst_ld);
-  else
-    rows_copy_kernel<false><<<warps_grid(rows), 256, 0, s>>>((const uint16_t*)src, rows, cols, src_ld, row_of, count,
-                                                             (uint16_t*)dst, dst_ld);
+  const auto kern = word ? (vec ? rows_copy_kernel<true, true> : rows_copy_kernel<false, true>)
+                         : (vec ? rows_copy_kernel<true, false> : rows_copy_kernel<false, false>);
+  kern<<<warps_grid(rows), 256, 0, s>>>((const uint16_t*)src, rows, cols, src_ld, row_of, count, (uint16_t*)dst, dst_ld,
+                                        word);
   return launched();
 }
 
@@ -730,7 +730,7 @@ cudaError_t launch_rows_scale(const Cotangent& up, const float* whole, const Row
 }
 
 cudaError_t launch_rows_fold(const void* e, const void* e_lo, int64_t N, int64_t Dk, const RowsView& R,
-                             const float* rows, const float* max_s, uint32_t* word, float* scale, void* out,
+                             const float* rows, const float* max_s, const uint32_t* word, float* scale, void* out,
                              void* out_lo, cudaStream_t s) {
   const __half *h = static_cast<const __half*>(e), *l = static_cast<const __half*>(e_lo);
   if (e_lo) {
@@ -738,9 +738,6 @@ cudaError_t launch_rows_fold(const void* e, const void* e_lo, int64_t N, int64_t
                                                          static_cast<__half*>(out), static_cast<__half*>(out_lo));
     return launched();
   }
-  absmax_half_kernel<<<warps_grid(ceil_div(N * Dk, 256)), 256, 0, s>>>(static_cast<const uint16_t*>(e), Dk, R.count, word);
-  cudaError_t err = launched();
-  if (err != cudaSuccess) return err;
   rows_fold_kernel<false><<<warps_grid(N), 256, 0, s>>>(h, nullptr, N, Dk, R.count, rows, max_s, word, scale,
                                                         static_cast<__half*>(out), nullptr);
   return launched();
