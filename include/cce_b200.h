@@ -356,7 +356,7 @@ CCE_API int cce_backward_peer(const void* e, const void* c, const void* bias, in
 typedef struct CcePolicyParams {
   double clip_low, clip_high;  /* ratios are clipped to [1 - clip_low, 1 + clip_high] */
   double dual_clip;            /* > 1: loss of a negative advantage bounded by -dual_clip A; 0: not */
-  double kl_coef;              /* weight of e^q - 1 - q, q = ref_logp - logp           */
+  double kl_coef;              /* weight of e^q - 1 - q, q = ref_logp - logp (0: only measured) */
   int32_t reduction;           /* CCE_REDUCE_*                                         */
   int32_t advantage_per_token; /* advantages [N], else [S]                             */
 } CcePolicyParams;
@@ -421,7 +421,9 @@ CCE_API int cce_preference_loss_backward(const float* coef, const float* grad_lo
  * The head's log-probabilities and the distillation loss.  No counterpart in
  * the reference.  Rows that do not count (targets equal to ignore_index, mask
  * bytes of 0) are taken out before the GEMMs; the logits are accumulated in
- * two levels to float32 accuracy, and the gradients are exact (no filter).
+ * two levels to float32 accuracy.  The gradients have no filter: float16 heads
+ * lose what is below 2^-39 of a row's largest dlogit, float32 heads below 2^-50
+ * (bfloat16 has float32's range).
  *
  * A forward call fills `saved` (cce_*_saved_bytes), which the backward call of
  * the same sizes reads; c and bias must not have changed in between.  It holds the
@@ -453,7 +455,7 @@ CCE_API int cce_logp_backward(const void* c, const void* bias, int bias_dtype, c
 #define CCE_DISTILL_MAX_K 1024
 
 typedef struct CceDistillParams {
-  double temperature;  /* the student's logits are divided by it                        */
+  double temperature;  /* the student's logits are divided by it; in [1e-30, 1e30]      */
   int32_t tail;        /* 0: teacher probabilities softmax(teacher_logp / temperature)
                           over its K entries; else e^teacher_logp as given, and the
                           mass they leave over against the student's outside of them   */

@@ -12,10 +12,11 @@ classifier, bias and log-probabilities are differentiable, the other tensors
 are constants.  Kernels: ``csrc/token_loss.cu``, ``csrc/rows_kernels.cu`` and
 the GEMMs of ``csrc/tc_rows.cuh``.
 
-The linear forms differ from ``linear_cross_entropy`` in two ways: gradients
-are exact (the filter of small softmax values is not applied: a policy
-gradient pushes the unlikely tokens too), and rows that do not count are taken
-out before the GEMMs.
+The linear forms differ from ``linear_cross_entropy`` in two ways: the filter of
+small softmax values is not applied (a policy gradient pushes the unlikely
+tokens too: float16 heads lose what is below 2^-39 of a row's largest dlogit,
+float32 heads below 2^-50), and rows that do not count are taken out before the
+GEMMs.
 
 Tokens come as padded rows ``[S, T]`` (a row is a sequence) or packed in one
 dimension with ``cu_seqlens`` (int32 offsets ``[S + 1]``).  Advantages and
@@ -70,7 +71,7 @@ class PreferenceRewards(NamedTuple):
 
 def _untraced(what):
     """torch.compile breaks its graph here: the call runs as it is, between two graphs."""
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_dynamo_compiling():
         raise RuntimeError(f"[{what}] cannot be part of a traced graph")
 
 
@@ -432,6 +433,7 @@ def linear_distillation_loss(e, c, teacher_ids, teacher_logprobs, bias=None, *, 
             over the K entries at the temperature.  With ``tail``: log-probabilities
             over the whole vocabulary at the temperature, used as they are
         bias: optional classifier bias ``[V]``
+        temperature: in [1e-30, 1e30]
         mask: bool ``[...]``; False leaves a row out
         reduction: "mean" over the rows that have an entry, "sum" or "none"
     Returns:
