@@ -422,8 +422,8 @@ CCE_API int cce_preference_loss_backward(const float* coef, const float* grad_lo
  * the reference.  Rows that do not count (targets equal to ignore_index, mask
  * bytes of 0) are taken out before the GEMMs; the logits are accumulated in
  * two levels to float32 accuracy.  The gradients have no filter: float16 heads
- * lose what is below 2^-39 of a row's largest dlogit, float32 heads below 2^-50
- * (bfloat16 has float32's range).
+ * lose what is below 2^-38 of a row's largest dlogit, float32 heads below 2^-48,
+ * bfloat16 heads softmax values below 2^-126.
  *
  * A forward call fills `saved` (cce_*_saved_bytes), which the backward call of
  * the same sizes reads; c and bias must not have changed in between.  It holds the

@@ -14,8 +14,8 @@ the GEMMs of ``csrc/tc_rows.cuh``.
 
 The linear forms differ from ``linear_cross_entropy`` in two ways: the filter of
 small softmax values is not applied (a policy gradient pushes the unlikely
-tokens too: float16 heads lose what is below 2^-39 of a row's largest dlogit,
-float32 heads below 2^-50), and rows that do not count are taken out before the
+tokens too: float16 heads lose what is below 2^-38 of a row's largest dlogit,
+float32 heads below 2^-48), and rows that do not count are taken out before the
 GEMMs.
 
 Tokens come as padded rows ``[S, T]`` (a row is a sequence) or packed in one

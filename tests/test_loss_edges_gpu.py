@@ -126,8 +126,10 @@ def _check_rows_apart(grads, e, c, b, w, mag, d, B, floor):
 
 
 # half the smallest step of a float16 part, 2^-25, in units of 2^-14 of dd; float32's
-# second part is in units of 2^-11 of the first's
-FLOORS = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 2.0 ** -50}
+# second part is in units of 2^-11 of the first's: 2^-50, and where that part, up to
+# 2^-25, is all there is, its product with the other operand's second part, 2^-12 of
+# it, is missing: 2^-51 more
+FLOORS = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39, torch.float32: 1.5 * 2.0 ** -50}
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -191,7 +193,7 @@ def _log_probs_of_rest(e, c, b, t, go, row, col):
     """Log-probabilities and gradients of all rows but one, whose e is far above the
     others' and whose cotangent is 0; the classifier's column ``col`` is as far above
     and masked.  What 22-bit parts with a common scale leave of the other values
-    besides is 2^-50 of the tensor's largest (2^-49: the scale is within a factor 2)."""
+    besides is 1.5 2^-50 of the power of two above the tensor's largest (FLOORS)."""
     rest = torch.arange(e.shape[0]) != row
     cols = torch.arange(c.shape[0]) != col
     xs = leaves(e, c, b)
@@ -200,7 +202,7 @@ def _log_probs_of_rest(e, c, b, t, go, row, col):
     e1, c1, b1, t1 = e[rest], c[cols], b[cols], t[rest] - (t[rest] > col).long()
     lq = torch.log_softmax(e1.double() @ c1.double().t() + b1.double(), 1)
     B = Bounds(e1, c1, b1)
-    floor = 2.0 ** -49 if e.dtype == torch.float32 else 0.0
+    floor = 2 * FLOORS[e.dtype] if e.dtype == torch.float32 else 0.0
     lost = floor * float(e.abs().max() * c1.abs().sum(1).max() + c.abs().max() * e1.abs().sum(1).max())
     B.dz += lost
     B.dlogp += 2 * lost
