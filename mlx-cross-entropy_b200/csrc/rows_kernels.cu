@@ -574,13 +574,14 @@ absmax_kernel(const float* __restrict__ x, int64_t rows, int64_t D, const int32_
 // hi has 11 bits down to 2^-14, so of values down to 2^-28 of the largest 22 bits are
 // held, and 2^-36 absolute (in units of 1 / s), 2^-50 of the largest, below.  The
 // product of two lo's is left out: half as much again there, and 2^-78 of the largest
-// values' product where both are that small.  (In hi's
-// own units lo would run out at 2^-25, and one row 2^20 above the others would leave
-// them 17 bits.)  |s x - hi| <= 4, so lo stays below 2^13.
+// values' product where both are that small.  (In hi's own units lo would run out at
+// 2^-25, and one row 2^20 above the others would leave them 17 bits.)
+// |s x - hi| <= 4, so lo stays below 2^13.
 __device__ __forceinline__ void split_parts(float y, __half& hi, __half& lo) {
   hi = __float2half_rn(y);
   lo = __float2half_rn((y - __half2float(hi)) * kLoUnits);
 }
+
 __global__ void __launch_bounds__(256)
 split_kernel(const float* __restrict__ x, int64_t rows, int64_t D, int64_t Dp, const int32_t* __restrict__ row_of,
              const int32_t* __restrict__ count, int vec, const uint32_t* __restrict__ word, float* __restrict__ scale,

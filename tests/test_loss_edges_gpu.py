@@ -159,6 +159,25 @@ def test_one_cotangent_far_above_the_others(dtype, chunks, monkeypatch):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_the_same_bits_again_and_from_a_graph_kept(dtype):
+    e, c, b, t, g = head(500, 96, 2500, dtype, 14, bias=torch.float32)
+    go = (torch.randn(500, generator=g) * 2.0 ** torch.randint(-12, 12, (500,), generator=g)).cuda()
+    tlp, ids = (v.cuda() for v in teacher(e, c, b, 12, g))
+    xs = leaves(e, c, b)
+
+    def run():
+        logp = mlx_cce.linear_log_probs(xs[0], xs[1], t.cuda(), xs[2])
+        rows = mlx_cce.linear_distillation_loss(xs[0], xs[1], ids, tlp, xs[2], tail=True, reduction="none")
+        return [(logp + rows).detach(), *torch.autograd.grad((logp, rows), xs, (go, go.flip(0)), retain_graph=True),
+                *torch.autograd.grad((logp, rows), xs, (go, go.flip(0)))]
+
+    first = run()
+    assert all(torch.equal(x, y) for x, y in zip(first[1:4], first[4:]))
+    for _ in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(first, run()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_teacher_probabilities_above_one(dtype, reduction):
     """With a tail the teacher's values are used as they are: a sum of 40 must not
